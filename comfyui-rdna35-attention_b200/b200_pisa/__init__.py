@@ -26,6 +26,7 @@ import torch
 
 from . import _lib
 from ._lib import LIB, check, ptr, stream_of, view
+from .rotary import axial_rope, qk_norm_rope, qk_norm_rope_backward
 
 __version__ = "0.1.0"
 
@@ -591,6 +592,7 @@ __all__ = [
     "MAX_BLOCKS",
     "SPATIAL_SPARSE_EXACT_BLOCKS",
     "SPATIAL_TOKENS",
+    "axial_rope",
     "block_mask_bias",
     "block_stats_hyd",
     "build_info",
@@ -605,4 +607,6 @@ __all__ = [
     "generic_forward",
     "pack_views",
     "prepare",
+    "qk_norm_rope",
+    "qk_norm_rope_backward",
 ]

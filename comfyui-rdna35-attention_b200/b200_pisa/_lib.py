@@ -57,6 +57,27 @@ class View(ctypes.Structure):
 
 _VIEW_P = ctypes.POINTER(View)
 
+POS_I32, POS_I64, POS_F32, POS_F64 = 0, 1, 2, 3
+MAX_AXES = 4
+
+
+class Rotary(ctypes.Structure):
+    _fields_ = [
+        ("positions", ctypes.c_void_p),
+        ("stride_b", ctypes.c_int64),
+        ("stride_t", ctypes.c_int64),
+        ("stride_axis", ctypes.c_int64),
+        ("pos_dtype", ctypes.c_int32),
+        ("n_axes", ctypes.c_int32),
+        ("axes_dims", ctypes.c_int32 * MAX_AXES),
+        ("interleaved", ctypes.c_int32),
+        ("inverse", ctypes.c_int32),
+        ("theta", ctypes.c_double * MAX_AXES),
+    ]
+
+
+_ROTARY_P = ctypes.POINTER(Rotary)
+
 SIGNATURES: dict[str, tuple] = {
     "b2_last_error": (ctypes.c_char_p, []),
     "b2_last_kernel": (ctypes.c_char_p, []),
@@ -85,6 +106,11 @@ SIGNATURES: dict[str, tuple] = {
     "b2_fixed_block_attention_masked": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _F32, _I32, _VP, _I64,
                                                        _VP]),
     "b2_pack_block_bias": (ctypes.c_int, [_VP, _I32, _I64, _I64, _I64, _I32, _I32, _VP, _VP]),
+    "b2_axial_rope": (ctypes.c_int, [_VIEW_P, _VIEW_P, _ROTARY_P, _VP]),
+    "b2_qk_norm_rope": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VP, _VP, _I32, _F32, _ROTARY_P, _VP]),
+    "b2_qk_norm_rope_workspace_bytes": (_I64, [_I32]),
+    "b2_qk_norm_rope_backward": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VP, _VP, _I32,
+                                                _F32, _ROTARY_P, _VP, _VP, _VP, _VP]),
     "b2_pack_rows": (ctypes.c_int, [_VIEW_P, _VP, _VP]),
     "b2_unpack_rows": (ctypes.c_int, [_VP, _VIEW_P, _VP]),
     "b2_merge_epilogue": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VIEW_P, _VP]),

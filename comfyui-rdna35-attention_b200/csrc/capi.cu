@@ -728,6 +728,121 @@ int b2_pack_block_bias(const void* mask, int32_t mask_dtype, int64_t stride_bh, 
   return ok();
 }
 
+}  // extern "C"
+
+namespace {
+int check_rotary(const b2_rotary* r, const b2_view* v) {
+  if (r == nullptr || r->positions == nullptr) return fail(B2_ERR_INVALID, "positions must be non-NULL");
+  if (r->pos_dtype < B2_POS_I32 || r->pos_dtype > B2_POS_F64) return fail(B2_ERR_INVALID, "unknown position dtype");
+  if (r->n_axes < 1 || r->n_axes > B2_MAX_AXES) return fail(B2_ERR_INVALID, "rotary axes must be 1..%d", B2_MAX_AXES);
+  int64_t sum = 0;
+  for (int i = 0; i < r->n_axes; ++i) {
+    if (r->axes_dims[i] <= 0 || r->axes_dims[i] % 2) return fail(B2_ERR_INVALID, "axis dims must be positive and even");
+    if (!(r->theta[i] > 0.0) || !(r->theta[i] < 1e300)) return fail(B2_ERR_INVALID, "theta must be positive and finite");
+    sum += r->axes_dims[i];
+  }
+  if (sum > v->head_dim) return fail(B2_ERR_INVALID, "axis dims sum to more than the head dimension");
+  return B2_OK;
+}
+
+int check_rotary_view(const b2_view* v, const char* name, const b2_view* like) {
+  const int rc = check_view(v, name);
+  if (rc) return rc;
+  if (v->order != B2_ORDER_LINEAR) return fail(B2_ERR_UNSUPPORTED, "%s must be in linear token order", name);
+  if (v->head_dim > 256 || v->head_dim % 8)
+    return fail(B2_ERR_UNSUPPORTED, "rotary positions support D <= 256, a multiple of 8");
+  if (like != nullptr && (!same_bht(v, like) || v->dtype != like->dtype))
+    return fail(B2_ERR_INVALID, "%s must have its input's [B,H,T,D] and dtype", name);
+  return B2_OK;
+}
+
+int check_qk(const b2_view* q, const b2_view* k, const void* qw, const void* kw, int32_t w_dtype, float eps,
+             const b2_rotary* rot) {
+  int rc;
+  if ((rc = check_rotary_view(q, "q", nullptr)) || (rc = check_rotary_view(k, "k", nullptr)) ||
+      (rc = check_rotary(rot, q)))
+    return rc;
+  if (q->batch != k->batch || q->tokens != k->tokens || q->head_dim != k->head_dim || q->dtype != k->dtype)
+    return fail(B2_ERR_INVALID, "q and k must share B, T, D and dtype");
+  if (w_dtype != B2_BF16 && w_dtype != B2_F16 && w_dtype != B2_F32) return fail(B2_ERR_INVALID, "unknown weight dtype");
+  if (!(eps >= 0.f)) return fail(B2_ERR_INVALID, "eps must be >= 0");
+  const uintptr_t mask = w_dtype == B2_F32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(qw) | reinterpret_cast<uintptr_t>(kw)) & mask)
+    return fail(B2_ERR_INVALID, "weights must be aligned to their type");
+  return B2_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int b2_axial_rope(const b2_view* x, const b2_view* out, const b2_rotary* rot, void* stream) {
+  int rc;
+  if ((rc = check_rotary_view(x, "x", nullptr)) || (rc = check_rotary_view(out, "out", x)) || (rc = check_rotary(rot, x)))
+    return rc;
+  RotaryCall c{};
+  c.x[0] = x;
+  c.y[0] = out;
+  c.rot = rot;
+  const cudaError_t err = launch_rotary(c, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "rotary launch");
+  return ok();
+}
+
+int b2_qk_norm_rope(const b2_view* q, const b2_view* k, const b2_view* q_out, const b2_view* k_out,
+                    const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                    const b2_rotary* rot, void* stream) {
+  int rc = check_qk(q, k, q_weight, k_weight, weight_dtype, eps, rot);
+  if (rc) return rc;
+  if ((rc = check_rotary_view(q_out, "q_out", q)) || (rc = check_rotary_view(k_out, "k_out", k))) return rc;
+  RotaryCall c{};
+  c.x[0] = q, c.x[1] = k;
+  c.y[0] = q_out, c.y[1] = k_out;
+  c.w[0] = q_weight, c.w[1] = k_weight;
+  c.w_dtype = weight_dtype;
+  c.norm = true;
+  c.eps = eps;
+  c.rot = rot;
+  const cudaError_t err = launch_rotary(c, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "norm and rotary launch");
+  return ok();
+}
+
+int64_t b2_qk_norm_rope_workspace_bytes(int32_t head_dim) {
+  if (head_dim <= 0 || head_dim > 256 || head_dim % 8) return -1;
+  return rotary_workspace_bytes(head_dim);
+}
+
+int b2_qk_norm_rope_backward(const b2_view* q, const b2_view* k, const b2_view* dq_out, const b2_view* dk_out,
+                             const b2_view* q_grad, const b2_view* k_grad, const void* q_weight, const void* k_weight,
+                             int32_t weight_dtype, float eps, const b2_rotary* rot, void* q_weight_grad,
+                             void* k_weight_grad, void* workspace, void* stream) {
+  int rc = check_qk(q, k, q_weight, k_weight, weight_dtype, eps, rot);
+  if (rc) return rc;
+  if ((rc = check_rotary_view(dq_out, "dq_out", q)) || (rc = check_rotary_view(dk_out, "dk_out", k)) ||
+      (rc = check_rotary_view(q_grad, "q_grad", q)) || (rc = check_rotary_view(k_grad, "k_grad", k)))
+    return rc;
+  const uintptr_t mask = weight_dtype == B2_F32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(q_weight_grad) | reinterpret_cast<uintptr_t>(k_weight_grad)) & mask)
+    return fail(B2_ERR_INVALID, "weight gradients must be aligned to their type");
+  if ((q_weight_grad != nullptr || k_weight_grad != nullptr) &&
+      (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return fail(B2_ERR_INVALID, "workspace must be non-NULL and 16-byte aligned");
+  RotaryCall c{};
+  c.x[0] = q, c.x[1] = k;
+  c.dy[0] = dq_out, c.dy[1] = dk_out;
+  c.y[0] = q_grad, c.y[1] = k_grad;
+  c.w[0] = q_weight, c.w[1] = k_weight;
+  c.dw[0] = q_weight_grad, c.dw[1] = k_weight_grad;
+  c.w_dtype = weight_dtype;
+  c.norm = true;
+  c.eps = eps;
+  c.rot = rot;
+  c.partial = static_cast<float*>(workspace);
+  const cudaError_t err = launch_rotary(c, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "norm and rotary gradient launch");
+  return ok();
+}
+
 int b2_pack_rows(const b2_view* src, void* dst, void* stream) {
   int rc = check_view(src, "src");
   if (rc) return rc;

@@ -88,6 +88,23 @@ cudaError_t launch_fixed_f32(const Rows& q, const Rows& k, const Rows& v, const 
                              cudaStream_t stream);
 cudaError_t launch_block_bias(const void* mask, int mask_dtype, int64_t s_bh, int64_t s_row, int64_t s_col,
                               int mask_rows_bh, int tokens, float* bias, cudaStream_t stream);
+// Norm + rotary positions (rotary.cu): one or two sides (queries, keys).
+// Forward: y from x.  Gradients (dy set): y receives dx, dw (may be NULL) the
+// weight gradients, partial is rotary_workspace_bytes() of scratch.
+struct RotaryCall {
+  const b2_view* x[2];
+  const b2_view* dy[2];
+  const b2_view* y[2];
+  const void* w[2];
+  void* dw[2];
+  int w_dtype;
+  bool norm;
+  float eps;
+  const b2_rotary* rot;
+  float* partial;
+};
+int64_t rotary_workspace_bytes(int head_dim);
+cudaError_t launch_rotary(const RotaryCall& call, cudaStream_t stream);
 // Host-side helpers of the C ABI layer (capi.cu): the shared statistics
 // argument checks and the thread-local error string behind b2_last_error.
 int check_stats_call(const b2_view* q, const b2_view* k, const b2_view* v, int mode, const void* q_centroids,

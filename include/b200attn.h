@@ -305,6 +305,47 @@ int b2_fixed_block_attention_masked(const b2_view* q, const b2_view* k,
                                     const float* bias, int64_t bias_bh_stride,
                                     void* stream);
 
+/* ---- Per-head RMS norm of queries and keys and rotary positions with several
+ * axes (time, height, width, ...) in one pass.  No counterpart in the
+ * reference, whose attention starts from normed and rotated q/k.
+ * b2_rotary: positions[b*stride_b + t*stride_t + a*stride_axis] (element
+ * strides; stride_b 0 for one set of positions for the whole batch) is the
+ * position of token t on axis a.  Axis a rotates axes_dims[a] columns (even)
+ * with rates theta[a]^(-2j/axes_dims[a]); the axes' pairs follow one another
+ * and cover the first R = sum(axes_dims) columns, the others pass through.
+ * interleaved: pair p is columns (2p, 2p+1), else (p, p + R/2).  inverse:
+ * rotate by the negative angle (the rotation's gradient).  Angles are reduced
+ * in FP64. */
+enum b2_pos_dtype { B2_POS_I32 = 0, B2_POS_I64 = 1, B2_POS_F32 = 2, B2_POS_F64 = 3 };
+#define B2_MAX_AXES 4
+typedef struct b2_rotary {
+  const void* positions;
+  int64_t stride_b, stride_t, stride_axis;
+  int32_t pos_dtype; /* enum b2_pos_dtype */
+  int32_t n_axes;    /* 1..B2_MAX_AXES */
+  int32_t axes_dims[B2_MAX_AXES];
+  int32_t interleaved, inverse;
+  double theta[B2_MAX_AXES];
+} b2_rotary;
+/* out = rotation(x) for x [B,H,T,D] (BF16, FP16, FP32; D <= 256, a multiple
+ * of 8, linear order). */
+int b2_axial_rope(const b2_view* x, const b2_view* out, const b2_rotary* rot, void* stream);
+/* out = rotation(x * rsqrt(mean(x^2) + eps) * weight) of q and k (equal B, T,
+ * D; own head counts), one rounding at the end.  Weights [D] of weight_dtype
+ * (enum b2_dtype), NULL for none. */
+int b2_qk_norm_rope(const b2_view* q, const b2_view* k, const b2_view* q_out, const b2_view* k_out,
+                    const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                    const b2_rotary* rot, void* stream);
+/* Its gradients: q_grad / k_grad (of q, k) from dq_out / dk_out (of the
+ * outputs), and the weights' in weight_dtype (NULL: not wanted).  workspace:
+ * b2_qk_norm_rope_workspace_bytes(D) bytes, read and written only by this
+ * call; results do not depend on the order blocks run in. */
+int64_t b2_qk_norm_rope_workspace_bytes(int32_t head_dim);
+int b2_qk_norm_rope_backward(const b2_view* q, const b2_view* k, const b2_view* dq_out, const b2_view* dk_out,
+                             const b2_view* q_grad, const b2_view* k_grad, const void* q_weight, const void* k_weight,
+                             int32_t weight_dtype, float eps, const b2_rotary* rot, void* q_weight_grad,
+                             void* k_weight_grad, void* workspace, void* stream);
+
 /* ---- Layout kernels. */
 /* pisa_kernels.cu:247-272: [B,H,T,D] tiled views -> contiguous [BH,T,D]. */
 int b2_pack_rows(const b2_view* src, void* dst, void* stream);

@@ -26,6 +26,7 @@ import torch
 
 from . import _lib
 from ._lib import LIB, check, ptr, stream_of, view
+from .exact import attention, attention_backward, attention_forward
 from .rotary import axial_rope, qk_norm_rope, qk_norm_rope_backward
 
 __version__ = "0.1.0"
@@ -592,6 +593,9 @@ __all__ = [
     "MAX_BLOCKS",
     "SPATIAL_SPARSE_EXACT_BLOCKS",
     "SPATIAL_TOKENS",
+    "attention",
+    "attention_backward",
+    "attention_forward",
     "axial_rope",
     "block_mask_bias",
     "block_stats_hyd",

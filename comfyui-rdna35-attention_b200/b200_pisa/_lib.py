@@ -106,6 +106,10 @@ SIGNATURES: dict[str, tuple] = {
     "b2_fixed_block_attention_masked": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _F32, _I32, _VP, _I64,
                                                        _VP]),
     "b2_pack_block_bias": (ctypes.c_int, [_VP, _I32, _I64, _I64, _I64, _I32, _I32, _VP, _VP]),
+    "b2_attention_forward": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _F32, _I32, _VP, _VP, _VP]),
+    "b2_attention_backward_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32]),
+    "b2_attention_backward": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VP, _VIEW_P, _VIEW_P,
+                                             _VIEW_P, _F32, _I32, _VP, _VP, _VP]),
     "b2_axial_rope": (ctypes.c_int, [_VIEW_P, _VIEW_P, _ROTARY_P, _VP]),
     "b2_qk_norm_rope": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VP, _VP, _I32, _F32, _ROTARY_P, _VP]),
     "b2_qk_norm_rope_workspace_bytes": (_I64, [_I32]),

@@ -1,0 +1,815 @@
+// Backward pass of exact attention: dQ, dK and dV from q, k, v, out, dout and
+// the forward pass's log-sum-exp, on tcgen05 with TMA-staged tiles.
+//
+//   P  = exp(scale q.k - lse)         recomputed, never stored
+//   delta = rowsum(dout * out)
+//   dV = P^T dout        dP = dout V^T        dS = P * (dP - delta)
+//   dQ = scale dS K      dK = scale dS^T Q
+//
+// Two kinds of CTA share one launch:
+//   dK/dV: owns 128 keys of one key/value head and walks the query tiles of
+//     every query head of its group: S^T = K Q^T, dP^T = V dO^T (keys are the
+//     rows, so P^T and dS^T are written back to tensor memory as they come and
+//     are the A operands of dV += P^T dO and dK += dS^T Q);
+//   dQ: owns 128 queries of one head and walks the key tiles: S = Q K^T,
+//     dP = dO V^T, dQ += dS K.
+// S and dP are so computed twice: seven products instead of the formula's
+// five.  In return no partial dQ leaves the CTA that owns it: no FP32 scratch
+// of dQ's size, no atomics, and results that do not depend on the order CTAs
+// run in.  A single pass would add 64 KB of FP32 reductions to L2 and a dS
+// tile in shared memory for each pair of tiles, and is bound by shared-memory
+// bandwidth (about 3750 cycles a pair at 128 B a cycle, against 7 * 512 for
+// the products here).
+//
+// Warp roles (320 threads, one CTA per SM): warp 0 TMA producer, warp 1 MMA
+// issuer and TMEM owner, warps 2..9 elementwise (warp % 4 is the TMEM lane
+// quadrant, warps 2-5 take columns 0-63 and 6-9 columns 64-127 of a tile).
+//
+// Precision: products of 16-bit operands accumulated in FP32; P and dS are
+// rounded to the inputs' type once, as operands.  FP16 has too small a range
+// for them, so there P is held times 2^8 and dS times a power of two chosen
+// from the largest norms of dO and V rows (|dP - delta| <= 2 |dO||V|), which
+// cannot overflow; both are taken out again in FP32 at the end.
+#include <cudaTypedefs.h>
+
+#include <type_traits>
+
+#include "kernels.h"
+#include "umma.cuh"
+
+namespace b2 {
+
+namespace {
+
+using namespace umma;
+
+constexpr int kTile = 128;
+constexpr int kThreads = 320;
+constexpr uint32_t kHalfBytes = kTile * 128;  // 128 rows x 64 16-bit columns
+constexpr uint32_t kStatBytes = 2 * kTile * 4;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kShiftP16 = 8;  // FP16: P is held times 2^8
+
+// TMEM columns
+constexpr uint32_t kColS = 0, kColDP = 128, kColAcc0 = 256, kColAcc1 = 384;
+
+struct GradArgs {
+  Rows dq, dk, dv;
+  const float* stat;       // [B*H][query tiles][2][128]: -lse*log2e (+ shift), -delta
+  const uint32_t* maxima;  // FP16: [B*Hk][2] bits of the largest squared norms of dO and V rows
+  const int32_t* key_lengths;
+  int heads, kv_heads, group;
+  int tq, tk, dim;
+  int q_tiles, k_tiles;
+  int n_dkv;  // CTAs of the dK/dV kind (they come first)
+  int causal;
+  float scale, scale_log2;
+  int* status;
+};
+
+struct __align__(8) Misc {
+  uint64_t own_full;      // the CTA's own two tiles
+  uint64_t a_full[2], a_empty[2];  // walked tiles: Q (with statistics) or K
+  uint64_t b_full[2], b_empty[2];  // dO or V
+  uint64_t s_full, s_read, p_full, dp_full, ds_full;
+  uint64_t acc0_done, acc1_done, all_done;
+  uint32_t tmem;
+  int abort_flag;
+};
+
+template <int HALVES>
+struct Smem {
+  static constexpr uint32_t tile = HALVES * kHalfBytes;
+  static constexpr uint32_t own0 = 0;
+  static constexpr uint32_t own1 = own0 + tile;
+  static constexpr uint32_t a = own1 + tile;      // [2]
+  static constexpr uint32_t b = a + 2 * tile;     // [2]
+  static constexpr uint32_t stat = b + 2 * tile;  // [2]
+  static constexpr uint32_t misc = stat + 2 * kStatBytes;
+  // one CTA per SM (each owns all 512 TMEM columns)
+  static constexpr uint32_t used = misc + sizeof(Misc);
+  static constexpr uint32_t total = used < 120 * 1024 ? 120 * 1024 : used;
+};
+static_assert(Smem<2>::total <= 232448, "shared memory budget");
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// 128 rows of one head as HALVES boxes of 64 columns.
+template <int HALVES>
+__device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int row, int h, int b) {
+#pragma unroll
+  for (int dh = 0; dh < HALVES; ++dh)
+    tma_load_4d(static_cast<char*>(dst) + dh * kHalfBytes, map, bar, dh * 64, row, h, b);
+}
+
+// D[128 x 128] = A B^T over the head dimension, both tiles K-major in shared memory.
+template <bool BF16, int HALVES>
+__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a_addr, uint32_t b_addr) {
+  constexpr uint32_t idesc = idesc_f16(128, 128, BF16, false, false);
+#pragma unroll
+  for (int kk = 0; kk < 4 * HALVES; ++kk) {
+    const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
+    mma_ss(d, smem_desc_sw128(a_addr + off, 16, 1024), smem_desc_sw128(b_addr + off, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+  }
+}
+
+// D[128 x D] (+)= A B with A (128 x 128, 16-bit) in tensor memory over the
+// first 32 columns of each 64-column half at `a`, B's rows as contraction.
+template <bool BF16, int HALVES>
+__device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint32_t b_addr, bool accumulate) {
+  constexpr uint32_t idesc = idesc_f16(128, 64 * HALVES, BF16, false, true);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk)
+    mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, smem_desc_sw128(b_addr + kk * 2048, kHalfBytes, 1024), idesc,
+           accumulate || kk > 0 ? 1u : 0u);
+}
+
+__device__ __forceinline__ uint64_t pack_f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack_f2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ int key_count(const GradArgs& a, int b) {
+  return a.key_lengths != nullptr ? min(max(a.key_lengths[b], 0), a.tk) : a.tk;
+}
+
+// FP16: the power of two dS is held times (P's 2^8 aside), so that
+// 2^8 * 2 max|dO| max|V| times it stays below 2^15.
+__device__ __forceinline__ float ds_gain(const GradArgs& a, int bhk) {
+  const float bound2 = __uint_as_float(a.maxima[2 * bhk]) * __uint_as_float(a.maxima[2 * bhk + 1]);
+  if (!(bound2 > 0.f) || !(bound2 < 3e38f)) return 1.f;
+  const int e = 15 - kShiftP16 - 1 - 1 - (ilogbf(bound2) >> 1);  // bound < 2^(ilogb(bound2)/2 + 1)
+  return ldexpf(1.f, min(max(e, -60), 60));
+}
+
+// Store 32 FP32 accumulator columns of one row, scaled, as 16-bit.
+template <typename T>
+__device__ __forceinline__ void store_cols(char* row, int c0, int dim, const uint32_t* r, float mul) {
+  uint32_t w[16];
+#pragma unroll
+  for (int c = 0; c < 32; c += 2) w[c / 2] = Cvt<T>::pack2(__uint_as_float(r[c]) * mul, __uint_as_float(r[c + 1]) * mul);
+  uint4* dst = reinterpret_cast<uint4*>(row + c0 * 2);
+#pragma unroll
+  for (int q4 = 0; q4 < 4; ++q4)
+    if (c0 + 8 * q4 < dim) dst[q4] = make_uint4(w[4 * q4], w[4 * q4 + 1], w[4 * q4 + 2], w[4 * q4 + 3]);
+}
+
+// One accumulator row (64 * HALVES columns at `taddr`) to global memory; a
+// row that sees nothing (or lies past the keys) is written as zeros.  The
+// loads are a warp's: every lane calls this, row NULL stores nothing.
+template <typename T, int HALVES>
+__device__ __forceinline__ void store_row(uint32_t taddr, char* row, int dim, float mul, bool zero) {
+#pragma unroll 1
+  for (int c0 = 0; c0 < 64 * HALVES; c0 += 32) {
+    uint32_t r[32];
+    tmem_ld32(taddr + c0, r);
+    tmem_wait_ld();
+    if (row == nullptr) continue;
+    if (zero) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) r[c] = 0u;
+    }
+    store_cols<T>(row, c0, dim, r, mul);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_zero_row(char* row, int dim) {
+  for (int c = 0; c < dim; c += 8) *reinterpret_cast<uint4*>(row + c * 2) = make_uint4(0u, 0u, 0u, 0u);
+}
+
+// ------------------------------------------------------------ dK and dV
+template <bool BF16, int HALVES>
+__device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensorMap* k_map, const CUtensorMap* v_map,
+                                        const CUtensorMap* do_map, const GradArgs& a, char* smem, Misc& m,
+                                        uint32_t tmem) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  using L = Smem<HALVES>;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int kt = blockIdx.x % a.k_tiles;
+  const int bhk = blockIdx.x / a.k_tiles;
+  const int b = bhk / a.kv_heads;
+  const int hk = bhk - b * a.kv_heads;
+  const int k0 = kt * kTile;
+  const int len = key_count(a, b);
+  const int off = a.tk - a.tq;  // causal: query i sees keys up to i + off
+  const int first = a.causal ? max(0, k0 - off) / kTile : 0;
+  const int per_head = k0 < len ? a.q_tiles - first : 0;
+  const int n = per_head * a.group;
+  volatile int* abort_flag = &m.abort_flag;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0 && !*abort_flag) {
+      mbar_expect_tx(&m.own_full, 2 * L::tile);
+      load_tile<HALVES>(smem + L::own0, k_map, &m.own_full, k0, hk, b);
+      load_tile<HALVES>(smem + L::own1, v_map, &m.own_full, k0, hk, b);
+      int na = 0, nb = 0;
+      for (int i = 0; i < n; ++i) {
+        const int s = i & 1;
+        const uint32_t free_parity = ((i >> 1) & 1) ^ 1;
+        const int g = i / per_head;
+        const int qt = first + i - g * per_head;
+        const int h = hk * a.group + g;
+        if (!mbar_wait(&m.a_empty[s], free_parity, abort_flag, a.status, 1)) break;
+        mbar_expect_tx(&m.a_full[s], L::tile + kStatBytes);
+        load_tile<HALVES>(smem + L::a + s * L::tile, q_map, &m.a_full[s], qt * kTile, h, b);
+        bulk_load(smem + L::stat + s * kStatBytes, a.stat + ((int64_t(b) * a.heads + h) * a.q_tiles + qt) * (2 * kTile),
+                  kStatBytes, &m.a_full[s]);
+        na = i + 1;
+        if (!mbar_wait(&m.b_empty[s], free_parity, abort_flag, a.status, 2)) break;
+        mbar_expect_tx(&m.b_full[s], L::tile);
+        load_tile<HALVES>(smem + L::b + s * L::tile, do_map, &m.b_full[s], qt * kTile, h, b);
+        nb = i + 1;
+      }
+      if (*abort_flag) {
+        drain_loads(m.a_full, 2, na, &m.own_full, a.status);
+        drain_loads(m.b_full, 2, nb, nullptr, a.status);
+      }
+    }
+  } else if (warp == 1) {
+    if (n > 0 && elect_one()) {
+      const uint32_t k_addr = smem_u32(smem + L::own0), v_addr = smem_u32(smem + L::own1);
+      auto q_addr = [&](int s) { return smem_u32(smem + L::a + s * L::tile); };
+      auto do_addr = [&](int s) { return smem_u32(smem + L::b + s * L::tile); };
+      bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3) && mbar_wait(&m.a_full[0], 0, abort_flag, a.status, 4);
+      if (ok) {
+        product_rows<BF16, HALVES>(tmem + kColS, k_addr, q_addr(0));
+        mma_commit(&m.s_full);
+        ok = mbar_wait(&m.b_full[0], 0, abort_flag, a.status, 5);
+      }
+      if (ok) {
+        product_rows<BF16, HALVES>(tmem + kColDP, v_addr, do_addr(0));
+        mma_commit(&m.dp_full);
+      }
+      for (int i = 0; ok && i < n; ++i) {
+        const int s = i & 1, t = s ^ 1;
+        const uint32_t ph = i & 1, next_ph = ((i + 1) >> 1) & 1;
+        const bool more = i + 1 < n;
+        // dV += P^T dO; then the next S may take the columns P was read from
+        if (!(ok = mbar_wait(&m.p_full, ph, abort_flag, a.status, 6))) break;
+        tc_fence_after();
+        product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColS, do_addr(s), i > 0);
+        mma_commit(&m.acc0_done);
+        mma_commit(&m.b_empty[s]);
+        if (more) {
+          ok = mbar_wait(&m.a_full[t], next_ph, abort_flag, a.status, 7) &&
+               mbar_wait(&m.acc0_done, ph, abort_flag, a.status, 8);
+          if (!ok) break;
+          product_rows<BF16, HALVES>(tmem + kColS, k_addr, q_addr(t));
+          mma_commit(&m.s_full);
+        }
+        // dK += dS^T Q; then the next dP
+        if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
+        tc_fence_after();
+        product_cols<BF16, HALVES>(tmem + kColAcc1, tmem + kColDP, q_addr(s), i > 0);
+        mma_commit(&m.acc1_done);
+        mma_commit(&m.a_empty[s]);
+        if (more) {
+          ok = mbar_wait(&m.b_full[t], next_ph, abort_flag, a.status, 10) &&
+               mbar_wait(&m.acc1_done, ph, abort_flag, a.status, 11);
+          if (!ok) break;
+          product_rows<BF16, HALVES>(tmem + kColDP, v_addr, do_addr(t));
+          mma_commit(&m.dp_full);
+        }
+      }
+      // every product completes before TMEM is read and released (bounded by
+      // time only, even after an abort)
+      mma_commit(&m.all_done);
+      int no_abort = 0;
+      mbar_wait(&m.all_done, 0, &no_abort, a.status, 12);
+    }
+  } else {
+    const int wg = (warp - 2) >> 2;
+    const int sub = warp & 3;
+    const int row = sub * 32 + lane;
+    const int key = k0 + row;
+    const uint32_t lanes = static_cast<uint32_t>(sub * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + kColS + wg * 64;
+    const uint32_t dp_addr = tmem + lanes + kColDP + wg * 64;
+    float gain = 1.f;
+    if constexpr (!BF16) gain = ds_gain(a, bhk);
+    const uint64_t gain2 = pack_f2(gain, gain);
+    const uint64_t scale2 = pack_f2(a.scale_log2, a.scale_log2);
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const int s = i & 1;
+      const uint32_t ph = i & 1;
+      const float* stat = reinterpret_cast<const float*>(smem + L::stat + s * kStatBytes) + wg * 64;
+      // causal: columns below `lim` are queries before the key
+      uint32_t bad0 = 0u, bad1 = 0u;
+      if (a.causal) {
+        const int lim = key - off - (first + i % per_head) * kTile - wg * 64;
+        const uint64_t bad = lim <= 0 ? 0ull : lim >= 64 ? ~0ull : (1ull << lim) - 1ull;
+        bad0 = static_cast<uint32_t>(bad);
+        bad1 = static_cast<uint32_t>(bad >> 32);
+      }
+      const bool masked = (bad0 | bad1) != 0u;
+      if (!(ok = mbar_wait(&m.a_full[s], (i >> 1) & 1, abort_flag, a.status, 13))) break;  // statistics
+      if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
+      tc_fence_after();
+      uint32_t v[64];
+      tmem_ld32(s_addr, v);
+      tmem_ld32(s_addr + 32, v + 32);
+      tmem_wait_ld();
+      uint32_t w[32];
+#pragma unroll
+      for (int c = 0; c < 64; c += 4) {
+        const float4 nl = *reinterpret_cast<const float4*>(stat + c);
+        float x[4];
+        unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, pack_f2(nl.x, nl.y)), x[0], x[1]);
+        unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, pack_f2(nl.z, nl.w)), x[2], x[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[c + e] = __float_as_uint(ex2(x[e]));
+      }
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (((c < 32 ? bad0 : bad1) >> (c & 31)) & 1u) v[c] = 0u;
+      }
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) w[c / 2] = Cvt<T>::pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+      tmem_st32(s_addr, w);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.p_full);
+      // dS = P (dP - delta)
+      if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t d[32];
+        tmem_ld32(dp_addr + c0, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 nd = *reinterpret_cast<const float4*>(stat + kTile + c0 + c);
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            uint64_t p = pack_f2(__uint_as_float(v[c0 + c + e]), __uint_as_float(v[c0 + c + e + 1]));
+            if constexpr (!BF16) p = mul_f2(p, gain2);
+            const uint64_t x = mul_f2(p, add_f2(pack_f2(__uint_as_float(d[c + e]), __uint_as_float(d[c + e + 1])),
+                                                e == 0 ? pack_f2(nd.x, nd.y) : pack_f2(nd.z, nd.w)));
+            float x0, x1;
+            unpack_f2(x, x0, x1);
+            if (masked) {  // 0 * inf
+              const uint32_t bw = c0 == 0 ? bad0 : bad1;
+              if ((bw >> (c + e)) & 1u) x0 = 0.f;
+              if ((bw >> (c + e + 1)) & 1u) x1 = 0.f;
+            }
+            w[(c0 + c + e) / 2] = Cvt<T>::pack2(x0, x1);
+          }
+        }
+      }
+      tmem_st32(dp_addr, w);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.ds_full);
+    }
+    // warps 2-5 store dV, 6-9 dK
+    const Rows& out = wg == 0 ? a.dv : a.dk;
+    char* orow = key < a.tk ? out.row(bhk, key) : nullptr;
+    if (n == 0) {
+      if (orow != nullptr) store_zero_row<T>(orow, a.dim);
+    } else {
+      ok = ok && mbar_wait(&m.all_done, 0, abort_flag, a.status, 16);
+      tc_fence_after();
+      if (ok && !*abort_flag) {
+        const float p_mul = BF16 ? 1.f : 1.f / (1 << kShiftP16);
+        const float mul = wg == 0 ? p_mul : a.scale * p_mul / gain;
+        store_row<T, HALVES>(tmem + lanes + (wg == 0 ? kColAcc0 : kColAcc1), orow, a.dim, mul, key >= len);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------ dQ
+template <bool BF16, int HALVES>
+__device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorMap* k_map, const CUtensorMap* v_map,
+                                       const CUtensorMap* do_map, const GradArgs& a, char* smem, Misc& m,
+                                       uint32_t tmem) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  using L = Smem<HALVES>;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int id = blockIdx.x - a.n_dkv;
+  const int bh = id / a.q_tiles;
+  const int qt = a.q_tiles - 1 - (id - bh * a.q_tiles);  // causal: the longest first
+  const int b = bh / a.heads;
+  const int h = bh - b * a.heads;
+  const int hk = h / a.group;
+  const int q0 = qt * kTile;
+  const int len = key_count(a, b);
+  const int off = a.tk - a.tq;
+  const int keys = a.causal ? min(len, min(q0 + kTile, a.tq) + off) : len;  // keys any of the rows sees
+  const int n = keys > 0 ? (keys + kTile - 1) / kTile : 0;
+  volatile int* abort_flag = &m.abort_flag;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0 && !*abort_flag) {
+      mbar_expect_tx(&m.own_full, 2 * L::tile);
+      load_tile<HALVES>(smem + L::own0, q_map, &m.own_full, q0, h, b);
+      load_tile<HALVES>(smem + L::own1, do_map, &m.own_full, q0, h, b);
+      int na = 0, nb = 0;
+      for (int i = 0; i < n; ++i) {
+        const int s = i & 1;
+        const uint32_t free_parity = ((i >> 1) & 1) ^ 1;
+        if (!mbar_wait(&m.a_empty[s], free_parity, abort_flag, a.status, 1)) break;
+        mbar_expect_tx(&m.a_full[s], L::tile);
+        load_tile<HALVES>(smem + L::a + s * L::tile, k_map, &m.a_full[s], i * kTile, hk, b);
+        na = i + 1;
+        if (!mbar_wait(&m.b_empty[s], free_parity, abort_flag, a.status, 2)) break;
+        mbar_expect_tx(&m.b_full[s], L::tile);
+        load_tile<HALVES>(smem + L::b + s * L::tile, v_map, &m.b_full[s], i * kTile, hk, b);
+        nb = i + 1;
+      }
+      if (*abort_flag) {
+        drain_loads(m.a_full, 2, na, &m.own_full, a.status);
+        drain_loads(m.b_full, 2, nb, nullptr, a.status);
+      }
+    }
+  } else if (warp == 1) {
+    if (n > 0 && elect_one()) {
+      const uint32_t q_addr = smem_u32(smem + L::own0), do_addr = smem_u32(smem + L::own1);
+      auto k_addr = [&](int s) { return smem_u32(smem + L::a + s * L::tile); };
+      auto v_addr = [&](int s) { return smem_u32(smem + L::b + s * L::tile); };
+      bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3) && mbar_wait(&m.a_full[0], 0, abort_flag, a.status, 4);
+      if (ok) {
+        product_rows<BF16, HALVES>(tmem + kColS, q_addr, k_addr(0));
+        mma_commit(&m.s_full);
+        ok = mbar_wait(&m.b_full[0], 0, abort_flag, a.status, 5);
+      }
+      if (ok) {
+        product_rows<BF16, HALVES>(tmem + kColDP, do_addr, v_addr(0));
+        mma_commit(&m.dp_full);
+        mma_commit(&m.b_empty[0]);
+      }
+      for (int i = 0; ok && i < n; ++i) {
+        const int s = i & 1, t = s ^ 1;
+        const uint32_t ph = i & 1, next_ph = ((i + 1) >> 1) & 1;
+        const bool more = i + 1 < n;
+        if (more) {  // the next S, once the elementwise warps hold this one
+          ok = mbar_wait(&m.a_full[t], next_ph, abort_flag, a.status, 7) &&
+               mbar_wait(&m.s_read, ph, abort_flag, a.status, 8);
+          if (!ok) break;
+          tc_fence_after();
+          product_rows<BF16, HALVES>(tmem + kColS, q_addr, k_addr(t));
+          mma_commit(&m.s_full);
+        }
+        // dQ += dS K; then the next dP may take the columns dS was read from
+        if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
+        tc_fence_after();
+        product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColDP, k_addr(s), i > 0);
+        mma_commit(&m.acc0_done);
+        mma_commit(&m.a_empty[s]);
+        if (more) {
+          ok = mbar_wait(&m.b_full[t], next_ph, abort_flag, a.status, 10) &&
+               mbar_wait(&m.acc0_done, ph, abort_flag, a.status, 11);
+          if (!ok) break;
+          product_rows<BF16, HALVES>(tmem + kColDP, do_addr, v_addr(t));
+          mma_commit(&m.dp_full);
+          mma_commit(&m.b_empty[t]);
+        }
+      }
+      mma_commit(&m.all_done);
+      int no_abort = 0;
+      mbar_wait(&m.all_done, 0, &no_abort, a.status, 12);
+    }
+  } else {
+    const int wg = (warp - 2) >> 2;
+    const int sub = warp & 3;
+    const int row = sub * 32 + lane;
+    const int query = q0 + row;
+    const uint32_t lanes = static_cast<uint32_t>(sub * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + kColS + wg * 64;
+    const uint32_t dp_addr = tmem + lanes + kColDP + wg * 64;
+    const float* stat = a.stat + (int64_t(bh) * a.q_tiles + qt) * (2 * kTile) + row;
+    const float nl = stat[0], nd = stat[kTile];
+    float gain = 1.f;
+    if constexpr (!BF16) gain = ds_gain(a, b * a.kv_heads + hk);
+    const uint64_t scale2 = pack_f2(a.scale_log2, a.scale_log2);
+    const uint64_t nl2 = pack_f2(nl, nl), nd2 = pack_f2(nd, nd), gain2 = pack_f2(gain, gain);
+    const int seen = a.causal ? min(len, query + off + 1) : len;  // keys this row sees
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const int s = i & 1;
+      const uint32_t ph = i & 1;
+      const int lim = seen - i * kTile - wg * 64;  // columns from `lim` on are masked
+      const bool masked = lim < 64;
+      const uint64_t bad = lim >= 64 ? 0ull : lim <= 0 ? ~0ull : ~0ull << lim;
+      const uint32_t bad0 = static_cast<uint32_t>(bad), bad1 = static_cast<uint32_t>(bad >> 32);
+      if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
+      tc_fence_after();
+      uint32_t v[64];
+      tmem_ld32(s_addr, v);
+      tmem_ld32(s_addr + 32, v + 32);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.s_read);
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        float x0, x1;
+        unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, nl2), x0, x1);
+        v[c] = __float_as_uint(ex2(x0));
+        v[c + 1] = __float_as_uint(ex2(x1));
+      }
+      // a partly valid last key tile: rows past the keys may hold anything,
+      // and dS's zeros times inf or NaN would reach dQ
+      const int k0 = i * kTile;
+      if (len < min(k0 + kTile, a.tk)) {
+        const int tid = threadIdx.x - 64;
+        const int from = len - k0, rows = min(kTile, a.tk - k0) - from;
+        char* tile = smem + L::a + s * L::tile;
+        for (int x = tid; x < rows * 8 * HALVES; x += 256) {
+          const int r = from + x / (8 * HALVES), ch = x % (8 * HALVES);
+          *reinterpret_cast<uint4*>(tile + (ch >> 3) * kHalfBytes + r * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+      }
+      if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
+      tc_fence_after();
+      uint32_t w[32];
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t d[32];
+        tmem_ld32(dp_addr + c0, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          uint64_t p = pack_f2(__uint_as_float(v[c0 + c]), __uint_as_float(v[c0 + c + 1]));
+          if constexpr (!BF16) p = mul_f2(p, gain2);
+          float x0, x1;
+          unpack_f2(mul_f2(p, add_f2(pack_f2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), nd2)), x0, x1);
+          if (masked) {
+            const uint32_t bw = c0 == 0 ? bad0 : bad1;
+            if ((bw >> c) & 1u) x0 = 0.f;
+            if ((bw >> (c + 1)) & 1u) x1 = 0.f;
+          }
+          w[(c0 + c) / 2] = Cvt<T>::pack2(x0, x1);
+        }
+      }
+      tmem_st32(dp_addr, w);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.ds_full);
+    }
+    char* orow = query < a.tq && (wg == 0 || n == 0) ? a.dq.row(bh, query) : nullptr;
+    if (n == 0) {
+      if (wg == 0 && orow != nullptr) store_zero_row<T>(orow, a.dim);
+    } else if (wg == 0) {
+      ok = ok && mbar_wait(&m.all_done, 0, abort_flag, a.status, 16);
+      tc_fence_after();
+      if (ok && !*abort_flag) {
+        const float mul = BF16 ? a.scale : a.scale / (gain * (1 << kShiftP16));
+        store_row<T, HALVES>(tmem + lanes + kColAcc0, orow, a.dim, mul, seen <= 0);
+      }
+    }
+  }
+}
+
+template <bool BF16, int HALVES>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
+                 const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap do_map,
+                 const __grid_constant__ GradArgs a) {
+  extern __shared__ __align__(1024) char smem[];
+  Misc& m = *reinterpret_cast<Misc*>(smem + Smem<HALVES>::misc);
+  const int warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0) {
+    m.abort_flag = 0;
+    if ((smem_u32(smem) & 1023u) != 0) {
+      m.abort_flag = 1;
+      atomicCAS(a.status, 0, 0x300);
+    }
+    mbar_init(&m.own_full, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&m.a_full[s], 1);
+      mbar_init(&m.a_empty[s], 1);
+      mbar_init(&m.b_full[s], 1);
+      mbar_init(&m.b_empty[s], 1);
+    }
+    mbar_init(&m.s_full, 1);
+    mbar_init(&m.s_read, 8);
+    mbar_init(&m.p_full, 8);
+    mbar_init(&m.dp_full, 1);
+    mbar_init(&m.ds_full, 8);
+    mbar_init(&m.acc0_done, 1);
+    mbar_init(&m.acc1_done, 1);
+    mbar_init(&m.all_done, 1);
+    fence_barrier_init();
+    fence_proxy_async_smem();
+  }
+  grid_dep_wait();  // the statistics come from the kernel before
+  if (warp == 1) tmem_alloc<512>(&m.tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = m.tmem;
+  if (static_cast<int>(blockIdx.x) < a.n_dkv)
+    dkv_cta<BF16, HALVES>(&q_map, &k_map, &v_map, &do_map, a, smem, m, tmem);
+  else
+    dq_cta<BF16, HALVES>(&q_map, &k_map, &v_map, &do_map, a, smem, m, tmem);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<512>(tmem);
+  }
+}
+
+// ------------------------------------------------------------ row statistics
+struct StatArgs {
+  Rows out, dout, v;
+  const float* lse;
+  float* stat;
+  uint32_t* maxima;
+  const int32_t* key_lengths;
+  int heads, kv_heads, group;
+  int tq, tk, dim;
+  int q_tiles;
+  int q_blocks;  // blocks of the query part; the rest walks V (FP16)
+};
+
+constexpr int kStatRows = 64;  // rows of a block: 16 groups of 16 lanes, 4 rows each
+
+// -lse*log2e and -delta of every query row, padded to whole tiles with rows
+// that give P = 0.  FP16: also the largest squared norms of dO rows and valid
+// V rows per key/value head (atomicMax of non-negative float bits: the order
+// does not matter).
+template <typename T>
+__global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_constant__ StatArgs a) {
+  constexpr bool kF16 = std::is_same<T, __half>::value;
+  const int g = threadIdx.x >> 4;
+  const int l = threadIdx.x & 15;
+  const bool active = 8 * l < a.dim;
+  if (static_cast<int>(blockIdx.x) < a.q_blocks) {
+    const int blocks_per_head = a.q_tiles * (kTile / kStatRows);
+    const int bh = blockIdx.x / blocks_per_head;
+    const int r0 = (blockIdx.x - bh * blocks_per_head) * kStatRows;
+    float most = 0.f;
+    uint4 o[4], d[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = r0 + u * 16 + g;
+      o[u] = d[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (active && r < a.tq) {
+        o[u] = reinterpret_cast<const uint4*>(a.out.row(bh, r))[l];
+        d[u] = reinterpret_cast<const uint4*>(a.dout.row(bh, r))[l];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = r0 + u * 16 + g;
+      const uint32_t ow[4] = {o[u].x, o[u].y, o[u].z, o[u].w}, dw[4] = {d[u].x, d[u].y, d[u].z, d[u].w};
+      float sum = 0.f, norm = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float o0, o1, d0, d1;
+        Cvt<T>::unpack2(ow[i], o0, o1);
+        Cvt<T>::unpack2(dw[i], d0, d1);
+        sum = fmaf(o0, d0, sum);
+        sum = fmaf(o1, d1, sum);
+        if constexpr (kF16) norm = fmaf(d0, d0, fmaf(d1, d1, norm));
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        if constexpr (kF16) norm += __shfl_xor_sync(0xffffffffu, norm, w);
+      }
+      most = fmaxf(most, norm);
+      if (l == 0) {
+        const float lse = r < a.tq ? a.lse[int64_t(bh) * a.tq + r] : -INFINITY;
+        float* dst = a.stat + (int64_t(bh) * a.q_tiles + r / kTile) * (2 * kTile) + r % kTile;
+        dst[0] = lse == -INFINITY ? -INFINITY : -lse * kLog2e + (kF16 ? static_cast<float>(kShiftP16) : 0.f);
+        dst[kTile] = -sum;
+      }
+    }
+    if constexpr (kF16) {
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+      if ((threadIdx.x & 31) == 0) {
+        const int b = bh / a.heads;
+        atomicMax(a.maxima + 2 * (b * a.kv_heads + (bh - b * a.heads) / a.group), __float_as_uint(most));
+      }
+    }
+  } else if constexpr (kF16) {
+    const int id = blockIdx.x - a.q_blocks;
+    const int blocks_per_head = (a.tk + kStatRows - 1) / kStatRows;
+    const int bhk = id / blocks_per_head;
+    const int r0 = (id - bhk * blocks_per_head) * kStatRows;
+    const int b = bhk / a.kv_heads;
+    const int len = a.key_lengths != nullptr ? min(a.key_lengths[b], a.tk) : a.tk;
+    float most = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int r = r0 + u * 16 + g;
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (active && r < len) x = reinterpret_cast<const uint4*>(a.v.row(bhk, r))[l];
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      float norm = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v0, v1;
+        Cvt<T>::unpack2(w[i], v0, v1);
+        norm = fmaf(v0, v0, fmaf(v1, v1, norm));
+      }
+#pragma unroll
+      for (int s = 8; s > 0; s >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, s);
+      most = fmaxf(most, norm);
+    }
+    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+    if ((threadIdx.x & 31) == 0) atomicMax(a.maxima + 2 * bhk + 1, __float_as_uint(most));
+  }
+}
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+template <bool BF16, int HALVES>
+cudaError_t launch_grad(unsigned blocks, const CUtensorMap* maps, const GradArgs& a, cudaStream_t st) {
+  const auto kernel = attn_grad_kernel<BF16, HALVES>;
+  const int smem = static_cast<int>(Smem<HALVES>::total);
+  const cudaError_t err = ensure_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (err != cudaSuccess) return err;
+  return launch_pdl(kernel, dim3(blocks), dim3(kThreads), size_t(smem), st, maps[0], maps[1], maps[2], maps[3], a);
+}
+
+}  // namespace
+
+int64_t attn_grad_workspace_bytes(int batch, int heads, int kv_heads, int tq) {
+  const int64_t q_tiles = (int64_t(tq) + kTile - 1) / kTile;
+  return static_cast<int64_t>(align256(size_t(batch) * heads * q_tiles * 2 * kTile * 4) +
+                              align256(size_t(batch) * kv_heads * 2 * 4));
+}
+
+cudaError_t launch_attn_grad(const AttnGradCall& c, int* status, cudaStream_t st) {
+  const b2_view &q = *c.q, &k = *c.k;
+  CUtensorMap maps[4];
+  const b2_view* views[4] = {c.q, c.k, c.v, c.dout};
+  for (int i = 0; i < 4; ++i)
+    if (!linear_rows_map(&maps[i], *views[i], kTile)) return cudaErrorInvalidValue;
+  const bool bf16 = q.dtype == B2_BF16;
+  StatArgs s{};
+  s.out = make_rows(*c.out), s.dout = make_rows(*c.dout), s.v = make_rows(*c.v);
+  s.lse = c.lse;
+  s.key_lengths = c.key_lengths;
+  s.heads = q.heads, s.kv_heads = k.heads, s.group = q.heads / k.heads;
+  s.tq = q.tokens, s.tk = k.tokens, s.dim = q.head_dim;
+  s.q_tiles = (q.tokens + kTile - 1) / kTile;
+  s.stat = static_cast<float*>(c.workspace);
+  const int64_t bh = int64_t(q.batch) * q.heads, bhk = int64_t(q.batch) * k.heads;
+  s.maxima = reinterpret_cast<uint32_t*>(static_cast<char*>(c.workspace) +
+                                         align256(size_t(bh) * s.q_tiles * 2 * kTile * 4));
+  s.q_blocks = static_cast<int>(bh * s.q_tiles * (kTile / kStatRows));
+  const int v_blocks = bf16 ? 0 : static_cast<int>(bhk * ((k.tokens + kStatRows - 1) / kStatRows));
+  cudaError_t err;
+  if (!bf16 && (err = cudaMemsetAsync(s.maxima, 0, size_t(bhk) * 8, st)) != cudaSuccess) return err;
+  if (bf16) attn_grad_stat_kernel<__nv_bfloat16><<<s.q_blocks, 256, 0, st>>>(s);
+  else attn_grad_stat_kernel<__half><<<s.q_blocks + v_blocks, 256, 0, st>>>(s);
+  if ((err = cudaGetLastError()) != cudaSuccess) return err;
+  GradArgs a{};
+  a.dq = make_rows(*c.dq), a.dk = make_rows(*c.dk), a.dv = make_rows(*c.dv);
+  a.stat = s.stat;
+  a.maxima = s.maxima;
+  a.key_lengths = c.key_lengths;
+  a.heads = s.heads, a.kv_heads = s.kv_heads, a.group = s.group;
+  a.tq = s.tq, a.tk = s.tk, a.dim = s.dim;
+  a.q_tiles = s.q_tiles;
+  a.k_tiles = (k.tokens + kTile - 1) / kTile;
+  a.n_dkv = static_cast<int>(bhk * a.k_tiles);
+  a.causal = c.causal;
+  a.scale = c.scale;
+  a.scale_log2 = c.scale * kLog2e;
+  a.status = status;
+  const unsigned blocks = static_cast<unsigned>(a.n_dkv + bh * a.q_tiles);
+  if (q.head_dim <= 64) return bf16 ? launch_grad<true, 1>(blocks, maps, a, st) : launch_grad<false, 1>(blocks, maps, a, st);
+  return bf16 ? launch_grad<true, 2>(blocks, maps, a, st) : launch_grad<false, 2>(blocks, maps, a, st);
+}
+
+}  // namespace b2

@@ -136,11 +136,12 @@ __device__ __forceinline__ Tile tile_at(const UmmaArgs& a, const Misc& m, int j,
   return t;
 }
 
-// TMA load of 64 rows (one key/query block) x 64 columns (half of D=128).
+// TMA load of 64 rows (one key/query block) x 64 columns (half of D=128) of
+// (batch, head) bh of `heads` heads.
 __device__ __forceinline__ void load_block(const CUtensorMap* map, const UmmaArgs& a, void* dst, uint64_t* bar,
-                                           int kind, int bh, int blk, int dh) {
-  const int b = bh / a.heads;
-  const int h = bh - b * a.heads;
+                                           int kind, int heads, int bh, int blk, int dh) {
+  const int b = bh / heads;
+  const int h = bh - b * heads;
   if (kind == 0) {
     tma_load_4d(dst, map, bar, dh * 64, blk * 64, h, b);
   } else {
@@ -180,7 +181,7 @@ __device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
 // S(j) = Q K(j)^T into the S buffer of warpgroup j%2; frees K slot on completion.
 // The buffer last held P(j-4): the caller issues S(j) only once that P.V has
 // completed (it reads P from these TMEM columns).
-template <bool BF16, int NW>
+template <bool BF16, int NW, int HALVES>
 __device__ __forceinline__ bool issue_s(Misc& m, char* k_s, uint32_t q_addr, uint32_t tmem, const UmmaArgs& a,
                                         volatile int* abort_flag, int j, long long* trace) {
   constexpr int kStages = Cfg<NW>::kStagesK;
@@ -194,7 +195,7 @@ __device__ __forceinline__ bool issue_s(Misc& m, char* k_s, uint32_t q_addr, uin
   const uint32_t idesc_s = idesc_f16(128, 64, BF16, false, false);
   const uint32_t k_addr = smem_u32(k_s + s * kSlotBytes);
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk) {
+  for (int kk = 0; kk < 4 * HALVES; ++kk) {
     const uint64_t da = smem_desc_sw128(q_addr + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024);
     const uint64_t db = smem_desc_sw128(k_addr + (kk >> 2) * 8192 + (kk & 3) * 32, 16, 1024);
     mma_ss(tmem + w * 256 + 128 + 64 * sb, da, db, idesc_s, kk > 0 ? 1u : 0u);
@@ -207,7 +208,7 @@ __device__ __forceinline__ bool issue_s(Misc& m, char* k_s, uint32_t q_addr, uin
 
 // O(w) += P(jj) V(jj) for key tile jj (warpgroup w = jj % 2); P is read from
 // TMEM, where the softmax wrote it over the tile's S columns.
-template <bool BF16, int NW>
+template <bool BF16, int NW, int HALVES>
 __device__ __forceinline__ bool issue_pv(Misc& m, char* smem, uint32_t tmem, const UmmaArgs& a,
                                          volatile int* abort_flag, int jj, long long* trace) {
   constexpr int kStages = Cfg<NW>::kStagesV;
@@ -217,7 +218,7 @@ __device__ __forceinline__ bool issue_pv(Misc& m, char* smem, uint32_t tmem, con
   if (!mbar_wait(&m.p_full[w][i & 1], (i >> 1) & 1, abort_flag, a.status, 2)) return false;
   if (!mbar_wait(&m.v_full[jj % kStages], (jj / kStages) & 1, abort_flag, a.status, 12)) return false;
   tc_fence_after();
-  const uint32_t idesc_o = idesc_f16(128, 128, BF16, false, true);
+  const uint32_t idesc_o = idesc_f16(128, 64 * HALVES, BF16, false, true);
   const uint32_t v_addr = smem_u32(smem + SmemLayout<NW>::v + (jj % kStages) * kSlotBytes);
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk) {
@@ -235,8 +236,12 @@ __device__ __forceinline__ bool issue_pv(Misc& m, char* smem, uint32_t tmem, con
 // DIAG with a mask): every row adds its FP32 mask terms a.bias to the scaled
 // scores, and a row whose keys are all masked stores NaN.  MIRROR (head-
 // sharded calls): every output row is also stored into a.n_mirror peer
-// copies of the output buffer.
-template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR>
+// copies of the output buffer.  GEN (general exact attention, mode ALL): keys
+// limited per batch (a.key_lengths) and causally (query i sees keys up to
+// i + a.causal_off), key/value heads shared by groups of query heads, rows
+// that see no key written as 0 with lse -inf; its value is the number of
+// 64-column halves of the head dimension the products cover.
+template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR, int GEN>
 __global__ void __launch_bounds__(Cfg<NW>::kThreads, Cfg<NW>::kCtasPerSm)
 attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap kc_map,
@@ -247,14 +252,17 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   constexpr int kThreads = Cfg<NW>::kThreads;
   constexpr int kStagesK = Cfg<NW>::kStagesK;
   constexpr int kStagesV = Cfg<NW>::kStagesV;
+  constexpr int kHalves = GEN == 1 ? 1 : 2;
   Misc& m = *reinterpret_cast<Misc*>(smem + SmemLayout<NW>::misc);
   char* q_s = smem + SmemLayout<NW>::q;
   char* k_s = smem + SmemLayout<NW>::k;
   char* v_s = smem + SmemLayout<NW>::v;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int pair = blockIdx.x;
+  // causal: the CTAs with the most keys first
+  const int pair = GEN && a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
   const int bh = blockIdx.y;
+  int kv_heads = a.heads, kv_bh = bh, tk_ = a.tk;
   int qa = 2 * pair;
   int qb = 2 * pair + 1;
   bool has_b = qb < a.nqb;  // the pairing kernel's output is read after grid_dep_wait
@@ -307,6 +315,16 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   // launched with programmatic stream serialization: everything below reads
   // the routing results (or the inputs) and writes the output
   grid_dep_wait();
+  if constexpr (GEN != 0) {
+    const int b = bh / a.heads;
+    kv_heads = a.kv_heads;
+    kv_bh = b * kv_heads + (bh - b * a.heads) / (a.heads / kv_heads);
+    if (a.key_lengths != nullptr) tk_ = min(max(a.key_lengths[b], 0), a.tk);
+    if (threadIdx.x == 0) {
+      const int keys = a.causal ? min(tk_, min(pair * 128 + 128, a.tq) + a.causal_off) : tk_;
+      m.nlist = m.ntiles = keys > 0 ? (keys + 63) / 64 : 0;
+    }
+  }
   if (a.pairs != nullptr) {
     qa = a.pairs[(int64_t(bh) * gridDim.x + pair) * 2];
     qb = a.pairs[(int64_t(bh) * gridDim.x + pair) * 2 + 1];
@@ -391,10 +409,10 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       tma_prefetch_desc(&q_map);
       tma_prefetch_desc(&k_map);
       if constexpr (!WITHHOLD) {
-        mbar_expect_tx(&m.q_full, kQBytes);
+        mbar_expect_tx(&m.q_full, kQBytes / 2 * kHalves);
         for (int half = 0; half < 2; ++half)
-          for (int dh = 0; dh < 2; ++dh)
-            load_block(&q_map, a, q_s + dh * 16384 + half * 8192, &m.q_full, a.q_kind, bh, half ? qb : qa, dh);
+          for (int dh = 0; dh < kHalves; ++dh)
+            load_block(&q_map, a, q_s + dh * 16384 + half * 8192, &m.q_full, a.q_kind, a.heads, bh, half ? qb : qa, dh);
       }
       // key tiles 0..n-1, then the two 64-column halves of H as "tiles" n, n+1
       const int total = n + (a.has_corr ? 2 : 0);
@@ -405,11 +423,11 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         char* slot = k_s + s * kSlotBytes;
         if (trace && j < 256) trace[6 * j] = clock64();
         if (j < n) {
-          mbar_expect_tx(&m.k_full[s], kSlotBytes);
+          mbar_expect_tx(&m.k_full[s], kSlotBytes / 2 * kHalves);
           const Tile t = tile_at(a, m, j, ntail);
-          for (int dh = 0; dh < 2; ++dh) {
+          for (int dh = 0; dh < kHalves; ++dh) {
             if (t.tail) tma_load_3d(slot + dh * 8192, &kc_map, &m.k_full[s], dh * 64, t.blk * 64, bh);
-            else load_block(&k_map, a, slot + dh * 8192, &m.k_full[s], a.kv_kind, bh, t.blk, dh);
+            else load_block(&k_map, a, slot + dh * 8192, &m.k_full[s], a.kv_kind, kv_heads, kv_bh, t.blk, dh);
           }
         } else {
           // H[:, 64*(j-n) : 64*(j-n)+64]: 128 rows x 128 B
@@ -428,11 +446,11 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         const int s = j % kStagesV;
         if (!mbar_wait(&m.v_empty[s], ((j / kStagesV) & 1) ^ 1, abort_flag, a.status, 13)) break;
         char* slot = v_s + s * kSlotBytes;
-        mbar_expect_tx(&m.v_full[s], kSlotBytes);
+        mbar_expect_tx(&m.v_full[s], kSlotBytes / 2 * kHalves);
         const Tile t = tile_at(a, m, j, ntail);
-        for (int dh = 0; dh < 2; ++dh) {
+        for (int dh = 0; dh < kHalves; ++dh) {
           if (t.tail) tma_load_3d(slot + dh * 8192, &vc_map, &m.v_full[s], dh * 64, t.blk * 64, bh);
-          else load_block(&v_map, a, slot + dh * 8192, &m.v_full[s], a.kv_kind, bh, t.blk, dh);
+          else load_block(&v_map, a, slot + dh * 8192, &m.v_full[s], a.kv_kind, kv_heads, kv_bh, t.blk, dh);
         }
       }
       if (*abort_flag) drain_loads(m.v_full, kStagesV, issued, nullptr, a.status);
@@ -458,7 +476,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           const int j = NW * ns + w;
           const bool buf_free = ns < 2 || (ns - 2 < npv && mbar_test_wait(&m.pv_done[w][ns & 1], ((ns - 2) >> 1) & 1));
           if (buf_free && mbar_test_wait(&m.k_full[j % kStagesK], (j / kStagesK) & 1)) {
-            ok = issue_s<BF16, NW>(m, k_s, q_addr, tmem, a, abort_flag, j, trace);
+            ok = issue_s<BF16, NW, kHalves>(m, k_s, q_addr, tmem, a, abort_flag, j, trace);
             ++ns;
             did = true;
           }
@@ -467,7 +485,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           const int j = NW * npv + w;
           if (mbar_test_wait(&m.p_full[w][npv & 1], (npv >> 1) & 1) &&
               mbar_test_wait(&m.v_full[j % kStagesV], (j / kStagesV) & 1)) {
-            ok = issue_pv<BF16, NW>(m, smem, tmem, a, abort_flag, j, trace);
+            ok = issue_pv<BF16, NW, kHalves>(m, smem, tmem, a, abort_flag, j, trace);
             ++npv;
             did = true;
           }
@@ -524,7 +542,8 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     const uint32_t o_base = tmem + lane_base + wg * 256;
     const int tq_row = qblk * 64 + (row & 63);
     float mrun = -INFINITY, lrun = 0.f, tmass = 0.f;
-    const int nb_ = a.nb, causal_ = a.causal, tk_ = a.tk;
+    const int nb_ = a.nb, causal_ = a.causal;
+    const int causal_row = tq_row + (GEN ? a.causal_off : 0);  // the last key the row sees
     const float log2_last_ = a.log2_last, scale_log2_ = a.scale_log2;
     int i = 0;
     bool ok = true;
@@ -540,7 +559,8 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       tc_fence_after();
       const uint32_t s_addr = o_base + 128 + 64 * sb;
       const int klen = t.tail ? 64 : min(64, tk_ - t.blk * 64);
-      const bool plain = !MASKED && !t.tail && klen == 64 && !causal_;
+      const bool plain =
+          !MASKED && !t.tail && klen == 64 && (!causal_ || (GEN != 0 && causal_row - t.blk * 64 >= 63));
       // masked columns of this tile as two 32-bit words (bit c = column c),
       // and the column that carries the last (ragged) block's log2 length
       uint32_t bad0 = 0u, bad1 = 0u;
@@ -560,7 +580,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         } else {
           bad = klen < 64 ? (~0ull << klen) : 0ull;
           if (causal_) {
-            const int lim = tq_row - t.blk * 64;  // columns > lim are masked
+            const int lim = causal_row - t.blk * 64;  // columns > lim are masked
             if (lim < 63) bad |= lim < 0 ? ~0ull : (~0ull << (lim + 1));
           }
         }
@@ -643,7 +663,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         }
         tc_fence_after();
 #pragma unroll 1
-        for (int c0 = 0; c0 < 128; c0 += 32) {
+        for (int c0 = 0; c0 < 64 * kHalves; c0 += 32) {
           uint32_t o[32];
           tmem_ld32(o_base + c0, o);
           tmem_wait_ld();
@@ -676,6 +696,23 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       }
       tmem_st32(s_addr, v);
       tmem_wait_st();
+      if constexpr (GEN != 0) {
+        // V rows past the batch's keys may hold anything: P is 0 there, but
+        // 0 * inf is not, so they are cleared in the tile first
+        if (klen < min(64, a.tk - t.blk * 64)) {
+          if (!mbar_wait(&m.v_full[j % kStagesV], (j / kStagesV) & 1, abort_flag, a.status, 25)) {
+            ok = false;
+            break;
+          }
+          char* tile = v_s + (j % kStagesV) * kSlotBytes;
+          const int rows = min(64, a.tk - t.blk * 64) - klen;
+          for (int x = threadIdx.x - 64; x < rows * 8 * kHalves; x += 128) {
+            const int r = klen + x / (8 * kHalves), ch = x % (8 * kHalves);
+            *reinterpret_cast<uint4*>(tile + (ch >> 3) * 8192 + r * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&m.p_full[wg][sb]);
@@ -711,7 +748,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     char* orow = store ? a.o.row(bh, tq_row) : nullptr;
     const uint32_t row_base = tmem + lane_base;
 #pragma unroll 1
-    for (int c0 = wg * (128 / NW); c0 < (wg + 1) * (128 / NW); c0 += 32) {
+    for (int c0 = wg * (128 / NW); c0 < (GEN == 1 ? 64 : (wg + 1) * (128 / NW)); c0 += 32) {
       // each warpgroup stores 128 / NW of the output columns
       uint32_t o0[32], o1[32], cr[32];
       tmem_ld32(row_base + c0, o0);
@@ -732,6 +769,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             f0 = fmaf(__uint_as_float(cr[c]), cw, f0);
             f1 = fmaf(__uint_as_float(cr[c + 1]), cw, f1);
           }
+          if (GEN != 0 && lt == 0.f) f0 = f1 = 0.f;  // no key seen: O may hold anything
           packed[c / 2] = Cvt<T>::pack2(f0 * inv, f1 * inv);
         }
         uint4* dst = reinterpret_cast<uint4*>(orow + c0 * 2);
@@ -791,7 +829,8 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       }
     }
     if (store && wg == 0 && a.lse != nullptr) {
-      a.lse[int64_t(bh) * a.tq + tq_row] = lt > 0.f ? (mm + __log2f(lt)) * 0.6931471805599453f : -INFINITY;
+      const float none = GEN != 0 && lt != 0.f ? lt : -INFINITY;  // NaN rows stay NaN
+      a.lse[int64_t(bh) * a.tq + tq_row] = lt > 0.f ? (mm + __log2f(lt)) * 0.6931471805599453f : none;
     }
   }
   tc_fence_before();
@@ -868,6 +907,19 @@ bool rows3_map(CUtensorMap* map, int dtype, const void* base, int rows, int batc
 
 }  // namespace
 
+bool linear_rows_map(CUtensorMap* map, const b2_view& v, int box_rows) {
+  // a dimension of one entry may carry any stride: give it one TMA accepts
+  const uint64_t row = uint64_t(v.head_dim) * 2;
+  const uint64_t st = v.tokens > 1 ? uint64_t(v.stride_t) * 2 : row;
+  const uint64_t sh = v.heads > 1 ? uint64_t(v.stride_h) * 2 : row;
+  const uint64_t sb = v.batch > 1 ? uint64_t(v.stride_b) * 2 : row;
+  if (st == 0 || sh == 0 || sb == 0) return false;
+  const cuuint64_t dims[4] = {cuuint64_t(v.head_dim), cuuint64_t(v.tokens), cuuint64_t(v.heads), cuuint64_t(v.batch)};
+  const cuuint64_t strides[3] = {st, sh, sb};
+  const cuuint32_t box[4] = {64, cuuint32_t(box_rows), 1, 1};
+  return encode(map, v.dtype, 4, v.base, dims, strides, box);
+}
+
 int* device_status_ptr() {
   void* ptr = nullptr;
   if (cudaGetSymbolAddress(&ptr, g_status) != cudaSuccess) return nullptr;
@@ -898,15 +950,15 @@ int attn_warpgroups() {
   return nw;
 }
 
-template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR>
+template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR, int GEN = 0>
 cudaError_t launch_variant(dim3 grid, cudaStream_t stream, const CUtensorMap& q_map, const CUtensorMap& k_map,
                            const CUtensorMap& v_map, const CUtensorMap& kc_map, const CUtensorMap& vc_map,
                            const CUtensorMap& h_map, const UmmaArgs& a) {
   const int smem = static_cast<int>(SmemLayout<NW>::total);
   const cudaError_t err =
-      ensure_smem(reinterpret_cast<const void*>(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR>), smem);
+      ensure_smem(reinterpret_cast<const void*>(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR, GEN>), smem);
   if (err != cudaSuccess) return err;
-  return launch_pdl(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR>, grid, dim3(Cfg<NW>::kThreads), size_t(smem), stream,
+  return launch_pdl(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR, GEN>, grid, dim3(Cfg<NW>::kThreads), size_t(smem), stream,
                     q_map, k_map, v_map, kc_map, vc_map, h_map, a);
 }
 
@@ -999,6 +1051,35 @@ cudaError_t launch_attn_umma(const b2_view& qv, const b2_view& kv, const b2_view
   if (err != cudaSuccess) return err;
   *launched = true;
   return cudaGetLastError();
+}
+
+cudaError_t launch_attn_general(const AttnGeneralCall& c, int* status, cudaStream_t stream) {
+  const b2_view &q = *c.q, &k = *c.k;
+  CUtensorMap q_map, k_map, v_map;
+  if (!linear_rows_map(&q_map, q, 64) || !linear_rows_map(&k_map, k, 64) || !linear_rows_map(&v_map, *c.v, 64))
+    return cudaErrorInvalidValue;
+  UmmaArgs a{};
+  a.heads = q.heads;
+  a.kv_heads = k.heads;
+  a.tq = q.tokens;
+  a.tk = k.tokens;
+  a.nqb = (q.tokens + 63) / 64;
+  a.frames = a.tiles_per_row = a.tiles_per_frame = 1;
+  a.scale_log2 = c.scale * 1.4426950408889634f;
+  a.causal = c.causal;
+  a.causal_off = k.tokens - q.tokens;
+  a.key_lengths = c.key_lengths;
+  a.o = make_rows(*c.out);
+  a.lse = c.lse;
+  a.status = status;
+  const dim3 grid((a.nqb + 1) / 2, q.batch * q.heads);
+  if (q.dtype == B2_BF16)
+    return q.head_dim <= 64
+               ? launch_variant<true, 1, false, false, false, 1>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a)
+               : launch_variant<true, 1, false, false, false, 2>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a);
+  return q.head_dim <= 64
+             ? launch_variant<false, 1, false, false, false, 1>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a)
+             : launch_variant<false, 1, false, false, false, 2>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a);
 }
 
 }  // namespace b2

@@ -731,6 +731,85 @@ int b2_pack_block_bias(const void* mask, int32_t mask_dtype, int64_t stride_bh, 
 }  // extern "C"
 
 namespace {
+int check_grad_view(const b2_view* v, const char* name, const b2_view* like) {
+  const int rc = check_view(v, name);
+  if (rc) return rc;
+  if (v->order != B2_ORDER_LINEAR) return fail(B2_ERR_UNSUPPORTED, "%s must be in linear token order", name);
+  if (like != nullptr && (!same_bht(v, like) || v->dtype != like->dtype))
+    return fail(B2_ERR_INVALID, "%s must have its counterpart's [B,H,T,D] and dtype", name);
+  // zero strides repeat rows: outputs would race, and TMA maps refuse them
+  if ((v->batch > 1 && v->stride_b <= 0) || (v->heads > 1 && v->stride_h <= 0) || (v->tokens > 1 && v->stride_t <= 0))
+    return fail(B2_ERR_INVALID, "%s strides must be positive", name);
+  return B2_OK;
+}
+
+int check_attention(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out, float scale,
+                    const int32_t* key_lengths) {
+  int rc;
+  if ((rc = check_grad_view(q, "q", nullptr)) || (rc = check_grad_view(k, "k", nullptr)) ||
+      (rc = check_grad_view(v, "v", k)) || (rc = check_grad_view(out, "out", q)))
+    return rc;
+  if (q->dtype == B2_F32) return fail(B2_ERR_UNSUPPORTED, "attention supports float16 and bfloat16");
+  if (q->dtype != k->dtype || q->batch != k->batch || q->head_dim != k->head_dim)
+    return fail(B2_ERR_INVALID, "q and k must share B, D and dtype");
+  if (q->heads % k->heads) return fail(B2_ERR_INVALID, "q heads must be a multiple of k/v heads");
+  if (q->head_dim > 128) return fail(B2_ERR_UNSUPPORTED, "attention supports D <= 128, a multiple of 8");
+  if (!(scale > 0.f) || !(scale < 3.4028235e38f))
+    return fail(B2_ERR_INVALID, "scale must be representable as a positive finite float32 value.");
+  if (reinterpret_cast<uintptr_t>(key_lengths) % 4) return fail(B2_ERR_INVALID, "key_lengths must be 4-byte aligned");
+  const int64_t bh = int64_t(q->batch) * q->heads;
+  if (bh > 65535) return fail(B2_ERR_UNSUPPORTED, "attention supports at most 65535 (batch, head) pairs");
+  if (q->tokens > (1 << 24) || k->tokens > (1 << 24))
+    return fail(B2_ERR_UNSUPPORTED, "attention supports at most 2^24 tokens");
+  if (bh * (int64_t(q->tokens) + k->tokens + 256) / 64 > 0x7fffffff)
+    return fail(B2_ERR_UNSUPPORTED, "too many tiles for one launch");
+  return B2_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int b2_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out, float scale,
+                         int32_t causal, const int32_t* key_lengths, float* lse, void* stream) {
+  const int rc = check_attention(q, k, v, out, scale, key_lengths);
+  if (rc) return rc;
+  int* status = device_status_ptr();
+  if (status == nullptr) return fail(B2_ERR_CUDA, "device status word unavailable");
+  const AttnGeneralCall c{q, k, v, out, key_lengths, scale, causal ? 1 : 0, lse};
+  const cudaError_t err = launch_attn_general(c, status, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "attention launch");
+  g_last_kernel = "tcgen05";
+  return ok();
+}
+
+int64_t b2_attention_backward_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || q_tokens <= 0) return -1;
+  return attn_grad_workspace_bytes(batch, heads, kv_heads, q_tokens);
+}
+
+int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
+                          const b2_view* dout, const float* lse, const b2_view* dq, const b2_view* dk,
+                          const b2_view* dv, float scale, int32_t causal, const int32_t* key_lengths, void* workspace,
+                          void* stream) {
+  int rc = check_attention(q, k, v, out, scale, key_lengths);
+  if (rc) return rc;
+  if ((rc = check_grad_view(dout, "dout", q)) || (rc = check_grad_view(dq, "dq", q)) ||
+      (rc = check_grad_view(dk, "dk", k)) || (rc = check_grad_view(dv, "dv", v)))
+    return rc;
+  if (lse == nullptr || reinterpret_cast<uintptr_t>(lse) % 4) return fail(B2_ERR_INVALID, "lse must be non-NULL");
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return fail(B2_ERR_INVALID, "workspace must be non-NULL and 16-byte aligned");
+  int* status = device_status_ptr();
+  if (status == nullptr) return fail(B2_ERR_CUDA, "device status word unavailable");
+  const AttnGradCall c{q, k, v, out, dout, dq, dk, dv, lse, key_lengths, scale, causal ? 1 : 0, workspace};
+  const cudaError_t err = launch_attn_grad(c, status, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "attention backward launch");
+  return ok();
+}
+
+}  // extern "C"
+
+namespace {
 int check_rotary(const b2_rotary* r, const b2_view* v) {
   if (r == nullptr || r->positions == nullptr) return fail(B2_ERR_INVALID, "positions must be non-NULL");
   if (r->pos_dtype < B2_POS_I32 || r->pos_dtype > B2_POS_F64) return fail(B2_ERR_INVALID, "unknown position dtype");

@@ -1,8 +1,13 @@
 // Internal launch interface shared by the C ABI layer and the kernels.
 #pragma once
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace b2 {
+// 4D TMA map (D,T,H,B) of a linear view: boxes of 64 columns x box_rows rows,
+// zeros past D and T.  False for views TMA cannot address.
+bool linear_rows_map(CUtensorMap* map, const b2_view& v, int box_rows);
 constexpr int kMaxMirrors = 7;  // peer copies of an output (head-sharded calls over up to 8 GPUs)
 // Parameters of the fused attention kernel (see attn_mma.cu).
 struct AttnParams {
@@ -54,6 +59,10 @@ struct UmmaArgs {
   int n_mirror;  // peer output copies, see AttnParams
   char* mirror[kMaxMirrors];
   int mirror_multicast;
+  // general exact attention: shared key/value heads, key limits
+  int kv_heads;
+  const int32_t* key_lengths;  // [B] or NULL
+  int causal_off;              // causal: query i sees keys up to i + causal_off
 };
 bool umma_supported(const b2_view& q, const b2_view& k, const b2_view& v, const b2_view& o);
 cudaError_t launch_attn_umma(const b2_view& qv, const b2_view& kv, const b2_view& vv, const b2_view& ov,
@@ -88,6 +97,27 @@ cudaError_t launch_fixed_f32(const Rows& q, const Rows& k, const Rows& v, const 
                              cudaStream_t stream);
 cudaError_t launch_block_bias(const void* mask, int mask_dtype, int64_t s_bh, int64_t s_row, int64_t s_col,
                               int mask_rows_bh, int tokens, float* bias, cudaStream_t stream);
+// Exact attention with shared key/value heads, per-batch key counts and a
+// causal mask aligned to the last key (attn_umma.cu).
+struct AttnGeneralCall {
+  const b2_view *q, *k, *v, *out;
+  const int32_t* key_lengths;
+  float scale;
+  int causal;
+  float* lse;
+};
+cudaError_t launch_attn_general(const AttnGeneralCall& call, int* status, cudaStream_t stream);
+struct AttnGradCall {
+  const b2_view *q, *k, *v, *out, *dout, *dq, *dk, *dv;
+  const float* lse;
+  const int32_t* key_lengths;
+  float scale;
+  int causal;
+  void* workspace;
+};
+// Backward pass of exact attention (attn_grad.cu).
+int64_t attn_grad_workspace_bytes(int batch, int heads, int kv_heads, int tq);
+cudaError_t launch_attn_grad(const AttnGradCall& call, int* status, cudaStream_t stream);
 // Norm + rotary positions (rotary.cu): one or two sides (queries, keys).
 // Forward: y from x.  Gradients (dy set): y receives dx, dw (may be NULL) the
 // weight gradients, partial is rotary_workspace_bytes() of scratch.

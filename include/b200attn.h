@@ -305,6 +305,29 @@ int b2_fixed_block_attention_masked(const b2_view* q, const b2_view* k,
                                     const float* bias, int64_t bias_bh_stride,
                                     void* stream);
 
+/* ---- Exact attention with its backward pass (no counterpart in the
+ * reference, which is forward-only).  q, out: [B,H,Tq,D]; k, v: [B,Hk,Tk,D]
+ * with H a multiple of Hk (query head h reads key/value head h / (H/Hk));
+ * BF16 or FP16, D <= 128 (a multiple of 8), linear order, positive strides.
+ * key_lengths: [B] int32 on the device or NULL; batch b has the keys
+ * [0, min(max(key_lengths[b], 0), Tk)), and K/V rows past them are not used
+ * whatever they hold.  causal: query i sees keys up to i + Tk - Tq.  A query
+ * that sees no key gives out = 0, lse = -inf and gradient 0.
+ * lse: [B,H,Tq] FP32, the natural log of the sum of exp(scale * scores); NULL
+ * if not wanted. */
+int b2_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out, float scale,
+                         int32_t causal, const int32_t* key_lengths, float* lse, void* stream);
+/* dq, dk, dv from dout and what the forward pass was given and wrote (out,
+ * lse; the same scale, causal and key_lengths).  Rows of dk/dv past a batch's
+ * keys are written as 0.  Probabilities are recomputed; workspace:
+ * b2_attention_backward_workspace_bytes() bytes for row statistics, read and
+ * written only by this call.  Results are bit-reproducible. */
+int64_t b2_attention_backward_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens);
+int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
+                          const b2_view* dout, const float* lse, const b2_view* dq, const b2_view* dk,
+                          const b2_view* dv, float scale, int32_t causal, const int32_t* key_lengths, void* workspace,
+                          void* stream);
+
 /* ---- Per-head RMS norm of queries and keys and rotary positions with several
  * axes (time, height, width, ...) in one pass.  No counterpart in the
  * reference, whose attention starts from normed and rotated q/k.

@@ -1,0 +1,256 @@
+"""Exact attention with gradients: refusals (CPU) and parity of both passes
+with a plain FP64 implementation (GPU).
+
+Tolerances.  One rounding of type t is at most u = finfo(t).eps / 2 of a value.
+With P the probabilities, the kernels round
+  * P once before P V and P^T dO (relative u a term; the row sum is not rounded);
+  * dS = P (dP - delta) once before the last two products; delta uses the
+    rounded output, off by u |out| |dout| summed over D;
+  * every result once.
+So, each term at its worst,
+  out: u (|P| |V|) + u |out|
+  dV:  u (|P|^T |dO|) + u |dV|
+  dQ:  scale ((u |dS| + P ddelta) |K|) + u |dQ|, ddelta = u sum |out||dout|
+  dK:  scale ((u |dS| + P ddelta)^T |Q|) + u |dK|
+plus the FP32 part: S is a D-term FP32 sum, exp2 and the statistics add under
+2^-18 relative to P in all for the logits here (|scaled logit| <= 64, whose
+product with scale and lse is rounded at 2^-24 of it), which is taken on every
+P and dS with |dP| + |delta| in place of |dP - delta|.  FP16: P is held times
+2^8, so what falls below FP16's normal range is at most 2^-14 of 2^-8 with a
+step of 2^-24 of 2^-8: 2^-33 a key absolute."""
+import math
+
+import pytest
+import torch
+
+from gpu_util import DEV
+
+gpu = pytest.mark.gpu
+FP32_PART = 2.0 ** -18
+
+
+def make(b, h, t, d, dtype, layout, seed, scale=1.0):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    if layout == "bthd":
+        return (torch.randn(b, t, h, d, generator=gen, device=DEV) * scale).to(dtype).permute(0, 2, 1, 3)
+    if layout == "bhtd":
+        return (torch.randn(b, h, t, d, generator=gen, device=DEV) * scale).to(dtype)
+    if layout == "fused":
+        return (torch.randn(b, t, 3, h, d, generator=gen, device=DEV) * scale).to(dtype)[:, :, 1].permute(0, 2, 1, 3)
+    assert layout == "sliced"
+    return (torch.randn(b, 2 * t, h + 1, d + 8, generator=gen, device=DEV) * scale).to(dtype)[:, ::2, 1:, 8:].permute(0, 2, 1, 3)
+
+
+def keep_mask(tq, tk, causal, lens, b):
+    keep = torch.ones(b, 1, tq, tk, dtype=torch.bool, device=DEV)
+    if causal:
+        i = torch.arange(tq, device=DEV)[:, None]
+        keep &= torch.arange(tk, device=DEV)[None] <= i + (tk - tq)
+    if lens is not None:
+        keep &= (torch.arange(tk, device=DEV)[None] < lens[:, None])[:, None, None]
+    return keep
+
+
+def reference(q, k, v, dout, scale, causal, lens):
+    """FP64 (out, lse, dq, dk, dv) and the allowed error of each but lse, as
+    functions of the rounding unit u (see the module docstring)."""
+    b, h, tq, d = q.shape
+    hk, tk = k.shape[1], k.shape[2]
+    g = h // hk
+    keep = keep_mask(tq, tk, causal, lens, b)
+    valid = keep.any(2)[:, :, :, None] if lens is None else (torch.arange(tk, device=DEV)[None] < lens[:, None])[:, None, :, None]
+    qd = q.double()
+    kd, vd = (torch.where(valid, x.double(), 0.0).repeat_interleave(g, 1) for x in (k, v))
+    s = (qd @ kd.transpose(-1, -2) * scale).masked_fill(~keep, -math.inf)
+    lse = torch.logsumexp(s, -1)
+    p = torch.where(keep, (s - torch.where(lse == -math.inf, 0.0, lse)[..., None]).exp(), 0.0)
+    out = p @ vd
+    res = {"out": out, "lse": lse}
+    fp32 = FP32_PART * p
+    allow = {"out": lambda u: (u * p + fp32) @ vd.abs() + u * out.abs()}
+    if dout is not None:
+        do = dout.double()
+        dp = do @ vd.transpose(-1, -2)
+        delta = (do * out).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        fold = lambda x: x.unflatten(1, (hk, g)).sum(2)  # noqa: E731
+        res.update(dq=scale * ds @ kd, dk=fold(scale * ds.transpose(-1, -2) @ qd), dv=fold(p.transpose(-1, -2) @ do))
+        rough = fp32 * (do.abs() @ vd.abs().transpose(-1, -2) + (do * out).abs().sum(-1, keepdim=True))
+        # the rounded output delta is made from is itself within allow["out"]
+        slip = lambda u: u * ds.abs() + p * (do.abs() * allow["out"](u)).sum(-1, keepdim=True) + rough  # noqa: E731
+        allow["dq"] = lambda u: scale * slip(u) @ kd.abs() + u * res["dq"].abs()
+        allow["dk"] = lambda u: fold(scale * slip(u).transpose(-1, -2) @ qd.abs()) + u * res["dk"].abs()
+        allow["dv"] = lambda u: fold((u * p + fp32).transpose(-1, -2) @ do.abs()) + u * res["dv"].abs()
+    return res, allow
+
+
+def close(name, got, want, allowed):
+    u16 = 2.0 ** -33 if got.dtype == torch.float16 else 0.0
+    floor = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps / 2 + u16 * 64
+    allowed = allowed * (1 + 2 ** -8) + floor  # products of the first-order terms
+    off = (got.double() - want).abs()
+    assert torch.isfinite(got).all(), f"{name} is not finite"
+    assert (off <= allowed).all(), f"{name} off by {off.max().item():.3g}, {(off / allowed).max().item():.3g} of the allowed"
+
+
+# ---------------------------------------------------------------- refusals (CPU)
+def _x(*shape, dtype=torch.bfloat16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("q,k,v,kw,match", [
+    (_x(2, 4, 8), _x(1, 2, 4, 8), _x(1, 2, 4, 8), {}, "same rank"),
+    (_x(1, 2, 0, 8), _x(1, 2, 4, 8), _x(1, 2, 4, 8), {}, "non-empty"),
+    (_x(1, 2, 4, 8), _x(1, 2, 4, 8), _x(1, 2, 5, 8), {}, "matching"),
+    (_x(1, 2, 4, 8), _x(2, 2, 4, 8), _x(2, 2, 4, 8), {}, "matching"),
+    (_x(1, 2, 4, 8), _x(1, 2, 4, 16), _x(1, 2, 4, 16), {}, "matching"),
+    (_x(1, 3, 4, 8), _x(1, 2, 4, 8), _x(1, 2, 4, 8), {}, "multiple of k/v heads"),
+    (_x(1, 2, 4, 8, dtype=torch.float32),) * 3 + ({}, "float16 or bfloat16"),
+    (_x(1, 2, 4, 8), _x(1, 2, 4, 8, dtype=torch.float16), _x(1, 2, 4, 8), {}, "float16 or bfloat16"),
+    (_x(1, 2, 4, 136),) * 3 + ({}, "D <= 128"),
+    (_x(1, 2, 4, 12),) * 3 + ({}, "multiple of 8"),
+    (_x(1, 2, 4, 8),) * 3 + (dict(scale=0.0), "scale"),
+    (_x(1, 2, 4, 8),) * 3 + (dict(scale=math.nan), "scale"),
+    (_x(1, 2, 4, 8),) * 3 + (dict(scale=1e300), "scale"),
+    (_x(1, 2, 4, 8),) * 3 + (dict(key_lengths=torch.zeros(2, dtype=torch.int32)), "key_lengths"),
+    (_x(1, 2, 4, 8),) * 3 + (dict(key_lengths=torch.zeros(1, dtype=torch.int64)), "key_lengths"),
+    (_x(1, 2, 4, 20)[..., 2:10],) * 3 + ({}, "16-byte"),
+    (_x(1, 2, 8, 8).transpose(2, 3),) * 3 + ({}, "contiguous head"),
+    (_x(1, 2, 4, 8),) * 3 + ({}, "one CUDA device"),
+])
+def test_attention_refuses(q, k, v, kw, match):
+    import b200_pisa
+
+    with pytest.raises(ValueError, match=match):
+        b200_pisa.attention(q, k, v, **kw)
+    with pytest.raises(ValueError, match=match):
+        b200_pisa.attention_forward(q, k, v, **kw)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(dout=_x(1, 2, 5, 8)), "dout"),
+    (dict(out=_x(1, 2, 4, 8, dtype=torch.float16)), "out"),
+    (dict(lse=torch.zeros(1, 2, 5)), "lse"),
+    (dict(lse=torch.zeros(1, 2, 4, dtype=torch.float64)), "lse"),
+    (dict(lse=None), "lse"),
+    (dict(), "one CUDA device"),
+])
+def test_attention_backward_refuses(change, match):
+    import b200_pisa
+
+    x = _x(1, 2, 4, 8)
+    kw = dict(dout=x, out=x, lse=torch.zeros(1, 2, 4))
+    kw.update(change)
+    with pytest.raises(ValueError, match=match):
+        b200_pisa.attention_backward(kw["dout"], x, x, x, kw["out"], kw["lse"])
+
+
+def test_c_entries_check_their_arguments():
+    import ctypes
+
+    from b200_pisa import _lib
+    from b200_pisa._args import row_view
+
+    lib = _lib.LIB
+    x, kv = _x(1, 4, 8, 64), _x(1, 2, 8, 64)
+    q, k = row_view(x), row_view(kv)
+    fake = ctypes.c_void_p(256)
+
+    def forward(q=q, k=k, v=k, out=q, scale=0.1, lens=None):
+        return lib.b2_attention_forward(*(ctypes.byref(a) for a in (q, k, v, out)), scale, 0, lens, None, None)
+
+    def backward(dq=q, dk=k, lse=fake, ws=fake):
+        args = [ctypes.byref(a) for a in (q, k, k, q, q)]
+        return lib.b2_attention_backward(*args, lse, ctypes.byref(dq), ctypes.byref(dk), ctypes.byref(k), 0.1, 0, None,
+                                         ws, None)
+
+    def changed(view, **fields):
+        new = _lib.View.from_buffer_copy(view)
+        for name, value in fields.items():
+            setattr(new, name, value)
+        return new
+
+    invalid, unsupported = _lib.B2_ERR_INVALID, _lib.B2_ERR_UNSUPPORTED
+    assert forward(scale=0.0) == invalid and forward(scale=math.inf) == invalid
+    assert forward(lens=ctypes.c_void_p(2)) == invalid
+    assert forward(k=changed(k, heads=3), v=changed(k, heads=3)) == invalid
+    assert forward(q=changed(q, stride_h=0)) == invalid  # broadcast rows
+    assert forward(out=changed(q, stride_t=-64)) == invalid
+    assert forward(q=changed(q, order=_lib.ORDER_TILED8, grid_h=8, grid_w=8, tokens=64)) == unsupported
+    assert forward(*(changed(a, dtype=_lib.B2_F32) for a in (q, k, k, q))) == unsupported
+    wide = dict(head_dim=136, stride_t=136)
+    assert forward(*(changed(a, **wide) for a in (q, k, k, q))) == unsupported
+    many = dict(batch=65536 // 2, stride_b=64)
+    assert forward(*(changed(a, **many) for a in (q, k, k, q))) == unsupported
+    assert backward(lse=None) == invalid and backward(ws=None) == invalid and backward(ws=ctypes.c_void_p(8)) == invalid
+    assert backward(dk=q) == invalid and backward(dq=changed(q, stride_t=0)) == invalid
+    assert lib.b2_attention_backward_workspace_bytes(0, 1, 1, 1) == -1
+    assert lib.b2_attention_backward_workspace_bytes(2, 4, 2, 129) >= 2 * 4 * 2 * 1024
+
+
+# ---------------------------------------------------------------- parity (GPU)
+CASES = [
+    # b, h, hk, tq, tk, d, dtype, causal, lens, layout
+    (1, 1, 1, 128, 128, 64, torch.bfloat16, False, None, "bhtd"),
+    (1, 1, 1, 128, 128, 128, torch.bfloat16, False, None, "bhtd"),
+    (1, 2, 2, 1, 1, 64, torch.bfloat16, False, None, "bthd"),
+    (1, 2, 1, 1, 300, 128, torch.float16, False, None, "bthd"),
+    (2, 2, 2, 300, 1, 40, torch.bfloat16, False, None, "fused"),
+    (1, 4, 2, 257, 129, 128, torch.float16, False, None, "sliced"),
+    (2, 3, 3, 65, 127, 8, torch.bfloat16, False, None, "bthd"),
+    (1, 7, 1, 200, 333, 72, torch.float16, False, None, "bthd"),
+    (3, 4, 4, 130, 260, 128, torch.bfloat16, False, (260, 0, 131), "bthd"),
+    (3, 4, 2, 130, 260, 64, torch.float16, False, (1, 128, 129), "fused"),
+    (2, 2, 2, 100, 64, 96, torch.bfloat16, False, (-5, 1000), "bhtd"),
+    (1, 2, 2, 385, 385, 128, torch.bfloat16, True, None, "bthd"),
+    (1, 4, 1, 513, 513, 64, torch.float16, True, None, "fused"),
+    (1, 2, 2, 100, 400, 128, torch.bfloat16, True, None, "bthd"),
+    (1, 2, 2, 1, 400, 128, torch.bfloat16, True, None, "bthd"),
+    (2, 2, 1, 400, 100, 128, torch.bfloat16, True, None, "bthd"),  # the first 300 queries see nothing
+    (2, 2, 1, 260, 260, 120, torch.float16, True, (200, 30), "sliced"),
+    (1, 2, 2, 1030, 2050, 128, torch.bfloat16, False, None, "bthd"),
+    (1, 2, 2, 2050, 1030, 48, torch.float16, False, None, "bthd"),
+]
+
+
+def run_case(b, h, hk, tq, tk, d, dtype, causal, lens, layout, seed=0, spread=1.0):
+    import b200_pisa
+
+    q = make(b, h, tq, d, dtype, layout, seed + 1, spread)
+    k, v = (make(b, hk, tk, d, dtype, layout, seed + i, spread if i == 2 else 1.0) for i in (2, 3))
+    dout = make(b, h, tq, d, dtype, "bthd", seed + 4)
+    lens_t = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=DEV)
+    if lens is not None:  # what lies past the keys does not matter
+        k, v = k.clone(), v.clone()
+        for i, n in enumerate(lens):
+            k[i, :, max(n, 0):], v[i, :, max(n, 0):] = math.nan, math.inf
+    out, lse = b200_pisa.attention_forward(q, k, v, causal=causal, key_lengths=lens_t)
+    grads = b200_pisa.attention_backward(dout, q, k, v, out, lse, causal=causal, key_lengths=lens_t)
+    again = b200_pisa.attention_backward(dout, q, k, v, out, lse, causal=causal, key_lengths=lens_t)
+    assert all(torch.equal(x, y) for x, y in zip(grads, again))
+    clamped = None if lens is None else lens_t.clamp(0, tk)
+    res, allow = reference(q, k, v, dout, d ** -0.5, causal, clamped)
+    u = torch.finfo(dtype).eps / 2
+    empty = res["lse"] == -math.inf
+    assert torch.equal(lse == -math.inf, empty)
+    # sums of up to Tk FP32 terms, exp2, log2: 2^-18 of the sum
+    assert ((lse.double() - res["lse"])[~empty].abs() <= FP32_PART * (1 + res["lse"][~empty].abs())).all()
+    for name, got in (("out", out), ("dq", grads[0]), ("dk", grads[1]), ("dv", grads[2])):
+        close(name, got, res[name], allow[name](u))
+    assert (out[empty] == 0).all() and (grads[0][empty] == 0).all()
+    if lens is not None:
+        for i, n in enumerate(lens):
+            assert (grads[1][i, :, max(n, 0):] == 0).all() and (grads[2][i, :, max(n, 0):] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c)).replace("torch.", ""))
+def test_forward_and_backward_match_fp64(case):
+    run_case(*case)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_peaked_rows(dtype):
+    """Logits spread by 3 * 3: most of a row's weight on few keys."""
+    run_case(1, 2, 2, 300, 500, 128, dtype, False, None, "bthd", seed=10, spread=3.0 ** 0.5)

@@ -47,6 +47,11 @@ constexpr int kTile = 128;
 constexpr int kThreads = 320;
 constexpr uint32_t kHalfBytes = kTile * 128;  // 128 rows x 64 16-bit columns
 constexpr uint32_t kStatBytes = 2 * kTile * 4;
+// Rings of the walked tiles.  K (or Q) is read by the first and the last
+// product of its tile pair, so the tile after the next is requested a whole
+// pair before its first use only with three stages: with two, each pair
+// waited for its load (9216^2 x 32 heads: 3.97 ms against 4.62 ms).
+constexpr int kStagesA = 3, kStagesB = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kShiftP16 = 8;  // FP16: P is held times 2^8
 
@@ -69,8 +74,9 @@ struct GradArgs {
 
 struct __align__(8) Misc {
   uint64_t own_full;      // the CTA's own two tiles
-  uint64_t a_full[2], a_empty[2];  // walked tiles: Q (with statistics) or K
-  uint64_t b_full[2], b_empty[2];  // dO or V
+  uint64_t a_full[kStagesA], a_empty[kStagesA];  // walked tiles: Q or K
+  uint64_t b_full[kStagesB], b_empty[kStagesB];  // dO or V
+  uint64_t stat_full[2], stat_empty[2];          // -lse and -delta of a query tile
   uint64_t s_full, s_read, p_full, dp_full, ds_full;
   uint64_t acc0_done, acc1_done, all_done;
   uint32_t tmem;
@@ -82,9 +88,9 @@ struct Smem {
   static constexpr uint32_t tile = HALVES * kHalfBytes;
   static constexpr uint32_t own0 = 0;
   static constexpr uint32_t own1 = own0 + tile;
-  static constexpr uint32_t a = own1 + tile;      // [2]
-  static constexpr uint32_t b = a + 2 * tile;     // [2]
-  static constexpr uint32_t stat = b + 2 * tile;  // [2]
+  static constexpr uint32_t a = own1 + tile;
+  static constexpr uint32_t b = a + kStagesA * tile;
+  static constexpr uint32_t stat = b + kStagesB * tile;  // [2]
   static constexpr uint32_t misc = stat + 2 * kStatBytes;
   // one CTA per SM (each owns all 512 TMEM columns)
   static constexpr uint32_t used = misc + sizeof(Misc);
@@ -107,26 +113,33 @@ __device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uin
     tma_load_4d(static_cast<char*>(dst) + dh * kHalfBytes, map, bar, dh * 64, row, h, b);
 }
 
+// Descriptors of a tile at shared-memory address `addr`, as rows of a product
+// (K-major) or as its contraction (MN-major, 64-column halves kHalfBytes
+// apart).  Steps inside a tile are added to the address field (16-byte
+// units), one 64-bit add per MMA: building each descriptor from its address
+// kept the issuing thread busy for 300 to 400 cycles a product.
+__device__ __forceinline__ uint64_t rows_desc(uint32_t addr) { return smem_desc_sw128(addr, 16, 1024); }
+__device__ __forceinline__ uint64_t cols_desc(uint32_t addr) { return smem_desc_sw128(addr, kHalfBytes, 1024); }
+
 // D[128 x 128] = A B^T over the head dimension, both tiles K-major in shared memory.
 template <bool BF16, int HALVES>
-__device__ __forceinline__ void product_rows(uint32_t d, uint32_t a_addr, uint32_t b_addr) {
+__device__ __forceinline__ void product_rows(uint32_t d, uint64_t a_desc, uint64_t b_desc) {
   constexpr uint32_t idesc = idesc_f16(128, 128, BF16, false, false);
 #pragma unroll
   for (int kk = 0; kk < 4 * HALVES; ++kk) {
-    const uint32_t off = (kk >> 2) * kHalfBytes + (kk & 3) * 32;
-    mma_ss(d, smem_desc_sw128(a_addr + off, 16, 1024), smem_desc_sw128(b_addr + off, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+    const uint32_t off = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
+    mma_ss(d, a_desc + off, b_desc + off, idesc, kk > 0 ? 1u : 0u);
   }
 }
 
 // D[128 x D] (+)= A B with A (128 x 128, 16-bit) in tensor memory over the
 // first 32 columns of each 64-column half at `a`, B's rows as contraction.
 template <bool BF16, int HALVES>
-__device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint32_t b_addr, bool accumulate) {
+__device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint64_t b_desc, bool accumulate) {
   constexpr uint32_t idesc = idesc_f16(128, 64 * HALVES, BF16, false, true);
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
-    mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, smem_desc_sw128(b_addr + kk * 2048, kHalfBytes, 1024), idesc,
-           accumulate || kk > 0 ? 1u : 0u);
+    mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b_desc + kk * (2048 >> 4), idesc, kk > 0 ? 1u : accumulate ? 1u : 0u);
 }
 
 __device__ __forceinline__ uint64_t pack_f2(float a, float b) {
@@ -151,6 +164,15 @@ __device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// Zero the 16-bit elements of 64 packed columns whose bit is set.
+__device__ __forceinline__ void clear_pairs(uint32_t (&w)[32], uint32_t bad0, uint32_t bad1) {
+#pragma unroll
+  for (int c = 0; c < 64; c += 2) {
+    const uint32_t two = (c < 32 ? bad0 : bad1) >> (c & 31);
+    w[c / 2] &= (two & 1u ? 0u : 0xFFFFu) | (two & 2u ? 0u : 0xFFFF0000u);
+  }
 }
 
 __device__ __forceinline__ int key_count(const GradArgs& a, int b) {
@@ -228,72 +250,78 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
       mbar_expect_tx(&m.own_full, 2 * L::tile);
       load_tile<HALVES>(smem + L::own0, k_map, &m.own_full, k0, hk, b);
       load_tile<HALVES>(smem + L::own1, v_map, &m.own_full, k0, hk, b);
-      int na = 0, nb = 0;
+      int na = 0, nb = 0, ns = 0;
       for (int i = 0; i < n; ++i) {
-        const int s = i & 1;
-        const uint32_t free_parity = ((i >> 1) & 1) ^ 1;
+        const int sa = i % kStagesA, sb = i % kStagesB, ss = i & 1;
         const int g = i / per_head;
         const int qt = first + i - g * per_head;
         const int h = hk * a.group + g;
-        if (!mbar_wait(&m.a_empty[s], free_parity, abort_flag, a.status, 1)) break;
-        mbar_expect_tx(&m.a_full[s], L::tile + kStatBytes);
-        load_tile<HALVES>(smem + L::a + s * L::tile, q_map, &m.a_full[s], qt * kTile, h, b);
-        bulk_load(smem + L::stat + s * kStatBytes, a.stat + ((int64_t(b) * a.heads + h) * a.q_tiles + qt) * (2 * kTile),
-                  kStatBytes, &m.a_full[s]);
+        if (!mbar_wait(&m.a_empty[sa], ((i / kStagesA) & 1) ^ 1, abort_flag, a.status, 1)) break;
+        mbar_expect_tx(&m.a_full[sa], L::tile);
+        load_tile<HALVES>(smem + L::a + sa * L::tile, q_map, &m.a_full[sa], qt * kTile, h, b);
         na = i + 1;
-        if (!mbar_wait(&m.b_empty[s], free_parity, abort_flag, a.status, 2)) break;
-        mbar_expect_tx(&m.b_full[s], L::tile);
-        load_tile<HALVES>(smem + L::b + s * L::tile, do_map, &m.b_full[s], qt * kTile, h, b);
+        if (!mbar_wait(&m.stat_empty[ss], ((i >> 1) & 1) ^ 1, abort_flag, a.status, 17)) break;
+        mbar_expect_tx(&m.stat_full[ss], kStatBytes);
+        bulk_load(smem + L::stat + ss * kStatBytes, a.stat + ((int64_t(b) * a.heads + h) * a.q_tiles + qt) * (2 * kTile),
+                  kStatBytes, &m.stat_full[ss]);
+        ns = i + 1;
+        if (!mbar_wait(&m.b_empty[sb], ((i / kStagesB) & 1) ^ 1, abort_flag, a.status, 2)) break;
+        mbar_expect_tx(&m.b_full[sb], L::tile);
+        load_tile<HALVES>(smem + L::b + sb * L::tile, do_map, &m.b_full[sb], qt * kTile, h, b);
         nb = i + 1;
       }
       if (*abort_flag) {
-        drain_loads(m.a_full, 2, na, &m.own_full, a.status);
-        drain_loads(m.b_full, 2, nb, nullptr, a.status);
+        drain_loads(m.a_full, kStagesA, na, &m.own_full, a.status);
+        drain_loads(m.b_full, kStagesB, nb, nullptr, a.status);
+        drain_loads(m.stat_full, 2, ns, nullptr, a.status);
       }
     }
   } else if (warp == 1) {
     if (n > 0 && elect_one()) {
-      const uint32_t k_addr = smem_u32(smem + L::own0), v_addr = smem_u32(smem + L::own1);
-      auto q_addr = [&](int s) { return smem_u32(smem + L::a + s * L::tile); };
-      auto do_addr = [&](int s) { return smem_u32(smem + L::b + s * L::tile); };
+      const uint32_t base = smem_u32(smem);
+      const uint64_t k_rows = rows_desc(base + L::own0), v_rows = rows_desc(base + L::own1);
+      const uint64_t q_rows = rows_desc(base + L::a), q_cols = cols_desc(base + L::a);  // stage 0; stages L::tile apart
+      const uint64_t do_rows = rows_desc(base + L::b), do_cols = cols_desc(base + L::b);
+      constexpr uint32_t step = L::tile >> 4;
       bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3) && mbar_wait(&m.a_full[0], 0, abort_flag, a.status, 4);
       if (ok) {
-        product_rows<BF16, HALVES>(tmem + kColS, k_addr, q_addr(0));
+        product_rows<BF16, HALVES>(tmem + kColS, k_rows, q_rows);
         mma_commit(&m.s_full);
         ok = mbar_wait(&m.b_full[0], 0, abort_flag, a.status, 5);
       }
       if (ok) {
-        product_rows<BF16, HALVES>(tmem + kColDP, v_addr, do_addr(0));
+        product_rows<BF16, HALVES>(tmem + kColDP, v_rows, do_rows);
         mma_commit(&m.dp_full);
       }
       for (int i = 0; ok && i < n; ++i) {
-        const int s = i & 1, t = s ^ 1;
-        const uint32_t ph = i & 1, next_ph = ((i + 1) >> 1) & 1;
+        const int sa = i % kStagesA, sb = i % kStagesB;
+        const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesB;  // the next tiles' stages and phases
+        const uint32_t ph = i & 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesB) & 1;
         const bool more = i + 1 < n;
         // dV += P^T dO; then the next S may take the columns P was read from
         if (!(ok = mbar_wait(&m.p_full, ph, abort_flag, a.status, 6))) break;
         tc_fence_after();
-        product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColS, do_addr(s), i > 0);
+        product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColS, do_cols + sb * step, i > 0);
         mma_commit(&m.acc0_done);
-        mma_commit(&m.b_empty[s]);
+        mma_commit(&m.b_empty[sb]);
         if (more) {
-          ok = mbar_wait(&m.a_full[t], next_ph, abort_flag, a.status, 7) &&
+          ok = mbar_wait(&m.a_full[ta], ta_ph, abort_flag, a.status, 7) &&
                mbar_wait(&m.acc0_done, ph, abort_flag, a.status, 8);
           if (!ok) break;
-          product_rows<BF16, HALVES>(tmem + kColS, k_addr, q_addr(t));
+          product_rows<BF16, HALVES>(tmem + kColS, k_rows, q_rows + ta * step);
           mma_commit(&m.s_full);
         }
         // dK += dS^T Q; then the next dP
         if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
         tc_fence_after();
-        product_cols<BF16, HALVES>(tmem + kColAcc1, tmem + kColDP, q_addr(s), i > 0);
+        product_cols<BF16, HALVES>(tmem + kColAcc1, tmem + kColDP, q_cols + sa * step, i > 0);
         mma_commit(&m.acc1_done);
-        mma_commit(&m.a_empty[s]);
+        mma_commit(&m.a_empty[sa]);
         if (more) {
-          ok = mbar_wait(&m.b_full[t], next_ph, abort_flag, a.status, 10) &&
+          ok = mbar_wait(&m.b_full[tb], tb_ph, abort_flag, a.status, 10) &&
                mbar_wait(&m.acc1_done, ph, abort_flag, a.status, 11);
           if (!ok) break;
-          product_rows<BF16, HALVES>(tmem + kColDP, v_addr, do_addr(t));
+          product_rows<BF16, HALVES>(tmem + kColDP, v_rows, do_rows + tb * step);
           mma_commit(&m.dp_full);
         }
       }
@@ -329,7 +357,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
         bad1 = static_cast<uint32_t>(bad >> 32);
       }
       const bool masked = (bad0 | bad1) != 0u;
-      if (!(ok = mbar_wait(&m.a_full[s], (i >> 1) & 1, abort_flag, a.status, 13))) break;  // statistics
+      if (!(ok = mbar_wait(&m.stat_full[s], (i >> 1) & 1, abort_flag, a.status, 13))) break;
       if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
       tc_fence_after();
       uint32_t v[64];
@@ -346,13 +374,9 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[c + e] = __float_as_uint(ex2(x[e]));
       }
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (((c < 32 ? bad0 : bad1) >> (c & 31)) & 1u) v[c] = 0u;
-      }
 #pragma unroll
       for (int c = 0; c < 64; c += 2) w[c / 2] = Cvt<T>::pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+      if (masked) clear_pairs(w, bad0, bad1);
       tmem_st32(s_addr, w);
       tmem_wait_st();
       tc_fence_before();
@@ -361,36 +385,33 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
       // dS = P (dP - delta)
       if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
       tc_fence_after();
+      uint32_t d[64];
+      tmem_ld32(dp_addr, d);
+      tmem_ld32(dp_addr + 32, d + 32);
+      tmem_wait_ld();
 #pragma unroll
-      for (int c0 = 0; c0 < 64; c0 += 32) {
-        uint32_t d[32];
-        tmem_ld32(dp_addr + c0, d);
-        tmem_wait_ld();
+      for (int c = 0; c < 64; c += 4) {
+        const float4 nd = *reinterpret_cast<const float4*>(stat + kTile + c);
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const float4 nd = *reinterpret_cast<const float4*>(stat + kTile + c0 + c);
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            uint64_t p = pack_f2(__uint_as_float(v[c0 + c + e]), __uint_as_float(v[c0 + c + e + 1]));
-            if constexpr (!BF16) p = mul_f2(p, gain2);
-            const uint64_t x = mul_f2(p, add_f2(pack_f2(__uint_as_float(d[c + e]), __uint_as_float(d[c + e + 1])),
-                                                e == 0 ? pack_f2(nd.x, nd.y) : pack_f2(nd.z, nd.w)));
-            float x0, x1;
-            unpack_f2(x, x0, x1);
-            if (masked) {  // 0 * inf
-              const uint32_t bw = c0 == 0 ? bad0 : bad1;
-              if ((bw >> (c + e)) & 1u) x0 = 0.f;
-              if ((bw >> (c + e + 1)) & 1u) x1 = 0.f;
-            }
-            w[(c0 + c + e) / 2] = Cvt<T>::pack2(x0, x1);
-          }
+        for (int e = c; e < c + 4; e += 2) {
+          uint64_t p = pack_f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+          if constexpr (!BF16) p = mul_f2(p, gain2);
+          const uint64_t x = mul_f2(p, add_f2(pack_f2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])),
+                                              e == c ? pack_f2(nd.x, nd.y) : pack_f2(nd.z, nd.w)));
+          float x0, x1;
+          unpack_f2(x, x0, x1);
+          w[e / 2] = Cvt<T>::pack2(x0, x1);
         }
       }
+      if (masked) clear_pairs(w, bad0, bad1);  // 0 * inf
       tmem_st32(dp_addr, w);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&m.ds_full);
+      if (lane == 0) {
+        mbar_arrive(&m.stat_empty[s]);
+        mbar_arrive(&m.ds_full);
+      }
     }
     // warps 2-5 store dV, 6-9 dK
     const Rows& out = wg == 0 ? a.dv : a.dk;
@@ -438,63 +459,65 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
       load_tile<HALVES>(smem + L::own1, do_map, &m.own_full, q0, h, b);
       int na = 0, nb = 0;
       for (int i = 0; i < n; ++i) {
-        const int s = i & 1;
-        const uint32_t free_parity = ((i >> 1) & 1) ^ 1;
-        if (!mbar_wait(&m.a_empty[s], free_parity, abort_flag, a.status, 1)) break;
-        mbar_expect_tx(&m.a_full[s], L::tile);
-        load_tile<HALVES>(smem + L::a + s * L::tile, k_map, &m.a_full[s], i * kTile, hk, b);
+        const int sa = i % kStagesA, sb = i % kStagesB;
+        if (!mbar_wait(&m.a_empty[sa], ((i / kStagesA) & 1) ^ 1, abort_flag, a.status, 1)) break;
+        mbar_expect_tx(&m.a_full[sa], L::tile);
+        load_tile<HALVES>(smem + L::a + sa * L::tile, k_map, &m.a_full[sa], i * kTile, hk, b);
         na = i + 1;
-        if (!mbar_wait(&m.b_empty[s], free_parity, abort_flag, a.status, 2)) break;
-        mbar_expect_tx(&m.b_full[s], L::tile);
-        load_tile<HALVES>(smem + L::b + s * L::tile, v_map, &m.b_full[s], i * kTile, hk, b);
+        if (!mbar_wait(&m.b_empty[sb], ((i / kStagesB) & 1) ^ 1, abort_flag, a.status, 2)) break;
+        mbar_expect_tx(&m.b_full[sb], L::tile);
+        load_tile<HALVES>(smem + L::b + sb * L::tile, v_map, &m.b_full[sb], i * kTile, hk, b);
         nb = i + 1;
       }
       if (*abort_flag) {
-        drain_loads(m.a_full, 2, na, &m.own_full, a.status);
-        drain_loads(m.b_full, 2, nb, nullptr, a.status);
+        drain_loads(m.a_full, kStagesA, na, &m.own_full, a.status);
+        drain_loads(m.b_full, kStagesB, nb, nullptr, a.status);
       }
     }
   } else if (warp == 1) {
     if (n > 0 && elect_one()) {
-      const uint32_t q_addr = smem_u32(smem + L::own0), do_addr = smem_u32(smem + L::own1);
-      auto k_addr = [&](int s) { return smem_u32(smem + L::a + s * L::tile); };
-      auto v_addr = [&](int s) { return smem_u32(smem + L::b + s * L::tile); };
+      const uint32_t base = smem_u32(smem);
+      const uint64_t q_rows = rows_desc(base + L::own0), do_rows = rows_desc(base + L::own1);
+      const uint64_t k_rows = rows_desc(base + L::a), k_cols = cols_desc(base + L::a);
+      const uint64_t v_rows = rows_desc(base + L::b);
+      constexpr uint32_t step = L::tile >> 4;
       bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3) && mbar_wait(&m.a_full[0], 0, abort_flag, a.status, 4);
       if (ok) {
-        product_rows<BF16, HALVES>(tmem + kColS, q_addr, k_addr(0));
+        product_rows<BF16, HALVES>(tmem + kColS, q_rows, k_rows);
         mma_commit(&m.s_full);
         ok = mbar_wait(&m.b_full[0], 0, abort_flag, a.status, 5);
       }
       if (ok) {
-        product_rows<BF16, HALVES>(tmem + kColDP, do_addr, v_addr(0));
+        product_rows<BF16, HALVES>(tmem + kColDP, do_rows, v_rows);
         mma_commit(&m.dp_full);
         mma_commit(&m.b_empty[0]);
       }
       for (int i = 0; ok && i < n; ++i) {
-        const int s = i & 1, t = s ^ 1;
-        const uint32_t ph = i & 1, next_ph = ((i + 1) >> 1) & 1;
+        const int sa = i % kStagesA, sb = i % kStagesB;
+        const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesB;  // the next tiles' stages and phases
+        const uint32_t ph = i & 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesB) & 1;
         const bool more = i + 1 < n;
         if (more) {  // the next S, once the elementwise warps hold this one
-          ok = mbar_wait(&m.a_full[t], next_ph, abort_flag, a.status, 7) &&
+          ok = mbar_wait(&m.a_full[ta], ta_ph, abort_flag, a.status, 7) &&
                mbar_wait(&m.s_read, ph, abort_flag, a.status, 8);
           if (!ok) break;
           tc_fence_after();
-          product_rows<BF16, HALVES>(tmem + kColS, q_addr, k_addr(t));
+          product_rows<BF16, HALVES>(tmem + kColS, q_rows, k_rows + ta * step);
           mma_commit(&m.s_full);
         }
         // dQ += dS K; then the next dP may take the columns dS was read from
         if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
         tc_fence_after();
-        product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColDP, k_addr(s), i > 0);
+        product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColDP, k_cols + sa * step, i > 0);
         mma_commit(&m.acc0_done);
-        mma_commit(&m.a_empty[s]);
+        mma_commit(&m.a_empty[sa]);
         if (more) {
-          ok = mbar_wait(&m.b_full[t], next_ph, abort_flag, a.status, 10) &&
+          ok = mbar_wait(&m.b_full[tb], tb_ph, abort_flag, a.status, 10) &&
                mbar_wait(&m.acc0_done, ph, abort_flag, a.status, 11);
           if (!ok) break;
-          product_rows<BF16, HALVES>(tmem + kColDP, do_addr, v_addr(t));
+          product_rows<BF16, HALVES>(tmem + kColDP, do_rows, v_rows + tb * step);
           mma_commit(&m.dp_full);
-          mma_commit(&m.b_empty[t]);
+          mma_commit(&m.b_empty[tb]);
         }
       }
       mma_commit(&m.all_done);
@@ -518,7 +541,6 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
     const int seen = a.causal ? min(len, query + off + 1) : len;  // keys this row sees
     bool ok = true;
     for (int i = 0; i < n; ++i) {
-      const int s = i & 1;
       const uint32_t ph = i & 1;
       const int lim = seen - i * kTile - wg * 64;  // columns from `lim` on are masked
       const bool masked = lim < 64;
@@ -546,7 +568,7 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
       if (len < min(k0 + kTile, a.tk)) {
         const int tid = threadIdx.x - 64;
         const int from = len - k0, rows = min(kTile, a.tk - k0) - from;
-        char* tile = smem + L::a + s * L::tile;
+        char* tile = smem + L::a + (i % kStagesA) * L::tile;
         for (int x = tid; x < rows * 8 * HALVES; x += 256) {
           const int r = from + x / (8 * HALVES), ch = x % (8 * HALVES);
           *reinterpret_cast<uint4*>(tile + (ch >> 3) * kHalfBytes + r * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -555,26 +577,19 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
       }
       if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
       tc_fence_after();
-      uint32_t w[32];
+      uint32_t w[32], d[64];
+      tmem_ld32(dp_addr, d);
+      tmem_ld32(dp_addr + 32, d + 32);
+      tmem_wait_ld();
 #pragma unroll
-      for (int c0 = 0; c0 < 64; c0 += 32) {
-        uint32_t d[32];
-        tmem_ld32(dp_addr + c0, d);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          uint64_t p = pack_f2(__uint_as_float(v[c0 + c]), __uint_as_float(v[c0 + c + 1]));
-          if constexpr (!BF16) p = mul_f2(p, gain2);
-          float x0, x1;
-          unpack_f2(mul_f2(p, add_f2(pack_f2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), nd2)), x0, x1);
-          if (masked) {
-            const uint32_t bw = c0 == 0 ? bad0 : bad1;
-            if ((bw >> c) & 1u) x0 = 0.f;
-            if ((bw >> (c + 1)) & 1u) x1 = 0.f;
-          }
-          w[(c0 + c) / 2] = Cvt<T>::pack2(x0, x1);
-        }
+      for (int c = 0; c < 64; c += 2) {
+        uint64_t p = pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+        if constexpr (!BF16) p = mul_f2(p, gain2);
+        float x0, x1;
+        unpack_f2(mul_f2(p, add_f2(pack_f2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), nd2)), x0, x1);
+        w[c / 2] = Cvt<T>::pack2(x0, x1);
       }
+      if (masked) clear_pairs(w, bad0, bad1);
       tmem_st32(dp_addr, w);
       tmem_wait_st();
       tc_fence_before();
@@ -610,11 +625,17 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       atomicCAS(a.status, 0, 0x300);
     }
     mbar_init(&m.own_full, 1);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < kStagesA; ++s) {
       mbar_init(&m.a_full[s], 1);
       mbar_init(&m.a_empty[s], 1);
+    }
+    for (int s = 0; s < kStagesB; ++s) {
       mbar_init(&m.b_full[s], 1);
       mbar_init(&m.b_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&m.stat_full[s], 1);
+      mbar_init(&m.stat_empty[s], 8);
     }
     mbar_init(&m.s_full, 1);
     mbar_init(&m.s_read, 8);

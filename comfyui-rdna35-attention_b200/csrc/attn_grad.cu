@@ -21,9 +21,9 @@
 // bandwidth (about 3750 cycles a pair at 128 B a cycle, against 7 * 512 for
 // the products here).
 //
-// Warp roles (320 threads, one CTA per SM): warp 0 TMA producer, warp 1 MMA
-// issuer and TMEM owner, warps 2..9 elementwise (warp % 4 is the TMEM lane
-// quadrant, warps 2-5 take columns 0-63 and 6-9 columns 64-127 of a tile).
+// Warp roles (576 threads, one CTA per SM): warp 0 TMA producer, warp 1 MMA
+// issuer and TMEM owner, warps 2..17 elementwise (warp % 4 is the TMEM lane
+// quadrant, and each group of four warps takes 32 columns of a tile).
 //
 // Precision: products of 16-bit operands accumulated in FP32; P and dS are
 // rounded to the inputs' type once, as operands.  FP16 has too small a range
@@ -44,7 +44,8 @@ namespace {
 using namespace umma;
 
 constexpr int kTile = 128;
-constexpr int kThreads = 320;
+constexpr int kElemWarps = 16;  // 4 TMEM lane quadrants x 4 column groups of 32
+constexpr int kThreads = 64 + 32 * kElemWarps;
 constexpr uint32_t kHalfBytes = kTile * 128;  // 128 rows x 64 16-bit columns
 constexpr uint32_t kStatBytes = 2 * kTile * 4;
 // Rings of the walked tiles.  K (or Q) is read by the first and the last
@@ -55,8 +56,11 @@ constexpr int kStagesA = 3, kStagesB = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kShiftP16 = 8;  // FP16: P is held times 2^8
 
-// TMEM columns
-constexpr uint32_t kColS = 0, kColDP = 128, kColAcc0 = 256, kColAcc1 = 384;
+// TMEM columns.  dK/dV: S and dP take turns in kColS (each is free again as
+// soon as the elementwise warps have loaded it), P and dS have columns of
+// their own.  dQ: S and dP have a place each, dS two.
+constexpr uint32_t kColS = 0, kColP = 128, kColDS = 192, kColAcc0 = 256, kColAcc1 = 384;
+constexpr uint32_t kColDP = 128, kColDS2 = 384;
 
 struct GradArgs {
   Rows dq, dk, dv;
@@ -77,8 +81,11 @@ struct __align__(8) Misc {
   uint64_t a_full[kStagesA], a_empty[kStagesA];  // walked tiles: Q or K
   uint64_t b_full[kStagesB], b_empty[kStagesB];  // dO or V
   uint64_t stat_full[2], stat_empty[2];          // -lse and -delta of a query tile
-  uint64_t s_full, s_read, p_full, dp_full, ds_full;
-  uint64_t acc0_done, acc1_done, all_done;
+  uint64_t s_full, s_read, p_full, dp_full, dp_read;
+  // dQ keeps two dS buffers in flight, each with barriers of its own: one
+  // barrier could run two phases ahead of a waiting warp and look unfinished
+  uint64_t ds_full[2], acc0_done[2];
+  uint64_t acc1_done, all_done;
   uint32_t tmem;
   int abort_flag;
 };
@@ -132,14 +139,14 @@ __device__ __forceinline__ void product_rows(uint32_t d, uint64_t a_desc, uint64
   }
 }
 
-// D[128 x D] (+)= A B with A (128 x 128, 16-bit) in tensor memory over the
-// first 32 columns of each 64-column half at `a`, B's rows as contraction.
+// D[128 x D] (+)= A B with A (128 x 128, 16-bit pairs: 64 columns) in tensor
+// memory at `a`, B's rows as contraction.
 template <bool BF16, int HALVES>
 __device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint64_t b_desc, bool accumulate) {
   constexpr uint32_t idesc = idesc_f16(128, 64 * HALVES, BF16, false, true);
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk)
-    mma_ts(d, a + (kk >> 2) * 64 + (kk & 3) * 8, b_desc + kk * (2048 >> 4), idesc, kk > 0 ? 1u : accumulate ? 1u : 0u);
+    mma_ts(d, a + kk * 8, b_desc + kk * (2048 >> 4), idesc, kk > 0 ? 1u : accumulate ? 1u : 0u);
 }
 
 __device__ __forceinline__ uint64_t pack_f2(float a, float b) {
@@ -166,11 +173,20 @@ __device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// Zero the 16-bit elements of 64 packed columns whose bit is set.
-__device__ __forceinline__ void clear_pairs(uint32_t (&w)[32], uint32_t bad0, uint32_t bad1) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Zero the 16-bit elements of 32 packed columns whose bit is set.
+__device__ __forceinline__ void clear_pairs(uint32_t (&w)[16], uint32_t bad) {
 #pragma unroll
-  for (int c = 0; c < 64; c += 2) {
-    const uint32_t two = (c < 32 ? bad0 : bad1) >> (c & 31);
+  for (int c = 0; c < 32; c += 2) {
+    const uint32_t two = bad >> c;
     w[c / 2] &= (two & 1u ? 0u : 0xFFFFu) | (two & 2u ? 0u : 0xFFFF0000u);
   }
 }
@@ -200,13 +216,13 @@ __device__ __forceinline__ void store_cols(char* row, int c0, int dim, const uin
     if (c0 + 8 * q4 < dim) dst[q4] = make_uint4(w[4 * q4], w[4 * q4 + 1], w[4 * q4 + 2], w[4 * q4 + 3]);
 }
 
-// One accumulator row (64 * HALVES columns at `taddr`) to global memory; a
-// row that sees nothing (or lies past the keys) is written as zeros.  The
-// loads are a warp's: every lane calls this, row NULL stores nothing.
-template <typename T, int HALVES>
-__device__ __forceinline__ void store_row(uint32_t taddr, char* row, int dim, float mul, bool zero) {
+// Columns [from, to) of one accumulator row at `taddr` to global memory; a row
+// that sees nothing (or lies past the keys) is written as zeros.  The loads
+// are a warp's: every lane calls this, row NULL stores nothing.
+template <typename T>
+__device__ __forceinline__ void store_row(uint32_t taddr, char* row, int from, int to, int dim, float mul, bool zero) {
 #pragma unroll 1
-  for (int c0 = 0; c0 < 64 * HALVES; c0 += 32) {
+  for (int c0 = from; c0 < to; c0 += 32) {
     uint32_t r[32];
     tmem_ld32(taddr + c0, r);
     tmem_wait_ld();
@@ -283,46 +299,44 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
       const uint64_t q_rows = rows_desc(base + L::a), q_cols = cols_desc(base + L::a);  // stage 0; stages L::tile apart
       const uint64_t do_rows = rows_desc(base + L::b), do_cols = cols_desc(base + L::b);
       constexpr uint32_t step = L::tile >> 4;
-      bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3) && mbar_wait(&m.a_full[0], 0, abort_flag, a.status, 4);
-      if (ok) {
-        product_rows<BF16, HALVES>(tmem + kColS, k_rows, q_rows);
-        mma_commit(&m.s_full);
-        ok = mbar_wait(&m.b_full[0], 0, abort_flag, a.status, 5);
-      }
-      if (ok) {
-        product_rows<BF16, HALVES>(tmem + kColDP, v_rows, do_rows);
-        mma_commit(&m.dp_full);
-      }
-      for (int i = 0; ok && i < n; ++i) {
-        const int sa = i % kStagesA, sb = i % kStagesB;
+      bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3);
+      // Order S(i+1), dV(i), dP(i+1), dK(i): S and dP wait for the elementwise
+      // warps to have loaded the other out of their common columns, and dV or
+      // dK runs while they do.
+      for (int i = -1; ok && i < n; ++i) {
+        const int sa = i < 0 ? 0 : i % kStagesA, sb = i & 1;
         const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesB;  // the next tiles' stages and phases
-        const uint32_t ph = i & 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesB) & 1;
+        const uint32_t ph = i & 1, next = ph ^ 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesB) & 1;
         const bool more = i + 1 < n;
-        // dV += P^T dO; then the next S may take the columns P was read from
-        if (!(ok = mbar_wait(&m.p_full, ph, abort_flag, a.status, 6))) break;
-        tc_fence_after();
-        product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColS, do_cols + sb * step, i > 0);
-        mma_commit(&m.acc0_done);
-        mma_commit(&m.b_empty[sb]);
         if (more) {
           ok = mbar_wait(&m.a_full[ta], ta_ph, abort_flag, a.status, 7) &&
-               mbar_wait(&m.acc0_done, ph, abort_flag, a.status, 8);
+               (i < 0 || mbar_wait(&m.dp_read, ph, abort_flag, a.status, 8));
           if (!ok) break;
+          tc_fence_after();
           product_rows<BF16, HALVES>(tmem + kColS, k_rows, q_rows + ta * step);
           mma_commit(&m.s_full);
         }
-        // dK += dS^T Q; then the next dP
-        if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
-        tc_fence_after();
-        product_cols<BF16, HALVES>(tmem + kColAcc1, tmem + kColDP, q_cols + sa * step, i > 0);
-        mma_commit(&m.acc1_done);
-        mma_commit(&m.a_empty[sa]);
+        if (i >= 0) {
+          if (!(ok = mbar_wait(&m.p_full, ph, abort_flag, a.status, 6))) break;
+          tc_fence_after();
+          product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColP, do_cols + sb * step, i > 0);
+          mma_commit(&m.acc0_done[0]);
+          mma_commit(&m.b_empty[sb]);
+        }
         if (more) {
           ok = mbar_wait(&m.b_full[tb], tb_ph, abort_flag, a.status, 10) &&
-               mbar_wait(&m.acc1_done, ph, abort_flag, a.status, 11);
+               mbar_wait(&m.s_read, next, abort_flag, a.status, 11);
           if (!ok) break;
-          product_rows<BF16, HALVES>(tmem + kColDP, v_rows, do_rows + tb * step);
+          tc_fence_after();
+          product_rows<BF16, HALVES>(tmem + kColS, v_rows, do_rows + tb * step);
           mma_commit(&m.dp_full);
+        }
+        if (i >= 0) {
+          if (!(ok = mbar_wait(&m.ds_full[0], ph, abort_flag, a.status, 9))) break;
+          tc_fence_after();
+          product_cols<BF16, HALVES>(tmem + kColAcc1, tmem + kColDS, q_cols + sa * step, i > 0);
+          mma_commit(&m.acc1_done);
+          mma_commit(&m.a_empty[sa]);
         }
       }
       // every product completes before TMEM is read and released (bounded by
@@ -332,52 +346,54 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
       mbar_wait(&m.all_done, 0, &no_abort, a.status, 12);
     }
   } else {
-    const int wg = (warp - 2) >> 2;
+    const int cg = (warp - 2) >> 2;  // column group: queries cg*32 .. +31 of a tile
     const int sub = warp & 3;
     const int row = sub * 32 + lane;
     const int key = k0 + row;
     const uint32_t lanes = static_cast<uint32_t>(sub * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + kColS + wg * 64;
-    const uint32_t dp_addr = tmem + lanes + kColDP + wg * 64;
+    const uint32_t s_addr = tmem + lanes + kColS + cg * 32;
+    const uint32_t p_addr = tmem + lanes + kColP + cg * 16, ds_addr = tmem + lanes + kColDS + cg * 16;
     float gain = 1.f;
     if constexpr (!BF16) gain = ds_gain(a, bhk);
     const uint64_t gain2 = pack_f2(gain, gain);
     const uint64_t scale2 = pack_f2(a.scale_log2, a.scale_log2);
     bool ok = true;
+    int qt = 0;  // query tile after the first
     for (int i = 0; i < n; ++i) {
       const int s = i & 1;
       const uint32_t ph = i & 1;
-      const float* stat = reinterpret_cast<const float*>(smem + L::stat + s * kStatBytes) + wg * 64;
-      // causal: columns below `lim` are queries before the key
-      uint32_t bad0 = 0u, bad1 = 0u;
+      const float* stat = reinterpret_cast<const float*>(smem + L::stat + s * kStatBytes) + cg * 32;
+      uint32_t bad = 0u;  // causal: columns below `lim` are queries before the key
       if (a.causal) {
-        const int lim = key - off - (first + i % per_head) * kTile - wg * 64;
-        const uint64_t bad = lim <= 0 ? 0ull : lim >= 64 ? ~0ull : (1ull << lim) - 1ull;
-        bad0 = static_cast<uint32_t>(bad);
-        bad1 = static_cast<uint32_t>(bad >> 32);
+        const int lim = key - off - (first + qt) * kTile - cg * 32;
+        bad = lim <= 0 ? 0u : lim >= 32 ? ~0u : (1u << lim) - 1u;
+        qt = qt + 1 < per_head ? qt + 1 : 0;
       }
-      const bool masked = (bad0 | bad1) != 0u;
       if (!(ok = mbar_wait(&m.stat_full[s], (i >> 1) & 1, abort_flag, a.status, 13))) break;
       if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
       tc_fence_after();
-      uint32_t v[64];
+      uint32_t v[32], w[16];
       tmem_ld32(s_addr, v);
-      tmem_ld32(s_addr + 32, v + 32);
       tmem_wait_ld();
-      uint32_t w[32];
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.s_read);
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
+      for (int c = 0; c < 32; c += 4) {
         const float4 nl = *reinterpret_cast<const float4*>(stat + c);
         float x[4];
         unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, pack_f2(nl.x, nl.y)), x[0], x[1]);
         unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, pack_f2(nl.z, nl.w)), x[2], x[3]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[c + e] = __float_as_uint(ex2(x[e]));
+        w[c / 2] = Cvt<T>::pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+        w[c / 2 + 1] = Cvt<T>::pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
       }
-#pragma unroll
-      for (int c = 0; c < 64; c += 2) w[c / 2] = Cvt<T>::pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-      if (masked) clear_pairs(w, bad0, bad1);
-      tmem_st32(s_addr, w);
+      if (bad != 0u) clear_pairs(w, bad);
+      // P's columns are free once the last dV has read them
+      if (i > 0 && !(ok = mbar_wait(&m.acc0_done[0], ph ^ 1, abort_flag, a.status, 18))) break;
+      tc_fence_after();
+      tmem_st16(p_addr, w);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -385,12 +401,14 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
       // dS = P (dP - delta)
       if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
       tc_fence_after();
-      uint32_t d[64];
-      tmem_ld32(dp_addr, d);
-      tmem_ld32(dp_addr + 32, d + 32);
+      uint32_t d[32];
+      tmem_ld32(s_addr, d);
       tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.dp_read);
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
+      for (int c = 0; c < 32; c += 4) {
         const float4 nd = *reinterpret_cast<const float4*>(stat + kTile + c);
 #pragma unroll
         for (int e = c; e < c + 4; e += 2) {
@@ -403,28 +421,32 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
           w[e / 2] = Cvt<T>::pack2(x0, x1);
         }
       }
-      if (masked) clear_pairs(w, bad0, bad1);  // 0 * inf
-      tmem_st32(dp_addr, w);
+      if (bad != 0u) clear_pairs(w, bad);  // 0 * inf
+      if (i > 0 && !(ok = mbar_wait(&m.acc1_done, ph ^ 1, abort_flag, a.status, 19))) break;
+      tc_fence_after();
+      tmem_st16(ds_addr, w);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&m.stat_empty[s]);
-        mbar_arrive(&m.ds_full);
+        mbar_arrive(&m.ds_full[0]);
       }
     }
-    // warps 2-5 store dV, 6-9 dK
-    const Rows& out = wg == 0 ? a.dv : a.dk;
+    // column groups 0 and 1 store the halves of dV, 2 and 3 those of dK
+    const bool is_dk = cg >= 2;
+    const Rows& out = is_dk ? a.dk : a.dv;
     char* orow = key < a.tk ? out.row(bhk, key) : nullptr;
     if (n == 0) {
-      if (orow != nullptr) store_zero_row<T>(orow, a.dim);
+      if (orow != nullptr && (cg & 1) == 0) store_zero_row<T>(orow, a.dim);
     } else {
       ok = ok && mbar_wait(&m.all_done, 0, abort_flag, a.status, 16);
       tc_fence_after();
       if (ok && !*abort_flag) {
         const float p_mul = BF16 ? 1.f : 1.f / (1 << kShiftP16);
-        const float mul = wg == 0 ? p_mul : a.scale * p_mul / gain;
-        store_row<T, HALVES>(tmem + lanes + (wg == 0 ? kColAcc0 : kColAcc1), orow, a.dim, mul, key >= len);
+        const float mul = is_dk ? a.scale * p_mul / gain : p_mul;
+        const int from = (cg & 1) * 32 * HALVES;
+        store_row<T>(tmem + lanes + (is_dk ? kColAcc1 : kColAcc0), orow, from, from + 32 * HALVES, a.dim, mul, key >= len);
       }
     }
   }
@@ -481,40 +503,34 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
       const uint64_t k_rows = rows_desc(base + L::a), k_cols = cols_desc(base + L::a);
       const uint64_t v_rows = rows_desc(base + L::b);
       constexpr uint32_t step = L::tile >> 4;
-      bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3) && mbar_wait(&m.a_full[0], 0, abort_flag, a.status, 4);
-      if (ok) {
-        product_rows<BF16, HALVES>(tmem + kColS, q_rows, k_rows);
-        mma_commit(&m.s_full);
-        ok = mbar_wait(&m.b_full[0], 0, abort_flag, a.status, 5);
-      }
-      if (ok) {
-        product_rows<BF16, HALVES>(tmem + kColDP, do_rows, v_rows);
-        mma_commit(&m.dp_full);
-        mma_commit(&m.b_empty[0]);
-      }
-      for (int i = 0; ok && i < n; ++i) {
-        const int sa = i % kStagesA, sb = i % kStagesB;
-        const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesB;  // the next tiles' stages and phases
+      bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3);
+      // Order S(i+1), dQ(i-1), dP(i+1): dQ runs one pair behind, so the
+      // elementwise warps are never waited for while products are left.
+      for (int i = -1; ok && i <= n; ++i) {
+        const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesB;
         const uint32_t ph = i & 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesB) & 1;
         const bool more = i + 1 < n;
-        if (more) {  // the next S, once the elementwise warps hold this one
+        if (more) {  // S's columns are free once the elementwise warps hold S(i)
           ok = mbar_wait(&m.a_full[ta], ta_ph, abort_flag, a.status, 7) &&
-               mbar_wait(&m.s_read, ph, abort_flag, a.status, 8);
+               (i < 0 || mbar_wait(&m.s_read, ph, abort_flag, a.status, 8));
           if (!ok) break;
           tc_fence_after();
           product_rows<BF16, HALVES>(tmem + kColS, q_rows, k_rows + ta * step);
           mma_commit(&m.s_full);
         }
-        // dQ += dS K; then the next dP may take the columns dS was read from
-        if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
-        tc_fence_after();
-        product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColDP, k_cols + sa * step, i > 0);
-        mma_commit(&m.acc0_done);
-        mma_commit(&m.a_empty[sa]);
+        if (i > 0) {
+          const int sa = (i - 1) % kStagesA;
+          if (!(ok = mbar_wait(&m.ds_full[ph ^ 1], ((i - 1) >> 1) & 1, abort_flag, a.status, 9))) break;
+          tc_fence_after();
+          product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColDS2 + (ph ^ 1) * 64, k_cols + sa * step, i > 1);
+          mma_commit(&m.acc0_done[ph ^ 1]);
+          mma_commit(&m.a_empty[sa]);
+        }
         if (more) {
           ok = mbar_wait(&m.b_full[tb], tb_ph, abort_flag, a.status, 10) &&
-               mbar_wait(&m.acc0_done, ph, abort_flag, a.status, 11);
+               (i < 0 || mbar_wait(&m.dp_read, ph, abort_flag, a.status, 11));
           if (!ok) break;
+          tc_fence_after();
           product_rows<BF16, HALVES>(tmem + kColDP, do_rows, v_rows + tb * step);
           mma_commit(&m.dp_full);
           mma_commit(&m.b_empty[tb]);
@@ -525,13 +541,14 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
       mbar_wait(&m.all_done, 0, &no_abort, a.status, 12);
     }
   } else {
-    const int wg = (warp - 2) >> 2;
+    const int cg = (warp - 2) >> 2;  // column group: keys cg*32 .. +31 of a tile
     const int sub = warp & 3;
     const int row = sub * 32 + lane;
     const int query = q0 + row;
     const uint32_t lanes = static_cast<uint32_t>(sub * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + kColS + wg * 64;
-    const uint32_t dp_addr = tmem + lanes + kColDP + wg * 64;
+    const uint32_t s_addr = tmem + lanes + kColS + cg * 32;
+    const uint32_t dp_addr = tmem + lanes + kColDP + cg * 32;
+    const uint32_t ds_addr = tmem + lanes + kColDS2 + cg * 16;
     const float* stat = a.stat + (int64_t(bh) * a.q_tiles + qt) * (2 * kTile) + row;
     const float nl = stat[0], nd = stat[kTile];
     float gain = 1.f;
@@ -542,21 +559,18 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
     bool ok = true;
     for (int i = 0; i < n; ++i) {
       const uint32_t ph = i & 1;
-      const int lim = seen - i * kTile - wg * 64;  // columns from `lim` on are masked
-      const bool masked = lim < 64;
-      const uint64_t bad = lim >= 64 ? 0ull : lim <= 0 ? ~0ull : ~0ull << lim;
-      const uint32_t bad0 = static_cast<uint32_t>(bad), bad1 = static_cast<uint32_t>(bad >> 32);
+      const int lim = seen - i * kTile - cg * 32;  // columns from `lim` on are masked
+      const uint32_t bad = lim >= 32 ? 0u : lim <= 0 ? ~0u : ~0u << lim;
       if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
       tc_fence_after();
-      uint32_t v[64];
+      uint32_t v[32], w[16];
       tmem_ld32(s_addr, v);
-      tmem_ld32(s_addr + 32, v + 32);
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&m.s_read);
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
+      for (int c = 0; c < 32; c += 2) {
         float x0, x1;
         unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, nl2), x0, x1);
         v[c] = __float_as_uint(ex2(x0));
@@ -569,7 +583,7 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
         const int tid = threadIdx.x - 64;
         const int from = len - k0, rows = min(kTile, a.tk - k0) - from;
         char* tile = smem + L::a + (i % kStagesA) * L::tile;
-        for (int x = tid; x < rows * 8 * HALVES; x += 256) {
+        for (int x = tid; x < rows * 8 * HALVES; x += 32 * kElemWarps) {
           const int r = from + x / (8 * HALVES), ch = x % (8 * HALVES);
           *reinterpret_cast<uint4*>(tile + (ch >> 3) * kHalfBytes + r * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
         }
@@ -577,34 +591,39 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
       }
       if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
       tc_fence_after();
-      uint32_t w[32], d[64];
+      uint32_t d[32];
       tmem_ld32(dp_addr, d);
-      tmem_ld32(dp_addr + 32, d + 32);
       tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.dp_read);
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
+      for (int c = 0; c < 32; c += 2) {
         uint64_t p = pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
         if constexpr (!BF16) p = mul_f2(p, gain2);
         float x0, x1;
         unpack_f2(mul_f2(p, add_f2(pack_f2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), nd2)), x0, x1);
         w[c / 2] = Cvt<T>::pack2(x0, x1);
       }
-      if (masked) clear_pairs(w, bad0, bad1);
-      tmem_st32(dp_addr, w);
+      if (bad != 0u) clear_pairs(w, bad);
+      // this dS buffer is free once dQ(i-2) has read it
+      if (i > 1 && !(ok = mbar_wait(&m.acc0_done[ph], ((i >> 1) & 1) ^ 1, abort_flag, a.status, 18))) break;
+      tc_fence_after();
+      tmem_st16(ds_addr + ph * 64, w);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&m.ds_full);
+      if (lane == 0) mbar_arrive(&m.ds_full[ph]);
     }
-    char* orow = query < a.tq && (wg == 0 || n == 0) ? a.dq.row(bh, query) : nullptr;
+    char* orow = query < a.tq ? a.dq.row(bh, query) : nullptr;
     if (n == 0) {
-      if (wg == 0 && orow != nullptr) store_zero_row<T>(orow, a.dim);
-    } else if (wg == 0) {
+      if (cg == 0 && orow != nullptr) store_zero_row<T>(orow, a.dim);
+    } else if (cg < 2) {
       ok = ok && mbar_wait(&m.all_done, 0, abort_flag, a.status, 16);
       tc_fence_after();
       if (ok && !*abort_flag) {
         const float mul = BF16 ? a.scale : a.scale / (gain * (1 << kShiftP16));
-        store_row<T, HALVES>(tmem + lanes + kColAcc0, orow, a.dim, mul, seen <= 0);
+        store_row<T>(tmem + lanes + kColAcc0, orow, cg * 32 * HALVES, (cg + 1) * 32 * HALVES, a.dim, mul, seen <= 0);
       }
     }
   }
@@ -635,14 +654,17 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&m.stat_full[s], 1);
-      mbar_init(&m.stat_empty[s], 8);
+      mbar_init(&m.stat_empty[s], kElemWarps);
     }
     mbar_init(&m.s_full, 1);
-    mbar_init(&m.s_read, 8);
-    mbar_init(&m.p_full, 8);
+    mbar_init(&m.s_read, kElemWarps);
+    mbar_init(&m.p_full, kElemWarps);
     mbar_init(&m.dp_full, 1);
-    mbar_init(&m.ds_full, 8);
-    mbar_init(&m.acc0_done, 1);
+    mbar_init(&m.ds_full[0], kElemWarps);
+    mbar_init(&m.ds_full[1], kElemWarps);
+    mbar_init(&m.dp_read, kElemWarps);
+    mbar_init(&m.acc0_done[0], 1);
+    mbar_init(&m.acc0_done[1], 1);
     mbar_init(&m.acc1_done, 1);
     mbar_init(&m.all_done, 1);
     fence_barrier_init();

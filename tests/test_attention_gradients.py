@@ -215,6 +215,7 @@ CASES = [
 
 def run_case(b, h, hk, tq, tk, d, dtype, causal, lens, layout, seed=0, spread=1.0):
     import b200_pisa
+    from b200_pisa import _lib
 
     q = make(b, h, tq, d, dtype, layout, seed + 1, spread)
     k, v = (make(b, hk, tk, d, dtype, layout, seed + i, spread if i == 2 else 1.0) for i in (2, 3))
@@ -227,6 +228,7 @@ def run_case(b, h, hk, tq, tk, d, dtype, causal, lens, layout, seed=0, spread=1.
     out, lse = b200_pisa.attention_forward(q, k, v, causal=causal, key_lengths=lens_t)
     grads = b200_pisa.attention_backward(dout, q, k, v, out, lse, causal=causal, key_lengths=lens_t)
     again = b200_pisa.attention_backward(dout, q, k, v, out, lse, causal=causal, key_lengths=lens_t)
+    _lib.check_status()  # no pipeline wait ran out
     assert all(torch.equal(x, y) for x, y in zip(grads, again))
     clamped = None if lens is None else lens_t.clamp(0, tk)
     res, allow = reference(q, k, v, dout, d ** -0.5, causal, clamped)

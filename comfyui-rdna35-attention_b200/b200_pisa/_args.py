@@ -1,14 +1,28 @@
 """Argument handling shared by the rotary and the differentiable attention
-entry points: row views, device guard, output storage."""
+entry points.
+
+A call's checks depend on the shapes, strides and types of its tensors alone,
+so each entry point does them once per combination, in a cached plan that also
+holds the packed b2_view of every tensor but its base address.  What is left
+per call is the addresses, the device and the stream: about 10 us of host time
+instead of 45, which is what the smallest calls cost."""
 from __future__ import annotations
 
 import contextlib
 import functools
+import struct
 
 import torch
 
 from . import _lib
 from ._lib import LIB, check
+
+#: calls of different shapes whose plans are kept
+PLANS = 1024
+
+_VIEW_TAIL = struct.Struct("=qqqiiiiiiii")
+_POINTER = struct.Struct("=Q")
+assert _POINTER.size + _VIEW_TAIL.size == _lib.ctypes.sizeof(_lib.View)
 
 
 @functools.lru_cache(maxsize=16)
@@ -17,44 +31,79 @@ def checked_device(index: int) -> int:
     return index
 
 
+_HERE = contextlib.nullcontext()
+
+
 def on_device(x: torch.Tensor):
     """Context in which x's device is the current one (kernels launch on the
     current device; the caller's may be another)."""
     index = checked_device(x.device.index)
-    return contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+    return _HERE if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def raw_stream(x: torch.Tensor) -> int:
+    """The current stream of x's device, as cudaStream_t."""
+    return torch._C._cuda_getCurrentRawStream(x.device.index)
 
 
 def require_one_device(name: str, *tensors: torch.Tensor | None) -> None:
-    present = [t for t in tensors if t is not None]
-    first = present[0].device
-    if first.type != "cuda" or any(t.device != first for t in present):
+    first = tensors[0].device
+    if first.type != "cuda" or any(t is not None and t.device != first for t in tensors):
         raise ValueError(f"{name} requires its tensors on one CUDA device.")
 
 
-def row_strides(x: torch.Tensor) -> tuple[int, ...]:
-    """Strides of x's leading dimensions, 0 where a dimension has one entry
+def row_strides(shape, strides) -> tuple[int, ...]:
+    """Strides of the leading dimensions, 0 where a dimension has one entry
     (its stride is never used and may be anything)."""
-    return tuple(s if n > 1 else 0 for n, s in zip(x.shape[:-1], x.stride()[:-1]))
+    return tuple(s if n > 1 else 0 for n, s in zip(shape[:-1], strides[:-1]))
 
 
-def addressable(x: torch.Tensor) -> bool:
-    """Whether the 16-byte row kernels can read x in place."""
-    es = x.element_size()
-    return ((x.stride(-1) == 1 or x.shape[-1] == 1) and x.data_ptr() % 16 == 0
-            and all(s * es % 16 == 0 and s >= 0 for s in row_strides(x)))
+def addressable(shape, strides, dtype: torch.dtype) -> bool:
+    """Whether the 16-byte row kernels can read such a tensor in place, given
+    a base address on a 16-byte boundary."""
+    return ((strides[-1] == 1 or shape[-1] == 1)
+            and all(s >= 0 and s * dtype.itemsize % 16 == 0 for s in row_strides(shape, strides)))
+
+
+def repeats(shape, strides) -> bool:
+    """Whether a dimension of several entries has stride 0 (a broadcast)."""
+    return any(n > 1 and s == 0 for n, s in zip(shape, strides))
+
+
+def view_tail(shape, strides, dtype: torch.dtype) -> bytes:
+    """The packed b2_view of a [B,H,T,D] tensor without its base address."""
+    return _VIEW_TAIL.pack(*row_strides(shape, strides), *shape, _lib.dtype_code(dtype), _lib.ORDER_LINEAR, 0, 0)
+
+
+def with_base(x: torch.Tensor, tail: bytes) -> bytes:
+    """The struct whose first member is x's address."""
+    return _POINTER.pack(x.data_ptr()) + tail
 
 
 def row_view(x: torch.Tensor) -> _lib.View:
     """b2_view of a [B,H,T,D] tensor whose rows are addressable."""
-    sb, sh, st = row_strides(x)
-    batch, heads, tokens, dim = x.shape
-    return _lib.View(x.data_ptr(), sb, sh, st, batch, heads, tokens, dim, _lib.dtype_code(x.dtype), _lib.ORDER_LINEAR,
-                     0, 0)
+    return _lib.View.from_buffer_copy(with_base(x, view_tail(x.shape, x.stride(), x.dtype)))
 
 
-def token_major(x: torch.Tensor, heads: int | None = None, tokens: int | None = None) -> torch.Tensor:
-    """New [B,H,T,D] view of contiguous [B,T,H,D] storage of x's shape, type
-    and device (the layout attention and the output projection read)."""
-    batch, h, t, dim = x.shape
-    storage = torch.empty((batch, tokens or t, heads or h, dim), device=x.device, dtype=x.dtype)
-    return storage.permute(0, 2, 1, 3)
+def token_major_strides(shape) -> tuple[int, int, int, int]:
+    """Strides of a [B,H,T,D] view of contiguous [B,T,H,D] storage, the layout
+    attention and the output projection read."""
+    _, h, t, d = shape
+    return (t * h * d, d, h * d, 1)
+
+
+def new_rows(like: torch.Tensor, shape, strides) -> torch.Tensor:
+    return torch.empty_strided(shape, strides, dtype=like.dtype, device=like.device)
+
+
+def signature(x: torch.Tensor):
+    return x.shape, x.stride(), x.dtype
+
+
+def as_rows(x: torch.Tensor, broadcast: bool = True) -> torch.Tensor:
+    """x where the kernels can read it in place, else a contiguous copy.
+    broadcast: whether stride 0 can be read in place (TMA cannot)."""
+    shape, strides, dtype = signature(x)
+    if x.data_ptr() % 16 == 0 and addressable(shape, strides, dtype) and (broadcast or not repeats(shape, strides)):
+        return x
+    return x.contiguous()

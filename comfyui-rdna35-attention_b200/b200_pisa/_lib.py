@@ -76,7 +76,6 @@ class Rotary(ctypes.Structure):
     ]
 
 
-_ROTARY_P = ctypes.POINTER(Rotary)
 
 SIGNATURES: dict[str, tuple] = {
     "b2_last_error": (ctypes.c_char_p, []),
@@ -106,15 +105,14 @@ SIGNATURES: dict[str, tuple] = {
     "b2_fixed_block_attention_masked": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _F32, _I32, _VP, _I64,
                                                        _VP]),
     "b2_pack_block_bias": (ctypes.c_int, [_VP, _I32, _I64, _I64, _I64, _I32, _I32, _VP, _VP]),
-    "b2_attention_forward": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _F32, _I32, _VP, _VP, _VP]),
+    # views and b2_rotary structs of these arrive packed (bytes) or by reference
+    "b2_attention_forward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _F32, _I32, _VP, _VP, _VP]),
     "b2_attention_backward_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32]),
-    "b2_attention_backward": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VP, _VIEW_P, _VIEW_P,
-                                             _VIEW_P, _F32, _I32, _VP, _VP, _VP]),
-    "b2_axial_rope": (ctypes.c_int, [_VIEW_P, _VIEW_P, _ROTARY_P, _VP]),
-    "b2_qk_norm_rope": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VP, _VP, _I32, _F32, _ROTARY_P, _VP]),
+    "b2_attention_backward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _F32, _I32, _VP, _VP, _VP]),
+    "b2_axial_rope": (ctypes.c_int, [_VP, _VP, _VP, _VP]),
+    "b2_qk_norm_rope": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _I32, _F32, _VP, _VP]),
     "b2_qk_norm_rope_workspace_bytes": (_I64, [_I32]),
-    "b2_qk_norm_rope_backward": (ctypes.c_int, [_VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VIEW_P, _VP, _VP, _I32,
-                                                _F32, _ROTARY_P, _VP, _VP, _VP, _VP]),
+    "b2_qk_norm_rope_backward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I32, _F32, _VP, _VP, _VP, _VP, _VP]),
     "b2_pack_rows": (ctypes.c_int, [_VIEW_P, _VP, _VP]),
     "b2_unpack_rows": (ctypes.c_int, [_VP, _VIEW_P, _VP]),
     "b2_merge_epilogue": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VIEW_P, _VP]),

@@ -11,13 +11,15 @@ storage."""
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._args import addressable, on_device, require_one_device, row_strides, row_view, token_major
-from ._lib import LIB, check, ptr, stream_of
+from ._args import (PLANS, addressable, as_rows, new_rows, on_device, raw_stream, repeats, require_one_device, signature,
+                    token_major_strides, view_tail, with_base)
+from ._lib import LIB, check, ptr
 
 MAX_HEAD_DIM = 128
 _DTYPES = (torch.bfloat16, torch.float16)
@@ -26,52 +28,63 @@ _DTYPES = (torch.bfloat16, torch.float16)
 def _four(name: str, x: torch.Tensor) -> torch.Tensor:
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"{name} must be a torch tensor.")
-    if x.ndim not in (3, 4) or 0 in x.shape:
-        raise ValueError(f"{name} must be a non-empty [B,H,T,D] or [BH,T,D] tensor.")
-    return x if x.ndim == 4 else x.unsqueeze(1)
-
-
-def _in_place(x: torch.Tensor) -> torch.Tensor:
-    """x, or a copy where TMA cannot read it in place: a broadcast dimension
-    (stride 0), a strided head dimension, rows off the 16-byte boundaries."""
-    if addressable(x) and all(s > 0 for s, n in zip(row_strides(x), x.shape) if n > 1):
+    if x.ndim == 4:
         return x
-    return x.contiguous()
+    if x.ndim != 3:
+        raise ValueError(f"{name} must be a non-empty [B,H,T,D] or [BH,T,D] tensor.")
+    return x.unsqueeze(1)
 
 
-def _check_input(name: str, x: torch.Tensor) -> torch.Tensor:
-    """A checked q, k or v; expanded inputs are copied, misaligned ones refused."""
-    if not addressable(x):
-        raise ValueError(f"{name} needs a contiguous head dimension and rows that start on 16-byte boundaries.")
-    return _in_place(x)
+@functools.lru_cache(maxsize=PLANS)
+def _plan(q_sig, k_sig, v_sig, lens_sig, scale):
+    """Checks of a call's shapes, strides and types (four-dimensional)."""
+    q_shape, k_shape, dtype = q_sig[0], k_sig[0], q_sig[2]
+    for name, (shape, _, _) in (("q", q_sig), ("k", k_sig), ("v", v_sig)):
+        if 0 in shape:
+            raise ValueError(f"{name} must be a non-empty [B,H,T,D] or [BH,T,D] tensor.")
+    if k_shape != v_sig[0] or q_shape[0] != k_shape[0] or q_shape[-1] != k_shape[-1]:
+        raise ValueError("attention expects q [B,H,Tq,D] and matching k/v [B,Hk,Tk,D].")
+    if q_shape[1] % k_shape[1]:
+        raise ValueError(f"q heads ({q_shape[1]}) must be a multiple of k/v heads ({k_shape[1]}).")
+    if dtype not in _DTYPES or k_sig[2] != dtype or v_sig[2] != dtype:
+        raise ValueError("attention supports matching float16 or bfloat16 q/k/v.")
+    if q_shape[-1] > MAX_HEAD_DIM or q_shape[-1] % 8:
+        raise ValueError(f"attention supports D <= {MAX_HEAD_DIM}, a multiple of 8.")
+    if lens_sig is not None and lens_sig != ((q_shape[0],), (1,), torch.int32):
+        raise ValueError(f"key_lengths must be a contiguous int32 [B] tensor, B={q_shape[0]}.")
+    scale = float(q_shape[-1] ** -0.5 if scale is None else scale)
+    if not 0.0 < ctypes.c_float(scale).value < math.inf:
+        raise ValueError("scale must be representable as a positive finite float32 value.")
+    for name, sig in (("q", q_sig), ("k", k_sig), ("v", v_sig)):
+        if not addressable(*sig):
+            raise ValueError(f"{name} needs a contiguous head dimension and rows that start on 16-byte boundaries.")
+    q_strides, k_strides = token_major_strides(q_shape), token_major_strides(k_shape)
+    return (scale, any(repeats(*sig[:2]) for sig in (q_sig, k_sig, v_sig)),
+            (view_tail(*q_sig), view_tail(*k_sig), view_tail(*v_sig)),
+            (q_strides, k_strides), (view_tail(q_shape, q_strides, dtype), view_tail(k_shape, k_strides, dtype)))
 
 
-def _check_call(q, k, v, scale, key_lengths):
-    """Checked four-dimensional (q, k, v) and the scale."""
+def _planned(q, k, v, scale, key_lengths):
+    """Checked four-dimensional (q, k, v) and their plan; expanded inputs
+    (stride 0) are copied, which TMA cannot read."""
     if len({x.ndim for x in (q, k, v) if isinstance(x, torch.Tensor)}) > 1:
         raise ValueError("q, k and v must have the same rank.")
     q, k, v = _four("q", q), _four("k", k), _four("v", v)
-    if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[-1] != k.shape[-1]:
-        raise ValueError("attention expects q [B,H,Tq,D] and matching k/v [B,Hk,Tk,D].")
-    if q.shape[1] % k.shape[1]:
-        raise ValueError(f"q heads ({q.shape[1]}) must be a multiple of k/v heads ({k.shape[1]}).")
-    if q.dtype not in _DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError("attention supports matching float16 or bfloat16 q/k/v.")
-    if q.shape[-1] > MAX_HEAD_DIM or q.shape[-1] % 8:
-        raise ValueError(f"attention supports D <= {MAX_HEAD_DIM}, a multiple of 8.")
+    lens_sig = None
     if key_lengths is not None:
         if not isinstance(key_lengths, torch.Tensor):
             raise TypeError("key_lengths must be a torch tensor or None.")
-        if key_lengths.shape != (q.shape[0],) or key_lengths.dtype != torch.int32 or not key_lengths.is_contiguous():
-            raise ValueError(f"key_lengths must be a contiguous int32 [B] tensor, B={q.shape[0]}.")
-    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
-    if not 0.0 < ctypes.c_float(scale).value < math.inf:
-        raise ValueError("scale must be representable as a positive finite float32 value.")
-    return _check_input("q", q), _check_input("k", k), _check_input("v", v), scale
-
-
-def _like_rank(x: torch.Tensor, rank: int) -> torch.Tensor:
-    return x if rank == 4 else x.squeeze(1)
+        shape, strides, dtype = signature(key_lengths)
+        lens_sig = (tuple(shape), strides if shape != (1,) else (1,), dtype)
+    scale = None if scale is None else float(scale)
+    plan = _plan(signature(q), signature(k), signature(v), lens_sig, scale)
+    for name, x in (("q", q), ("k", k), ("v", v)):
+        if x.data_ptr() % 16:
+            raise ValueError(f"{name} needs a contiguous head dimension and rows that start on 16-byte boundaries.")
+    if plan[1]:
+        q, k, v = (as_rows(x, broadcast=False) for x in (q, k, v))
+        plan = _plan(signature(q), signature(k), signature(v), lens_sig, scale)
+    return q, k, v, plan
 
 
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None, *,
@@ -81,16 +94,16 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
     [B] on the device, batch b attends to its first key_lengths[b] keys (what
     the K/V rows past them hold does not matter).  causal: query i sees keys
     up to i + Tk - Tq.  A query that sees no key gives out 0 and lse -inf."""
-    rank = q.ndim if isinstance(q, torch.Tensor) else 0
-    q, k, v, scale = _check_call(q, k, v, scale, key_lengths)
+    flat = isinstance(q, torch.Tensor) and q.ndim == 3
+    q, k, v, (scale, _, tails, strides, out_tails) = _planned(q, k, v, scale, key_lengths)
     require_one_device("attention", q, k, v, key_lengths)
     with on_device(q):
-        out = token_major(q)
+        out = new_rows(q, q.shape, strides[0])
         lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32)
-        check(LIB.b2_attention_forward(ctypes.byref(row_view(q)), ctypes.byref(row_view(k)), ctypes.byref(row_view(v)),
-                                       ctypes.byref(row_view(out)), scale, int(bool(causal)), ptr(key_lengths), ptr(lse),
-                                       stream_of(q)))
-    return _like_rank(out, rank), _like_rank(lse, rank)
+        check(LIB.b2_attention_forward(with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]),
+                                       with_base(out, out_tails[0]), scale, 1 if causal else 0, ptr(key_lengths), ptr(lse),
+                                       raw_stream(q)))
+    return (out.squeeze(1), lse.squeeze(1)) if flat else (out, lse)
 
 
 def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
@@ -100,26 +113,28 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     and what it returned.  Probabilities are recomputed from lse; dk and dv of
     a shared head are summed over its group in FP32; rows of dk and dv past a
     batch's keys are 0.  Bit-reproducible."""
-    rank = q.ndim if isinstance(q, torch.Tensor) else 0
-    q, k, v, scale = _check_call(q, k, v, scale, key_lengths)
+    flat = isinstance(q, torch.Tensor) and q.ndim == 3
+    q, k, v, (scale, _, tails, strides, grad_tails) = _planned(q, k, v, scale, key_lengths)
     out, dout = _four("out", out), _four("dout", dout)
     for name, x in (("out", out), ("dout", dout)):
         if x.shape != q.shape or x.dtype != q.dtype:
             raise ValueError(f"{name} must have q's shape and dtype.")
-    if not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32 or lse.numel() != math.prod(q.shape[:3]) \
-            or lse.shape != (q.shape[:3] if rank == 4 else (q.shape[0], q.shape[2])):
+    batch, heads, tokens, _ = q.shape
+    if not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32 \
+            or lse.shape != ((batch, tokens) if flat else (batch, heads, tokens)):
         raise ValueError("lse must be attention_forward's float32 [B,H,Tq] tensor.")
-    require_one_device("attention_backward", q, k, v, out, dout, lse, key_lengths)
-    out, dout, lse = _in_place(out), _in_place(dout), lse.contiguous()
+    require_one_device("attention_backward", q, k, v, key_lengths, out, dout, lse)
     with on_device(q):
-        dq, dk, dv = token_major(q), token_major(k), token_major(v)
-        ws = torch.empty(LIB.b2_attention_backward_workspace_bytes(q.shape[0], q.shape[1], k.shape[1], q.shape[2]),
-                         device=q.device, dtype=torch.uint8)
-        views = [ctypes.byref(row_view(x)) for x in (q, k, v, out, dout)]
-        grads = [ctypes.byref(row_view(x)) for x in (dq, dk, dv)]
-        check(LIB.b2_attention_backward(*views, ptr(lse), *grads, scale, int(bool(causal)), ptr(key_lengths), ptr(ws),
-                                        stream_of(q)))
-    return _like_rank(dq, rank), _like_rank(dk, rank), _like_rank(dv, rank)
+        out, dout, lse = as_rows(out, broadcast=False), as_rows(dout, broadcast=False), lse.contiguous()
+        dq, dk, dv = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1]), new_rows(k, k.shape, strides[1])
+        ws = torch.empty(LIB.b2_attention_backward_workspace_bytes(batch, heads, k.shape[1], tokens), device=q.device,
+                         dtype=torch.uint8)
+        check(LIB.b2_attention_backward(
+            with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]),
+            with_base(out, view_tail(*signature(out))), with_base(dout, view_tail(*signature(dout))), ptr(lse),
+            with_base(dq, grad_tails[0]), with_base(dk, grad_tails[1]), with_base(dv, grad_tails[1]), scale,
+            1 if causal else 0, ptr(key_lengths), ptr(ws), raw_stream(q)))
+    return (dq.squeeze(1), dk.squeeze(1), dv.squeeze(1)) if flat else (dq, dk, dv)
 
 
 class _Attention(torch.autograd.Function):

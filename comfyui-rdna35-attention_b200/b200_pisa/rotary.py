@@ -7,68 +7,95 @@ contiguous [B,T,H,D] storage, which the attention entry points read in place.
 """
 from __future__ import annotations
 
-import ctypes
+import functools
 import math
+import operator
+import struct
 from collections.abc import Sequence
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._args import addressable, on_device, require_one_device, row_view, token_major
-from ._lib import LIB, check, ptr, stream_of
+from ._args import (PLANS, addressable, as_rows, new_rows, on_device, raw_stream, require_one_device, signature,
+                    token_major_strides, view_tail, with_base)
+from ._lib import LIB, check, ptr
 
 MAX_ROTARY_DIM = 256
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _POS_CODES = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float32: _lib.POS_F32,
               torch.float64: _lib.POS_F64}
+_ROTARY_TAIL = struct.Struct("=qqqii4iii4d")
+assert 8 + _ROTARY_TAIL.size == _lib.ctypes.sizeof(_lib.Rotary)
 
 
-def _check_rows(name: str, x: torch.Tensor) -> None:
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"{name} must be a torch tensor.")
-    if x.ndim != 4 or 0 in x.shape:
+def _check_rows(name: str, shape, strides, dtype) -> None:
+    if len(shape) != 4 or 0 in shape:
         raise ValueError(f"{name} must be a non-empty [B,H,T,D] tensor.")
-    if x.dtype not in _DTYPES:
+    if dtype not in _DTYPES:
         raise ValueError(f"{name} must be bfloat16, float16 or float32.")
-    if x.shape[-1] > MAX_ROTARY_DIM or x.shape[-1] % 8:
+    if shape[-1] > MAX_ROTARY_DIM or shape[-1] % 8:
         raise ValueError(f"rotary positions support D <= {MAX_ROTARY_DIM}, a multiple of 8.")
-    if not addressable(x):
+    if not addressable(shape, strides, dtype):
         raise ValueError(f"{name} needs a contiguous head dimension and rows that start on 16-byte boundaries.")
 
 
-def _rotary(x: torch.Tensor, positions: torch.Tensor, axes_dims: Sequence[int], theta, interleaved: bool,
-            inverse: bool) -> _lib.Rotary:
-    """Checked b2_rotary of the call; the caller keeps ``positions`` alive."""
-    if not isinstance(positions, torch.Tensor):
-        raise TypeError("positions must be a torch tensor.")
-    dims = [int(d) for d in axes_dims]
-    if not 1 <= len(dims) <= _lib.MAX_AXES or any(d <= 0 or d % 2 for d in dims) or sum(dims) > x.shape[-1]:
-        raise ValueError(f"axes_dims must be 1..{_lib.MAX_AXES} positive even sizes that sum to at most D={x.shape[-1]}.")
-    thetas = [float(t) for t in theta] if isinstance(theta, Sequence) else [float(theta)] * len(dims)
+def _check_tensors(**tensors) -> None:
+    """What a plan cannot know: that these are tensors, and their addresses."""
+    for name, x in tensors.items():
+        if not isinstance(x, torch.Tensor):
+            raise TypeError(f"{name} must be a torch tensor.")
+        if name != "positions" and x.data_ptr() % 16:
+            raise ValueError(f"{name} needs a contiguous head dimension and rows that start on 16-byte boundaries.")
+
+
+def _rotary_tail(shape, pos_sig, axes_dims, theta, interleaved: bool, inverse: bool) -> bytes:
+    """The checked b2_rotary of a call without the positions' address."""
+    dims = list(axes_dims)
+    if not 1 <= len(dims) <= _lib.MAX_AXES or any(d <= 0 or d % 2 for d in dims) or sum(dims) > shape[-1]:
+        raise ValueError(f"axes_dims must be 1..{_lib.MAX_AXES} positive even sizes that sum to at most D={shape[-1]}.")
+    thetas = list(theta) if isinstance(theta, tuple) else [theta] * len(dims)
     if len(thetas) != len(dims) or not all(0.0 < t < math.inf for t in thetas):
         raise ValueError("theta must be one positive number, or one for each axis.")
-    batch, _, tokens, _ = x.shape
-    if positions.dtype not in _POS_CODES:
+    batch, _, tokens, _ = shape
+    pos_shape, strides, dtype = pos_sig
+    if dtype not in _POS_CODES:
         raise ValueError("positions must be int32, int64, float32 or float64.")
+    if tuple(pos_shape) not in ((tokens, len(dims)), (batch, tokens, len(dims))):
+        raise ValueError(f"positions must be [T,{len(dims)}] or [B,T,{len(dims)}] with B={batch}, T={tokens}.")
+    strides = strides if len(strides) == 3 else (0, *strides)
+    pad = [0] * (_lib.MAX_AXES - len(dims))
+    return _ROTARY_TAIL.pack(*strides, _POS_CODES[dtype], len(dims), *dims, *pad, interleaved, inverse, *thetas, *pad)
+
+
+def _hashable(axes_dims, theta):
+    """The rotation's sizes and rates as plain numbers, for the plan's key."""
+    theta = tuple(float(t) for t in theta) if isinstance(theta, Sequence) else float(theta)
+    return tuple(operator.index(d) for d in axes_dims), theta
+
+
+@functools.lru_cache(maxsize=PLANS)
+def _rope_plan(sig, pos_sig, axes_dims, theta, interleaved, inverse):
+    _check_rows("x", *sig)
+    shape, _, dtype = sig
+    out_strides = token_major_strides(shape)
+    return (_rotary_tail(shape, pos_sig, axes_dims, theta, interleaved, inverse), view_tail(*sig),
+            view_tail(shape, out_strides, dtype), out_strides)
+
+
+def _no_position_gradient(positions) -> None:
     if positions.requires_grad:
         raise ValueError("positions have no gradient here; detach them.")
-    if tuple(positions.shape) not in ((tokens, len(dims)), (batch, tokens, len(dims))):
-        raise ValueError(f"positions must be [T,{len(dims)}] or [B,T,{len(dims)}] with B={batch}, T={tokens}.")
-    sb, st, sa = positions.stride() if positions.ndim == 3 else (0, *positions.stride())
-    rot = _lib.Rotary(positions.data_ptr(), sb, st, sa, _POS_CODES[positions.dtype], len(dims))
-    rot.axes_dims[:len(dims)] = dims
-    rot.theta[:len(dims)] = thetas
-    rot.interleaved, rot.inverse = int(bool(interleaved)), int(bool(inverse))
-    return rot
 
 
 def _rope_call(x: torch.Tensor, positions: torch.Tensor, axes_dims, theta, interleaved, inverse) -> torch.Tensor:
-    rot = _rotary(x, positions, axes_dims, theta, interleaved, inverse)
+    _check_tensors(x=x, positions=positions)
+    _no_position_gradient(positions)
+    rot, tail, out_tail, out_strides = _rope_plan(signature(x), signature(positions), axes_dims, theta, interleaved, inverse)
     require_one_device("axial_rope", x, positions)
     with on_device(x):
-        out = token_major(x)
-        check(LIB.b2_axial_rope(ctypes.byref(row_view(x)), ctypes.byref(row_view(out)), ctypes.byref(rot), stream_of(x)))
+        out = new_rows(x, x.shape, out_strides)
+        check(LIB.b2_axial_rope(with_base(x, tail), with_base(out, out_tail), with_base(positions, rot), raw_stream(x)))
     return out
 
 
@@ -84,8 +111,7 @@ class _AxialRope(torch.autograd.Function):
     def backward(ctx, dy):
         axes_dims, theta, interleaved, inverse = ctx.rotation
         (positions,) = ctx.saved_tensors
-        dy = dy if addressable(dy) else dy.contiguous()
-        return _rope_call(dy, positions, axes_dims, theta, interleaved, not inverse), None, None, None, None, None
+        return _rope_call(as_rows(dy), positions, axes_dims, theta, interleaved, not inverse), None, None, None, None, None
 
 
 def axial_rope(x: torch.Tensor, positions: torch.Tensor, axes_dims: Sequence[int], *, theta=10000.0,
@@ -100,52 +126,63 @@ def axial_rope(x: torch.Tensor, positions: torch.Tensor, axes_dims: Sequence[int
     (p, p + R/2).  inverse rotates back.  Angles are reduced in FP64, so far
     positions keep their accuracy; the result is rounded once to x's type.
     Differentiable in x."""
-    _check_rows("x", x)
-    rotation = (tuple(axes_dims), theta, interleaved, inverse)
-    if torch.is_grad_enabled() and x.requires_grad:
+    rotation = (*_hashable(axes_dims, theta), bool(interleaved), bool(inverse))
+    if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
         return _AxialRope.apply(x, positions, *rotation)
     return _rope_call(x, positions, *rotation)
 
 
-def _check_weight(name: str, w: torch.Tensor | None, x: torch.Tensor) -> None:
-    if w is None:
+def _check_weight(name: str, sig, dim: int) -> None:
+    if sig is None:
         return
-    if not isinstance(w, torch.Tensor):
-        raise TypeError(f"{name} must be a torch tensor or None.")
-    if w.shape != (x.shape[-1],) or w.dtype not in _DTYPES:
-        raise ValueError(f"{name} must be a [D] bfloat16, float16 or float32 tensor, D={x.shape[-1]}.")
-    if w.stride(0) != 1:
+    shape, strides, dtype = sig
+    if tuple(shape) != (dim,) or dtype not in _DTYPES:
+        raise ValueError(f"{name} must be a [D] bfloat16, float16 or float32 tensor, D={dim}.")
+    if strides[0] != 1:
         raise ValueError(f"{name} must be contiguous.")
 
 
-def _check_qk(q, k, q_weight, k_weight, eps) -> float:
-    _check_rows("q", q)
-    _check_rows("k", k)
-    if q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:] or q.dtype != k.dtype:
+@functools.lru_cache(maxsize=PLANS)
+def _qk_plan(q_sig, k_sig, wq_sig, wk_sig, pos_sig, axes_dims, eps, theta, interleaved):
+    _check_rows("q", *q_sig)
+    _check_rows("k", *k_sig)
+    q_shape, k_shape, dtype = q_sig[0], k_sig[0], q_sig[2]
+    if q_shape[0] != k_shape[0] or q_shape[2:] != k_shape[2:] or dtype != k_sig[2]:
         raise ValueError("q and k must share B, T, D and dtype (head counts may differ).")
-    _check_weight("q_weight", q_weight, q)
-    _check_weight("k_weight", k_weight, k)
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+    _check_weight("q_weight", wq_sig, q_shape[-1])
+    _check_weight("k_weight", wk_sig, q_shape[-1])
+    if wq_sig is not None and wk_sig is not None and wq_sig[2] != wk_sig[2]:
         raise ValueError("q_weight and k_weight must share one dtype.")
-    eps = float(eps)
     if not 0.0 <= eps < math.inf:
         raise ValueError("eps must be a finite number >= 0.")
-    return eps
+    weight = wq_sig or wk_sig
+    strides = tuple(token_major_strides(s) for s in (q_shape, k_shape))
+    return (_rotary_tail(q_shape, pos_sig, axes_dims, theta, interleaved, False),
+            (view_tail(*q_sig), view_tail(*k_sig)),
+            tuple(view_tail(s, st, dtype) for s, st in zip((q_shape, k_shape), strides)), strides,
+            _lib.B2_F32 if weight is None else _lib.dtype_code(weight[2]))
 
 
-def _weight_code(q_weight, k_weight) -> int:
-    w = q_weight if q_weight is not None else k_weight
-    return _lib.B2_F32 if w is None else _lib.dtype_code(w.dtype)
+def _plan_of(q, k, q_weight, k_weight, positions, axes_dims, eps, theta, interleaved):
+    _check_tensors(q=q, k=k, positions=positions)
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and not isinstance(w, torch.Tensor):
+            raise TypeError(f"{name} must be a torch tensor or None.")
+    _no_position_gradient(positions)
+    return _qk_plan(signature(q), signature(k), None if q_weight is None else signature(q_weight),
+                    None if k_weight is None else signature(k_weight), signature(positions), axes_dims, eps, theta,
+                    interleaved)
 
 
 def _norm_rope_call(q, k, q_weight, k_weight, positions, axes_dims, eps, theta, interleaved):
-    rot = _rotary(q, positions, axes_dims, theta, interleaved, False)
+    rot, tails, out_tails, strides, w_code = _plan_of(q, k, q_weight, k_weight, positions, axes_dims, eps, theta,
+                                                      interleaved)
     require_one_device("qk_norm_rope", q, k, q_weight, k_weight, positions)
     with on_device(q):
-        q_out, k_out = token_major(q), token_major(k)
-        check(LIB.b2_qk_norm_rope(ctypes.byref(row_view(q)), ctypes.byref(row_view(k)), ctypes.byref(row_view(q_out)),
-                                  ctypes.byref(row_view(k_out)), ptr(q_weight), ptr(k_weight),
-                                  _weight_code(q_weight, k_weight), eps, ctypes.byref(rot), stream_of(q)))
+        q_out, k_out = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1])
+        check(LIB.b2_qk_norm_rope(with_base(q, tails[0]), with_base(k, tails[1]), with_base(q_out, out_tails[0]),
+                                  with_base(k_out, out_tails[1]), ptr(q_weight), ptr(k_weight), w_code, eps,
+                                  with_base(positions, rot), raw_stream(q)))
     return q_out, k_out
 
 
@@ -157,22 +194,25 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     k_weight_grad) from the gradients of its two outputs; the weights' are
     None without weights or with weight_grads=False.  The statistics are
     recomputed from q and k.  Bit-reproducible."""
-    eps = _check_qk(q, k, q_weight, k_weight, eps)
+    axes_dims, theta = _hashable(axes_dims, theta)
+    rot, tails, out_tails, strides, w_code = _plan_of(q, k, q_weight, k_weight, positions, axes_dims, float(eps), theta,
+                                                      bool(interleaved))
     for name, dy, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
         if not isinstance(dy, torch.Tensor) or dy.shape != x.shape or dy.dtype != x.dtype:
             raise ValueError(f"{name} must be a tensor of its output's shape and dtype.")
-    rot = _rotary(q, positions, axes_dims, theta, interleaved, False)
-    require_one_device("qk_norm_rope_backward", q, k, dq_out, dk_out, q_weight, k_weight, positions)
-    dq_out, dk_out = (x if addressable(x) else x.contiguous() for x in (dq_out, dk_out))
+    require_one_device("qk_norm_rope_backward", q, k, q_weight, k_weight, positions, dq_out, dk_out)
     with on_device(q):
-        dq, dk = token_major(q), token_major(k)
+        dq_out, dk_out = as_rows(dq_out), as_rows(dk_out)
+        dq, dk = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1])
         dwq, dwk = (torch.empty_like(w) if w is not None and weight_grads else None for w in (q_weight, k_weight))
         ws = None
         if dwq is not None or dwk is not None:
             ws = torch.empty(LIB.b2_qk_norm_rope_workspace_bytes(q.shape[-1]), device=q.device, dtype=torch.uint8)
-        views = [ctypes.byref(row_view(x)) for x in (q, k, dq_out, dk_out, dq, dk)]
-        check(LIB.b2_qk_norm_rope_backward(*views, ptr(q_weight), ptr(k_weight), _weight_code(q_weight, k_weight), eps,
-                                           ctypes.byref(rot), ptr(dwq), ptr(dwk), ptr(ws), stream_of(q)))
+        check(LIB.b2_qk_norm_rope_backward(
+            with_base(q, tails[0]), with_base(k, tails[1]), with_base(dq_out, view_tail(*signature(dq_out))),
+            with_base(dk_out, view_tail(*signature(dk_out))), with_base(dq, out_tails[0]), with_base(dk, out_tails[1]),
+            ptr(q_weight), ptr(k_weight), w_code, float(eps), with_base(positions, rot), ptr(dwq), ptr(dwk), ptr(ws),
+            raw_stream(q)))
     return dq, dk, dwq, dwk
 
 
@@ -198,9 +238,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     its weight [D] (None for none) and rotate it by the tokens' positions
     (``axial_rope``), in one launch with one rounding at the end.
     Differentiable in q, k and the weights."""
-    eps = _check_qk(q, k, q_weight, k_weight, eps)
-    args = (q, k, q_weight, k_weight, positions, tuple(axes_dims), eps, theta, interleaved)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
+    axes_dims, theta = _hashable(axes_dims, theta)
+    args = (q, k, q_weight, k_weight, positions, axes_dims, float(eps), theta, bool(interleaved))
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args[:4]):
         return _QkNormRope.apply(*args)
     return _norm_rope_call(*args)
 

@@ -25,6 +25,7 @@
 // shared memory (one sincospif per thread for H = 16, D = 128) and every group
 // then walks heads of one token, four rows in flight.
 #include <math.h>
+#include <string.h>
 
 #include "kernels.h"
 
@@ -460,6 +461,35 @@ RowSet rows_of(const b2_view* v) {
   return RowSet{static_cast<char*>(v->base), v->stride_b, v->stride_h, v->stride_t};
 }
 
+// Turns per position and axis of every pair.  The last rotation's are kept
+// per thread (64 calls of pow are 2.5 us of host time for D = 128).
+struct Rates {
+  int n_axes = 0;
+  int32_t dims[B2_MAX_AXES];
+  double theta[B2_MAX_AXES];
+  int pairs;
+  double turn[kMaxPairs];
+  uint8_t axis[kMaxPairs];
+};
+
+const Rates& rates_of(const b2_rotary& r) {
+  static thread_local Rates k;
+  bool same = k.n_axes == r.n_axes;
+  for (int i = 0; same && i < r.n_axes; ++i) same = k.dims[i] == r.axes_dims[i] && k.theta[i] == r.theta[i];
+  if (same) return k;
+  k.n_axes = r.n_axes;
+  k.pairs = 0;
+  for (int x = 0; x < r.n_axes; ++x) {
+    k.dims[x] = r.axes_dims[x];
+    k.theta[x] = r.theta[x];
+    for (int j = 0; j < r.axes_dims[x] / 2; ++j, ++k.pairs) {
+      k.turn[k.pairs] = pow(r.theta[x], -2.0 * j / r.axes_dims[x]) / 6.283185307179586476925286766559;
+      k.axis[k.pairs] = static_cast<uint8_t>(x);
+    }
+  }
+  return k;
+}
+
 template <typename T>
 cudaError_t launch_typed(const RotaryArgs& a, int layout, bool norm, bool grad, int sides, int64_t tiles,
                          cudaStream_t st) {
@@ -514,14 +544,10 @@ cudaError_t launch_rotary(const RotaryCall& c, cudaStream_t st) {
   a.w_dtype = c.w_dtype;
   a.eps = c.eps;
   a.partial = c.partial;
-  int p = 0;
-  for (int x = 0; x < c.rot->n_axes; ++x) {
-    const int d = c.rot->axes_dims[x];
-    for (int j = 0; j < d / 2; ++j, ++p) {
-      a.turn[p] = pow(c.rot->theta[x], -2.0 * j / d) / 6.283185307179586476925286766559;
-      a.axis[p] = static_cast<uint8_t>(x);
-    }
-  }
+  const Rates& rates = rates_of(*c.rot);
+  const int p = rates.pairs;
+  memcpy(a.turn, rates.turn, sizeof(double) * p);
+  memcpy(a.axis, rates.axis, p);
   a.rot_pairs = p;
   // halves of fewer than four aligned pairs a lane (R % 8 != 0) go pair by pair
   const int layout = a.interleaved ? kInterleaved : (p % 4 == 0 ? kHalves : kScalar);

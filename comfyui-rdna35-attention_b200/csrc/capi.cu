@@ -830,6 +830,7 @@ int check_rotary_view(const b2_view* v, const char* name, const b2_view* like) {
   if (v->order != B2_ORDER_LINEAR) return fail(B2_ERR_UNSUPPORTED, "%s must be in linear token order", name);
   if (v->head_dim > 256 || v->head_dim % 8)
     return fail(B2_ERR_UNSUPPORTED, "rotary positions support D <= 256, a multiple of 8");
+  if (int64_t(v->batch) * v->tokens > (1 << 30)) return fail(B2_ERR_UNSUPPORTED, "%s has more than 2^30 tokens", name);
   if (like != nullptr && (!same_bht(v, like) || v->dtype != like->dtype))
     return fail(B2_ERR_INVALID, "%s must have its input's [B,H,T,D] and dtype", name);
   return B2_OK;

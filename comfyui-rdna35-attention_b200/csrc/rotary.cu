@@ -20,10 +20,11 @@
 //
 // Layout: a group of G lanes owns a row, each lane four pairs (G = 16 for
 // D = 128), so a 16-bit row moves with one 16-byte access a lane (interleaved
-// pairs) or two of 8 bytes (halves).  A block takes `tt` tokens of one side
-// (queries or keys); its 256 threads compute the tokens' cos / sin once into
-// shared memory (one sincospif per thread for H = 16, D = 128) and every group
-// then walks heads of one token, four rows in flight.
+// pairs) or two of 8 bytes (halves).  A block takes `tt` tokens; its 256
+// threads compute the tokens' cos / sin once into shared memory (one
+// sincospif per thread for 16 + 16 heads, D = 128) while the first rows are on
+// their way; every group then walks heads of one token, query heads first,
+// four rows in flight.
 #include <math.h>
 #include <string.h>
 
@@ -36,9 +37,27 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 128;     // D <= 256
 constexpr int kMaxTokens = 16;     // tokens of a block
-constexpr int kGradBlocks = 148 * 4;  // blocks of one side in the backward pass: partial weight gradients
+// Blocks of the forward pass: four on an SM, which stride over the tiles.
+constexpr int kBlocks = 148 * 4;
+// Blocks of one side in the backward pass (two sides fill the SMs with three
+// blocks each), and so partial weight gradients.
+constexpr int kGradBlocks = 222;
 
 enum Layout { kInterleaved = 0, kHalves = 1, kScalar = 2 };
+
+// Rows are read once: leave L1 alone.
+__device__ __forceinline__ uint4 load16(const char* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 load8(const char* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
 
 struct RowSet {
   char* base;
@@ -57,6 +76,7 @@ struct RotaryArgs {
   const void* pos;
   int64_t pb, pt, pa;
   int pos_dtype;
+  int sides;
   int batch, tokens, dim;
   int rot_pairs;    // rotated pairs; pairs past them pass through
   int interleaved;  // used by the scalar layout
@@ -70,12 +90,8 @@ struct RotaryArgs {
   uint8_t axis[kMaxPairs];
 };
 
-__device__ __forceinline__ char* row_ptr(const RowSet& r, int64_t b, int h, int64_t t, int es) {
-  return r.base + (b * r.sb + int64_t(h) * r.sh + t * r.st) * es;
-}
-
-__device__ __forceinline__ double position(const RotaryArgs& a, int64_t b, int64_t t, int axis) {
-  const int64_t i = b * a.pb + t * a.pt + int64_t(axis) * a.pa;
+__device__ __forceinline__ double position(const RotaryArgs& a, int b, int t, int axis) {
+  const int64_t i = int64_t(b) * a.pb + int64_t(t) * a.pt + int64_t(axis) * a.pa;
   switch (a.pos_dtype) {
     case B2_POS_I32: return static_cast<double>(static_cast<const int32_t*>(a.pos)[i]);
     case B2_POS_I64: return static_cast<double>(static_cast<const int64_t*>(a.pos)[i]);
@@ -130,15 +146,15 @@ struct Raw {
         }
       }
     } else if constexpr (sizeof(T) == 4) {
-      const uint4 a = *reinterpret_cast<const uint4*>(row + c0 * 4);
-      const uint4 b = *reinterpret_cast<const uint4*>(row + c1 * 4);
+      const uint4 a = load16(row + c0 * 4);
+      const uint4 b = load16(row + c1 * 4);
       w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
     } else if constexpr (LAYOUT == kInterleaved) {
-      const uint4 a = *reinterpret_cast<const uint4*>(row + c0 * 2);
+      const uint4 a = load16(row + c0 * 2);
       w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
     } else {
-      const uint2 a = *reinterpret_cast<const uint2*>(row + c0 * 2);
-      const uint2 b = *reinterpret_cast<const uint2*>(row + c1 * 2);
+      const uint2 a = load8(row + c0 * 2);
+      const uint2 b = load8(row + c1 * 2);
       w[0] = a.x, w[1] = a.y, w[2] = b.x, w[3] = b.y;
     }
   }
@@ -204,15 +220,16 @@ __device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
   return __half2float(static_cast<const __half*>(w)[i]);
 }
 
-// cos / sin of the block's tokens: cs[token][pair].
-__device__ __forceinline__ void fill_angles(const RotaryArgs& a, float2* cs, int64_t n0, int tt, int64_t n_tokens) {
-  for (int i = threadIdx.x; i < tt * a.rot_pairs; i += kThreads) {
-    const int tok = i / a.rot_pairs;
+// cos / sin of a tile's tokens: cs[token][pair].
+__device__ __forceinline__ void fill_angles(const RotaryArgs& a, float2* cs, int n0, int n_tokens) {
+  const int b0 = n0 / a.tokens, t0 = n0 - b0 * a.tokens;
+  const int count = min(1 << a.tt_log2, n_tokens - n0) * a.rot_pairs;
+  for (int i = threadIdx.x; i < count; i += kThreads) {
+    const int tok = static_cast<int>(static_cast<unsigned>(i) / static_cast<unsigned>(a.rot_pairs));
     const int p = i - tok * a.rot_pairs;
-    const int64_t n = n0 + tok;
-    if (n >= n_tokens) break;
-    const int64_t b = n / a.tokens;
-    double turns = position(a, b, n - b * a.tokens, a.axis[p]) * a.turn[p];
+    int b = b0, at = t0 + tok;
+    while (at >= a.tokens) at -= a.tokens, ++b;  // a tile may span batches
+    double turns = position(a, b, at, a.axis[p]) * a.turn[p];
     turns -= rint(turns);
     float s, c;
     sincospif(2.0f * static_cast<float>(turns), &s, &c);
@@ -221,9 +238,10 @@ __device__ __forceinline__ void fill_angles(const RotaryArgs& a, float2* cs, int
 }
 
 struct Lane {
-  int l, tok, gi, gpt;  // lane in its group, token of the block, group among the token's, groups per token
+  int l, tok, gi, gpt, gpt_log2;  // lane in its group, token of the block, group among the token's, groups per token
   int c0, c1;
   bool active;          // the lane's pairs exist
+  bool rotates;         // and are rotated (vector layouts)
 };
 
 template <int LAYOUT>
@@ -231,15 +249,17 @@ __device__ __forceinline__ Lane lane_of(const RotaryArgs& a) {
   Lane t;
   const int g = threadIdx.x >> a.group_log2;
   t.l = threadIdx.x & ((1 << a.group_log2) - 1);
-  const int gpt_log2 = 8 - a.group_log2 - a.tt_log2;
-  t.gpt = 1 << gpt_log2;
+  t.gpt_log2 = 8 - a.group_log2 - a.tt_log2;
+  t.gpt = 1 << t.gpt_log2;
   t.gi = g & (t.gpt - 1);
-  t.tok = g >> gpt_log2;
+  t.tok = g >> t.gpt_log2;
   t.active = LAYOUT == kScalar ? true : 8 * t.l < a.dim;
+  t.rotates = 4 * t.l < a.rot_pairs;
   chunks<LAYOUT>(t.l, a.rot_pairs, t.c0, t.c1);
   return t;
 }
 
+// cos and sin of a lane's pairs, (1, 0) for those that pass through.
 template <int LAYOUT>
 __device__ __forceinline__ void load_angles(const RotaryArgs& a, const float2* cs, const Lane& t, float2 (&ang)[4]) {
 #pragma unroll
@@ -249,165 +269,210 @@ __device__ __forceinline__ void load_angles(const RotaryArgs& a, const float2* c
   }
 }
 
+// The sides' weights in the order of the lanes' pairs: ws[side][8 l + 2 i + m].
 template <int LAYOUT>
-__device__ __forceinline__ void load_weights(const RotaryArgs& a, const Side& s, const Lane& t, float (&w)[8]) {
-  const int pairs = a.dim >> 1;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const int p = pair_of<LAYOUT>(t.l, i);
-      w[2 * i + m] =
-          s.w != nullptr && p < pairs
-              ? weight_at(s.w, a.w_dtype, element<LAYOUT>(p, m, a.rot_pairs, a.interleaved != 0))
-              : 1.f;
-    }
+__device__ __forceinline__ void fill_weights(const RotaryArgs& a, int side, float* ws) {
+  const int l = threadIdx.x >> 3, i = (threadIdx.x >> 1) & 3, m = threadIdx.x & 1;
+  const int p = pair_of<LAYOUT>(l, i);
+  const void* w = a.side[side].w;
+  ws[side * kThreads + threadIdx.x] =
+      w != nullptr && p < (a.dim >> 1) ? weight_at(w, a.w_dtype, element<LAYOUT>(p, m, a.rot_pairs, a.interleaved != 0)) : 1.f;
+}
+__device__ __forceinline__ void load_weights(const float* ws, int side, int l, float (&w)[8]) {
+  const float4 lo = *reinterpret_cast<const float4*>(ws + side * kThreads + 8 * l);
+  const float4 hi = *reinterpret_cast<const float4*>(ws + side * kThreads + 8 * l + 4);
+  w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w, w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
 }
 
 // Sum over the lanes of a row's group; every lane of the warp takes part.
 __device__ __forceinline__ float group_sum(float v, int group_log2) {
-  for (int off = 1 << group_log2 >> 1; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+#pragma unroll
+  for (int k = 5; k > 0; --k)
+    if (group_log2 >= k) v += __shfl_xor_sync(0xffffffffu, v, 1 << (k - 1));
   return v;
 }
 
-// Pairs past the rotated ones keep their bits (an identity rotation would
-// turn x + 0 * inf into NaN).
+// (v_a, v_b) = (v_a k.x - v_b k.y, v_a k.z + v_b k.w) for the rotated pairs,
+// (v_a k.x, v_b k.w) for the others: a rotation by nothing would turn
+// x + 0 * inf into NaN.  All pairs of a lane rotate or none does, but in the
+// scalar layout.
 template <int LAYOUT>
-__device__ __forceinline__ void rotate(const float2 (&ang)[4], float (&v)[8], int l, int rot_pairs, bool back) {
+__device__ __forceinline__ void turn(const float4 (&k)[4], float (&v)[8], const Lane& t, int rot_pairs) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if (pair_of<LAYOUT>(l, i) < rot_pairs) {
-      const float c = ang[i].x, s = back ? -ang[i].y : ang[i].y;
-      const float x = v[2 * i], y = v[2 * i + 1];
-      v[2 * i] = x * c - y * s;
-      v[2 * i + 1] = x * s + y * c;
+    const float x = v[2 * i], y = v[2 * i + 1];
+    if (LAYOUT == kScalar ? pair_of<LAYOUT>(t.l, i) < rot_pairs : t.rotates) {
+      v[2 * i] = x * k[i].x - y * k[i].y;
+      v[2 * i + 1] = x * k[i].z + y * k[i].w;
+    } else {
+      v[2 * i] = x * k[i].x;
+      v[2 * i + 1] = y * k[i].w;
     }
   }
 }
 
+// The rows of one token that a group walks: heads gi, gi + gpt, ...
+struct Walk {
+  const char* p;
+  int64_t step;  // bytes between the rows
+  __device__ __forceinline__ Walk(const RowSet& r, int b, int tok, const Lane& t, int es)
+      : p(r.base + (int64_t(b) * r.sb + int64_t(tok) * r.st + t.gi * r.sh) * es), step(t.gpt * r.sh * es) {}
+  __device__ __forceinline__ char* at(int u) const { return const_cast<char*>(p) + u * step; }
+  __device__ __forceinline__ void next(int u) { p += u * step; }
+};
+
 template <typename T, int LAYOUT, bool NORM>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  constexpr int U = 4;  // rows in flight per group
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && LAYOUT != kScalar ? 4 : 2)
+rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  constexpr int U = 4;  // rows of a group in flight
   __shared__ float2 cs[kMaxTokens * kMaxPairs];
-  const Side& s = a.side[blockIdx.y];
-  const int tt = 1 << a.tt_log2;
-  const int64_t n_tokens = int64_t(a.batch) * a.tokens;
-  const int64_t n0 = int64_t(blockIdx.x) * tt;
+  __shared__ __align__(16) float ws[NORM ? 2 * kThreads : 4];
+  const int n_tokens = a.batch * a.tokens;
   const Lane t = lane_of<LAYOUT>(a);
   const int pairs = a.dim >> 1;
   const bool inter = a.interleaved != 0;
-  const int64_t n = n0 + t.tok;
-  const int64_t b = n / a.tokens;
-  const int64_t tok = n - b * a.tokens;
-  const bool here = n < n_tokens && t.active;
   const float inv_dim = 1.f / static_cast<float>(a.dim);
-  float w[8];
-  if constexpr (NORM) load_weights<LAYOUT>(a, s, t, w);
-  fill_angles(a, cs, n0, tt, n_tokens);
-  __syncthreads();
-  float2 ang[4];
-  load_angles<LAYOUT>(a, cs, t, ang);
-  // every thread of the block runs the same number of steps: the group sums
-  // are full-warp shuffles
-  for (int h0 = 0; h0 < s.heads; h0 += U * t.gpt) {
-    Raw<T, LAYOUT> raw[U];
+  if constexpr (NORM) {
+    fill_weights<LAYOUT>(a, 0, ws);
+    fill_weights<LAYOUT>(a, 1, ws);
+  }
+  for (int n0 = blockIdx.x << a.tt_log2; n0 < n_tokens; n0 += gridDim.x << a.tt_log2) {
+    const int n = n0 + t.tok;
+    const int b = n / a.tokens;
+    const int tok = n - b * a.tokens;
+    float2 ang[4];
+    for (int side = 0; side < a.sides; ++side) {
+      const Side& s = a.side[side];
+      Walk x(s.x, b, tok, t, sizeof(T)), y(s.y, b, tok, t, sizeof(T));
+      int left = n < n_tokens && t.active ? (s.heads - t.gi + t.gpt - 1) >> t.gpt_log2 : 0;  // rows of this group
+      // every thread of the block runs the same number of steps: the group
+      // sums are full-warp shuffles
+      const int steps = (s.heads + t.gpt - 1) >> t.gpt_log2;
+      float4 k[4];  // rotation times weights
+      for (int step = 0; step < steps; step += U, left -= U) {
+        Raw<T, LAYOUT> raw[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = h0 + u * t.gpt + t.gi;
-      if (here && h < s.heads)
-        raw[u].load(row_ptr(s.x, b, h, tok, sizeof(T)), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
-      else
-        for (int i = 0; i < Raw<T, LAYOUT>::kWords; ++i) raw[u].w[i] = 0u;
-    }
+        for (int u = 0; u < U; ++u) {
+          if (u < left) raw[u].load(x.at(u), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
+          else
+            for (int i = 0; i < Raw<T, LAYOUT>::kWords; ++i) raw[u].w[i] = 0u;
+        }
+        x.next(U);
+        if (step == 0) {
+          if (side == 0) {  // with the first rows on their way
+            __syncthreads();  // the last tile's angles are read
+            fill_angles(a, cs, n0, n_tokens);
+            __syncthreads();
+            load_angles<LAYOUT>(a, cs, t, ang);
+          }
+          float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+          if constexpr (NORM) load_weights(ws, side, t.l, w);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (h0 + u * t.gpt >= s.heads) break;
-      const int h = h0 + u * t.gpt + t.gi;
-      float v[8];
-      raw[u].widen(v);
-      if constexpr (NORM) {
-        float sum = 0.f;
+          for (int i = 0; i < 4; ++i)
+            k[i] = make_float4(w[2 * i] * ang[i].x, w[2 * i + 1] * ang[i].y, w[2 * i] * ang[i].y, w[2 * i + 1] * ang[i].x);
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
-        const float r = rsqrtf(group_sum(sum, a.group_log2) * inv_dim + a.eps);
+        for (int u = 0; u < U; ++u) {
+          if (step + u >= steps) break;
+          float v[8];
+          raw[u].widen(v);
+          if constexpr (NORM) {
+            float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= r * w[i];
-      }
-      rotate<LAYOUT>(ang, v, t.l, a.rot_pairs, false);
-      if (here && h < s.heads) {
-        raw[u].narrow(v);
-        raw[u].store(row_ptr(s.y, b, h, tok, sizeof(T)), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
+            for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
+            const float rstd = rsqrtf(group_sum(sum, a.group_log2) * inv_dim + a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] *= rstd;
+          }
+          turn<LAYOUT>(k, v, t, a.rot_pairs);
+          if (u < left) {
+            raw[u].narrow(v);
+            raw[u].store(y.at(u), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
+          }
+        }
+        y.next(U);
       }
     }
   }
 }
 
-// Gradients of norm + rotation.  Blocks stride over the token tiles, so a
-// lane's weight gradients stay in registers until the end and the partials
-// are few; their order, and so the result, is fixed.
+// Gradients of norm + rotation.  Blocks stride over the token tiles of one
+// side, so a lane's weight gradients stay in registers until the end and the
+// partials are few; their order, and so the result, is fixed.
 template <typename T, int LAYOUT>
-__global__ void __launch_bounds__(kThreads) rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && LAYOUT != kScalar ? 3 : 2)
+rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int U = 2;
   __shared__ float2 cs[kMaxTokens * kMaxPairs];
   const Side& s = a.side[blockIdx.y];
-  const int tt = 1 << a.tt_log2;
-  const int64_t n_tokens = int64_t(a.batch) * a.tokens;
+  __shared__ __align__(16) float ws[2 * kThreads];
+  const int n_tokens = a.batch * a.tokens;
   const Lane t = lane_of<LAYOUT>(a);
   const int pairs = a.dim >> 1;
   const bool inter = a.interleaved != 0;
   const float inv_dim = 1.f / static_cast<float>(a.dim);
+  const int steps = (s.heads + t.gpt - 1) >> t.gpt_log2;
   float w[8], dw[8] = {};
-  load_weights<LAYOUT>(a, s, t, w);
-  for (int64_t n0 = int64_t(blockIdx.x) * tt; n0 < n_tokens; n0 += int64_t(gridDim.x) * tt) {
-    const int64_t n = n0 + t.tok;
-    const int64_t b = n / a.tokens;
-    const int64_t tok = n - b * a.tokens;
-    const bool here = n < n_tokens && t.active;
-    __syncthreads();
-    fill_angles(a, cs, n0, tt, n_tokens);
-    __syncthreads();
-    float2 ang[4];
-    load_angles<LAYOUT>(a, cs, t, ang);
-    for (int h0 = 0; h0 < s.heads; h0 += U * t.gpt) {
+  fill_weights<LAYOUT>(a, blockIdx.y, ws);
+  __syncthreads();
+  load_weights(ws, blockIdx.y, t.l, w);
+  for (int n0 = blockIdx.x << a.tt_log2; n0 < n_tokens; n0 += gridDim.x << a.tt_log2) {
+    const int n = n0 + t.tok;
+    const int b = n / a.tokens;
+    const int tok = n - b * a.tokens;
+    Walk wx(s.x, b, tok, t, sizeof(T)), wdy(s.dy, b, tok, t, sizeof(T)), wy(s.y, b, tok, t, sizeof(T));
+    int left = n < n_tokens && t.active ? (s.heads - t.gi + t.gpt - 1) >> t.gpt_log2 : 0;
+    float4 k[4];  // the rotation back
+    for (int step = 0; step < steps; step += U, left -= U) {
       Raw<T, LAYOUT> rx[U], rdy[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int h = h0 + u * t.gpt + t.gi;
-        if (here && h < s.heads) {
-          rx[u].load(row_ptr(s.x, b, h, tok, sizeof(T)), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
-          rdy[u].load(row_ptr(s.dy, b, h, tok, sizeof(T)), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
+        if (u < left) {
+          rx[u].load(wx.at(u), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
+          rdy[u].load(wdy.at(u), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
         } else {
           for (int i = 0; i < Raw<T, LAYOUT>::kWords; ++i) rx[u].w[i] = rdy[u].w[i] = 0u;
         }
       }
+      wx.next(U), wdy.next(U);
+      if (step == 0) {
+        __syncthreads();  // the last tile's angles are read
+        fill_angles(a, cs, n0, n_tokens);
+        __syncthreads();
+        float2 ang[4];
+        load_angles<LAYOUT>(a, cs, t, ang);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) k[i] = make_float4(ang[i].x, -ang[i].y, -ang[i].y, ang[i].x);
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (h0 + u * t.gpt >= s.heads) break;
-        const int h = h0 + u * t.gpt + t.gi;
+        if (step + u >= steps) break;
         float x[8], g[8];
         rx[u].widen(x);
         rdy[u].widen(g);
-        rotate<LAYOUT>(ang, g, t.l, a.rot_pairs, true);  // dz
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-        const float r = rsqrtf(group_sum(sum, a.group_log2) * inv_dim + a.eps);
-        float dot = 0.f;
+        turn<LAYOUT>(k, g, t, a.rot_pairs);  // dz
+        float sum = 0.f, dot = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          x[i] *= r;                          // xh
-          dw[i] = fmaf(g[i], x[i], dw[i]);
-          g[i] *= w[i];
-          dot = fmaf(g[i], x[i], dot);
+          sum = fmaf(x[i], x[i], sum);
+          dot = fmaf(g[i] * w[i], x[i], dot);
         }
-        dot = group_sum(dot, a.group_log2) * inv_dim;
+        sum = group_sum(sum, a.group_log2);
+        dot = group_sum(dot, a.group_log2);
+        const float r = rsqrtf(sum * inv_dim + a.eps);
+        const float back = -dot * inv_dim * r * r * r;  // xh mean(g w xh) r = -back x
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = r * fmaf(-x[i], dot, g[i]);
-        if (here && h < s.heads) {
+        for (int i = 0; i < 8; ++i) {
+          g[i] *= r;
+          dw[i] = fmaf(g[i], x[i], dw[i]);
+          g[i] = fmaf(g[i], w[i], back * x[i]);
+        }
+        if (u < left) {
           rx[u].narrow(g);
-          rx[u].store(row_ptr(s.y, b, h, tok, sizeof(T)), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
+          rx[u].store(wy.at(u), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
         }
       }
+      wy.next(U);
     }
   }
   if (s.dw == nullptr) return;
@@ -503,7 +568,7 @@ cudaError_t launch_typed(const RotaryArgs& a, int layout, bool norm, bool grad, 
     return launch_pdl(rotary_dw_kernel, dim3((a.dim + 31) / 32, sides), dim3(32, 32), size_t(0), st, a,
                       static_cast<int>(grid.x));
   }
-  const dim3 grid(static_cast<unsigned>(tiles), sides);
+  const dim3 grid(static_cast<unsigned>(tiles < kBlocks ? tiles : kBlocks));
   if (norm) {
     if (layout == kInterleaved) rotary_kernel<T, kInterleaved, true><<<grid, kThreads, 0, st>>>(a);
     else if (layout == kHalves) rotary_kernel<T, kHalves, true><<<grid, kThreads, 0, st>>>(a);
@@ -524,7 +589,8 @@ cudaError_t launch_rotary(const RotaryCall& c, cudaStream_t st) {
   RotaryArgs a{};
   const b2_view& v = *c.x[0];
   const int sides = c.x[1] != nullptr ? 2 : 1;
-  int most_heads = 0;
+  const bool grad = c.dy[0] != nullptr;
+  int rows = 0;  // of a token that a block walks
   for (int i = 0; i < sides; ++i) {
     Side& s = a.side[i];
     s.x = rows_of(c.x[i]);
@@ -533,11 +599,12 @@ cudaError_t launch_rotary(const RotaryCall& c, cudaStream_t st) {
     s.w = c.w[i];
     s.dw = c.dw[i];
     s.heads = c.x[i]->heads;
-    most_heads = s.heads > most_heads ? s.heads : most_heads;
+    rows = grad ? (s.heads > rows ? s.heads : rows) : rows + s.heads;
   }
   a.pos = c.rot->positions;
   a.pb = c.rot->stride_b, a.pt = c.rot->stride_t, a.pa = c.rot->stride_axis;
   a.pos_dtype = c.rot->pos_dtype;
+  a.sides = sides;
   a.batch = v.batch, a.tokens = v.tokens, a.dim = v.head_dim;
   a.interleaved = c.rot->interleaved;
   a.inverse = c.rot->inverse;
@@ -549,21 +616,25 @@ cudaError_t launch_rotary(const RotaryCall& c, cudaStream_t st) {
   memcpy(a.turn, rates.turn, sizeof(double) * p);
   memcpy(a.axis, rates.axis, p);
   a.rot_pairs = p;
-  // halves of fewer than four aligned pairs a lane (R % 8 != 0) go pair by pair
-  const int layout = a.interleaved ? kInterleaved : (p % 4 == 0 ? kHalves : kScalar);
+  // rotations that end inside a lane's four pairs (R % 8 != 0) go pair by pair
+  const int layout = p % 4 ? kScalar : a.interleaved ? kInterleaved : kHalves;
   a.group_log2 = 5;
   if (layout != kScalar)
     while (a.group_log2 > 0 && (8 << (a.group_log2 - 1)) >= a.dim) --a.group_log2;
-  // tokens of a block: about eight rows a group, so that a block's cos / sin
-  // and set-up are spread over many rows; fewer while the grid would leave
-  // SMs without a block
+  // Tokens of a tile: the number that takes the fewest row steps of the
+  // busiest block, counting a tile's set-up (angles, two barriers) as four.
   const int groups_log2 = 8 - a.group_log2;
   const int64_t n_tokens = int64_t(a.batch) * a.tokens;
-  int tt_log2 = groups_log2 < 4 ? groups_log2 : 4;
-  while (tt_log2 > 0 && ((most_heads << tt_log2) > (8 << groups_log2) || (n_tokens >> tt_log2) * sides < 148 * 2)) --tt_log2;
+  const int blocks = grad ? kGradBlocks : kBlocks;
+  int tt_log2 = 0;
+  int64_t best = 0;
+  for (int x = 0; x <= groups_log2 && x <= 4; ++x) {
+    const int64_t rounds = (((n_tokens + (1 << x) - 1) >> x) + blocks - 1) / blocks;
+    const int64_t cost = rounds * ((((int64_t(rows) << x) + (1 << groups_log2) - 1) >> groups_log2) + 4);
+    if (x == 0 || cost < best) best = cost, tt_log2 = x;
+  }
   a.tt_log2 = tt_log2;
   const int64_t tiles = (n_tokens + (1 << tt_log2) - 1) >> tt_log2;
-  const bool grad = c.dy[0] != nullptr;
   switch (v.dtype) {
     case B2_BF16: return launch_typed<__nv_bfloat16>(a, layout, c.norm, grad, sides, tiles, st);
     case B2_F16: return launch_typed<__half>(a, layout, c.norm, grad, sides, tiles, st);

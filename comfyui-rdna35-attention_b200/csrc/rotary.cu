@@ -23,8 +23,10 @@
 // pairs) or two of 8 bytes (halves).  A block takes `tt` tokens; its 256
 // threads compute the tokens' cos / sin once into shared memory (one
 // sincospif per thread for 16 + 16 heads, D = 128) while the first rows are on
-// their way; every group then walks heads of one token, query heads first,
-// four rows in flight.
+// their way; every group then walks heads of one token, query heads first, four rows in
+// flight.  The backward pass, with two rows to read for one it writes, fetches
+// them by asynchronous copies into slots that only their own thread reads:
+// 148 us against 204 (2 x 9170 x 56 x 128) for loads into registers.
 #include <math.h>
 #include <string.h>
 
@@ -177,6 +179,29 @@ struct Raw {
       *reinterpret_cast<uint2*>(row + c1 * 2) = make_uint2(w[2], w[3]);
     }
   }
+  // The same through shared memory: fetch() starts copies into a slot of the
+  // lane's own, take() reads it once they have landed.  No other thread
+  // touches the slot, so waiting for the thread's own copies is enough.
+  static constexpr int kSlot = sizeof(T) * 8;
+  __device__ __forceinline__ static void fetch(char* slot, const char* row, int c0, int c1) {
+    const uint32_t to = smem_u32(slot);
+    if constexpr (sizeof(T) == 4) {
+      cp_async16(to, row + c0 * 4, 16);
+      cp_async16(to + 16, row + c1 * 4, 16);
+    } else if constexpr (LAYOUT == kInterleaved) {
+      cp_async16(to, row + c0 * 2, 16);
+    } else {
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to), "l"(row + c0 * 2));
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to + 8), "l"(row + c1 * 2));
+    }
+  }
+  __device__ __forceinline__ void take(const char* slot) {
+#pragma unroll
+    for (int i = 0; i < kWords; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(slot + i * 4);
+      w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+    }
+  }
   // member m of pair i sits at eight-element slot: interleaved 2i+m, halves
   // (and the scalar layout) 4m+i
   static __device__ __forceinline__ constexpr int slot(int i, int m) { return LAYOUT == kInterleaved ? 2 * i + m : 4 * m + i; }
@@ -220,8 +245,19 @@ __device__ __forceinline__ float weight_at(const void* w, int dtype, int i) {
   return __half2float(static_cast<const __half*>(w)[i]);
 }
 
+// The pairs' rates in shared memory: lanes index them differently, which the
+// constant bank of the parameters answers one address at a time (10 us of a
+// 9216-token call).
+struct RateTable {
+  double turn[kMaxPairs];
+  uint8_t axis[kMaxPairs];
+};
+__device__ __forceinline__ void fill_rates(const RotaryArgs& a, RateTable& r) {
+  for (int p = threadIdx.x; p < a.rot_pairs; p += kThreads) r.turn[p] = a.turn[p], r.axis[p] = a.axis[p];
+}
+
 // cos / sin of a tile's tokens: cs[token][pair].
-__device__ __forceinline__ void fill_angles(const RotaryArgs& a, float2* cs, int n0, int n_tokens) {
+__device__ __forceinline__ void fill_angles(const RotaryArgs& a, const RateTable& r, float2* cs, int n0, int n_tokens) {
   const int b0 = n0 / a.tokens, t0 = n0 - b0 * a.tokens;
   const int count = min(1 << a.tt_log2, n_tokens - n0) * a.rot_pairs;
   for (int i = threadIdx.x; i < count; i += kThreads) {
@@ -229,7 +265,7 @@ __device__ __forceinline__ void fill_angles(const RotaryArgs& a, float2* cs, int
     const int p = i - tok * a.rot_pairs;
     int b = b0, at = t0 + tok;
     while (at >= a.tokens) at -= a.tokens, ++b;  // a tile may span batches
-    double turns = position(a, b, at, a.axis[p]) * a.turn[p];
+    double turns = position(a, b, at, r.axis[p]) * r.turn[p];
     turns -= rint(turns);
     float s, c;
     sincospif(2.0f * static_cast<float>(turns), &s, &c);
@@ -284,12 +320,21 @@ __device__ __forceinline__ void load_weights(const float* ws, int side, int l, f
   w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w, w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
 }
 
-// Sum over the lanes of a row's group; every lane of the warp takes part.
-__device__ __forceinline__ float group_sum(float v, int group_log2) {
+// Sums over the lanes of a row's group; every lane of the warp takes part.
+template <int N>
+__device__ __forceinline__ void group_sums(float (&v)[N], int group_log2) {
 #pragma unroll
   for (int k = 5; k > 0; --k)
-    if (group_log2 >= k) v += __shfl_xor_sync(0xffffffffu, v, 1 << (k - 1));
-  return v;
+    if (group_log2 >= k) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], 1 << (k - 1));
+    }
+}
+
+__device__ __forceinline__ float group_sum(float v, int group_log2) {
+  float one[1] = {v};
+  group_sums<1>(one, group_log2);
+  return one[0];
 }
 
 // (v_a, v_b) = (v_a k.x - v_b k.y, v_a k.z + v_b k.w) for the rotated pairs,
@@ -311,14 +356,25 @@ __device__ __forceinline__ void turn(const float4 (&k)[4], float (&v)[8], const 
   }
 }
 
-// The rows of one token that a group walks: heads gi, gi + gpt, ...
+// Shared-memory bytes of the fetched rows: `rows` in flight for every thread.
+template <typename T, int LAYOUT>
+__host__ __device__ constexpr int fetch_bytes(int rows) {
+  return LAYOUT == kScalar ? 0 : rows * kThreads * Raw<T, LAYOUT>::kSlot;
+}
+// Rows of x and of dy in flight for a thread of the backward pass.  Forward
+// keeps its four rows in registers instead: computing four at a time hides
+// the group sums, and measured 114 us against 126 (32760 x 40 x 128) for the
+// same ring of slots.
+constexpr int kAheadGrad = 4;
+
+// A group's rows of one token and side: heads gi, gi + gpt, ...
 struct Walk {
-  const char* p;
+  char* p;
   int64_t step;  // bytes between the rows
   __device__ __forceinline__ Walk(const RowSet& r, int b, int tok, const Lane& t, int es)
       : p(r.base + (int64_t(b) * r.sb + int64_t(tok) * r.st + t.gi * r.sh) * es), step(t.gpt * r.sh * es) {}
-  __device__ __forceinline__ char* at(int u) const { return const_cast<char*>(p) + u * step; }
-  __device__ __forceinline__ void next(int u) { p += u * step; }
+  __device__ __forceinline__ char* at(int u) const { return p + u * step; }
+  __device__ __forceinline__ void next(int u = 1) { p += u * step; }
 };
 
 template <typename T, int LAYOUT, bool NORM>
@@ -326,12 +382,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && LAYOUT != kScalar 
 rotary_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int U = 4;  // rows of a group in flight
   __shared__ float2 cs[kMaxTokens * kMaxPairs];
+  __shared__ RateTable rates;
   __shared__ __align__(16) float ws[NORM ? 2 * kThreads : 4];
   const int n_tokens = a.batch * a.tokens;
   const Lane t = lane_of<LAYOUT>(a);
   const int pairs = a.dim >> 1;
   const bool inter = a.interleaved != 0;
   const float inv_dim = 1.f / static_cast<float>(a.dim);
+  fill_rates(a, rates);
   if constexpr (NORM) {
     fill_weights<LAYOUT>(a, 0, ws);
     fill_weights<LAYOUT>(a, 1, ws);
@@ -361,7 +419,7 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
         if (step == 0) {
           if (side == 0) {  // with the first rows on their way
             __syncthreads();  // the last tile's angles are read
-            fill_angles(a, cs, n0, n_tokens);
+            fill_angles(a, rates, cs, n0, n_tokens);
             __syncthreads();
             load_angles<LAYOUT>(a, cs, t, ang);
           }
@@ -402,17 +460,22 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
 template <typename T, int LAYOUT>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && LAYOUT != kScalar ? 3 : 2)
 rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
-  constexpr int U = 2;
+  using R = Raw<T, LAYOUT>;
+  extern __shared__ __align__(16) char slots[];
   __shared__ float2 cs[kMaxTokens * kMaxPairs];
-  const Side& s = a.side[blockIdx.y];
+  __shared__ RateTable rates;
   __shared__ __align__(16) float ws[2 * kThreads];
+  const Side& s = a.side[blockIdx.y];
   const int n_tokens = a.batch * a.tokens;
   const Lane t = lane_of<LAYOUT>(a);
   const int pairs = a.dim >> 1;
   const bool inter = a.interleaved != 0;
   const float inv_dim = 1.f / static_cast<float>(a.dim);
   const int steps = (s.heads + t.gpt - 1) >> t.gpt_log2;
+  char* const own = slots + threadIdx.x * R::kSlot;
+  constexpr int kStage = 2 * kThreads * R::kSlot;  // x, then dy
   float w[8], dw[8] = {};
+  fill_rates(a, rates);
   fill_weights<LAYOUT>(a, blockIdx.y, ws);
   __syncthreads();
   load_weights(ws, blockIdx.y, t.l, w);
@@ -421,58 +484,76 @@ rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
     const int b = n / a.tokens;
     const int tok = n - b * a.tokens;
     Walk wx(s.x, b, tok, t, sizeof(T)), wdy(s.dy, b, tok, t, sizeof(T)), wy(s.y, b, tok, t, sizeof(T));
-    int left = n < n_tokens && t.active ? (s.heads - t.gi + t.gpt - 1) >> t.gpt_log2 : 0;
+    const int rows = n < n_tokens && t.active ? (s.heads - t.gi + t.gpt - 1) >> t.gpt_log2 : 0;
+    auto fetch = [&](int j) {
+      if constexpr (LAYOUT != kScalar) {
+        if (j < rows) {
+          char* slot = own + (j % kAheadGrad) * kStage;
+          R::fetch(slot, wx.p, t.c0, t.c1);
+          R::fetch(slot + kThreads * R::kSlot, wdy.p, t.c0, t.c1);
+        }
+        wx.next(), wdy.next();
+        cp_async_commit();
+      }
+    };
+#pragma unroll 1
+    for (int j = 0; j < kAheadGrad; ++j) fetch(j);
+    __syncthreads();  // the last tile's angles are read
+    fill_angles(a, rates, cs, n0, n_tokens);
+    __syncthreads();
     float4 k[4];  // the rotation back
-    for (int step = 0; step < steps; step += U, left -= U) {
-      Raw<T, LAYOUT> rx[U], rdy[U];
+    {
+      float2 ang[4];
+      load_angles<LAYOUT>(a, cs, t, ang);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (u < left) {
-          rx[u].load(wx.at(u), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
-          rdy[u].load(wdy.at(u), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
+      for (int i = 0; i < 4; ++i) k[i] = make_float4(ang[i].x, -ang[i].y, -ang[i].y, ang[i].x);
+    }
+#pragma unroll 1
+    for (int j = 0; j < steps; ++j) {
+      R rx, rdy;
+      if constexpr (LAYOUT == kScalar) {
+        if (j < rows) {
+          rx.load(wx.p, t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
+          rdy.load(wdy.p, t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
         } else {
-          for (int i = 0; i < Raw<T, LAYOUT>::kWords; ++i) rx[u].w[i] = rdy[u].w[i] = 0u;
+          rx = rdy = R{};
         }
+        wx.next(), wdy.next();
+      } else {
+        cp_async_wait<kAheadGrad - 1>();
+        rx.take(own + (j % kAheadGrad) * kStage);
+        rdy.take(own + (j % kAheadGrad) * kStage + kThreads * R::kSlot);
       }
-      wx.next(U), wdy.next(U);
-      if (step == 0) {
-        __syncthreads();  // the last tile's angles are read
-        fill_angles(a, cs, n0, n_tokens);
-        __syncthreads();
-        float2 ang[4];
-        load_angles<LAYOUT>(a, cs, t, ang);
+      float x[8], g[8];
+      rx.widen(x);
+      rdy.widen(g);
+      fetch(j + kAheadGrad);
+      if (j >= rows) {  // what a slot held before may be NaN
 #pragma unroll
-        for (int i = 0; i < 4; ++i) k[i] = make_float4(ang[i].x, -ang[i].y, -ang[i].y, ang[i].x);
+        for (int i = 0; i < 8; ++i) x[i] = g[i] = 0.f;
       }
+      turn<LAYOUT>(k, g, t, a.rot_pairs);  // dz
+      float sum = 0.f, dot = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (step + u >= steps) break;
-        float x[8], g[8];
-        rx[u].widen(x);
-        rdy[u].widen(g);
-        turn<LAYOUT>(k, g, t, a.rot_pairs);  // dz
-        float sum = 0.f, dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          sum = fmaf(x[i], x[i], sum);
-          dot = fmaf(g[i] * w[i], x[i], dot);
-        }
-        sum = group_sum(sum, a.group_log2);
-        dot = group_sum(dot, a.group_log2);
-        const float r = rsqrtf(sum * inv_dim + a.eps);
-        const float back = -dot * inv_dim * r * r * r;  // xh mean(g w xh) r = -back x
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          g[i] *= r;
-          dw[i] = fmaf(g[i], x[i], dw[i]);
-          g[i] = fmaf(g[i], w[i], back * x[i]);
-        }
-        if (u < left) {
-          rx[u].narrow(g);
-          rx[u].store(wy.at(u), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
-        }
+      for (int i = 0; i < 8; ++i) {
+        sum = fmaf(x[i], x[i], sum);
+        dot = fmaf(g[i] * w[i], x[i], dot);
       }
-      wy.next(U);
+      float sums[2] = {sum, dot};
+      group_sums<2>(sums, a.group_log2);
+      const float r = rsqrtf(sums[0] * inv_dim + a.eps);
+      const float back = -sums[1] * inv_dim * r * r * r;  // xh mean(g w xh) r = -back x
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        g[i] *= r;
+        dw[i] = fmaf(g[i], x[i], dw[i]);
+        g[i] = fmaf(g[i], w[i], back * x[i]);
+      }
+      if (j < rows) {
+        rx.narrow(g);
+        rx.store(wy.p, t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
+      }
+      wy.next();
     }
   }
   if (s.dw == nullptr) return;
@@ -555,30 +636,27 @@ const Rates& rates_of(const b2_rotary& r) {
   return k;
 }
 
+template <typename T, int LAYOUT>
+cudaError_t launch_layout(const RotaryArgs& a, bool norm, bool grad, int64_t tiles, cudaStream_t st) {
+  using Kernel = void (*)(const RotaryArgs);
+  const Kernel kernel = grad ? Kernel(rotary_grad_kernel<T, LAYOUT>)
+                             : norm ? Kernel(rotary_kernel<T, LAYOUT, true>) : Kernel(rotary_kernel<T, LAYOUT, false>);
+  const int smem = grad ? fetch_bytes<T, LAYOUT>(2 * kAheadGrad) : 0;
+  cudaError_t err = ensure_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (err != cudaSuccess) return err;
+  const int most = grad ? kGradBlocks : kBlocks;
+  const dim3 grid(static_cast<unsigned>(tiles < most ? tiles : most), grad ? a.sides : 1);
+  kernel<<<grid, kThreads, smem, st>>>(a);
+  if ((err = cudaGetLastError()) != cudaSuccess || (a.side[0].dw == nullptr && a.side[1].dw == nullptr)) return err;
+  return launch_pdl(rotary_dw_kernel, dim3((a.dim + 31) / 32, a.sides), dim3(32, 32), size_t(0), st, a,
+                    static_cast<int>(grid.x));
+}
+
 template <typename T>
-cudaError_t launch_typed(const RotaryArgs& a, int layout, bool norm, bool grad, int sides, int64_t tiles,
-                         cudaStream_t st) {
-  if (grad) {
-    const dim3 grid(static_cast<unsigned>(tiles < kGradBlocks ? tiles : kGradBlocks), sides);
-    if (layout == kInterleaved) rotary_grad_kernel<T, kInterleaved><<<grid, kThreads, 0, st>>>(a);
-    else if (layout == kHalves) rotary_grad_kernel<T, kHalves><<<grid, kThreads, 0, st>>>(a);
-    else rotary_grad_kernel<T, kScalar><<<grid, kThreads, 0, st>>>(a);
-    const cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess || (a.side[0].dw == nullptr && a.side[1].dw == nullptr)) return err;
-    return launch_pdl(rotary_dw_kernel, dim3((a.dim + 31) / 32, sides), dim3(32, 32), size_t(0), st, a,
-                      static_cast<int>(grid.x));
-  }
-  const dim3 grid(static_cast<unsigned>(tiles < kBlocks ? tiles : kBlocks));
-  if (norm) {
-    if (layout == kInterleaved) rotary_kernel<T, kInterleaved, true><<<grid, kThreads, 0, st>>>(a);
-    else if (layout == kHalves) rotary_kernel<T, kHalves, true><<<grid, kThreads, 0, st>>>(a);
-    else rotary_kernel<T, kScalar, true><<<grid, kThreads, 0, st>>>(a);
-  } else {
-    if (layout == kInterleaved) rotary_kernel<T, kInterleaved, false><<<grid, kThreads, 0, st>>>(a);
-    else if (layout == kHalves) rotary_kernel<T, kHalves, false><<<grid, kThreads, 0, st>>>(a);
-    else rotary_kernel<T, kScalar, false><<<grid, kThreads, 0, st>>>(a);
-  }
-  return cudaGetLastError();
+cudaError_t launch_typed(const RotaryArgs& a, int layout, bool norm, bool grad, int64_t tiles, cudaStream_t st) {
+  if (layout == kInterleaved) return launch_layout<T, kInterleaved>(a, norm, grad, tiles, st);
+  if (layout == kHalves) return launch_layout<T, kHalves>(a, norm, grad, tiles, st);
+  return launch_layout<T, kScalar>(a, norm, grad, tiles, st);
 }
 
 }  // namespace
@@ -636,9 +714,9 @@ cudaError_t launch_rotary(const RotaryCall& c, cudaStream_t st) {
   a.tt_log2 = tt_log2;
   const int64_t tiles = (n_tokens + (1 << tt_log2) - 1) >> tt_log2;
   switch (v.dtype) {
-    case B2_BF16: return launch_typed<__nv_bfloat16>(a, layout, c.norm, grad, sides, tiles, st);
-    case B2_F16: return launch_typed<__half>(a, layout, c.norm, grad, sides, tiles, st);
-    default: return launch_typed<float>(a, layout, c.norm, grad, sides, tiles, st);
+    case B2_BF16: return launch_typed<__nv_bfloat16>(a, layout, c.norm, grad, tiles, st);
+    case B2_F16: return launch_typed<__half>(a, layout, c.norm, grad, tiles, st);
+    default: return launch_typed<float>(a, layout, c.norm, grad, tiles, st);
   }
 }
 

@@ -49,21 +49,25 @@ constexpr int kThreads = 64 + 32 * kElemWarps;
 constexpr uint32_t kHalfBytes = kTile * 128;  // 128 rows x 64 16-bit columns
 constexpr uint32_t kStatBytes = 2 * kTile * 4;
 // Rings of the walked tiles.  K (or Q) is read by the first and the last
-// product of its tile pair, so the tile after the next is requested a whole
-// pair before its first use only with three stages: with two, each pair
-// waited for its load (9216^2 x 32 heads: 3.97 ms against 4.62 ms).
-constexpr int kStagesA = 3, kStagesB = 2;
+// product of its tile pair, so with two stages each pair waits for its load.
+// The second ring gets what the CTA's own tiles leave.
+constexpr int kStagesA = 3, kStagesDkv = 2, kStagesDq = 3, kMaxB = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kShiftP16 = 8;  // FP16: P is held times 2^8
 
-// TMEM columns.  dK/dV: S and dP take turns in kColS (each is free again as
-// soon as the elementwise warps have loaded it), P and dS have columns of
-// their own.  dQ: S and dP have a place each, dS two.
-constexpr uint32_t kColS = 0, kColP = 128, kColDS = 192, kColAcc0 = 256, kColAcc1 = 384;
-constexpr uint32_t kColDP = 128, kColDS2 = 384;
+// TMEM columns.
+//   dK/dV: S and dP take turns in kColX (each is free again as soon as the
+//     elementwise warps have loaded it), P, dS, dV, dK.
+//   dQ: S, dP, dQ, dS, and Q: as the A operand of S it costs no shared-memory
+//     reads there, whose 128 bytes a cycle A and B of a 128 x 128 product
+//     take all of (1.53 ms against 1.69 for all of dQ).  The same for V in the
+//     dK/dV CTAs needs P and dS to share columns, and their products to wait
+//     for one another: 2.20 ms against 2.06.
+constexpr uint32_t kColX = 0, kColP = 128, kColDS = 192, kColDV = 256, kColDK = 384;
+constexpr uint32_t kColS = 0, kColDP = 128, kColDQ = 256, kColDSq = 384, kColQ = 448;
 
 struct GradArgs {
-  Rows dq, dk, dv;
+  Rows q, dq, dk, dv;
   const float* stat;       // [B*H][query tiles][2][128]: -lse*log2e (+ shift), -delta
   const uint32_t* maxima;  // FP16: [B*Hk][2] bits of the largest squared norms of dO and V rows
   const int32_t* key_lengths;
@@ -77,15 +81,13 @@ struct GradArgs {
 };
 
 struct __align__(8) Misc {
-  uint64_t own_full;      // the CTA's own two tiles
+  uint64_t own_full;      // the CTA's own tile (two for dK/dV) in shared memory
+  uint64_t own_tmem;      // dQ: Q in tensor memory
   uint64_t a_full[kStagesA], a_empty[kStagesA];  // walked tiles: Q or K
-  uint64_t b_full[kStagesB], b_empty[kStagesB];  // dO or V
+  uint64_t b_full[kMaxB], b_empty[kMaxB];  // dO or V
   uint64_t stat_full[2], stat_empty[2];          // -lse and -delta of a query tile
-  uint64_t s_full, s_read, p_full, dp_full, dp_read;
-  // dQ keeps two dS buffers in flight, each with barriers of its own: one
-  // barrier could run two phases ahead of a waiting warp and look unfinished
-  uint64_t ds_full[2], acc0_done[2];
-  uint64_t acc1_done, all_done;
+  uint64_t s_full, s_read, p_full, dp_full, dp_read, ds_full;
+  uint64_t dk_done, all_done;
   uint32_t tmem;
   int abort_flag;
 };
@@ -93,11 +95,10 @@ struct __align__(8) Misc {
 template <int HALVES>
 struct Smem {
   static constexpr uint32_t tile = HALVES * kHalfBytes;
-  static constexpr uint32_t own0 = 0;
-  static constexpr uint32_t own1 = own0 + tile;
-  static constexpr uint32_t a = own1 + tile;
-  static constexpr uint32_t b = a + kStagesA * tile;
-  static constexpr uint32_t stat = b + kStagesB * tile;  // [2]
+  static constexpr uint32_t a = 0;
+  static constexpr uint32_t own = a + kStagesA * tile;  // dK/dV: K and V; dQ: dO
+  static constexpr uint32_t b_dkv = own + 2 * tile, b_dq = own + tile;
+  static constexpr uint32_t stat = own + 4 * tile;  // [2]
   static constexpr uint32_t misc = stat + 2 * kStatBytes;
   // one CTA per SM (each owns all 512 TMEM columns)
   static constexpr uint32_t used = misc + sizeof(Misc);
@@ -139,6 +140,15 @@ __device__ __forceinline__ void product_rows(uint32_t d, uint64_t a_desc, uint64
   }
 }
 
+// The same with A (16-bit pairs: 32 * HALVES columns) in tensor memory at `a`.
+template <bool BF16, int HALVES>
+__device__ __forceinline__ void product_rows_ts(uint32_t d, uint32_t a, uint64_t b_desc) {
+  constexpr uint32_t idesc = idesc_f16(128, 128, BF16, false, false);
+#pragma unroll
+  for (int kk = 0; kk < 4 * HALVES; ++kk)
+    mma_ts(d, a + kk * 8, b_desc + (((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4), idesc, kk > 0 ? 1u : 0u);
+}
+
 // D[128 x D] (+)= A B with A (128 x 128, 16-bit pairs: 64 columns) in tensor
 // memory at `a`, B's rows as contraction.
 template <bool BF16, int HALVES>
@@ -173,6 +183,16 @@ __device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// Powers of two of a pair of columns.  (Computing half of them with a
+// polynomial on the FMA pipes instead changed nothing: 2.04 against 2.06 ms
+// for dK/dV, 1.74 against 1.69 ms for dQ at 9216^2 x 32 heads.)
+__device__ __forceinline__ void exp2_pair(uint64_t x2, uint32_t& p0, uint32_t& p1) {
+  float a, b;
+  unpack_f2(x2, a, b);
+  p0 = __float_as_uint(ex2(a));
+  p1 = __float_as_uint(ex2(b));
+}
+
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(
@@ -180,6 +200,22 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+// One row of the CTA's own operand to tensor memory: columns cg*32 .. +31 of
+// the head dimension (zeros past it, and for no row) by column group cg.
+template <int HALVES>
+__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const char* row, int cg, int dim) {
+  if (cg >= 2 * HALVES) return;
+  uint32_t w[16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (row != nullptr && cg * 32 + 8 * i < dim) x = *reinterpret_cast<const uint4*>(row + cg * 64 + 16 * i);
+    w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
+  }
+  tmem_st16(taddr + cg * 16, w);
+  tmem_wait_st();
 }
 
 // Zero the 16-bit elements of 32 packed columns whose bit is set.
@@ -264,11 +300,11 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
   if (warp == 0) {
     if (lane == 0 && n > 0 && !*abort_flag) {
       mbar_expect_tx(&m.own_full, 2 * L::tile);
-      load_tile<HALVES>(smem + L::own0, k_map, &m.own_full, k0, hk, b);
-      load_tile<HALVES>(smem + L::own1, v_map, &m.own_full, k0, hk, b);
+      load_tile<HALVES>(smem + L::own, k_map, &m.own_full, k0, hk, b);
+      load_tile<HALVES>(smem + L::own + L::tile, v_map, &m.own_full, k0, hk, b);
       int na = 0, nb = 0, ns = 0;
       for (int i = 0; i < n; ++i) {
-        const int sa = i % kStagesA, sb = i % kStagesB, ss = i & 1;
+        const int sa = i % kStagesA, sb = i % kStagesDkv, ss = i & 1;
         const int g = i / per_head;
         const int qt = first + i - g * per_head;
         const int h = hk * a.group + g;
@@ -281,46 +317,45 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
         bulk_load(smem + L::stat + ss * kStatBytes, a.stat + ((int64_t(b) * a.heads + h) * a.q_tiles + qt) * (2 * kTile),
                   kStatBytes, &m.stat_full[ss]);
         ns = i + 1;
-        if (!mbar_wait(&m.b_empty[sb], ((i / kStagesB) & 1) ^ 1, abort_flag, a.status, 2)) break;
+        if (!mbar_wait(&m.b_empty[sb], ((i / kStagesDkv) & 1) ^ 1, abort_flag, a.status, 2)) break;
         mbar_expect_tx(&m.b_full[sb], L::tile);
-        load_tile<HALVES>(smem + L::b + sb * L::tile, do_map, &m.b_full[sb], qt * kTile, h, b);
+        load_tile<HALVES>(smem + L::b_dkv + sb * L::tile, do_map, &m.b_full[sb], qt * kTile, h, b);
         nb = i + 1;
       }
       if (*abort_flag) {
         drain_loads(m.a_full, kStagesA, na, &m.own_full, a.status);
-        drain_loads(m.b_full, kStagesB, nb, nullptr, a.status);
+        drain_loads(m.b_full, kStagesDkv, nb, nullptr, a.status);
         drain_loads(m.stat_full, 2, ns, nullptr, a.status);
       }
     }
   } else if (warp == 1) {
     if (n > 0 && elect_one()) {
       const uint32_t base = smem_u32(smem);
-      const uint64_t k_rows = rows_desc(base + L::own0), v_rows = rows_desc(base + L::own1);
+      const uint64_t k_rows = rows_desc(base + L::own), v_rows = rows_desc(base + L::own + L::tile);
       const uint64_t q_rows = rows_desc(base + L::a), q_cols = cols_desc(base + L::a);  // stage 0; stages L::tile apart
-      const uint64_t do_rows = rows_desc(base + L::b), do_cols = cols_desc(base + L::b);
+      const uint64_t do_rows = rows_desc(base + L::b_dkv), do_cols = cols_desc(base + L::b_dkv);
       constexpr uint32_t step = L::tile >> 4;
       bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3);
       // Order S(i+1), dV(i), dP(i+1), dK(i): S and dP wait for the elementwise
       // warps to have loaded the other out of their common columns, and dV or
       // dK runs while they do.
       for (int i = -1; ok && i < n; ++i) {
-        const int sa = i < 0 ? 0 : i % kStagesA, sb = i & 1;
-        const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesB;  // the next tiles' stages and phases
-        const uint32_t ph = i & 1, next = ph ^ 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesB) & 1;
+        const int sa = i < 0 ? 0 : i % kStagesA, sb = i < 0 ? 0 : i % kStagesDkv;
+        const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesDkv;  // the next tiles' stages and phases
+        const uint32_t ph = i & 1, next = ph ^ 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesDkv) & 1;
         const bool more = i + 1 < n;
         if (more) {
           ok = mbar_wait(&m.a_full[ta], ta_ph, abort_flag, a.status, 7) &&
                (i < 0 || mbar_wait(&m.dp_read, ph, abort_flag, a.status, 8));
           if (!ok) break;
           tc_fence_after();
-          product_rows<BF16, HALVES>(tmem + kColS, k_rows, q_rows + ta * step);
+          product_rows<BF16, HALVES>(tmem + kColX, k_rows, q_rows + ta * step);
           mma_commit(&m.s_full);
         }
         if (i >= 0) {
           if (!(ok = mbar_wait(&m.p_full, ph, abort_flag, a.status, 6))) break;
           tc_fence_after();
-          product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColP, do_cols + sb * step, i > 0);
-          mma_commit(&m.acc0_done[0]);
+          product_cols<BF16, HALVES>(tmem + kColDV, tmem + kColP, do_cols + sb * step, i > 0);
           mma_commit(&m.b_empty[sb]);
         }
         if (more) {
@@ -328,14 +363,14 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
                mbar_wait(&m.s_read, next, abort_flag, a.status, 11);
           if (!ok) break;
           tc_fence_after();
-          product_rows<BF16, HALVES>(tmem + kColS, v_rows, do_rows + tb * step);
+          product_rows<BF16, HALVES>(tmem + kColX, v_rows, do_rows + tb * step);
           mma_commit(&m.dp_full);
         }
         if (i >= 0) {
-          if (!(ok = mbar_wait(&m.ds_full[0], ph, abort_flag, a.status, 9))) break;
+          if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
           tc_fence_after();
-          product_cols<BF16, HALVES>(tmem + kColAcc1, tmem + kColDS, q_cols + sa * step, i > 0);
-          mma_commit(&m.acc1_done);
+          product_cols<BF16, HALVES>(tmem + kColDK, tmem + kColDS, q_cols + sa * step, i > 0);
+          mma_commit(&m.dk_done);
           mma_commit(&m.a_empty[sa]);
         }
       }
@@ -351,7 +386,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
     const int row = sub * 32 + lane;
     const int key = k0 + row;
     const uint32_t lanes = static_cast<uint32_t>(sub * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + kColS + cg * 32;
+    const uint32_t s_addr = tmem + lanes + kColX + cg * 32;
     const uint32_t p_addr = tmem + lanes + kColP + cg * 16, ds_addr = tmem + lanes + kColDS + cg * 16;
     float gain = 1.f;
     if constexpr (!BF16) gain = ds_gain(a, bhk);
@@ -381,32 +416,29 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
         const float4 nl = *reinterpret_cast<const float4*>(stat + c);
-        float x[4];
-        unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, pack_f2(nl.x, nl.y)), x[0], x[1]);
-        unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, pack_f2(nl.z, nl.w)), x[2], x[3]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[c + e] = __float_as_uint(ex2(x[e]));
+        exp2_pair(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, pack_f2(nl.x, nl.y)),
+                  v[c], v[c + 1]);
+        exp2_pair(fma_f2(pack_f2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, pack_f2(nl.z, nl.w)),
+                  v[c + 2], v[c + 3]);
         w[c / 2] = Cvt<T>::pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
         w[c / 2 + 1] = Cvt<T>::pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
       }
       if (bad != 0u) clear_pairs(w, bad);
-      // P's columns are free once the last dV has read them
-      if (i > 0 && !(ok = mbar_wait(&m.acc0_done[0], ph ^ 1, abort_flag, a.status, 18))) break;
-      tc_fence_after();
-      tmem_st16(p_addr, w);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&m.p_full);
-      // dS = P (dP - delta)
+      // dP(i) was issued after dV(i-1), so with it done P's columns are free
       if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
       tc_fence_after();
       uint32_t d[32];
+      tmem_st16(p_addr, w);
       tmem_ld32(s_addr, d);
+      tmem_wait_st();
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&m.dp_read);
+      if (lane == 0) {
+        mbar_arrive(&m.dp_read);
+        mbar_arrive(&m.p_full);
+      }
+      // dS = P (dP - delta)
 #pragma unroll
       for (int c = 0; c < 32; c += 4) {
         const float4 nd = *reinterpret_cast<const float4*>(stat + kTile + c);
@@ -422,7 +454,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
         }
       }
       if (bad != 0u) clear_pairs(w, bad);  // 0 * inf
-      if (i > 0 && !(ok = mbar_wait(&m.acc1_done, ph ^ 1, abort_flag, a.status, 19))) break;
+      if (i > 0 && !(ok = mbar_wait(&m.dk_done, ph ^ 1, abort_flag, a.status, 19))) break;  // the last dS is read
       tc_fence_after();
       tmem_st16(ds_addr, w);
       tmem_wait_st();
@@ -430,7 +462,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(&m.stat_empty[s]);
-        mbar_arrive(&m.ds_full[0]);
+        mbar_arrive(&m.ds_full);
       }
     }
     // column groups 0 and 1 store the halves of dV, 2 and 3 those of dK
@@ -446,7 +478,7 @@ __device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensor
         const float p_mul = BF16 ? 1.f : 1.f / (1 << kShiftP16);
         const float mul = is_dk ? a.scale * p_mul / gain : p_mul;
         const int from = (cg & 1) * 32 * HALVES;
-        store_row<T>(tmem + lanes + (is_dk ? kColAcc1 : kColAcc0), orow, from, from + 32 * HALVES, a.dim, mul, key >= len);
+        store_row<T>(tmem + lanes + (is_dk ? kColDK : kColDV), orow, from, from + 32 * HALVES, a.dim, mul, key >= len);
       }
     }
   }
@@ -476,60 +508,57 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
 
   if (warp == 0) {
     if (lane == 0 && n > 0 && !*abort_flag) {
-      mbar_expect_tx(&m.own_full, 2 * L::tile);
-      load_tile<HALVES>(smem + L::own0, q_map, &m.own_full, q0, h, b);
-      load_tile<HALVES>(smem + L::own1, do_map, &m.own_full, q0, h, b);
+      mbar_expect_tx(&m.own_full, L::tile);
+      load_tile<HALVES>(smem + L::own, do_map, &m.own_full, q0, h, b);
       int na = 0, nb = 0;
       for (int i = 0; i < n; ++i) {
-        const int sa = i % kStagesA, sb = i % kStagesB;
+        const int sa = i % kStagesA, sb = i % kStagesDq;
         if (!mbar_wait(&m.a_empty[sa], ((i / kStagesA) & 1) ^ 1, abort_flag, a.status, 1)) break;
         mbar_expect_tx(&m.a_full[sa], L::tile);
         load_tile<HALVES>(smem + L::a + sa * L::tile, k_map, &m.a_full[sa], i * kTile, hk, b);
         na = i + 1;
-        if (!mbar_wait(&m.b_empty[sb], ((i / kStagesB) & 1) ^ 1, abort_flag, a.status, 2)) break;
+        if (!mbar_wait(&m.b_empty[sb], ((i / kStagesDq) & 1) ^ 1, abort_flag, a.status, 2)) break;
         mbar_expect_tx(&m.b_full[sb], L::tile);
-        load_tile<HALVES>(smem + L::b + sb * L::tile, v_map, &m.b_full[sb], i * kTile, hk, b);
+        load_tile<HALVES>(smem + L::b_dq + sb * L::tile, v_map, &m.b_full[sb], i * kTile, hk, b);
         nb = i + 1;
       }
       if (*abort_flag) {
         drain_loads(m.a_full, kStagesA, na, &m.own_full, a.status);
-        drain_loads(m.b_full, kStagesB, nb, nullptr, a.status);
+        drain_loads(m.b_full, kStagesDq, nb, nullptr, a.status);
       }
     }
   } else if (warp == 1) {
     if (n > 0 && elect_one()) {
       const uint32_t base = smem_u32(smem);
-      const uint64_t q_rows = rows_desc(base + L::own0), do_rows = rows_desc(base + L::own1);
+      const uint64_t do_rows = rows_desc(base + L::own);
       const uint64_t k_rows = rows_desc(base + L::a), k_cols = cols_desc(base + L::a);
-      const uint64_t v_rows = rows_desc(base + L::b);
+      const uint64_t v_rows = rows_desc(base + L::b_dq);
       constexpr uint32_t step = L::tile >> 4;
-      bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3);
-      // Order S(i+1), dQ(i-1), dP(i+1): dQ runs one pair behind, so the
-      // elementwise warps are never waited for while products are left.
-      for (int i = -1; ok && i <= n; ++i) {
-        const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesB;
-        const uint32_t ph = i & 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesB) & 1;
+      bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3) && mbar_wait(&m.own_tmem, 0, abort_flag, a.status, 4);
+      tc_fence_after();
+      // Order S(i+1), dQ(i), dP(i+1): S runs ahead of the exponentials of the
+      // tile before, dP under those of its own.
+      for (int i = -1; ok && i < n; ++i) {
+        const int sa = i < 0 ? 0 : i % kStagesA;
+        const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesDq;
+        const uint32_t ph = i & 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesDq) & 1;
         const bool more = i + 1 < n;
-        if (more) {  // S's columns are free once the elementwise warps hold S(i)
+        if (more) {  // the elementwise warps hold S(i)
           ok = mbar_wait(&m.a_full[ta], ta_ph, abort_flag, a.status, 7) &&
                (i < 0 || mbar_wait(&m.s_read, ph, abort_flag, a.status, 8));
           if (!ok) break;
           tc_fence_after();
-          product_rows<BF16, HALVES>(tmem + kColS, q_rows, k_rows + ta * step);
+          product_rows_ts<BF16, HALVES>(tmem + kColS, tmem + kColQ, k_rows + ta * step);
           mma_commit(&m.s_full);
         }
-        if (i > 0) {
-          const int sa = (i - 1) % kStagesA;
-          if (!(ok = mbar_wait(&m.ds_full[ph ^ 1], ((i - 1) >> 1) & 1, abort_flag, a.status, 9))) break;
+        if (i >= 0) {
+          if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
           tc_fence_after();
-          product_cols<BF16, HALVES>(tmem + kColAcc0, tmem + kColDS2 + (ph ^ 1) * 64, k_cols + sa * step, i > 1);
-          mma_commit(&m.acc0_done[ph ^ 1]);
+          product_cols<BF16, HALVES>(tmem + kColDQ, tmem + kColDSq, k_cols + sa * step, i > 0);
           mma_commit(&m.a_empty[sa]);
         }
-        if (more) {
-          ok = mbar_wait(&m.b_full[tb], tb_ph, abort_flag, a.status, 10) &&
-               (i < 0 || mbar_wait(&m.dp_read, ph, abort_flag, a.status, 11));
-          if (!ok) break;
+        if (more) {  // and dP(i) (ds_full says so)
+          if (!(ok = mbar_wait(&m.b_full[tb], tb_ph, abort_flag, a.status, 10))) break;
           tc_fence_after();
           product_rows<BF16, HALVES>(tmem + kColDP, do_rows, v_rows + tb * step);
           mma_commit(&m.dp_full);
@@ -548,7 +577,13 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
     const uint32_t lanes = static_cast<uint32_t>(sub * 32) << 16;
     const uint32_t s_addr = tmem + lanes + kColS + cg * 32;
     const uint32_t dp_addr = tmem + lanes + kColDP + cg * 32;
-    const uint32_t ds_addr = tmem + lanes + kColDS2 + cg * 16;
+    const uint32_t ds_addr = tmem + lanes + kColDSq + cg * 16;
+    if (n > 0) {
+      row_to_tmem<HALVES>(tmem + lanes + kColQ, query < a.tq ? a.q.row(bh, query) : nullptr, cg, a.dim);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.own_tmem);
+    }
     const float* stat = a.stat + (int64_t(bh) * a.q_tiles + qt) * (2 * kTile) + row;
     const float nl = stat[0], nd = stat[kTile];
     float gain = 1.f;
@@ -571,10 +606,7 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
       if (lane == 0) mbar_arrive(&m.s_read);
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
-        float x0, x1;
-        unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, nl2), x0, x1);
-        v[c] = __float_as_uint(ex2(x0));
-        v[c + 1] = __float_as_uint(ex2(x1));
+        exp2_pair(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, nl2), v[c], v[c + 1]);
       }
       // a partly valid last key tile: rows past the keys may hold anything,
       // and dS's zeros times inf or NaN would reach dQ
@@ -594,9 +626,6 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
       uint32_t d[32];
       tmem_ld32(dp_addr, d);
       tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&m.dp_read);
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
         uint64_t p = pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
@@ -606,14 +635,12 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
         w[c / 2] = Cvt<T>::pack2(x0, x1);
       }
       if (bad != 0u) clear_pairs(w, bad);
-      // this dS buffer is free once dQ(i-2) has read it
-      if (i > 1 && !(ok = mbar_wait(&m.acc0_done[ph], ((i >> 1) & 1) ^ 1, abort_flag, a.status, 18))) break;
-      tc_fence_after();
-      tmem_st16(ds_addr + ph * 64, w);
+      // dP(i) was issued after dQ(i-1), so dS's columns are free
+      tmem_st16(ds_addr, w);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&m.ds_full[ph]);
+      if (lane == 0) mbar_arrive(&m.ds_full);
     }
     char* orow = query < a.tq ? a.dq.row(bh, query) : nullptr;
     if (n == 0) {
@@ -623,7 +650,7 @@ __device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorM
       tc_fence_after();
       if (ok && !*abort_flag) {
         const float mul = BF16 ? a.scale : a.scale / (gain * (1 << kShiftP16));
-        store_row<T>(tmem + lanes + kColAcc0, orow, cg * 32 * HALVES, (cg + 1) * 32 * HALVES, a.dim, mul, seen <= 0);
+        store_row<T>(tmem + lanes + kColDQ, orow, cg * 32 * HALVES, (cg + 1) * 32 * HALVES, a.dim, mul, seen <= 0);
       }
     }
   }
@@ -648,7 +675,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       mbar_init(&m.a_full[s], 1);
       mbar_init(&m.a_empty[s], 1);
     }
-    for (int s = 0; s < kStagesB; ++s) {
+    for (int s = 0; s < kMaxB; ++s) {
       mbar_init(&m.b_full[s], 1);
       mbar_init(&m.b_empty[s], 1);
     }
@@ -660,12 +687,10 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     mbar_init(&m.s_read, kElemWarps);
     mbar_init(&m.p_full, kElemWarps);
     mbar_init(&m.dp_full, 1);
-    mbar_init(&m.ds_full[0], kElemWarps);
-    mbar_init(&m.ds_full[1], kElemWarps);
+    mbar_init(&m.ds_full, kElemWarps);
     mbar_init(&m.dp_read, kElemWarps);
-    mbar_init(&m.acc0_done[0], 1);
-    mbar_init(&m.acc0_done[1], 1);
-    mbar_init(&m.acc1_done, 1);
+    mbar_init(&m.dk_done, 1);
+    mbar_init(&m.own_tmem, kElemWarps);
     mbar_init(&m.all_done, 1);
     fence_barrier_init();
     fence_proxy_async_smem();
@@ -837,7 +862,7 @@ cudaError_t launch_attn_grad(const AttnGradCall& c, int* status, cudaStream_t st
   else attn_grad_stat_kernel<__half><<<s.q_blocks + v_blocks, 256, 0, st>>>(s);
   if ((err = cudaGetLastError()) != cudaSuccess) return err;
   GradArgs a{};
-  a.dq = make_rows(*c.dq), a.dk = make_rows(*c.dk), a.dv = make_rows(*c.dv);
+  a.q = make_rows(q), a.dq = make_rows(*c.dq), a.dk = make_rows(*c.dk), a.dv = make_rows(*c.dv);
   a.stat = s.stat;
   a.maxima = s.maxima;
   a.key_lengths = c.key_lengths;

@@ -107,7 +107,7 @@ SIGNATURES: dict[str, tuple] = {
     "b2_pack_block_bias": (ctypes.c_int, [_VP, _I32, _I64, _I64, _I64, _I32, _I32, _VP, _VP]),
     # views and b2_rotary structs of these arrive packed (bytes) or by reference
     "b2_attention_forward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _F32, _I32, _VP, _VP, _VP]),
-    "b2_attention_backward_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32]),
+    "b2_attention_backward_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32]),
     "b2_attention_backward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _F32, _I32, _VP, _VP, _VP]),
     "b2_axial_rope": (ctypes.c_int, [_VP, _VP, _VP, _VP]),
     "b2_qk_norm_rope": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _I32, _F32, _VP, _VP]),

@@ -127,7 +127,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     with on_device(q):
         out, dout, lse = as_rows(out, broadcast=False), as_rows(dout, broadcast=False), lse.contiguous()
         dq, dk, dv = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1]), new_rows(k, k.shape, strides[1])
-        ws = torch.empty(LIB.b2_attention_backward_workspace_bytes(batch, heads, k.shape[1], tokens), device=q.device,
+        ws = torch.empty(LIB.b2_attention_backward_workspace_bytes(batch, heads, k.shape[1], tokens, k.shape[2]), device=q.device,
                          dtype=torch.uint8)
         check(LIB.b2_attention_backward(
             with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]),

@@ -6,30 +6,35 @@
 //   dV = P^T dout        dP = dout V^T        dS = P * (dP - delta)
 //   dQ = scale dS K      dK = scale dS^T Q
 //
-// Two kinds of CTA share one launch:
-//   dK/dV: owns 128 keys of one key/value head and walks the query tiles of
-//     every query head of its group: S^T = K Q^T, dP^T = V dO^T (keys are the
-//     rows, so P^T and dS^T are written back to tensor memory as they come and
-//     are the A operands of dV += P^T dO and dK += dS^T Q);
-//   dQ: owns 128 queries of one head and walks the key tiles: S = Q K^T,
+// Two kinds of work item share one launch of persistent CTAs, one per SM,
+// which take items from a counter (the longer dK/dV items first):
+//   dK/dV: 128 keys of one key/value head against the query tiles of every
+//     query head of its group: S^T = K Q^T, dP^T = V dO^T (keys are the rows,
+//     so P^T and dS^T are written back to tensor memory as they come and are
+//     the A operands of dV += P^T dO and dK += dS^T Q);
+//   dQ: 128 queries of one head against the key tiles: S = Q K^T,
 //     dP = dO V^T, dQ += dS K.
 // S and dP are so computed twice: seven products instead of the formula's
 // five.  In return no partial dQ leaves the CTA that owns it: no FP32 scratch
-// of dQ's size, no atomics, and results that do not depend on the order CTAs
-// run in.  A single pass would add 64 KB of FP32 reductions to L2 and a dS
-// tile in shared memory for each pair of tiles, and is bound by shared-memory
-// bandwidth (about 3750 cycles a pair at 128 B a cycle, against 7 * 512 for
-// the products here).
+// of dQ's size, no atomics on results, and results that do not depend on the
+// order items run in.  A single pass would add 64 KB of FP32 reductions to L2
+// and a dS tile in shared memory for each pair of tiles, and is bound by
+// shared-memory bandwidth (about 3750 cycles a pair at 128 B a cycle, against
+// 7 * 512 for the products here).
 //
-// Warp roles (576 threads, one CTA per SM): warp 0 TMA producer, warp 1 MMA
-// issuer and TMEM owner, warps 2..17 elementwise (warp % 4 is the TMEM lane
-// quadrant, and each group of four warps takes 32 columns of a tile).
+// Warp roles (576 threads): warp 0 TMA producer and item scheduler, warp 1
+// MMA issuer and TMEM owner, warps 2..17 elementwise (warp % 4 is the TMEM
+// lane quadrant, and each group of four warps takes 32 columns of a tile).
+// Rings, barriers and tensor memory live across items: an item's first tiles
+// load and its first S and dP run while the one before stores its results.
 //
 // Precision: products of 16-bit operands accumulated in FP32; P and dS are
-// rounded to the inputs' type once, as operands.  FP16 has too small a range
-// for them, so there P is held times 2^8 and dS times a power of two chosen
-// from the largest norms of dO and V rows (|dP - delta| <= 2 |dO||V|), which
-// cannot overflow; both are taken out again in FP32 at the end.
+// rounded once, as operands: P to the type of v, dS to that of q and k.  FP16
+// has too small a range for them.  With FP16 v, P is held times 2^8; FP16 dS
+// is held times a power of two chosen from the largest norms of dO and V rows
+// (|dP - delta| <= 2 |dO||V|), which cannot overflow; both are taken out again
+// in FP32 at the end.  QK16: q and k are FP16 copies (times a power of two
+// each) of what v's BF16 could hold less exactly, and dQ, dK leave in FP32.
 #include <cudaTypedefs.h>
 
 #include <type_traits>
@@ -50,10 +55,10 @@ constexpr uint32_t kHalfBytes = kTile * 128;  // 128 rows x 64 16-bit columns
 constexpr uint32_t kStatBytes = 2 * kTile * 4;
 // Rings of the walked tiles.  K (or Q) is read by the first and the last
 // product of its tile pair, so with two stages each pair waits for its load.
-// The second ring gets what the CTA's own tiles leave.
-constexpr int kStagesA = 3, kStagesDkv = 2, kStagesDq = 3, kMaxB = 3;
+constexpr int kStagesA = 3, kStagesB = 2;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kShiftP16 = 8;  // FP16: P is held times 2^8
+constexpr int kShiftP16 = 8;  // FP16 v: P is held times 2^8
+constexpr int kStatRows = 64;  // rows of a block of the statistics kernel
 
 // TMEM columns.
 //   dK/dV: S and dP take turns in kColX (each is free again as soon as the
@@ -61,33 +66,39 @@ constexpr int kShiftP16 = 8;  // FP16: P is held times 2^8
 //   dQ: S, dP, dQ, dS, and Q: as the A operand of S it costs no shared-memory
 //     reads there, whose 128 bytes a cycle A and B of a 128 x 128 product
 //     take all of (1.53 ms against 1.69 for all of dQ).  The same for V in the
-//     dK/dV CTAs needs P and dS to share columns, and their products to wait
+//     dK/dV items needs P and dS to share columns, and their products to wait
 //     for one another: 2.20 ms against 2.06.
 constexpr uint32_t kColX = 0, kColP = 128, kColDS = 192, kColDV = 256, kColDK = 384;
 constexpr uint32_t kColS = 0, kColDP = 128, kColDQ = 256, kColDSq = 384, kColQ = 448;
 
 struct GradArgs {
-  Rows q, dq, dk, dv;
+  Rows dq, dk, dv;
   const float* stat;       // [B*H][query tiles][2][128]: -lse*log2e (+ shift), -delta
-  const uint32_t* maxima;  // FP16: [B*Hk][2] bits of the largest squared norms of dO and V rows
+  const float* do_norm;    // [B*H][2 * query tiles] largest squared norms of dO rows, by 64 rows
+  const float* v_norm;     // [B*Hk][v_blocks] the same of the valid V rows
+  const float* qk_scale;   // QK16: the powers of two q and k are held times, or NULL
+  int* counter;            // the next item
   const int32_t* key_lengths;
   int heads, kv_heads, group;
   int tq, tk, dim;
-  int q_tiles, k_tiles;
-  int n_dkv;  // CTAs of the dK/dV kind (they come first)
+  int q_tiles, k_tiles, v_blocks;
+  int n_dkv, n_items;  // items of the dK/dV kind (they come first), and all
   int causal;
   float scale, scale_log2;
   int* status;
 };
 
 struct __align__(8) Misc {
-  uint64_t own_full;      // the CTA's own tile (two for dK/dV) in shared memory
-  uint64_t own_tmem;      // dQ: Q in tensor memory
+  uint64_t item_full[2], item_empty[2];
+  uint64_t own_full, own_empty;  // the item's own two tiles in shared memory
+  uint64_t own_tmem;             // dQ: Q in tensor memory
   uint64_t a_full[kStagesA], a_empty[kStagesA];  // walked tiles: Q or K
-  uint64_t b_full[kMaxB], b_empty[kMaxB];  // dO or V
+  uint64_t b_full[kStagesB], b_empty[kStagesB];  // dO or V
   uint64_t stat_full[2], stat_empty[2];          // -lse and -delta of a query tile
-  uint64_t s_full, s_read, p_full, dp_full, dp_read, ds_full;
-  uint64_t dk_done, all_done;
+  uint64_t s_full, s_read, p_full, dp_full, dp_read, ds_full, dk_done;
+  uint64_t acc_full, acc_free;  // the item's results are complete; are stored
+  uint64_t exit_done;
+  int item[2];
   uint32_t tmem;
   int abort_flag;
 };
@@ -95,10 +106,10 @@ struct __align__(8) Misc {
 template <int HALVES>
 struct Smem {
   static constexpr uint32_t tile = HALVES * kHalfBytes;
-  static constexpr uint32_t a = 0;
-  static constexpr uint32_t own = a + kStagesA * tile;  // dK/dV: K and V; dQ: dO
-  static constexpr uint32_t b_dkv = own + 2 * tile, b_dq = own + tile;
-  static constexpr uint32_t stat = own + 4 * tile;  // [2]
+  static constexpr uint32_t own = 0;  // dK/dV: K and V; dQ: dO and Q
+  static constexpr uint32_t a = own + 2 * tile;
+  static constexpr uint32_t b = a + kStagesA * tile;
+  static constexpr uint32_t stat = b + kStagesB * tile;  // [2]
   static constexpr uint32_t misc = stat + 2 * kStatBytes;
   // one CTA per SM (each owns all 512 TMEM columns)
   static constexpr uint32_t used = misc + sizeof(Misc);
@@ -202,16 +213,16 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
-// One row of the CTA's own operand to tensor memory: columns cg*32 .. +31 of
-// the head dimension (zeros past it, and for no row) by column group cg.
+// Columns cg*32 .. +31 of row `row` of a tile in shared memory (as TMA wrote
+// it: 128-byte rows, 16-byte chunks swizzled by the row) to tensor memory.
 template <int HALVES>
-__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const char* row, int cg, int dim) {
+__device__ __forceinline__ void row_to_tmem(uint32_t taddr, const char* tile, int row, int cg) {
   if (cg >= 2 * HALVES) return;
+  const char* src = tile + (cg >> 1) * kHalfBytes + row * 128;
   uint32_t w[16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-    if (row != nullptr && cg * 32 + 8 * i < dim) x = *reinterpret_cast<const uint4*>(row + cg * 64 + 16 * i);
+    const uint4 x = *reinterpret_cast<const uint4*>(src + ((((cg & 1) * 4 + i) ^ (row & 7)) << 4));
     w[4 * i] = x.x, w[4 * i + 1] = x.y, w[4 * i + 2] = x.z, w[4 * i + 3] = x.w;
   }
   tmem_st16(taddr + cg * 16, w);
@@ -231,432 +242,554 @@ __device__ __forceinline__ int key_count(const GradArgs& a, int b) {
   return a.key_lengths != nullptr ? min(max(a.key_lengths[b], 0), a.tk) : a.tk;
 }
 
-// FP16: the power of two dS is held times (P's 2^8 aside), so that
-// 2^8 * 2 max|dO| max|V| times it stays below 2^15.
-__device__ __forceinline__ float ds_gain(const GradArgs& a, int bhk) {
-  const float bound2 = __uint_as_float(a.maxima[2 * bhk]) * __uint_as_float(a.maxima[2 * bhk + 1]);
+// A warp's largest of n non-negative values.
+__device__ __forceinline__ float warp_most(const float* x, int64_t n, int lane) {
+  float most = 0.f;
+  for (int64_t i = lane; i < n; i += 32) most = fmaxf(most, x[i]);
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
+  return most;
+}
+
+// FP16 dS: the power of two it is held times (the shift of P aside), so that
+// 2^shift * 2 max|dO| max|V| times it stays below 2^15.
+__device__ __forceinline__ float ds_gain(const GradArgs& a, int b, int hk, int shift, int lane) {
+  const int64_t bh = int64_t(b) * a.heads + int64_t(hk) * a.group, bhk = int64_t(b) * a.kv_heads + hk;
+  const float bound2 = warp_most(a.do_norm + bh * 2 * a.q_tiles, int64_t(a.group) * 2 * a.q_tiles, lane) *
+                       warp_most(a.v_norm + bhk * a.v_blocks, a.v_blocks, lane);
   if (!(bound2 > 0.f) || !(bound2 < 3e38f)) return 1.f;
-  const int e = 15 - kShiftP16 - 1 - 1 - (ilogbf(bound2) >> 1);  // bound < 2^(ilogb(bound2)/2 + 1)
+  const int e = 15 - shift - 1 - 1 - (ilogbf(bound2) >> 1);  // bound < 2^(ilogb(bound2)/2 + 1)
   return ldexpf(1.f, min(max(e, -60), 60));
 }
 
-// Store 32 FP32 accumulator columns of one row, scaled, as 16-bit.
-template <typename T>
-__device__ __forceinline__ void store_cols(char* row, int c0, int dim, const uint32_t* r, float mul) {
-  uint32_t w[16];
+// 4 x 4 transpose of 16-byte chunks in every four lanes: chunk j of lane q
+// becomes chunk q of lane j.
+__device__ __forceinline__ void transpose_quads(uint32_t (&w)[16], int lane) {
 #pragma unroll
-  for (int c = 0; c < 32; c += 2) w[c / 2] = Cvt<T>::pack2(__uint_as_float(r[c]) * mul, __uint_as_float(r[c + 1]) * mul);
-  uint4* dst = reinterpret_cast<uint4*>(row + c0 * 2);
+  for (int bit = 1; bit <= 2; bit <<= 1) {
+    const bool upper = (lane & bit) != 0;
 #pragma unroll
-  for (int q4 = 0; q4 < 4; ++q4)
-    if (c0 + 8 * q4 < dim) dst[q4] = make_uint4(w[4 * q4], w[4 * q4 + 1], w[4 * q4 + 2], w[4 * q4 + 3]);
+    for (int c = 0; c < 4; ++c) {
+      if (c & bit) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t& lo = w[4 * c + e];
+        uint32_t& hi = w[4 * (c + bit) + e];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? lo : hi, bit);
+        if (upper) lo = got;
+        else hi = got;
+      }
+    }
+  }
 }
 
-// Columns [from, to) of one accumulator row at `taddr` to global memory; a row
-// that sees nothing (or lies past the keys) is written as zeros.  The loads
-// are a warp's: every lane calls this, row NULL stores nothing.
-template <typename T>
-__device__ __forceinline__ void store_row(uint32_t taddr, char* row, int from, int to, int dim, float mul, bool zero) {
+// Rows of a result tile in global memory.
+struct OutTile {
+  char* base;  // row 0
+  int64_t step;
+  int rows, dim;  // that exist; columns
+};
+
+// Columns [from, to) of a warp's 32 accumulator rows at `taddr` to global
+// memory, scaled; `zero` rows (that see nothing, or lie past the keys) as
+// zeros.  Four lanes store 64 bytes of a row together: stored by its own lane
+// alone, each row's 16 bytes touch a line of their own, and a tile took 4500
+// cycles.
+template <typename TO>
+__device__ __forceinline__ void store_rows(uint32_t taddr, const OutTile& o, int row, int lane, int from, int to, float mul,
+                                           bool zero) {
+  constexpr int kCols = 64 / sizeof(TO);  // columns of 64 bytes
+  const int q = lane & 3;
 #pragma unroll 1
   for (int c0 = from; c0 < to; c0 += 32) {
     uint32_t r[32];
     tmem_ld32(taddr + c0, r);
     tmem_wait_ld();
-    if (row == nullptr) continue;
-    if (zero) {
 #pragma unroll
-      for (int c = 0; c < 32; ++c) r[c] = 0u;
+    for (int part = 0; part < 32; part += kCols) {
+      uint32_t w[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        if constexpr (sizeof(TO) == 4) w[e] = __float_as_uint(__uint_as_float(r[part + e]) * mul);
+        else w[e] = Cvt<TO>::pack2(__uint_as_float(r[part + 2 * e]) * mul, __uint_as_float(r[part + 2 * e + 1]) * mul);
+        if (zero) w[e] = 0u;
+      }
+      transpose_quads(w, lane);
+      const int col = c0 + part + q * (kCols / 4);
+      char* dst = o.base + int64_t(row - q) * o.step + col * int(sizeof(TO));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (row - q + j < o.rows && col < o.dim)
+          *reinterpret_cast<uint4*>(dst + j * o.step) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
     }
-    store_cols<T>(row, c0, dim, r, mul);
   }
 }
 
-template <typename T>
+template <typename TO>
 __device__ __forceinline__ void store_zero_row(char* row, int dim) {
-  for (int c = 0; c < dim; c += 8) *reinterpret_cast<uint4*>(row + c * 2) = make_uint4(0u, 0u, 0u, 0u);
+  for (int c = 0; c < dim * int(sizeof(TO)); c += 16) *reinterpret_cast<uint4*>(row + c) = make_uint4(0u, 0u, 0u, 0u);
 }
 
-// ------------------------------------------------------------ dK and dV
-template <bool BF16, int HALVES>
-__device__ __forceinline__ void dkv_cta(const CUtensorMap* q_map, const CUtensorMap* k_map, const CUtensorMap* v_map,
-                                        const CUtensorMap* do_map, const GradArgs& a, char* smem, Misc& m,
-                                        uint32_t tmem) {
-  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  using L = Smem<HALVES>;
-  const int warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31;
-  const int kt = blockIdx.x % a.k_tiles;
-  const int bhk = blockIdx.x / a.k_tiles;
-  const int b = bhk / a.kv_heads;
-  const int hk = bhk - b * a.kv_heads;
-  const int k0 = kt * kTile;
-  const int len = key_count(a, b);
-  const int off = a.tk - a.tq;  // causal: query i sees keys up to i + off
-  const int first = a.causal ? max(0, k0 - off) / kTile : 0;
-  const int per_head = k0 < len ? a.q_tiles - first : 0;
-  const int n = per_head * a.group;
-  volatile int* abort_flag = &m.abort_flag;
+// ------------------------------------------------------------ items
+struct Work {
+  bool dkv;
+  int b, h, hk;  // batch, query head (dQ), key/value head
+  int r0;        // the first of its own 128 rows
+  int len;       // keys of the batch
+  int n;         // tile pairs
+  int first, per_head;  // dK/dV: the first query tile, and how many of each head
+};
 
-  if (warp == 0) {
-    if (lane == 0 && n > 0 && !*abort_flag) {
-      mbar_expect_tx(&m.own_full, 2 * L::tile);
-      load_tile<HALVES>(smem + L::own, k_map, &m.own_full, k0, hk, b);
-      load_tile<HALVES>(smem + L::own + L::tile, v_map, &m.own_full, k0, hk, b);
-      int na = 0, nb = 0, ns = 0;
-      for (int i = 0; i < n; ++i) {
-        const int sa = i % kStagesA, sb = i % kStagesDkv, ss = i & 1;
-        const int g = i / per_head;
-        const int qt = first + i - g * per_head;
-        const int h = hk * a.group + g;
-        if (!mbar_wait(&m.a_empty[sa], ((i / kStagesA) & 1) ^ 1, abort_flag, a.status, 1)) break;
-        mbar_expect_tx(&m.a_full[sa], L::tile);
-        load_tile<HALVES>(smem + L::a + sa * L::tile, q_map, &m.a_full[sa], qt * kTile, h, b);
-        na = i + 1;
-        if (!mbar_wait(&m.stat_empty[ss], ((i >> 1) & 1) ^ 1, abort_flag, a.status, 17)) break;
-        mbar_expect_tx(&m.stat_full[ss], kStatBytes);
-        bulk_load(smem + L::stat + ss * kStatBytes, a.stat + ((int64_t(b) * a.heads + h) * a.q_tiles + qt) * (2 * kTile),
-                  kStatBytes, &m.stat_full[ss]);
-        ns = i + 1;
-        if (!mbar_wait(&m.b_empty[sb], ((i / kStagesDkv) & 1) ^ 1, abort_flag, a.status, 2)) break;
-        mbar_expect_tx(&m.b_full[sb], L::tile);
-        load_tile<HALVES>(smem + L::b_dkv + sb * L::tile, do_map, &m.b_full[sb], qt * kTile, h, b);
-        nb = i + 1;
+__device__ __forceinline__ Work decode(const GradArgs& a, int id) {
+  Work w;
+  const int off = a.tk - a.tq;  // causal: query i sees keys up to i + off
+  w.dkv = id < a.n_dkv;
+  if (w.dkv) {
+    const int bhk = id / a.k_tiles;
+    w.r0 = (id - bhk * a.k_tiles) * kTile;
+    w.b = bhk / a.kv_heads;
+    w.h = 0;
+    w.hk = bhk - w.b * a.kv_heads;
+    w.len = key_count(a, w.b);
+    w.first = a.causal ? max(0, w.r0 - off) / kTile : 0;
+    w.per_head = w.r0 < w.len ? a.q_tiles - w.first : 0;
+    w.n = w.per_head * a.group;
+  } else {
+    id -= a.n_dkv;
+    const int bh = id / a.q_tiles;
+    w.r0 = (a.q_tiles - 1 - (id - bh * a.q_tiles)) * kTile;  // causal: the longest first
+    w.b = bh / a.heads;
+    w.h = bh - w.b * a.heads;
+    w.hk = w.h / a.group;
+    w.len = key_count(a, w.b);
+    const int keys = a.causal ? min(w.len, min(w.r0 + kTile, a.tq) + off) : w.len;  // that any of the rows sees
+    w.first = w.per_head = 0;
+    w.n = keys > 0 ? (keys + kTile - 1) / kTile : 0;
+  }
+  return w;
+}
+
+// A place in a ring of barriers: stage and the parity of its current phase.
+template <int STAGES>
+struct Place {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++s == STAGES) s = 0, ph ^= 1u;
+  }
+};
+
+// The next item, published by the producer (-1: none left, or aborted).
+__device__ __forceinline__ int next_item(Misc& m, Place<2>& at, volatile int* abort_flag, int* status) {
+  if (!mbar_wait(&m.item_full[at.s], at.ph, abort_flag, status, 20)) return -1;
+  return *const_cast<volatile int*>(&m.item[at.s]);
+}
+
+// ------------------------------------------------------------ TMA producer
+template <int HALVES>
+__device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, const CUtensorMap* v_map,
+                        const CUtensorMap* do_map, const GradArgs& a, char* smem, Misc& m) {
+  using L = Smem<HALVES>;
+  volatile int* abort_flag = &m.abort_flag;
+  Place<2> at, st;
+  Place<kStagesA> pa;
+  Place<kStagesB> pb;
+  int na = 0, nb = 0, ns = 0, owns = 0;
+  bool ok = !*abort_flag;
+  while (ok) {
+    const int id = atomicAdd(a.counter, 1);
+    if (!(ok = mbar_wait(&m.item_empty[at.s], at.ph ^ 1, abort_flag, a.status, 21))) break;
+    *const_cast<volatile int*>(&m.item[at.s]) = id < a.n_items ? id : -1;
+    mbar_arrive(&m.item_full[at.s]);
+    at.next();
+    if (id >= a.n_items) break;
+    const Work w = decode(a, id);
+    int g = 0, qt = w.first;  // dK/dV: head of the group and query tile
+    for (int i = 0; ok && i < w.n; ++i) {
+      const int h = w.hk * a.group + g;
+      const int row = (w.dkv ? qt : i) * kTile, head = w.dkv ? h : w.hk;
+      if (!(ok = mbar_wait(&m.a_empty[pa.s], pa.ph ^ 1, abort_flag, a.status, 1))) break;
+      mbar_expect_tx(&m.a_full[pa.s], L::tile);
+      load_tile<HALVES>(smem + L::a + pa.s * L::tile, w.dkv ? q_map : k_map, &m.a_full[pa.s], row, head, w.b);
+      pa.next(), ++na;
+      if (w.dkv) {
+        if (!(ok = mbar_wait(&m.stat_empty[st.s], st.ph ^ 1, abort_flag, a.status, 17))) break;
+        mbar_expect_tx(&m.stat_full[st.s], kStatBytes);
+        bulk_load(smem + L::stat + st.s * kStatBytes,
+                  a.stat + ((int64_t(w.b) * a.heads + h) * a.q_tiles + qt) * (2 * kTile), kStatBytes, &m.stat_full[st.s]);
+        st.next(), ++ns;
       }
-      if (*abort_flag) {
-        drain_loads(m.a_full, kStagesA, na, &m.own_full, a.status);
-        drain_loads(m.b_full, kStagesDkv, nb, nullptr, a.status);
-        drain_loads(m.stat_full, 2, ns, nullptr, a.status);
+      if (!(ok = mbar_wait(&m.b_empty[pb.s], pb.ph ^ 1, abort_flag, a.status, 2))) break;
+      mbar_expect_tx(&m.b_full[pb.s], L::tile);
+      load_tile<HALVES>(smem + L::b + pb.s * L::tile, w.dkv ? do_map : v_map, &m.b_full[pb.s], row, head, w.b);
+      pb.next(), ++nb;
+      if (i == 0) {  // the own tiles, once the item before has read its own
+        if (!(ok = mbar_wait(&m.own_empty, (owns & 1) ^ 1, abort_flag, a.status, 22))) break;
+        mbar_expect_tx(&m.own_full, 2 * L::tile);
+        load_tile<HALVES>(smem + L::own, w.dkv ? k_map : do_map, &m.own_full, w.r0, w.dkv ? w.hk : w.h, w.b);
+        load_tile<HALVES>(smem + L::own + L::tile, w.dkv ? v_map : q_map, &m.own_full, w.r0, w.dkv ? w.hk : w.h, w.b);
+        ++owns;
       }
+      if (++qt == w.first + w.per_head) qt = w.first, ++g;
     }
-  } else if (warp == 1) {
-    if (n > 0 && elect_one()) {
-      const uint32_t base = smem_u32(smem);
-      const uint64_t k_rows = rows_desc(base + L::own), v_rows = rows_desc(base + L::own + L::tile);
-      const uint64_t q_rows = rows_desc(base + L::a), q_cols = cols_desc(base + L::a);  // stage 0; stages L::tile apart
-      const uint64_t do_rows = rows_desc(base + L::b_dkv), do_cols = cols_desc(base + L::b_dkv);
-      constexpr uint32_t step = L::tile >> 4;
-      bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3);
-      // Order S(i+1), dV(i), dP(i+1), dK(i): S and dP wait for the elementwise
-      // warps to have loaded the other out of their common columns, and dV or
-      // dK runs while they do.
-      for (int i = -1; ok && i < n; ++i) {
-        const int sa = i < 0 ? 0 : i % kStagesA, sb = i < 0 ? 0 : i % kStagesDkv;
-        const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesDkv;  // the next tiles' stages and phases
-        const uint32_t ph = i & 1, next = ph ^ 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesDkv) & 1;
-        const bool more = i + 1 < n;
+  }
+  if (*abort_flag) {
+    int no_abort = 0;
+    drain_loads(m.a_full, kStagesA, na, nullptr, a.status);
+    drain_loads(m.b_full, kStagesB, nb, nullptr, a.status);
+    drain_loads(m.stat_full, 2, ns, nullptr, a.status);
+    if (owns > 0) mbar_wait(&m.own_full, (owns - 1) & 1, &no_abort, a.status, 31);
+  }
+}
+
+// ------------------------------------------------------------ MMA issuer
+template <bool VBF16, bool QBF16, int HALVES>
+__device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
+  using L = Smem<HALVES>;
+  volatile int* abort_flag = &m.abort_flag;
+  const uint32_t base = smem_u32(smem);
+  constexpr uint32_t step = L::tile >> 4;  // stages are L::tile apart
+  const uint64_t own0 = rows_desc(base + L::own), own1 = rows_desc(base + L::own + L::tile);
+  const uint64_t a_rows = rows_desc(base + L::a), a_cols = cols_desc(base + L::a);
+  const uint64_t b_rows = rows_desc(base + L::b), b_cols = cols_desc(base + L::b);
+  Place<2> at;
+  Place<kStagesA> ca, ta;  // stages of tile i and of tile i + 1
+  Place<kStagesB> cb, tb;
+  uint32_t it = 0;   // tile pairs so far: every barrier of a pair completes once a pair
+  int owns = 0, dqs = 0;
+  bool ok = true;
+  while (ok) {
+    const int id = next_item(m, at, abort_flag, a.status);
+    if (id < 0) break;
+    mbar_arrive(&m.item_empty[at.s]);
+    at.next();
+    const Work w = decode(a, id);
+    if (w.n == 0) continue;
+    // the last item's products are complete: nothing is read any more from
+    // the columns and tiles that this one fills
+    ok = (owns == 0 || mbar_wait(&m.acc_full, (owns - 1) & 1, abort_flag, a.status, 24)) &&
+         mbar_wait(&m.own_full, owns & 1, abort_flag, a.status, 3) &&
+         (w.dkv || mbar_wait(&m.own_tmem, dqs & 1, abort_flag, a.status, 4));
+    if (!ok) break;
+    tc_fence_after();
+    for (int i = -1; i < w.n; ++i) {
+      const uint32_t ph = (it + i) & 1, next = ph ^ 1;
+      const bool more = i + 1 < w.n;
+      if (w.dkv) {
+        // Order S(i+1), dV(i), dP(i+1), dK(i): S and dP wait for the
+        // elementwise warps to have loaded the other out of their common
+        // columns, and dV or dK runs while they do.
         if (more) {
-          ok = mbar_wait(&m.a_full[ta], ta_ph, abort_flag, a.status, 7) &&
+          ok = mbar_wait(&m.a_full[ta.s], ta.ph, abort_flag, a.status, 7) &&
                (i < 0 || mbar_wait(&m.dp_read, ph, abort_flag, a.status, 8));
           if (!ok) break;
           tc_fence_after();
-          product_rows<BF16, HALVES>(tmem + kColX, k_rows, q_rows + ta * step);
+          product_rows<QBF16, HALVES>(tmem + kColX, own0, a_rows + ta.s * step);
           mma_commit(&m.s_full);
+          ta.next();
         }
         if (i >= 0) {
-          if (!(ok = mbar_wait(&m.p_full, ph, abort_flag, a.status, 6))) break;
+          ok = mbar_wait(&m.p_full, ph, abort_flag, a.status, 6) &&
+               (i > 0 || owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 25));
+          if (!ok) break;
           tc_fence_after();
-          product_cols<BF16, HALVES>(tmem + kColDV, tmem + kColP, do_cols + sb * step, i > 0);
-          mma_commit(&m.b_empty[sb]);
+          product_cols<VBF16, HALVES>(tmem + kColDV, tmem + kColP, b_cols + cb.s * step, i > 0);
+          mma_commit(&m.b_empty[cb.s]);
+          cb.next();
         }
         if (more) {
-          ok = mbar_wait(&m.b_full[tb], tb_ph, abort_flag, a.status, 10) &&
+          ok = mbar_wait(&m.b_full[tb.s], tb.ph, abort_flag, a.status, 10) &&
                mbar_wait(&m.s_read, next, abort_flag, a.status, 11);
           if (!ok) break;
           tc_fence_after();
-          product_rows<BF16, HALVES>(tmem + kColX, v_rows, do_rows + tb * step);
+          product_rows<VBF16, HALVES>(tmem + kColX, own1, b_rows + tb.s * step);
           mma_commit(&m.dp_full);
+          tb.next();
         }
         if (i >= 0) {
           if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
           tc_fence_after();
-          product_cols<BF16, HALVES>(tmem + kColDK, tmem + kColDS, q_cols + sa * step, i > 0);
+          product_cols<QBF16, HALVES>(tmem + kColDK, tmem + kColDS, a_cols + ca.s * step, i > 0);
           mma_commit(&m.dk_done);
-          mma_commit(&m.a_empty[sa]);
+          mma_commit(&m.a_empty[ca.s]);
+          ca.next();
         }
-      }
-      // every product completes before TMEM is read and released (bounded by
-      // time only, even after an abort)
-      mma_commit(&m.all_done);
-      int no_abort = 0;
-      mbar_wait(&m.all_done, 0, &no_abort, a.status, 12);
-    }
-  } else {
-    const int cg = (warp - 2) >> 2;  // column group: queries cg*32 .. +31 of a tile
-    const int sub = warp & 3;
-    const int row = sub * 32 + lane;
-    const int key = k0 + row;
-    const uint32_t lanes = static_cast<uint32_t>(sub * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + kColX + cg * 32;
-    const uint32_t p_addr = tmem + lanes + kColP + cg * 16, ds_addr = tmem + lanes + kColDS + cg * 16;
-    float gain = 1.f;
-    if constexpr (!BF16) gain = ds_gain(a, bhk);
-    const uint64_t gain2 = pack_f2(gain, gain);
-    const uint64_t scale2 = pack_f2(a.scale_log2, a.scale_log2);
-    bool ok = true;
-    int qt = 0;  // query tile after the first
-    for (int i = 0; i < n; ++i) {
-      const int s = i & 1;
-      const uint32_t ph = i & 1;
-      const float* stat = reinterpret_cast<const float*>(smem + L::stat + s * kStatBytes) + cg * 32;
-      uint32_t bad = 0u;  // causal: columns below `lim` are queries before the key
-      if (a.causal) {
-        const int lim = key - off - (first + qt) * kTile - cg * 32;
-        bad = lim <= 0 ? 0u : lim >= 32 ? ~0u : (1u << lim) - 1u;
-        qt = qt + 1 < per_head ? qt + 1 : 0;
-      }
-      if (!(ok = mbar_wait(&m.stat_full[s], (i >> 1) & 1, abort_flag, a.status, 13))) break;
-      if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
-      tc_fence_after();
-      uint32_t v[32], w[16];
-      tmem_ld32(s_addr, v);
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&m.s_read);
-#pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        const float4 nl = *reinterpret_cast<const float4*>(stat + c);
-        exp2_pair(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, pack_f2(nl.x, nl.y)),
-                  v[c], v[c + 1]);
-        exp2_pair(fma_f2(pack_f2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, pack_f2(nl.z, nl.w)),
-                  v[c + 2], v[c + 3]);
-        w[c / 2] = Cvt<T>::pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-        w[c / 2 + 1] = Cvt<T>::pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
-      }
-      if (bad != 0u) clear_pairs(w, bad);
-      // dP(i) was issued after dV(i-1), so with it done P's columns are free
-      if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
-      tc_fence_after();
-      uint32_t d[32];
-      tmem_st16(p_addr, w);
-      tmem_ld32(s_addr, d);
-      tmem_wait_st();
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&m.dp_read);
-        mbar_arrive(&m.p_full);
-      }
-      // dS = P (dP - delta)
-#pragma unroll
-      for (int c = 0; c < 32; c += 4) {
-        const float4 nd = *reinterpret_cast<const float4*>(stat + kTile + c);
-#pragma unroll
-        for (int e = c; e < c + 4; e += 2) {
-          uint64_t p = pack_f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
-          if constexpr (!BF16) p = mul_f2(p, gain2);
-          const uint64_t x = mul_f2(p, add_f2(pack_f2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])),
-                                              e == c ? pack_f2(nd.x, nd.y) : pack_f2(nd.z, nd.w)));
-          float x0, x1;
-          unpack_f2(x, x0, x1);
-          w[e / 2] = Cvt<T>::pack2(x0, x1);
-        }
-      }
-      if (bad != 0u) clear_pairs(w, bad);  // 0 * inf
-      if (i > 0 && !(ok = mbar_wait(&m.dk_done, ph ^ 1, abort_flag, a.status, 19))) break;  // the last dS is read
-      tc_fence_after();
-      tmem_st16(ds_addr, w);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&m.stat_empty[s]);
-        mbar_arrive(&m.ds_full);
-      }
-    }
-    // column groups 0 and 1 store the halves of dV, 2 and 3 those of dK
-    const bool is_dk = cg >= 2;
-    const Rows& out = is_dk ? a.dk : a.dv;
-    char* orow = key < a.tk ? out.row(bhk, key) : nullptr;
-    if (n == 0) {
-      if (orow != nullptr && (cg & 1) == 0) store_zero_row<T>(orow, a.dim);
-    } else {
-      ok = ok && mbar_wait(&m.all_done, 0, abort_flag, a.status, 16);
-      tc_fence_after();
-      if (ok && !*abort_flag) {
-        const float p_mul = BF16 ? 1.f : 1.f / (1 << kShiftP16);
-        const float mul = is_dk ? a.scale * p_mul / gain : p_mul;
-        const int from = (cg & 1) * 32 * HALVES;
-        store_row<T>(tmem + lanes + (is_dk ? kColDK : kColDV), orow, from, from + 32 * HALVES, a.dim, mul, key >= len);
-      }
-    }
-  }
-}
-
-// ------------------------------------------------------------ dQ
-template <bool BF16, int HALVES>
-__device__ __forceinline__ void dq_cta(const CUtensorMap* q_map, const CUtensorMap* k_map, const CUtensorMap* v_map,
-                                       const CUtensorMap* do_map, const GradArgs& a, char* smem, Misc& m,
-                                       uint32_t tmem) {
-  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
-  using L = Smem<HALVES>;
-  const int warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31;
-  const int id = blockIdx.x - a.n_dkv;
-  const int bh = id / a.q_tiles;
-  const int qt = a.q_tiles - 1 - (id - bh * a.q_tiles);  // causal: the longest first
-  const int b = bh / a.heads;
-  const int h = bh - b * a.heads;
-  const int hk = h / a.group;
-  const int q0 = qt * kTile;
-  const int len = key_count(a, b);
-  const int off = a.tk - a.tq;
-  const int keys = a.causal ? min(len, min(q0 + kTile, a.tq) + off) : len;  // keys any of the rows sees
-  const int n = keys > 0 ? (keys + kTile - 1) / kTile : 0;
-  volatile int* abort_flag = &m.abort_flag;
-
-  if (warp == 0) {
-    if (lane == 0 && n > 0 && !*abort_flag) {
-      mbar_expect_tx(&m.own_full, L::tile);
-      load_tile<HALVES>(smem + L::own, do_map, &m.own_full, q0, h, b);
-      int na = 0, nb = 0;
-      for (int i = 0; i < n; ++i) {
-        const int sa = i % kStagesA, sb = i % kStagesDq;
-        if (!mbar_wait(&m.a_empty[sa], ((i / kStagesA) & 1) ^ 1, abort_flag, a.status, 1)) break;
-        mbar_expect_tx(&m.a_full[sa], L::tile);
-        load_tile<HALVES>(smem + L::a + sa * L::tile, k_map, &m.a_full[sa], i * kTile, hk, b);
-        na = i + 1;
-        if (!mbar_wait(&m.b_empty[sb], ((i / kStagesDq) & 1) ^ 1, abort_flag, a.status, 2)) break;
-        mbar_expect_tx(&m.b_full[sb], L::tile);
-        load_tile<HALVES>(smem + L::b_dq + sb * L::tile, v_map, &m.b_full[sb], i * kTile, hk, b);
-        nb = i + 1;
-      }
-      if (*abort_flag) {
-        drain_loads(m.a_full, kStagesA, na, &m.own_full, a.status);
-        drain_loads(m.b_full, kStagesDq, nb, nullptr, a.status);
-      }
-    }
-  } else if (warp == 1) {
-    if (n > 0 && elect_one()) {
-      const uint32_t base = smem_u32(smem);
-      const uint64_t do_rows = rows_desc(base + L::own);
-      const uint64_t k_rows = rows_desc(base + L::a), k_cols = cols_desc(base + L::a);
-      const uint64_t v_rows = rows_desc(base + L::b_dq);
-      constexpr uint32_t step = L::tile >> 4;
-      bool ok = mbar_wait(&m.own_full, 0, abort_flag, a.status, 3) && mbar_wait(&m.own_tmem, 0, abort_flag, a.status, 4);
-      tc_fence_after();
-      // Order S(i+1), dQ(i), dP(i+1): S runs ahead of the exponentials of the
-      // tile before, dP under those of its own.
-      for (int i = -1; ok && i < n; ++i) {
-        const int sa = i < 0 ? 0 : i % kStagesA;
-        const int ta = (i + 1) % kStagesA, tb = (i + 1) % kStagesDq;
-        const uint32_t ph = i & 1, ta_ph = ((i + 1) / kStagesA) & 1, tb_ph = ((i + 1) / kStagesDq) & 1;
-        const bool more = i + 1 < n;
+      } else {
+        // Order S(i+1), dQ(i), dP(i+1): S runs ahead of the exponentials of
+        // the tile before, dP under those of its own.
         if (more) {  // the elementwise warps hold S(i)
-          ok = mbar_wait(&m.a_full[ta], ta_ph, abort_flag, a.status, 7) &&
+          ok = mbar_wait(&m.a_full[ta.s], ta.ph, abort_flag, a.status, 7) &&
                (i < 0 || mbar_wait(&m.s_read, ph, abort_flag, a.status, 8));
           if (!ok) break;
           tc_fence_after();
-          product_rows_ts<BF16, HALVES>(tmem + kColS, tmem + kColQ, k_rows + ta * step);
+          product_rows_ts<QBF16, HALVES>(tmem + kColS, tmem + kColQ, a_rows + ta.s * step);
           mma_commit(&m.s_full);
+          ta.next();
         }
         if (i >= 0) {
-          if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
+          ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9) &&
+               (i > 0 || owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 25));
+          if (!ok) break;
           tc_fence_after();
-          product_cols<BF16, HALVES>(tmem + kColDQ, tmem + kColDSq, k_cols + sa * step, i > 0);
-          mma_commit(&m.a_empty[sa]);
+          product_cols<QBF16, HALVES>(tmem + kColDQ, tmem + kColDSq, a_cols + ca.s * step, i > 0);
+          mma_commit(&m.a_empty[ca.s]);
+          ca.next();
         }
         if (more) {  // and dP(i) (ds_full says so)
-          if (!(ok = mbar_wait(&m.b_full[tb], tb_ph, abort_flag, a.status, 10))) break;
+          if (!(ok = mbar_wait(&m.b_full[tb.s], tb.ph, abort_flag, a.status, 10))) break;
           tc_fence_after();
-          product_rows<BF16, HALVES>(tmem + kColDP, do_rows, v_rows + tb * step);
+          product_rows<VBF16, HALVES>(tmem + kColDP, own0, b_rows + tb.s * step);
           mma_commit(&m.dp_full);
-          mma_commit(&m.b_empty[tb]);
+          mma_commit(&m.b_empty[tb.s]);
+          tb.next(), cb.next();
         }
       }
-      mma_commit(&m.all_done);
-      int no_abort = 0;
-      mbar_wait(&m.all_done, 0, &no_abort, a.status, 12);
     }
-  } else {
-    const int cg = (warp - 2) >> 2;  // column group: keys cg*32 .. +31 of a tile
-    const int sub = warp & 3;
-    const int row = sub * 32 + lane;
-    const int query = q0 + row;
-    const uint32_t lanes = static_cast<uint32_t>(sub * 32) << 16;
-    const uint32_t s_addr = tmem + lanes + kColS + cg * 32;
-    const uint32_t dp_addr = tmem + lanes + kColDP + cg * 32;
-    const uint32_t ds_addr = tmem + lanes + kColDSq + cg * 16;
-    if (n > 0) {
-      row_to_tmem<HALVES>(tmem + lanes + kColQ, query < a.tq ? a.q.row(bh, query) : nullptr, cg, a.dim);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&m.own_tmem);
+    if (!ok) break;
+    mma_commit(&m.acc_full);
+    mma_commit(&m.own_empty);
+    it += w.n;
+    ++owns;
+    dqs += w.dkv ? 0 : 1;
+  }
+  // every product completes before TMEM is released (bounded by time only,
+  // even after an abort)
+  mma_commit(&m.exit_done);
+  int no_abort = 0;
+  mbar_wait(&m.exit_done, 0, &no_abort, a.status, 12);
+}
+
+// ------------------------------------------------------------ elementwise
+template <bool VBF16, bool QBF16, bool OUT32, int HALVES>
+__device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
+  using T = typename std::conditional<VBF16, __nv_bfloat16, __half>::type;   // v, dO, P
+  using TS = typename std::conditional<QBF16, __nv_bfloat16, __half>::type;  // q, k, dS
+  using TO = typename std::conditional<OUT32, float, TS>::type;              // dQ, dK
+  using L = Smem<HALVES>;
+  constexpr int kShift = VBF16 ? 0 : kShiftP16;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int cg = (warp - 2) >> 2;  // column group: columns cg*32 .. +31 of a tile
+  const int sub = warp & 3;
+  const int row = sub * 32 + lane;
+  const uint32_t lanes = static_cast<uint32_t>(sub * 32) << 16;
+  const int off = a.tk - a.tq;
+  volatile int* abort_flag = &m.abort_flag;
+  float q_scale = 1.f, k_scale = 1.f;
+  if (a.qk_scale != nullptr) q_scale = a.qk_scale[0], k_scale = a.qk_scale[1];
+  const float mul_s = a.scale_log2 / (q_scale * k_scale);
+  const uint64_t scale2 = pack_f2(mul_s, mul_s);
+  Place<2> at, st;
+  uint32_t it = 0;
+  int owns = 0;
+  bool ok = true;
+  bool q_ready = false;  // dQ: the item's Q is in tensor memory already
+  auto fetch = [&](Work& w) {
+    const int id = next_item(m, at, abort_flag, a.status);
+    if (id < 0) return false;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&m.item_empty[at.s]);
+    at.next();
+    w = decode(a, id);
+    return true;
+  };
+  // Q of a dQ item (owns: the item's number among those with products)
+  auto take_q = [&](int number) {
+    if (!mbar_wait(&m.own_full, number & 1, abort_flag, a.status, 27)) return false;
+    row_to_tmem<HALVES>(tmem + lanes + kColQ, smem + L::own + L::tile, row, cg);
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&m.own_tmem);
+    return true;
+  };
+  Work w;
+  bool have = fetch(w);
+  while (have) {
+    const int own = w.r0 + row;  // key or query
+    const int64_t bhk = int64_t(w.b) * a.kv_heads + w.hk, bh = int64_t(w.b) * a.heads + w.h;
+    if (w.n == 0) {  // column groups 0 and 1: zeros for dV and dK, or dQ
+      if (w.dkv && own < a.tk && cg == 0) store_zero_row<T>(a.dv.row(static_cast<int>(bhk), own), a.dim);
+      if (w.dkv && own < a.tk && cg == 1) store_zero_row<TO>(a.dk.row(static_cast<int>(bhk), own), a.dim);
+      if (!w.dkv && own < a.tq && cg == 0) store_zero_row<TO>(a.dq.row(static_cast<int>(bh), own), a.dim);
+      have = fetch(w);
+      continue;
     }
-    const float* stat = a.stat + (int64_t(bh) * a.q_tiles + qt) * (2 * kTile) + row;
-    const float nl = stat[0], nd = stat[kTile];
     float gain = 1.f;
-    if constexpr (!BF16) gain = ds_gain(a, b * a.kv_heads + hk);
-    const uint64_t scale2 = pack_f2(a.scale_log2, a.scale_log2);
-    const uint64_t nl2 = pack_f2(nl, nl), nd2 = pack_f2(nd, nd), gain2 = pack_f2(gain, gain);
-    const int seen = a.causal ? min(len, query + off + 1) : len;  // keys this row sees
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      const uint32_t ph = i & 1;
-      const int lim = seen - i * kTile - cg * 32;  // columns from `lim` on are masked
-      const uint32_t bad = lim >= 32 ? 0u : lim <= 0 ? ~0u : ~0u << lim;
-      if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
-      tc_fence_after();
-      uint32_t v[32], w[16];
-      tmem_ld32(s_addr, v);
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&m.s_read);
-#pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        exp2_pair(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, nl2), v[c], v[c + 1]);
-      }
-      // a partly valid last key tile: rows past the keys may hold anything,
-      // and dS's zeros times inf or NaN would reach dQ
-      const int k0 = i * kTile;
-      if (len < min(k0 + kTile, a.tk)) {
-        const int tid = threadIdx.x - 64;
-        const int from = len - k0, rows = min(kTile, a.tk - k0) - from;
-        char* tile = smem + L::a + (i % kStagesA) * L::tile;
-        for (int x = tid; x < rows * 8 * HALVES; x += 32 * kElemWarps) {
-          const int r = from + x / (8 * HALVES), ch = x % (8 * HALVES);
-          *reinterpret_cast<uint4*>(tile + (ch >> 3) * kHalfBytes + r * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (!QBF16) gain = ds_gain(a, w.b, w.hk, kShift, lane);
+    const uint64_t gain2 = pack_f2(gain, gain);
+    if (w.dkv) {
+      const uint32_t s_addr = tmem + lanes + kColX + cg * 32;
+      const uint32_t p_addr = tmem + lanes + kColP + cg * 16, ds_addr = tmem + lanes + kColDS + cg * 16;
+      int lim = own - off - w.first * kTile - cg * 32;  // causal: columns below it are queries before the key
+      int qt = 0;
+      for (int i = 0; i < w.n; ++i) {
+        const uint32_t ph = (it + i) & 1;
+        const float* stat = reinterpret_cast<const float*>(smem + L::stat + st.s * kStatBytes) + cg * 32;
+        uint32_t bad = 0u;
+        if (a.causal) {
+          bad = lim <= 0 ? 0u : lim >= 32 ? ~0u : (1u << lim) - 1u;
+          lim -= kTile;
+          if (++qt == w.per_head) lim += w.per_head * kTile, qt = 0;
         }
-        fence_proxy_async_smem();
-      }
-      if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
-      tc_fence_after();
-      uint32_t d[32];
-      tmem_ld32(dp_addr, d);
-      tmem_wait_ld();
+        if (!(ok = mbar_wait(&m.stat_full[st.s], st.ph, abort_flag, a.status, 13))) break;
+        if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
+        tc_fence_after();
+        uint32_t v[32], p[16];
+        tmem_ld32(s_addr, v);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.s_read);
 #pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        uint64_t p = pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-        if constexpr (!BF16) p = mul_f2(p, gain2);
-        float x0, x1;
-        unpack_f2(mul_f2(p, add_f2(pack_f2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), nd2)), x0, x1);
-        w[c / 2] = Cvt<T>::pack2(x0, x1);
+        for (int c = 0; c < 32; c += 4) {
+          const float4 nl = *reinterpret_cast<const float4*>(stat + c);
+          exp2_pair(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, pack_f2(nl.x, nl.y)), v[c],
+                    v[c + 1]);
+          exp2_pair(fma_f2(pack_f2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3])), scale2, pack_f2(nl.z, nl.w)),
+                    v[c + 2], v[c + 3]);
+          p[c / 2] = Cvt<T>::pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+          p[c / 2 + 1] = Cvt<T>::pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+        }
+        if (bad != 0u) clear_pairs(p, bad);
+        // dP(i) was issued after dV(i-1), so with it done P's columns are free
+        if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
+        tc_fence_after();
+        uint32_t d[32];
+        tmem_st16(p_addr, p);
+        tmem_ld32(s_addr, d);
+        tmem_wait_st();
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&m.dp_read);
+          mbar_arrive(&m.p_full);
+        }
+        // dS = P (dP - delta)
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 nd = *reinterpret_cast<const float4*>(stat + kTile + c);
+#pragma unroll
+          for (int e = c; e < c + 4; e += 2) {
+            uint64_t pe = pack_f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+            if constexpr (!QBF16) pe = mul_f2(pe, gain2);
+            const uint64_t x = mul_f2(pe, add_f2(pack_f2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])),
+                                                 e == c ? pack_f2(nd.x, nd.y) : pack_f2(nd.z, nd.w)));
+            float x0, x1;
+            unpack_f2(x, x0, x1);
+            p[e / 2] = Cvt<TS>::pack2(x0, x1);
+          }
+        }
+        if (bad != 0u) clear_pairs(p, bad);  // 0 * inf
+        if (i > 0 && !(ok = mbar_wait(&m.dk_done, ph ^ 1, abort_flag, a.status, 19))) break;  // the last dS is read
+        tc_fence_after();
+        tmem_st16(ds_addr, p);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&m.stat_empty[st.s]);
+          mbar_arrive(&m.ds_full);
+        }
+        st.next();
       }
-      if (bad != 0u) clear_pairs(w, bad);
-      // dP(i) was issued after dQ(i-1), so dS's columns are free
-      tmem_st16(ds_addr, w);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&m.ds_full);
-    }
-    char* orow = query < a.tq ? a.dq.row(bh, query) : nullptr;
-    if (n == 0) {
-      if (cg == 0 && orow != nullptr) store_zero_row<T>(orow, a.dim);
-    } else if (cg < 2) {
-      ok = ok && mbar_wait(&m.all_done, 0, abort_flag, a.status, 16);
-      tc_fence_after();
-      if (ok && !*abort_flag) {
-        const float mul = BF16 ? a.scale : a.scale / (gain * (1 << kShiftP16));
-        store_row<T>(tmem + lanes + kColDQ, orow, cg * 32 * HALVES, (cg + 1) * 32 * HALVES, a.dim, mul, seen <= 0);
+    } else {
+      const uint32_t s_addr = tmem + lanes + kColS + cg * 32;
+      const uint32_t dp_addr = tmem + lanes + kColDP + cg * 32;
+      const uint32_t ds_addr = tmem + lanes + kColDSq + cg * 16;
+      if (!q_ready) {
+        // Q takes columns that a dK/dV item's results may still be read from
+        ok = (owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 26)) && take_q(owns);
+        if (!ok) break;
+      }
+      const float* stat = a.stat + (bh * a.q_tiles + w.r0 / kTile) * (2 * kTile) + row;
+      const float nl = stat[0], nd = stat[kTile];
+      const uint64_t nl2 = pack_f2(nl, nl), nd2 = pack_f2(nd, nd);
+      const int seen = a.causal ? min(w.len, own + off + 1) : w.len;  // keys this row sees
+      for (int i = 0; i < w.n; ++i) {
+        const uint32_t ph = (it + i) & 1;
+        const int lim = seen - i * kTile - cg * 32;  // columns from `lim` on are masked
+        const uint32_t bad = lim >= 32 ? 0u : lim <= 0 ? ~0u : ~0u << lim;
+        if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
+        tc_fence_after();
+        uint32_t v[32];
+        tmem_ld32(s_addr, v);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.s_read);
+#pragma unroll
+        for (int c = 0; c < 32; c += 2)
+          exp2_pair(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, nl2), v[c], v[c + 1]);
+        // a partly valid last key tile: rows past the keys may hold anything,
+        // and dS's zeros times inf or NaN would reach dQ
+        const int k0 = i * kTile;
+        if (w.len < min(k0 + kTile, a.tk)) {
+          const int tid = threadIdx.x - 64;
+          const int from = w.len - k0, rows = min(kTile, a.tk - k0) - from;
+          char* tile = smem + L::a + ((it + i) % kStagesA) * L::tile;
+          for (int x = tid; x < rows * 8 * HALVES; x += 32 * kElemWarps) {
+            const int r = from + x / (8 * HALVES), ch = x % (8 * HALVES);
+            *reinterpret_cast<uint4*>(tile + (ch >> 3) * kHalfBytes + r * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+        }
+        if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
+        tc_fence_after();
+        uint32_t d[32], ds[16];
+        tmem_ld32(dp_addr, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          uint64_t p = pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+          if constexpr (!QBF16) p = mul_f2(p, gain2);
+          float x0, x1;
+          unpack_f2(mul_f2(p, add_f2(pack_f2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), nd2)), x0, x1);
+          ds[c / 2] = Cvt<TS>::pack2(x0, x1);
+        }
+        if (bad != 0u) clear_pairs(ds, bad);
+        // dP(i) was issued after dQ(i-1), so dS's columns are free
+        tmem_st16(ds_addr, ds);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.ds_full);
       }
     }
+    ok = ok && mbar_wait(&m.acc_full, owns & 1, abort_flag, a.status, 16);
+    if (!ok || *abort_flag) break;
+    tc_fence_after();
+    // between dQ items the next Q goes in first, so that the next S and dP run
+    // while this item's results are stored
+    Work next;
+    have = fetch(next);
+    q_ready = have && !w.dkv && !next.dkv && next.n > 0;
+    if (q_ready && !take_q(owns + 1)) break;
+    const float p_mul = 1.f / static_cast<float>(1 << kShift);
+    if (w.dkv) {  // column groups 0 and 1 store the halves of dV, 2 and 3 those of dK
+      const int from = (cg & 1) * 32 * HALVES, to = from + 32 * HALVES;
+      if (cg >= 2) {
+        const OutTile o{a.dk.row(static_cast<int>(bhk), w.r0), a.dk.st * int64_t(sizeof(TO)), a.tk - w.r0, a.dim};
+        store_rows<TO>(tmem + lanes + kColDK, o, row, lane, from, to, a.scale * p_mul / (gain * q_scale), own >= w.len);
+      } else {
+        const OutTile o{a.dv.row(static_cast<int>(bhk), w.r0), a.dv.st * int64_t(sizeof(T)), a.tk - w.r0, a.dim};
+        store_rows<T>(tmem + lanes + kColDV, o, row, lane, from, to, p_mul, own >= w.len);
+      }
+    } else if (cg < 2 * HALVES) {
+      const OutTile o{a.dq.row(static_cast<int>(bh), w.r0), a.dq.st * int64_t(sizeof(TO)), a.tq - w.r0, a.dim};
+      const bool none = (a.causal ? min(w.len, own + off + 1) : w.len) <= 0;
+      store_rows<TO>(tmem + lanes + kColDQ, o, row, lane, cg * 32, cg * 32 + 32, a.scale * p_mul / (gain * k_scale), none);
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&m.acc_free);
+    it += w.n;
+    ++owns;
+    w = next;
   }
 }
 
-template <bool BF16, int HALVES>
+template <bool VBF16, bool QBF16, bool OUT32, int HALVES>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap do_map,
@@ -670,41 +803,49 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       m.abort_flag = 1;
       atomicCAS(a.status, 0, 0x300);
     }
-    mbar_init(&m.own_full, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&m.item_full[s], 1);
+      mbar_init(&m.item_empty[s], 1 + kElemWarps);
+      mbar_init(&m.stat_full[s], 1);
+      mbar_init(&m.stat_empty[s], kElemWarps);
+    }
     for (int s = 0; s < kStagesA; ++s) {
       mbar_init(&m.a_full[s], 1);
       mbar_init(&m.a_empty[s], 1);
     }
-    for (int s = 0; s < kMaxB; ++s) {
+    for (int s = 0; s < kStagesB; ++s) {
       mbar_init(&m.b_full[s], 1);
       mbar_init(&m.b_empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&m.stat_full[s], 1);
-      mbar_init(&m.stat_empty[s], kElemWarps);
-    }
+    mbar_init(&m.own_full, 1);
+    mbar_init(&m.own_empty, 1);
+    mbar_init(&m.own_tmem, kElemWarps);
     mbar_init(&m.s_full, 1);
     mbar_init(&m.s_read, kElemWarps);
     mbar_init(&m.p_full, kElemWarps);
     mbar_init(&m.dp_full, 1);
-    mbar_init(&m.ds_full, kElemWarps);
     mbar_init(&m.dp_read, kElemWarps);
+    mbar_init(&m.ds_full, kElemWarps);
     mbar_init(&m.dk_done, 1);
-    mbar_init(&m.own_tmem, kElemWarps);
-    mbar_init(&m.all_done, 1);
+    mbar_init(&m.acc_full, 1);
+    mbar_init(&m.acc_free, kElemWarps);
+    mbar_init(&m.exit_done, 1);
     fence_barrier_init();
     fence_proxy_async_smem();
   }
-  grid_dep_wait();  // the statistics come from the kernel before
+  grid_dep_wait();  // the statistics and the counter come from the kernel before
   if (warp == 1) tmem_alloc<512>(&m.tmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = m.tmem;
-  if (static_cast<int>(blockIdx.x) < a.n_dkv)
-    dkv_cta<BF16, HALVES>(&q_map, &k_map, &v_map, &do_map, a, smem, m, tmem);
-  else
-    dq_cta<BF16, HALVES>(&q_map, &k_map, &v_map, &do_map, a, smem, m, tmem);
+  if (warp == 0) {
+    if ((threadIdx.x & 31) == 0) produce<HALVES>(&q_map, &k_map, &v_map, &do_map, a, smem, m);
+  } else if (warp == 1) {
+    if (elect_one()) issue<VBF16, QBF16, HALVES>(a, smem, m, tmem);
+  } else {
+    elementwise<VBF16, QBF16, OUT32, HALVES>(a, smem, m, tmem);
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -715,91 +856,86 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
 
 // ------------------------------------------------------------ row statistics
 struct StatArgs {
-  Rows out, dout, v;
+  Rows out, out_low, dout, v;  // out_low: what out's type could not hold of the output, or no base
   const float* lse;
   float* stat;
-  uint32_t* maxima;
+  float* do_norm;
+  float* v_norm;
+  int* counter;
   const int32_t* key_lengths;
-  int heads, kv_heads, group;
+  int heads, kv_heads;
   int tq, tk, dim;
-  int q_tiles;
-  int q_blocks;  // blocks of the query part; the rest walks V (FP16)
+  int q_tiles, v_blocks;
+  int q_blocks;  // blocks of the query part; the rest walks V (NORMS)
 };
 
-constexpr int kStatRows = 64;  // rows of a block: 16 groups of 16 lanes, 4 rows each
-
 // -lse*log2e and -delta of every query row, padded to whole tiles with rows
-// that give P = 0.  FP16: also the largest squared norms of dO rows and valid
-// V rows per key/value head (atomicMax of non-negative float bits: the order
-// does not matter).
-template <typename T>
+// that give P = 0.  NORMS: also the largest squared norms of 64 dO rows and of
+// 64 valid V rows.  Block 0 resets the item counter of the kernel after.
+template <typename T, bool NORMS>
 __global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_constant__ StatArgs a) {
-  constexpr bool kF16 = std::is_same<T, __half>::value;
+  constexpr int kShift = std::is_same<T, __half>::value ? kShiftP16 : 0;
+  __shared__ float part[8];
   const int g = threadIdx.x >> 4;
   const int l = threadIdx.x & 15;
   const bool active = 8 * l < a.dim;
-  if (static_cast<int>(blockIdx.x) < a.q_blocks) {
-    const int blocks_per_head = a.q_tiles * (kTile / kStatRows);
-    const int bh = blockIdx.x / blocks_per_head;
-    const int r0 = (blockIdx.x - bh * blocks_per_head) * kStatRows;
-    float most = 0.f;
+  const bool queries = static_cast<int>(blockIdx.x) < a.q_blocks;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.counter = 0;
+  const int id = queries ? blockIdx.x : blockIdx.x - a.q_blocks;
+  const int per_head = queries ? a.q_tiles * (kTile / kStatRows) : a.v_blocks;
+  const int head = id / per_head;
+  const int r0 = (id - head * per_head) * kStatRows;
+  float most = 0.f;
+  if (queries) {
     uint4 o[4], d[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int r = r0 + u * 16 + g;
       o[u] = d[u] = make_uint4(0u, 0u, 0u, 0u);
       if (active && r < a.tq) {
-        o[u] = reinterpret_cast<const uint4*>(a.out.row(bh, r))[l];
-        d[u] = reinterpret_cast<const uint4*>(a.dout.row(bh, r))[l];
+        o[u] = reinterpret_cast<const uint4*>(a.out.row(head, r))[l];
+        d[u] = reinterpret_cast<const uint4*>(a.dout.row(head, r))[l];
       }
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int r = r0 + u * 16 + g;
       const uint32_t ow[4] = {o[u].x, o[u].y, o[u].z, o[u].w}, dw[4] = {d[u].x, d[u].y, d[u].z, d[u].w};
+      uint4 low = make_uint4(0u, 0u, 0u, 0u);
+      if (a.out_low.base != nullptr && active && r < a.tq) low = reinterpret_cast<const uint4*>(a.out_low.row(head, r))[l];
+      const uint32_t lw[4] = {low.x, low.y, low.z, low.w};
       float sum = 0.f, norm = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float o0, o1, d0, d1;
+        float o0, o1, l0, l1, d0, d1;
         Cvt<T>::unpack2(ow[i], o0, o1);
+        Cvt<T>::unpack2(lw[i], l0, l1);
         Cvt<T>::unpack2(dw[i], d0, d1);
-        sum = fmaf(o0, d0, sum);
-        sum = fmaf(o1, d1, sum);
-        if constexpr (kF16) norm = fmaf(d0, d0, fmaf(d1, d1, norm));
+        sum = fmaf(o0 + l0, d0, sum);
+        sum = fmaf(o1 + l1, d1, sum);
+        if constexpr (NORMS) norm = fmaf(d0, d0, fmaf(d1, d1, norm));
       }
 #pragma unroll
       for (int w = 8; w > 0; w >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, w);
-        if constexpr (kF16) norm += __shfl_xor_sync(0xffffffffu, norm, w);
+        if constexpr (NORMS) norm += __shfl_xor_sync(0xffffffffu, norm, w);
       }
       most = fmaxf(most, norm);
       if (l == 0) {
-        const float lse = r < a.tq ? a.lse[int64_t(bh) * a.tq + r] : -INFINITY;
-        float* dst = a.stat + (int64_t(bh) * a.q_tiles + r / kTile) * (2 * kTile) + r % kTile;
-        dst[0] = lse == -INFINITY ? -INFINITY : -lse * kLog2e + (kF16 ? static_cast<float>(kShiftP16) : 0.f);
+        const float lse = r < a.tq ? a.lse[int64_t(head) * a.tq + r] : -INFINITY;
+        float* dst = a.stat + (int64_t(head) * a.q_tiles + r / kTile) * (2 * kTile) + r % kTile;
+        dst[0] = lse == -INFINITY ? -INFINITY : -lse * kLog2e + static_cast<float>(kShift);
         dst[kTile] = -sum;
       }
     }
-    if constexpr (kF16) {
-      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-      if ((threadIdx.x & 31) == 0) {
-        const int b = bh / a.heads;
-        atomicMax(a.maxima + 2 * (b * a.kv_heads + (bh - b * a.heads) / a.group), __float_as_uint(most));
-      }
-    }
-  } else if constexpr (kF16) {
-    const int id = blockIdx.x - a.q_blocks;
-    const int blocks_per_head = (a.tk + kStatRows - 1) / kStatRows;
-    const int bhk = id / blocks_per_head;
-    const int r0 = (id - bhk * blocks_per_head) * kStatRows;
-    const int b = bhk / a.kv_heads;
+  } else if constexpr (NORMS) {
+    const int b = head / a.kv_heads;
     const int len = a.key_lengths != nullptr ? min(a.key_lengths[b], a.tk) : a.tk;
-    float most = 0.f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int r = r0 + u * 16 + g;
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (active && r < len) x = reinterpret_cast<const uint4*>(a.v.row(bhk, r))[l];
+      if (active && r < len) x = reinterpret_cast<const uint4*>(a.v.row(head, r))[l];
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
       float norm = 0.f;
 #pragma unroll
@@ -812,28 +948,65 @@ __global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_consta
       for (int s = 8; s > 0; s >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, s);
       most = fmaxf(most, norm);
     }
+  }
+  if constexpr (NORMS) {
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
-    if ((threadIdx.x & 31) == 0) atomicMax(a.maxima + 2 * bhk + 1, __float_as_uint(most));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 8; ++w) most = fmaxf(most, part[w]);
+      (queries ? a.do_norm : a.v_norm)[int64_t(head) * per_head + r0 / kStatRows] = most;
+    }
   }
 }
 
 size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
-template <bool BF16, int HALVES>
-cudaError_t launch_grad(unsigned blocks, const CUtensorMap* maps, const GradArgs& a, cudaStream_t st) {
-  const auto kernel = attn_grad_kernel<BF16, HALVES>;
+// Byte offsets in the workspace.
+struct Layout {
+  size_t stat, do_norm, v_norm, counter, total;
+};
+Layout layout_of(int64_t bh, int64_t bhk, int64_t q_tiles, int64_t v_blocks) {
+  Layout l;
+  l.stat = 0;
+  l.do_norm = align256(size_t(bh) * q_tiles * kStatBytes);
+  l.v_norm = l.do_norm + align256(size_t(bh) * q_tiles * 2 * 4);
+  l.counter = l.v_norm + align256(size_t(bhk) * v_blocks * 4);
+  l.total = l.counter + 256;
+  return l;
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 1;
+  return n;
+}
+
+template <bool VBF16, bool QBF16, bool OUT32, int HALVES>
+cudaError_t launch_grad(const CUtensorMap* maps, const GradArgs& a, cudaStream_t st) {
+  const auto kernel = attn_grad_kernel<VBF16, QBF16, OUT32, HALVES>;
   const int smem = static_cast<int>(Smem<HALVES>::total);
   const cudaError_t err = ensure_smem(reinterpret_cast<const void*>(kernel), smem);
   if (err != cudaSuccess) return err;
-  return launch_pdl(kernel, dim3(blocks), dim3(kThreads), size_t(smem), st, maps[0], maps[1], maps[2], maps[3], a);
+  const int sms = sm_count();
+  return launch_pdl(kernel, dim3(a.n_items < sms ? a.n_items : sms), dim3(kThreads), size_t(smem), st, maps[0], maps[1],
+                    maps[2], maps[3], a);
+}
+
+template <int HALVES>
+cudaError_t launch_halves(bool v_bf16, bool qk16, const CUtensorMap* maps, const GradArgs& a, cudaStream_t st) {
+  if (qk16)
+    return v_bf16 ? launch_grad<true, false, true, HALVES>(maps, a, st) : launch_grad<false, false, true, HALVES>(maps, a, st);
+  return v_bf16 ? launch_grad<true, true, false, HALVES>(maps, a, st) : launch_grad<false, false, false, HALVES>(maps, a, st);
 }
 
 }  // namespace
 
-int64_t attn_grad_workspace_bytes(int batch, int heads, int kv_heads, int tq) {
-  const int64_t q_tiles = (int64_t(tq) + kTile - 1) / kTile;
-  return static_cast<int64_t>(align256(size_t(batch) * heads * q_tiles * 2 * kTile * 4) +
-                              align256(size_t(batch) * kv_heads * 2 * 4));
+int64_t attn_grad_workspace_bytes(int batch, int heads, int kv_heads, int tq, int tk) {
+  return static_cast<int64_t>(layout_of(int64_t(batch) * heads, int64_t(batch) * kv_heads, (int64_t(tq) + kTile - 1) / kTile,
+                                        (int64_t(tk) + kStatRows - 1) / kStatRows)
+                                  .total);
 }
 
 cudaError_t launch_attn_grad(const AttnGradCall& c, int* status, cudaStream_t st) {
@@ -842,42 +1015,48 @@ cudaError_t launch_attn_grad(const AttnGradCall& c, int* status, cudaStream_t st
   const b2_view* views[4] = {c.q, c.k, c.v, c.dout};
   for (int i = 0; i < 4; ++i)
     if (!linear_rows_map(&maps[i], *views[i], kTile)) return cudaErrorInvalidValue;
-  const bool bf16 = q.dtype == B2_BF16;
+  const bool v_bf16 = c.v->dtype == B2_BF16, qk16 = c.qk_scale != nullptr;
+  const int64_t bh = int64_t(q.batch) * q.heads, bhk = int64_t(q.batch) * k.heads;
   StatArgs s{};
   s.out = make_rows(*c.out), s.dout = make_rows(*c.dout), s.v = make_rows(*c.v);
+  if (c.out_low != nullptr) s.out_low = make_rows(*c.out_low);
   s.lse = c.lse;
   s.key_lengths = c.key_lengths;
-  s.heads = q.heads, s.kv_heads = k.heads, s.group = q.heads / k.heads;
+  s.heads = q.heads, s.kv_heads = k.heads;
   s.tq = q.tokens, s.tk = k.tokens, s.dim = q.head_dim;
   s.q_tiles = (q.tokens + kTile - 1) / kTile;
-  s.stat = static_cast<float*>(c.workspace);
-  const int64_t bh = int64_t(q.batch) * q.heads, bhk = int64_t(q.batch) * k.heads;
-  s.maxima = reinterpret_cast<uint32_t*>(static_cast<char*>(c.workspace) +
-                                         align256(size_t(bh) * s.q_tiles * 2 * kTile * 4));
+  s.v_blocks = (k.tokens + kStatRows - 1) / kStatRows;
+  const Layout l = layout_of(bh, bhk, s.q_tiles, s.v_blocks);
+  char* ws = static_cast<char*>(c.workspace);
+  s.stat = reinterpret_cast<float*>(ws + l.stat);
+  s.do_norm = reinterpret_cast<float*>(ws + l.do_norm);
+  s.v_norm = reinterpret_cast<float*>(ws + l.v_norm);
+  s.counter = reinterpret_cast<int*>(ws + l.counter);
   s.q_blocks = static_cast<int>(bh * s.q_tiles * (kTile / kStatRows));
-  const int v_blocks = bf16 ? 0 : static_cast<int>(bhk * ((k.tokens + kStatRows - 1) / kStatRows));
-  cudaError_t err;
-  if (!bf16 && (err = cudaMemsetAsync(s.maxima, 0, size_t(bhk) * 8, st)) != cudaSuccess) return err;
-  if (bf16) attn_grad_stat_kernel<__nv_bfloat16><<<s.q_blocks, 256, 0, st>>>(s);
-  else attn_grad_stat_kernel<__half><<<s.q_blocks + v_blocks, 256, 0, st>>>(s);
-  if ((err = cudaGetLastError()) != cudaSuccess) return err;
+  const bool norms = !v_bf16 || qk16;  // dS in FP16
+  const int blocks = s.q_blocks + (norms ? static_cast<int>(bhk * s.v_blocks) : 0);
+  if (!v_bf16) attn_grad_stat_kernel<__half, true><<<blocks, 256, 0, st>>>(s);
+  else if (norms) attn_grad_stat_kernel<__nv_bfloat16, true><<<blocks, 256, 0, st>>>(s);
+  else attn_grad_stat_kernel<__nv_bfloat16, false><<<blocks, 256, 0, st>>>(s);
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return err;
   GradArgs a{};
-  a.q = make_rows(q), a.dq = make_rows(*c.dq), a.dk = make_rows(*c.dk), a.dv = make_rows(*c.dv);
-  a.stat = s.stat;
-  a.maxima = s.maxima;
+  a.dq = make_rows(*c.dq), a.dk = make_rows(*c.dk), a.dv = make_rows(*c.dv);
+  a.stat = s.stat, a.do_norm = s.do_norm, a.v_norm = s.v_norm;
+  a.qk_scale = c.qk_scale;
+  a.counter = s.counter;
   a.key_lengths = c.key_lengths;
-  a.heads = s.heads, a.kv_heads = s.kv_heads, a.group = s.group;
+  a.heads = s.heads, a.kv_heads = s.kv_heads, a.group = q.heads / k.heads;
   a.tq = s.tq, a.tk = s.tk, a.dim = s.dim;
-  a.q_tiles = s.q_tiles;
+  a.q_tiles = s.q_tiles, a.v_blocks = s.v_blocks;
   a.k_tiles = (k.tokens + kTile - 1) / kTile;
   a.n_dkv = static_cast<int>(bhk * a.k_tiles);
+  a.n_items = static_cast<int>(a.n_dkv + bh * a.q_tiles);
   a.causal = c.causal;
   a.scale = c.scale;
   a.scale_log2 = c.scale * kLog2e;
   a.status = status;
-  const unsigned blocks = static_cast<unsigned>(a.n_dkv + bh * a.q_tiles);
-  if (q.head_dim <= 64) return bf16 ? launch_grad<true, 1>(blocks, maps, a, st) : launch_grad<false, 1>(blocks, maps, a, st);
-  return bf16 ? launch_grad<true, 2>(blocks, maps, a, st) : launch_grad<false, 2>(blocks, maps, a, st);
+  return q.head_dim <= 64 ? launch_halves<1>(v_bf16, qk16, maps, a, st) : launch_halves<2>(v_bf16, qk16, maps, a, st);
 }
 
 }  // namespace b2

@@ -782,9 +782,10 @@ int b2_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, c
   return ok();
 }
 
-int64_t b2_attention_backward_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens) {
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || q_tokens <= 0) return -1;
-  return attn_grad_workspace_bytes(batch, heads, kv_heads, q_tokens);
+int64_t b2_attention_backward_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens,
+                                              int32_t k_tokens) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || q_tokens <= 0 || k_tokens <= 0) return -1;
+  return attn_grad_workspace_bytes(batch, heads, kv_heads, q_tokens, k_tokens);
 }
 
 int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
@@ -801,7 +802,7 @@ int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, 
     return fail(B2_ERR_INVALID, "workspace must be non-NULL and 16-byte aligned");
   int* status = device_status_ptr();
   if (status == nullptr) return fail(B2_ERR_CUDA, "device status word unavailable");
-  const AttnGradCall c{q, k, v, out, dout, dq, dk, dv, lse, key_lengths, scale, causal ? 1 : 0, workspace};
+  const AttnGradCall c{q, k, v, out, dout, dq, dk, dv, nullptr, nullptr, lse, key_lengths, scale, causal ? 1 : 0, workspace};
   const cudaError_t err = launch_attn_grad(c, status, static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) return cuda_fail(err, "attention backward launch");
   return ok();

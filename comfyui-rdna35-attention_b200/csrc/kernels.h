@@ -109,6 +109,8 @@ struct AttnGeneralCall {
 cudaError_t launch_attn_general(const AttnGeneralCall& call, int* status, cudaStream_t stream);
 struct AttnGradCall {
   const b2_view *q, *k, *v, *out, *dout, *dq, *dk, *dv;
+  const b2_view* out_low;  // what out's type could not hold of the output, or NULL
+  const float* qk_scale;   // FP16 q, k held times these powers of two (dq, dk in FP32), or NULL
   const float* lse;
   const int32_t* key_lengths;
   float scale;
@@ -116,7 +118,7 @@ struct AttnGradCall {
   void* workspace;
 };
 // Backward pass of exact attention (attn_grad.cu).
-int64_t attn_grad_workspace_bytes(int batch, int heads, int kv_heads, int tq);
+int64_t attn_grad_workspace_bytes(int batch, int heads, int kv_heads, int tq, int tk);
 cudaError_t launch_attn_grad(const AttnGradCall& call, int* status, cudaStream_t stream);
 // Norm + rotary positions (rotary.cu): one or two sides (queries, keys).
 // Forward: y from x.  Gradients (dy set): y receives dx, dw (may be NULL) the

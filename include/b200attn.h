@@ -322,7 +322,8 @@ int b2_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, c
  * keys are written as 0.  Probabilities are recomputed; workspace:
  * b2_attention_backward_workspace_bytes() bytes for row statistics, read and
  * written only by this call.  Results are bit-reproducible. */
-int64_t b2_attention_backward_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens);
+int64_t b2_attention_backward_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens,
+                                              int32_t k_tokens);
 int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
                           const b2_view* dout, const float* lse, const b2_view* dq, const b2_view* dk,
                           const b2_view* dv, float scale, int32_t causal, const int32_t* key_lengths, void* workspace,

@@ -184,8 +184,8 @@ def test_c_entries_check_their_arguments():
     assert forward(*(changed(a, **many) for a in (q, k, k, q))) == unsupported
     assert backward(lse=None) == invalid and backward(ws=None) == invalid and backward(ws=ctypes.c_void_p(8)) == invalid
     assert backward(dk=q) == invalid and backward(dq=changed(q, stride_t=0)) == invalid
-    assert lib.b2_attention_backward_workspace_bytes(0, 1, 1, 1) == -1
-    assert lib.b2_attention_backward_workspace_bytes(2, 4, 2, 129) >= 2 * 4 * 2 * 1024
+    assert lib.b2_attention_backward_workspace_bytes(0, 1, 1, 1, 1) == -1
+    assert lib.b2_attention_backward_workspace_bytes(2, 4, 2, 129, 5) >= 2 * 4 * 2 * 1024
 
 
 # ---------------------------------------------------------------- parity (GPU)

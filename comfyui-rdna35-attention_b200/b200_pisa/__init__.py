@@ -27,6 +27,7 @@ import torch
 from . import _lib
 from ._lib import LIB, check, ptr, stream_of, view
 from .exact import attention, attention_backward, attention_forward
+from .fused import norm_rope_attention
 from .rotary import axial_rope, qk_norm_rope, qk_norm_rope_backward
 
 __version__ = "0.1.0"
@@ -610,6 +611,7 @@ __all__ = [
     "generic_block_stats",
     "generic_forward",
     "pack_views",
+    "norm_rope_attention",
     "prepare",
     "qk_norm_rope",
     "qk_norm_rope_backward",

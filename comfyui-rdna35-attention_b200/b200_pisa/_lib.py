@@ -106,9 +106,13 @@ SIGNATURES: dict[str, tuple] = {
                                                        _VP]),
     "b2_pack_block_bias": (ctypes.c_int, [_VP, _I32, _I64, _I64, _I64, _I32, _I32, _VP, _VP]),
     # views and b2_rotary structs of these arrive packed (bytes) or by reference
-    "b2_attention_forward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _F32, _I32, _VP, _VP, _VP]),
+    "b2_attention_forward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _F32, _I32, _VP, _VP, _VP, _VP]),
     "b2_attention_backward_workspace_bytes": (_I64, [_I32, _I32, _I32, _I32, _I32]),
-    "b2_attention_backward": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _F32, _I32, _VP, _VP, _VP]),
+    "b2_attention_backward": (ctypes.c_int, [*[_VP] * 10, _F32, _I32, _VP, _VP, _VP]),
+    "b2_norm_rope_attention_saved_bytes": (_I64, [_I32] * 5),
+    "b2_norm_rope_attention_workspace_bytes": (_I64, [_I32] * 5),
+    "b2_norm_rope_attention_forward": (ctypes.c_int, [*[_VP] * 6, _I32, _F32, _VP, _F32, _I32, *[_VP] * 5]),
+    "b2_norm_rope_attention_backward": (ctypes.c_int, [*[_VP] * 9, _I32, _F32, _VP, _F32, _I32, *[_VP] * 9]),
     "b2_axial_rope": (ctypes.c_int, [_VP, _VP, _VP, _VP]),
     "b2_qk_norm_rope": (ctypes.c_int, [_VP, _VP, _VP, _VP, _VP, _VP, _I32, _F32, _VP, _VP]),
     "b2_qk_norm_rope_workspace_bytes": (_I64, [_I32]),

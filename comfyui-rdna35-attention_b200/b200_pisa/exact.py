@@ -22,6 +22,8 @@ from ._args import (PLANS, addressable, as_rows, new_rows, on_device, raw_stream
 from ._lib import LIB, check, ptr
 
 MAX_HEAD_DIM = 128
+#: keys of a batch up to which out's rounding error is kept for the backward pass (kLowKeys of the library)
+LOW_KEYS = 64
 _DTYPES = (torch.bfloat16, torch.float16)
 
 
@@ -87,70 +89,101 @@ def _planned(q, k, v, scale, key_lengths):
     return q, k, v, plan
 
 
+def new_low(q: torch.Tensor, strides, key_tokens: int, key_lengths) -> torch.Tensor | None:
+    """Room for what BF16 cannot hold of the output, where the backward pass
+    may need it: batches of at most LOW_KEYS keys."""
+    if q.dtype != torch.bfloat16 or (key_lengths is None and key_tokens > LOW_KEYS):
+        return None
+    return new_rows(q, q.shape, strides)
+
+
+def with_optional(x: torch.Tensor | None, tail: bytes) -> bytes | None:
+    return None if x is None else with_base(x, tail)
+
+
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None, *,
-                      causal: bool = False, key_lengths: torch.Tensor | None = None):
+                      causal: bool = False, key_lengths: torch.Tensor | None = None, with_low: bool = False):
     """(out, lse) of softmax(scale q k^T) v: out like q, lse FP32 [B,H,Tq]
     ([BH,Tq]) the natural log of the sum of exponentials.  key_lengths: int32
     [B] on the device, batch b attends to its first key_lengths[b] keys (what
     the K/V rows past them hold does not matter).  causal: query i sees keys
-    up to i + Tk - Tq.  A query that sees no key gives out 0 and lse -inf."""
+    up to i + Tk - Tq.  A query that sees no key gives out 0 and lse -inf.
+
+    with_low: (out, lse, out_low), for attention_backward: out's rounding
+    error (like out, BF16) in batches of at most 64 keys, whose gradients it
+    is the largest error of; None where no batch can have so few."""
     flat = isinstance(q, torch.Tensor) and q.ndim == 3
     q, k, v, (scale, _, tails, strides, out_tails) = _planned(q, k, v, scale, key_lengths)
     require_one_device("attention", q, k, v, key_lengths)
     with on_device(q):
         out = new_rows(q, q.shape, strides[0])
+        low = new_low(q, strides[0], k.shape[2], key_lengths) if with_low else None
         lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32)
         check(LIB.b2_attention_forward(with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]),
                                        with_base(out, out_tails[0]), scale, 1 if causal else 0, ptr(key_lengths), ptr(lse),
-                                       raw_stream(q)))
-    return (out.squeeze(1), lse.squeeze(1)) if flat else (out, lse)
+                                       with_optional(low, out_tails[0]), raw_stream(q)))
+    if flat:
+        out, lse, low = out.squeeze(1), lse.squeeze(1), None if low is None else low.squeeze(1)
+    return (out, lse, low) if with_low else (out, lse)
+
+
+def check_saved(q: torch.Tensor, flat: bool, lse, **rows) -> list:
+    """Checked four-dimensional ``rows`` (like q) a backward pass is given."""
+    got = []
+    for name, x in rows.items():
+        if x is not None or name != "out_low":
+            x = _four(name, x)
+            if x.shape != q.shape or x.dtype != q.dtype:
+                raise ValueError(f"{name} must have q's shape and dtype.")
+        got.append(x)
+    batch, heads, tokens, _ = q.shape
+    if not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32 \
+            or lse.shape != ((batch, tokens) if flat else (batch, heads, tokens)):
+        raise ValueError("lse must be the forward pass's float32 [B,H,Tq] tensor.")
+    return got
 
 
 def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
                        lse: torch.Tensor, scale: float | None = None, *, causal: bool = False,
-                       key_lengths: torch.Tensor | None = None):
+                       key_lengths: torch.Tensor | None = None, out_low: torch.Tensor | None = None):
     """(dq, dk, dv) of attention_forward's call from the gradient of its out
-    and what it returned.  Probabilities are recomputed from lse; dk and dv of
-    a shared head are summed over its group in FP32; rows of dk and dv past a
-    batch's keys are 0.  Bit-reproducible."""
+    and what it returned (out_low is optional).  Probabilities are recomputed
+    from lse; dk and dv of a shared head are summed over its group in FP32;
+    rows of dk and dv past a batch's keys are 0.  Bit-reproducible."""
     flat = isinstance(q, torch.Tensor) and q.ndim == 3
     q, k, v, (scale, _, tails, strides, grad_tails) = _planned(q, k, v, scale, key_lengths)
-    out, dout = _four("out", out), _four("dout", dout)
-    for name, x in (("out", out), ("dout", dout)):
-        if x.shape != q.shape or x.dtype != q.dtype:
-            raise ValueError(f"{name} must have q's shape and dtype.")
+    out, dout, out_low = check_saved(q, flat, lse, out=out, dout=dout, out_low=out_low)
+    require_one_device("attention_backward", q, k, v, key_lengths, out, dout, lse, out_low)
     batch, heads, tokens, _ = q.shape
-    if not isinstance(lse, torch.Tensor) or lse.dtype != torch.float32 \
-            or lse.shape != ((batch, tokens) if flat else (batch, heads, tokens)):
-        raise ValueError("lse must be attention_forward's float32 [B,H,Tq] tensor.")
-    require_one_device("attention_backward", q, k, v, key_lengths, out, dout, lse)
     with on_device(q):
         out, dout, lse = as_rows(out, broadcast=False), as_rows(dout, broadcast=False), lse.contiguous()
+        low = None if out_low is None else as_rows(out_low, broadcast=False)
         dq, dk, dv = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1]), new_rows(k, k.shape, strides[1])
-        ws = torch.empty(LIB.b2_attention_backward_workspace_bytes(batch, heads, k.shape[1], tokens, k.shape[2]), device=q.device,
-                         dtype=torch.uint8)
+        ws = torch.empty(LIB.b2_attention_backward_workspace_bytes(batch, heads, k.shape[1], tokens, k.shape[2]),
+                         device=q.device, dtype=torch.uint8)
         check(LIB.b2_attention_backward(
             with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]),
-            with_base(out, view_tail(*signature(out))), with_base(dout, view_tail(*signature(dout))), ptr(lse),
-            with_base(dq, grad_tails[0]), with_base(dk, grad_tails[1]), with_base(dv, grad_tails[1]), scale,
-            1 if causal else 0, ptr(key_lengths), ptr(ws), raw_stream(q)))
+            with_base(out, view_tail(*signature(out))), None if low is None else with_base(low, view_tail(*signature(low))),
+            with_base(dout, view_tail(*signature(dout))), ptr(lse), with_base(dq, grad_tails[0]),
+            with_base(dk, grad_tails[1]), with_base(dv, grad_tails[1]), scale, 1 if causal else 0, ptr(key_lengths),
+            ptr(ws), raw_stream(q)))
     return (dq.squeeze(1), dk.squeeze(1), dv.squeeze(1)) if flat else (dq, dk, dv)
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, causal, key_lengths):
-        out, lse = attention_forward(q, k, v, scale, causal=causal, key_lengths=key_lengths)
-        ctx.save_for_backward(q, k, v, out, lse, key_lengths)
+        out, lse, low = attention_forward(q, k, v, scale, causal=causal, key_lengths=key_lengths, with_low=True)
+        ctx.save_for_backward(q, k, v, out, lse, low, key_lengths)
         ctx.call = (scale, causal)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, key_lengths = ctx.saved_tensors
+        q, k, v, out, lse, low, key_lengths = ctx.saved_tensors
         scale, causal = ctx.call
-        grads = attention_backward(dout, q, k, v, out, lse, scale, causal=causal, key_lengths=key_lengths)
+        grads = attention_backward(dout, q, k, v, out, lse, scale, causal=causal, key_lengths=key_lengths, out_low=low)
         return (*grads, None, None, None)
 
 

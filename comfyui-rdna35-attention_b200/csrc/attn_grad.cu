@@ -887,6 +887,9 @@ __global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_consta
   const int r0 = (id - head * per_head) * kStatRows;
   float most = 0.f;
   if (queries) {
+    bool use_low = a.out_low.base != nullptr;
+    if (use_low && a.key_lengths != nullptr) use_low = min(max(a.key_lengths[head / a.heads], 0), a.tk) <= kLowKeys;
+    else if (use_low) use_low = a.tk <= kLowKeys;
     uint4 o[4], d[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -902,7 +905,7 @@ __global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_consta
       const int r = r0 + u * 16 + g;
       const uint32_t ow[4] = {o[u].x, o[u].y, o[u].z, o[u].w}, dw[4] = {d[u].x, d[u].y, d[u].z, d[u].w};
       uint4 low = make_uint4(0u, 0u, 0u, 0u);
-      if (a.out_low.base != nullptr && active && r < a.tq) low = reinterpret_cast<const uint4*>(a.out_low.row(head, r))[l];
+      if (use_low && active && r < a.tq) low = reinterpret_cast<const uint4*>(a.out_low.row(head, r))[l];
       const uint32_t lw[4] = {low.x, low.y, low.z, low.w};
       float sum = 0.f, norm = 0.f;
 #pragma unroll

@@ -240,8 +240,9 @@ __device__ __forceinline__ bool issue_pv(Misc& m, char* smem, uint32_t tmem, con
 // limited per batch (a.key_lengths) and causally (query i sees keys up to
 // i + a.causal_off), key/value heads shared by groups of query heads, rows
 // that see no key written as 0 with lse -inf; its value is the number of
-// 64-column halves of the head dimension the products cover.
-template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR, int GEN>
+// 64-column halves of the head dimension the products cover.  QK16: q and k
+// are FP16 copies held times a.qk_scale, whatever the type of v.
+template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR, int GEN, bool QK16>
 __global__ void __launch_bounds__(Cfg<NW>::kThreads, Cfg<NW>::kCtasPerSm)
 attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap kc_map,
@@ -476,7 +477,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           const int j = NW * ns + w;
           const bool buf_free = ns < 2 || (ns - 2 < npv && mbar_test_wait(&m.pv_done[w][ns & 1], ((ns - 2) >> 1) & 1));
           if (buf_free && mbar_test_wait(&m.k_full[j % kStagesK], (j / kStagesK) & 1)) {
-            ok = issue_s<BF16, NW, kHalves>(m, k_s, q_addr, tmem, a, abort_flag, j, trace);
+            ok = issue_s<BF16 && !QK16, NW, kHalves>(m, k_s, q_addr, tmem, a, abort_flag, j, trace);
             ++ns;
             did = true;
           }
@@ -544,7 +545,9 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     float mrun = -INFINITY, lrun = 0.f, tmass = 0.f;
     const int nb_ = a.nb, causal_ = a.causal;
     const int causal_row = tq_row + (GEN ? a.causal_off : 0);  // the last key the row sees
-    const float log2_last_ = a.log2_last, scale_log2_ = a.scale_log2;
+    const float log2_last_ = a.log2_last;
+    float scale_log2_ = a.scale_log2;
+    if constexpr (QK16) scale_log2_ /= a.qk_scale[0] * a.qk_scale[1];
     int i = 0;
     bool ok = true;
     for (int j = wg; j < n; j += NW, ++i) {
@@ -746,6 +749,10 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     const float inv = lt > 0.f ? 1.f / lt : (MASKED ? __int_as_float(0x7fc00000) : 0.f);
     const float cw = tt * a.corr_scale;
     char* orow = store ? a.o.row(bh, tq_row) : nullptr;
+    char* low_row = nullptr;
+    if constexpr (GEN != 0) {
+      if (store && a.o_low.base != nullptr && tk_ <= kLowKeys) low_row = a.o_low.row(bh, tq_row);
+    }
     const uint32_t row_base = tmem + lane_base;
 #pragma unroll 1
     for (int c0 = wg * (128 / NW); c0 < (GEN == 1 ? 64 : (wg + 1) * (128 / NW)); c0 += 32) {
@@ -771,6 +778,24 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           }
           if (GEN != 0 && lt == 0.f) f0 = f1 = 0.f;  // no key seen: O may hold anything
           packed[c / 2] = Cvt<T>::pack2(f0 * inv, f1 * inv);
+        }
+        if constexpr (GEN != 0) {
+          if (low_row != nullptr) {  // what the output's type cannot hold
+            uint32_t low[16];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              float h0, h1;
+              Cvt<T>::unpack2(packed[c / 2], h0, h1);
+              const float w0 = lt == 0.f ? 0.f : a0 * inv;
+              low[c / 2] = Cvt<T>::pack2(lt == 0.f ? 0.f : fmaf(__uint_as_float(o0[c]), w0, -h0),
+                                         lt == 0.f ? 0.f : fmaf(__uint_as_float(o0[c + 1]), w0, -h1));
+            }
+            uint4* dst = reinterpret_cast<uint4*>(low_row + c0 * 2);
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+              if (c0 + 8 * q4 < a.o.dim)
+                dst[q4] = make_uint4(low[4 * q4], low[4 * q4 + 1], low[4 * q4 + 2], low[4 * q4 + 3]);
+          }
         }
         uint4* dst = reinterpret_cast<uint4*>(orow + c0 * 2);
         if (a.o.dim == 128) {
@@ -950,15 +975,15 @@ int attn_warpgroups() {
   return nw;
 }
 
-template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR, int GEN = 0>
+template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR, int GEN = 0, bool QK16 = false>
 cudaError_t launch_variant(dim3 grid, cudaStream_t stream, const CUtensorMap& q_map, const CUtensorMap& k_map,
                            const CUtensorMap& v_map, const CUtensorMap& kc_map, const CUtensorMap& vc_map,
                            const CUtensorMap& h_map, const UmmaArgs& a) {
   const int smem = static_cast<int>(SmemLayout<NW>::total);
   const cudaError_t err =
-      ensure_smem(reinterpret_cast<const void*>(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR, GEN>), smem);
+      ensure_smem(reinterpret_cast<const void*>(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR, GEN, QK16>), smem);
   if (err != cudaSuccess) return err;
-  return launch_pdl(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR, GEN>, grid, dim3(Cfg<NW>::kThreads), size_t(smem), stream,
+  return launch_pdl(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR, GEN, QK16>, grid, dim3(Cfg<NW>::kThreads), size_t(smem), stream,
                     q_map, k_map, v_map, kc_map, vc_map, h_map, a);
 }
 
@@ -1072,14 +1097,20 @@ cudaError_t launch_attn_general(const AttnGeneralCall& c, int* status, cudaStrea
   a.o = make_rows(*c.out);
   a.lse = c.lse;
   a.status = status;
+  if (c.out_low != nullptr) a.o_low = make_rows(*c.out_low);
+  a.qk_scale = c.qk_scale;
   const dim3 grid((a.nqb + 1) / 2, q.batch * q.heads);
-  if (q.dtype == B2_BF16)
-    return q.head_dim <= 64
-               ? launch_variant<true, 1, false, false, false, 1>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a)
-               : launch_variant<true, 1, false, false, false, 2>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a);
-  return q.head_dim <= 64
-             ? launch_variant<false, 1, false, false, false, 1>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a)
-             : launch_variant<false, 1, false, false, false, 2>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a);
+  auto launch = [&](auto bf16, auto halves) {
+    constexpr bool kBf16 = decltype(bf16)::value;
+    constexpr int kGen = decltype(halves)::value;
+    if (c.qk_scale != nullptr)
+      return launch_variant<kBf16, 1, false, false, false, kGen, true>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a);
+    return launch_variant<kBf16, 1, false, false, false, kGen>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a);
+  };
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (c.v->dtype == B2_BF16) return q.head_dim <= 64 ? launch(std::true_type{}, One{}) : launch(std::true_type{}, Two{});
+  return q.head_dim <= 64 ? launch(std::false_type{}, One{}) : launch(std::false_type{}, Two{});
 }
 
 }  // namespace b2

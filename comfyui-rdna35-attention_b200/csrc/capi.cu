@@ -770,12 +770,12 @@ int check_attention(const b2_view* q, const b2_view* k, const b2_view* v, const 
 extern "C" {
 
 int b2_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out, float scale,
-                         int32_t causal, const int32_t* key_lengths, float* lse, void* stream) {
-  const int rc = check_attention(q, k, v, out, scale, key_lengths);
-  if (rc) return rc;
+                         int32_t causal, const int32_t* key_lengths, float* lse, const b2_view* out_low, void* stream) {
+  int rc = check_attention(q, k, v, out, scale, key_lengths);
+  if (rc || (out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q)))) return rc;
   int* status = device_status_ptr();
   if (status == nullptr) return fail(B2_ERR_CUDA, "device status word unavailable");
-  const AttnGeneralCall c{q, k, v, out, key_lengths, scale, causal ? 1 : 0, lse};
+  const AttnGeneralCall c{q, k, v, out, key_lengths, scale, causal ? 1 : 0, lse, out_low, nullptr};
   const cudaError_t err = launch_attn_general(c, status, static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) return cuda_fail(err, "attention launch");
   g_last_kernel = "tcgen05";
@@ -789,12 +789,12 @@ int64_t b2_attention_backward_workspace_bytes(int32_t batch, int32_t heads, int3
 }
 
 int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
-                          const b2_view* dout, const float* lse, const b2_view* dq, const b2_view* dk,
-                          const b2_view* dv, float scale, int32_t causal, const int32_t* key_lengths, void* workspace,
+                          const b2_view* out_low, const b2_view* dout, const float* lse, const b2_view* dq,
+                          const b2_view* dk, const b2_view* dv, float scale, int32_t causal, const int32_t* key_lengths, void* workspace,
                           void* stream) {
   int rc = check_attention(q, k, v, out, scale, key_lengths);
   if (rc) return rc;
-  if ((rc = check_grad_view(dout, "dout", q)) || (rc = check_grad_view(dq, "dq", q)) ||
+  if ((out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q))) || (rc = check_grad_view(dout, "dout", q)) || (rc = check_grad_view(dq, "dq", q)) ||
       (rc = check_grad_view(dk, "dk", k)) || (rc = check_grad_view(dv, "dv", v)))
     return rc;
   if (lse == nullptr || reinterpret_cast<uintptr_t>(lse) % 4) return fail(B2_ERR_INVALID, "lse must be non-NULL");
@@ -802,7 +802,7 @@ int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, 
     return fail(B2_ERR_INVALID, "workspace must be non-NULL and 16-byte aligned");
   int* status = device_status_ptr();
   if (status == nullptr) return fail(B2_ERR_CUDA, "device status word unavailable");
-  const AttnGradCall c{q, k, v, out, dout, dq, dk, dv, nullptr, nullptr, lse, key_lengths, scale, causal ? 1 : 0, workspace};
+  const AttnGradCall c{q, k, v, out, dout, dq, dk, dv, out_low, nullptr, lse, key_lengths, scale, causal ? 1 : 0, workspace};
   const cudaError_t err = launch_attn_grad(c, status, static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) return cuda_fail(err, "attention backward launch");
   return ok();
@@ -920,6 +920,150 @@ int b2_qk_norm_rope_backward(const b2_view* q, const b2_view* k, const b2_view* 
   c.rot = rot;
   c.partial = static_cast<float*>(workspace);
   const cudaError_t err = launch_rotary(c, static_cast<cudaStream_t>(stream));
+  if (err != cudaSuccess) return cuda_fail(err, "norm and rotary gradient launch");
+  return ok();
+}
+
+}  // extern "C"
+
+namespace {
+// What b2_norm_rope_attention_forward keeps for the backward pass, and the
+// backward pass's workspace.
+struct FusedSaved {
+  size_t q, k, scale, total;
+};
+FusedSaved fused_saved(int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens, int64_t dim) {
+  FusedSaved f;
+  f.q = 0;
+  f.k = align256(size_t(batch * heads * tokens * dim) * 2);
+  f.scale = f.k + align256(size_t(batch * kv_heads * tokens * dim) * 2);
+  f.total = f.scale + 256;
+  return f;
+}
+struct FusedWork {
+  size_t dq, dk, attention, partial, total;
+};
+FusedWork fused_work(int64_t batch, int64_t heads, int64_t kv_heads, int64_t tokens, int64_t dim) {
+  FusedWork f;
+  f.dq = 0;
+  f.dk = align256(size_t(batch * heads * tokens * dim) * 4);
+  f.attention = f.dk + align256(size_t(batch * kv_heads * tokens * dim) * 4);
+  f.partial = f.attention + align256(static_cast<size_t>(attn_grad_workspace_bytes(int(batch), int(heads), int(kv_heads),
+                                                                                    int(tokens), int(tokens))));
+  f.total = f.partial + static_cast<size_t>(rotary_workspace_bytes(int(dim)));
+  return f;
+}
+// [B,H,T,D] view of contiguous [B,T,H,D] storage of another type.
+b2_view token_major(const b2_view& like, void* base, int dtype) {
+  b2_view v = like;
+  v.base = base;
+  v.dtype = dtype;
+  v.stride_h = like.head_dim;
+  v.stride_t = int64_t(like.heads) * like.head_dim;
+  v.stride_b = v.stride_t * like.tokens;
+  return v;
+}
+int check_fused(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out, const void* qw, const void* kw,
+                int32_t w_dtype, float eps, const b2_rotary* rot, float scale, const int32_t* key_lengths,
+                const void* saved) {
+  int rc;
+  if ((rc = check_qk(q, k, qw, kw, w_dtype, eps, rot)) || (rc = check_attention(q, k, v, out, scale, key_lengths))) return rc;
+  if (rot->inverse) return fail(B2_ERR_UNSUPPORTED, "norm_rope_attention rotates forward only");
+  if (saved == nullptr || reinterpret_cast<uintptr_t>(saved) % 256)
+    return fail(B2_ERR_INVALID, "saved must be non-NULL and 256-byte aligned");
+  return B2_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int64_t b2_norm_rope_attention_saved_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens,
+                                           int32_t head_dim) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || tokens <= 0 || head_dim <= 0 || head_dim > 128 || head_dim % 8) return -1;
+  return static_cast<int64_t>(fused_saved(batch, heads, kv_heads, tokens, head_dim).total);
+}
+
+int64_t b2_norm_rope_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens,
+                                               int32_t head_dim) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || tokens <= 0 || head_dim <= 0 || head_dim > 128 || head_dim % 8) return -1;
+  return static_cast<int64_t>(fused_work(batch, heads, kv_heads, tokens, head_dim).total);
+}
+
+int b2_norm_rope_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
+                                   const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                                   const b2_rotary* rot, float scale, int32_t causal, const int32_t* key_lengths,
+                                   void* saved, float* lse, const b2_view* out_low, void* stream) {
+  int rc = check_fused(q, k, v, out, q_weight, k_weight, weight_dtype, eps, rot, scale, key_lengths, saved);
+  if (rc || (out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q)))) return rc;
+  int* status = device_status_ptr();
+  if (status == nullptr) return fail(B2_ERR_CUDA, "device status word unavailable");
+  const FusedSaved f = fused_saved(q->batch, q->heads, k->heads, q->tokens, q->head_dim);
+  char* base = static_cast<char*>(saved);
+  float* qk_scale = reinterpret_cast<float*>(base + f.scale);
+  const b2_view q16 = token_major(*q, base + f.q, B2_F16), k16 = token_major(*k, base + f.k, B2_F16);
+  RotaryCall r{};
+  r.x[0] = q, r.x[1] = k;
+  r.y[0] = &q16, r.y[1] = &k16;
+  r.w[0] = q_weight, r.w[1] = k_weight;
+  r.w_dtype = weight_dtype;
+  r.norm = true;
+  r.eps = eps;
+  r.rot = rot;
+  r.scale = qk_scale;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t err = launch_rotary(r, st);
+  if (err != cudaSuccess) return cuda_fail(err, "norm and rotary launch");
+  const AttnGeneralCall c{&q16, &k16, v, out, key_lengths, scale, causal ? 1 : 0, lse, out_low, qk_scale};
+  err = launch_attn_general(c, status, st);
+  if (err != cudaSuccess) return cuda_fail(err, "attention launch");
+  g_last_kernel = "tcgen05";
+  return ok();
+}
+
+int b2_norm_rope_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
+                                    const b2_view* out_low, const b2_view* dout, const float* lse, const void* q_weight,
+                                    const void* k_weight, int32_t weight_dtype, float eps, const b2_rotary* rot,
+                                    float scale, int32_t causal, const int32_t* key_lengths, const void* saved,
+                                    const b2_view* dq, const b2_view* dk, const b2_view* dv, void* q_weight_grad,
+                                    void* k_weight_grad, void* workspace, void* stream) {
+  int rc = check_fused(q, k, v, out, q_weight, k_weight, weight_dtype, eps, rot, scale, key_lengths, saved);
+  if (rc) return rc;
+  if ((out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q))) || (rc = check_grad_view(dout, "dout", q)) ||
+      (rc = check_grad_view(dq, "dq", q)) || (rc = check_grad_view(dk, "dk", k)) || (rc = check_grad_view(dv, "dv", v)))
+    return rc;
+  if (lse == nullptr || reinterpret_cast<uintptr_t>(lse) % 4) return fail(B2_ERR_INVALID, "lse must be non-NULL");
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(B2_ERR_INVALID, "workspace must be non-NULL and 256-byte aligned");
+  const uintptr_t mask = weight_dtype == B2_F32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(q_weight_grad) | reinterpret_cast<uintptr_t>(k_weight_grad)) & mask)
+    return fail(B2_ERR_INVALID, "weight gradients must be aligned to their type");
+  int* status = device_status_ptr();
+  if (status == nullptr) return fail(B2_ERR_CUDA, "device status word unavailable");
+  const FusedSaved f = fused_saved(q->batch, q->heads, k->heads, q->tokens, q->head_dim);
+  const FusedWork w = fused_work(q->batch, q->heads, k->heads, q->tokens, q->head_dim);
+  char* base = static_cast<char*>(const_cast<void*>(saved));
+  char* ws = static_cast<char*>(workspace);
+  const float* qk_scale = reinterpret_cast<const float*>(base + f.scale);
+  const b2_view q16 = token_major(*q, base + f.q, B2_F16), k16 = token_major(*k, base + f.k, B2_F16);
+  const b2_view dq32 = token_major(*q, ws + w.dq, B2_F32), dk32 = token_major(*k, ws + w.dk, B2_F32);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const AttnGradCall c{&q16, &k16, v, out, dout, &dq32, &dk32, dv, out_low, qk_scale, lse, key_lengths, scale,
+                       causal ? 1 : 0, ws + w.attention};
+  cudaError_t err = launch_attn_grad(c, status, st);
+  if (err != cudaSuccess) return cuda_fail(err, "attention backward launch");
+  RotaryCall r{};
+  r.x[0] = q, r.x[1] = k;
+  r.dy[0] = &dq32, r.dy[1] = &dk32;
+  r.y[0] = dq, r.y[1] = dk;
+  r.w[0] = q_weight, r.w[1] = k_weight;
+  r.dw[0] = q_weight_grad, r.dw[1] = k_weight_grad;
+  r.w_dtype = weight_dtype;
+  r.norm = true;
+  r.eps = eps;
+  r.rot = rot;
+  r.partial = reinterpret_cast<float*>(ws + w.partial);
+  r.lengths = key_lengths;
+  err = launch_rotary(r, st);
   if (err != cudaSuccess) return cuda_fail(err, "norm and rotary gradient launch");
   return ok();
 }

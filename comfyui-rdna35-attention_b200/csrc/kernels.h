@@ -8,6 +8,11 @@ namespace b2 {
 // 4D TMA map (D,T,H,B) of a linear view: boxes of 64 columns x box_rows rows,
 // zeros past D and T.  False for views TMA cannot address.
 bool linear_rows_map(CUtensorMap* map, const b2_view& v, int box_rows);
+// Where a batch has at most this many keys, the forward pass also writes what
+// the output's type cannot hold: delta = rowsum(dout * out) then cancels
+// against few dP terms, and BF16's rounding of out would be the largest error
+// of dQ and dK (5e-3 of dQ for 2 keys, 1e-3 from 64 on).
+constexpr int kLowKeys = 64;
 constexpr int kMaxMirrors = 7;  // peer copies of an output (head-sharded calls over up to 8 GPUs)
 // Parameters of the fused attention kernel (see attn_mma.cu).
 struct AttnParams {
@@ -63,6 +68,8 @@ struct UmmaArgs {
   int kv_heads;
   const int32_t* key_lengths;  // [B] or NULL
   int causal_off;              // causal: query i sees keys up to i + causal_off
+  Rows o_low;                  // what o's type cannot hold of the output (rows of few keys), or no base
+  const float* qk_scale;       // the powers of two FP16 q and k are held times
 };
 bool umma_supported(const b2_view& q, const b2_view& k, const b2_view& v, const b2_view& o);
 cudaError_t launch_attn_umma(const b2_view& qv, const b2_view& kv, const b2_view& vv, const b2_view& ov,
@@ -105,6 +112,8 @@ struct AttnGeneralCall {
   float scale;
   int causal;
   float* lse;
+  const b2_view* out_low;   // or NULL
+  const float* qk_scale;    // FP16 q, k held times these (whatever v's type), or NULL
 };
 cudaError_t launch_attn_general(const AttnGeneralCall& call, int* status, cudaStream_t stream);
 struct AttnGradCall {
@@ -123,6 +132,7 @@ cudaError_t launch_attn_grad(const AttnGradCall& call, int* status, cudaStream_t
 // Norm + rotary positions (rotary.cu): one or two sides (queries, keys).
 // Forward: y from x.  Gradients (dy set): y receives dx, dw (may be NULL) the
 // weight gradients, partial is rotary_workspace_bytes() of scratch.
+// scale (with norm): y in FP16, held times the power of two written there per side.
 struct RotaryCall {
   const b2_view* x[2];
   const b2_view* dy[2];
@@ -134,6 +144,8 @@ struct RotaryCall {
   float eps;
   const b2_rotary* rot;
   float* partial;
+  float* scale;
+  const int32_t* lengths;  // gradients: tokens of each batch that side 1 has (the others get 0), or NULL
 };
 int64_t rotary_workspace_bytes(int head_dim);
 cudaError_t launch_rotary(const RotaryCall& call, cudaStream_t stream);

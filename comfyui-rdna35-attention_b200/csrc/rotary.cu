@@ -30,6 +30,8 @@
 #include <math.h>
 #include <string.h>
 
+#include <type_traits>
+
 #include "kernels.h"
 
 namespace b2 {
@@ -88,6 +90,8 @@ struct RotaryArgs {
   int group_log2;   // lanes of a row
   int tt_log2;      // tokens of a block
   float* partial;   // [side][kGradBlocks][dim] weight-gradient partials
+  const int32_t* lengths;  // backward: tokens of each batch that side 1 has, or NULL
+  float* scale;     // FP16 output of other inputs: the powers of two the sides are held times
   double turn[kMaxPairs];
   uint8_t axis[kMaxPairs];
 };
@@ -356,11 +360,6 @@ __device__ __forceinline__ void turn(const float4 (&k)[4], float (&v)[8], const 
   }
 }
 
-// Shared-memory bytes of the fetched rows: `rows` in flight for every thread.
-template <typename T, int LAYOUT>
-__host__ __device__ constexpr int fetch_bytes(int rows) {
-  return LAYOUT == kScalar ? 0 : rows * kThreads * Raw<T, LAYOUT>::kSlot;
-}
 // Rows of x and of dy in flight for a thread of the backward pass.  Forward
 // keeps its four rows in registers instead: computing four at a time hides
 // the group sums, and measured 114 us against 126 (32760 x 40 x 128) for the
@@ -377,7 +376,28 @@ struct Walk {
   __device__ __forceinline__ void next(int u = 1) { p += u * step; }
 };
 
-template <typename T, int LAYOUT, bool NORM>
+// The power of two a normed side is held times in FP16, from its largest
+// weight: |y| <= sqrt(2 D) max|w|, which becomes 2^13 .. 2^14.
+__device__ __forceinline__ float side_scale(const RotaryArgs& a, int side, float* shared) {
+  float most = 0.f;
+  for (int d = threadIdx.x; d < a.dim; d += kThreads)
+    most = fmaxf(most, a.side[side].w != nullptr ? fabsf(weight_at(a.side[side].w, a.w_dtype, d)) : 1.f);
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = most;
+  __syncthreads();
+  most = shared[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 32; ++w) most = fmaxf(most, shared[w]);
+  const float bound = most * sqrtf(2.f * a.dim);
+  if (!(bound > 0.f) || !(bound < 3e38f)) return 1.f;
+  return ldexpf(1.f, min(max(13 - ilogbf(bound), -60), 60));
+}
+
+// TO: the output's type, T but for the FP16 copies that attention's products
+// read (the scale above then multiplies the weights).
+template <typename T, typename TO, int LAYOUT, bool NORM>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && LAYOUT != kScalar ? 4 : 2)
 rotary_kernel(const __grid_constant__ RotaryArgs a) {
   constexpr int U = 4;  // rows of a group in flight
@@ -393,6 +413,14 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
   if constexpr (NORM) {
     fill_weights<LAYOUT>(a, 0, ws);
     fill_weights<LAYOUT>(a, 1, ws);
+    if (a.scale != nullptr) {
+      __shared__ float shared[kThreads / 32];
+      for (int side = 0; side < a.sides; ++side) {
+        const float scale = side_scale(a, side, shared);
+        ws[side * kThreads + threadIdx.x] *= scale;
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.scale[side] = scale;
+      }
+    }
   }
   for (int n0 = blockIdx.x << a.tt_log2; n0 < n_tokens; n0 += gridDim.x << a.tt_log2) {
     const int n = n0 + t.tok;
@@ -401,7 +429,7 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
     float2 ang[4];
     for (int side = 0; side < a.sides; ++side) {
       const Side& s = a.side[side];
-      Walk x(s.x, b, tok, t, sizeof(T)), y(s.y, b, tok, t, sizeof(T));
+      Walk x(s.x, b, tok, t, sizeof(T)), y(s.y, b, tok, t, sizeof(TO));
       int left = n < n_tokens && t.active ? (s.heads - t.gi + t.gpt - 1) >> t.gpt_log2 : 0;  // rows of this group
       // every thread of the block runs the same number of steps: the group
       // sums are full-warp shuffles
@@ -444,8 +472,9 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
           }
           turn<LAYOUT>(k, v, t, a.rot_pairs);
           if (u < left) {
-            raw[u].narrow(v);
-            raw[u].store(y.at(u), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
+            Raw<TO, LAYOUT> to;
+            to.narrow(v);
+            to.store(y.at(u), t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
           }
         }
         y.next(U);
@@ -457,10 +486,11 @@ rotary_kernel(const __grid_constant__ RotaryArgs a) {
 // Gradients of norm + rotation.  Blocks stride over the token tiles of one
 // side, so a lane's weight gradients stay in registers until the end and the
 // partials are few; their order, and so the result, is fixed.
-template <typename T, int LAYOUT>
+template <typename T, typename TD, int LAYOUT>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && LAYOUT != kScalar ? 3 : 2)
 rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
   using R = Raw<T, LAYOUT>;
+  using RD = Raw<TD, LAYOUT>;  // dy
   extern __shared__ __align__(16) char slots[];
   __shared__ float2 cs[kMaxTokens * kMaxPairs];
   __shared__ RateTable rates;
@@ -472,8 +502,9 @@ rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
   const bool inter = a.interleaved != 0;
   const float inv_dim = 1.f / static_cast<float>(a.dim);
   const int steps = (s.heads + t.gpt - 1) >> t.gpt_log2;
-  char* const own = slots + threadIdx.x * R::kSlot;
-  constexpr int kStage = 2 * kThreads * R::kSlot;  // x, then dy
+  constexpr int kStage = kThreads * (R::kSlot + RD::kSlot);  // x, then dy
+  char* const own_x = slots + threadIdx.x * R::kSlot;
+  char* const own_dy = slots + kThreads * R::kSlot + threadIdx.x * RD::kSlot;
   float w[8], dw[8] = {};
   fill_rates(a, rates);
   fill_weights<LAYOUT>(a, blockIdx.y, ws);
@@ -483,14 +514,15 @@ rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
     const int n = n0 + t.tok;
     const int b = n / a.tokens;
     const int tok = n - b * a.tokens;
-    Walk wx(s.x, b, tok, t, sizeof(T)), wdy(s.dy, b, tok, t, sizeof(T)), wy(s.y, b, tok, t, sizeof(T));
+    Walk wx(s.x, b, tok, t, sizeof(T)), wdy(s.dy, b, tok, t, sizeof(TD)), wy(s.y, b, tok, t, sizeof(T));
     const int rows = n < n_tokens && t.active ? (s.heads - t.gi + t.gpt - 1) >> t.gpt_log2 : 0;
+    // keys past a batch's count: whatever they hold, their gradient is 0
+    const bool dead = a.lengths != nullptr && blockIdx.y == 1 && n < n_tokens && tok >= a.lengths[b];
     auto fetch = [&](int j) {
       if constexpr (LAYOUT != kScalar) {
         if (j < rows) {
-          char* slot = own + (j % kAheadGrad) * kStage;
-          R::fetch(slot, wx.p, t.c0, t.c1);
-          R::fetch(slot + kThreads * R::kSlot, wdy.p, t.c0, t.c1);
+          R::fetch(own_x + (j % kAheadGrad) * kStage, wx.p, t.c0, t.c1);
+          RD::fetch(own_dy + (j % kAheadGrad) * kStage, wdy.p, t.c0, t.c1);
         }
         wx.next(), wdy.next();
         cp_async_commit();
@@ -510,25 +542,28 @@ rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
     }
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
-      R rx, rdy;
+      R rx;
+      RD rdy;
       if constexpr (LAYOUT == kScalar) {
         if (j < rows) {
           rx.load(wx.p, t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
           rdy.load(wdy.p, t.l, t.c0, t.c1, a.rot_pairs, inter, pairs);
         } else {
-          rx = rdy = R{};
+          rx = R{};
+          rdy = RD{};
         }
         wx.next(), wdy.next();
       } else {
         cp_async_wait<kAheadGrad - 1>();
-        rx.take(own + (j % kAheadGrad) * kStage);
-        rdy.take(own + (j % kAheadGrad) * kStage + kThreads * R::kSlot);
+        rx.take(own_x + (j % kAheadGrad) * kStage);
+        rdy.take(own_dy + (j % kAheadGrad) * kStage);
       }
       float x[8], g[8];
       rx.widen(x);
       rdy.widen(g);
       fetch(j + kAheadGrad);
-      if (j >= rows) {  // what a slot held before may be NaN
+      const bool counts = j < rows && !dead;
+      if (!counts) {  // what a slot held before may be NaN
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = g[i] = 0.f;
       }
@@ -541,7 +576,7 @@ rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
       }
       float sums[2] = {sum, dot};
       group_sums<2>(sums, a.group_log2);
-      const float r = rsqrtf(sums[0] * inv_dim + a.eps);
+      const float r = counts ? rsqrtf(sums[0] * inv_dim + a.eps) : 0.f;  // eps may be 0
       const float back = -sums[1] * inv_dim * r * r * r;  // xh mean(g w xh) r = -back x
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -636,12 +671,20 @@ const Rates& rates_of(const b2_rotary& r) {
   return k;
 }
 
-template <typename T, int LAYOUT>
+// T: inputs; TX: the other type of the call (forward: the output's, backward: dy's).
+template <typename T, typename TX, int LAYOUT>
 cudaError_t launch_layout(const RotaryArgs& a, bool norm, bool grad, int64_t tiles, cudaStream_t st) {
   using Kernel = void (*)(const RotaryArgs);
-  const Kernel kernel = grad ? Kernel(rotary_grad_kernel<T, LAYOUT>)
-                             : norm ? Kernel(rotary_kernel<T, LAYOUT, true>) : Kernel(rotary_kernel<T, LAYOUT, false>);
-  const int smem = grad ? fetch_bytes<T, LAYOUT>(2 * kAheadGrad) : 0;
+  Kernel kernel;
+  int smem = 0;
+  if (grad) {
+    kernel = rotary_grad_kernel<T, TX, LAYOUT>;
+    if (LAYOUT != kScalar) smem = kAheadGrad * kThreads * (Raw<T, LAYOUT>::kSlot + Raw<TX, LAYOUT>::kSlot);
+  } else if constexpr (std::is_same<T, TX>::value) {
+    kernel = norm ? Kernel(rotary_kernel<T, TX, LAYOUT, true>) : Kernel(rotary_kernel<T, TX, LAYOUT, false>);
+  } else {
+    return cudaErrorInvalidValue;
+  }
   cudaError_t err = ensure_smem(reinterpret_cast<const void*>(kernel), smem);
   if (err != cudaSuccess) return err;
   const int most = grad ? kGradBlocks : kBlocks;
@@ -652,11 +695,19 @@ cudaError_t launch_layout(const RotaryArgs& a, bool norm, bool grad, int64_t til
                     static_cast<int>(grid.x));
 }
 
-template <typename T>
+template <typename T, typename TX>
 cudaError_t launch_typed(const RotaryArgs& a, int layout, bool norm, bool grad, int64_t tiles, cudaStream_t st) {
-  if (layout == kInterleaved) return launch_layout<T, kInterleaved>(a, norm, grad, tiles, st);
-  if (layout == kHalves) return launch_layout<T, kHalves>(a, norm, grad, tiles, st);
-  return launch_layout<T, kScalar>(a, norm, grad, tiles, st);
+  if (layout == kInterleaved) return launch_layout<T, TX, kInterleaved>(a, norm, grad, tiles, st);
+  if (layout == kHalves) return launch_layout<T, TX, kHalves>(a, norm, grad, tiles, st);
+  return launch_layout<T, TX, kScalar>(a, norm, grad, tiles, st);
+}
+
+// The FP16 copies of BF16 queries and keys.
+template <int LAYOUT>
+cudaError_t launch_copies(const RotaryArgs& a, int64_t tiles, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(tiles < kBlocks ? tiles : kBlocks));
+  rotary_kernel<__nv_bfloat16, __half, LAYOUT, true><<<grid, kThreads, 0, st>>>(a);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -713,10 +764,20 @@ cudaError_t launch_rotary(const RotaryCall& c, cudaStream_t st) {
   }
   a.tt_log2 = tt_log2;
   const int64_t tiles = (n_tokens + (1 << tt_log2) - 1) >> tt_log2;
+  a.scale = c.scale;
+  a.lengths = c.lengths;
+  if (c.scale != nullptr && v.dtype == B2_BF16)
+    return layout == kInterleaved ? launch_copies<kInterleaved>(a, tiles, st)
+                                  : layout == kHalves ? launch_copies<kHalves>(a, tiles, st) : launch_copies<kScalar>(a, tiles, st);
+  const bool dy32 = grad && c.dy[0]->dtype == B2_F32;
   switch (v.dtype) {
-    case B2_BF16: return launch_typed<__nv_bfloat16>(a, layout, c.norm, grad, tiles, st);
-    case B2_F16: return launch_typed<__half>(a, layout, c.norm, grad, tiles, st);
-    default: return launch_typed<float>(a, layout, c.norm, grad, tiles, st);
+    case B2_BF16:
+      return dy32 ? launch_typed<__nv_bfloat16, float>(a, layout, c.norm, grad, tiles, st)
+                  : launch_typed<__nv_bfloat16, __nv_bfloat16>(a, layout, c.norm, grad, tiles, st);
+    case B2_F16:
+      return dy32 ? launch_typed<__half, float>(a, layout, c.norm, grad, tiles, st)
+                  : launch_typed<__half, __half>(a, layout, c.norm, grad, tiles, st);
+    default: return launch_typed<float, float>(a, layout, c.norm, grad, tiles, st);
   }
 }
 

@@ -314,19 +314,21 @@ int b2_fixed_block_attention_masked(const b2_view* q, const b2_view* k,
  * whatever they hold.  causal: query i sees keys up to i + Tk - Tq.  A query
  * that sees no key gives out = 0, lse = -inf and gradient 0.
  * lse: [B,H,Tq] FP32, the natural log of the sum of exp(scale * scores); NULL
- * if not wanted. */
+ * if not wanted.  out_low (NULL if not wanted): like out, receives out's
+ * rounding error in batches of at most 64 keys, where the backward pass needs
+ * it; elsewhere it is neither written nor read. */
 int b2_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out, float scale,
-                         int32_t causal, const int32_t* key_lengths, float* lse, void* stream);
+                         int32_t causal, const int32_t* key_lengths, float* lse, const b2_view* out_low, void* stream);
 /* dq, dk, dv from dout and what the forward pass was given and wrote (out,
- * lse; the same scale, causal and key_lengths).  Rows of dk/dv past a batch's
+ * lse, out_low or NULL; the same scale, causal and key_lengths).  Rows of dk/dv past a batch's
  * keys are written as 0.  Probabilities are recomputed; workspace:
  * b2_attention_backward_workspace_bytes() bytes for row statistics, read and
  * written only by this call.  Results are bit-reproducible. */
 int64_t b2_attention_backward_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t q_tokens,
                                               int32_t k_tokens);
 int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
-                          const b2_view* dout, const float* lse, const b2_view* dq, const b2_view* dk,
-                          const b2_view* dv, float scale, int32_t causal, const int32_t* key_lengths, void* workspace,
+                          const b2_view* out_low, const b2_view* dout, const float* lse, const b2_view* dq,
+                          const b2_view* dk, const b2_view* dv, float scale, int32_t causal, const int32_t* key_lengths, void* workspace,
                           void* stream);
 
 /* ---- Per-head RMS norm of queries and keys and rotary positions with several
@@ -369,6 +371,30 @@ int b2_qk_norm_rope_backward(const b2_view* q, const b2_view* k, const b2_view* 
                              const b2_view* q_grad, const b2_view* k_grad, const void* q_weight, const void* k_weight,
                              int32_t weight_dtype, float eps, const b2_rotary* rot, void* q_weight_grad,
                              void* k_weight_grad, void* workspace, void* stream);
+
+/* ---- b2_qk_norm_rope followed by b2_attention, as one differentiable
+ * operator (self-attention: q and k share T): the normed and rotated queries
+ * and keys stay in the library, as FP16 held times a power of two per side,
+ * and their gradients in FP32, so BF16 models lose no accuracy between the
+ * two steps.  q, out: [B,H,T,D]; k, v: [B,Hk,T,D]; weights, rot (not
+ * inverse), scale, causal, key_lengths, lse and out_low as above.  saved:
+ * b2_norm_rope_attention_saved_bytes() bytes (256-byte aligned) that the
+ * forward pass writes and the backward pass reads; workspace (256-byte
+ * aligned) is read and written only by the call. */
+int64_t b2_norm_rope_attention_saved_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens,
+                                           int32_t head_dim);
+int64_t b2_norm_rope_attention_workspace_bytes(int32_t batch, int32_t heads, int32_t kv_heads, int32_t tokens,
+                                               int32_t head_dim);
+int b2_norm_rope_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
+                                   const void* q_weight, const void* k_weight, int32_t weight_dtype, float eps,
+                                   const b2_rotary* rot, float scale, int32_t causal, const int32_t* key_lengths,
+                                   void* saved, float* lse, const b2_view* out_low, void* stream);
+int b2_norm_rope_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
+                                    const b2_view* out_low, const b2_view* dout, const float* lse, const void* q_weight,
+                                    const void* k_weight, int32_t weight_dtype, float eps, const b2_rotary* rot,
+                                    float scale, int32_t causal, const int32_t* key_lengths, const void* saved,
+                                    const b2_view* dq, const b2_view* dk, const b2_view* dv, void* q_weight_grad,
+                                    void* k_weight_grad, void* workspace, void* stream);
 
 /* ---- Layout kernels. */
 /* pisa_kernels.cu:247-272: [B,H,T,D] tiled views -> contiguous [BH,T,D]. */

@@ -157,11 +157,11 @@ def test_c_entries_check_their_arguments():
     fake = ctypes.c_void_p(256)
 
     def forward(q=q, k=k, v=k, out=q, scale=0.1, lens=None):
-        return lib.b2_attention_forward(*(ctypes.byref(a) for a in (q, k, v, out)), scale, 0, lens, None, None)
+        return lib.b2_attention_forward(*(ctypes.byref(a) for a in (q, k, v, out)), scale, 0, lens, None, None, None)
 
     def backward(dq=q, dk=k, lse=fake, ws=fake):
-        args = [ctypes.byref(a) for a in (q, k, k, q, q)]
-        return lib.b2_attention_backward(*args, lse, ctypes.byref(dq), ctypes.byref(dk), ctypes.byref(k), 0.1, 0, None,
+        args = [ctypes.byref(a) for a in (q, k, k, q)]
+        return lib.b2_attention_backward(*args, None, ctypes.byref(q), lse, ctypes.byref(dq), ctypes.byref(dk), ctypes.byref(k), 0.1, 0, None,
                                          ws, None)
 
     def changed(view, **fields):

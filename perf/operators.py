@@ -366,13 +366,14 @@ def _run_own(s):
         if case["pass"] == "forward":
             return y
         return y.detach(), torch.autograd.grad(y, s["q"], s["dq"])[0]
+    if case["op"] == "layer":
+        out = b200_pisa.norm_rope_attention(s["q"], s["k"], s["v"], s["wq"], s["wk"], s["pos"], _axes(case), eps=EPS,
+                                            causal=case["causal"], key_lengths=s["lens"], **rotation)
+        dv, *grads = torch.autograd.grad(out, [s[n] for n in ("v", "q", "k", "wq", "wk")], s["dout"])
+        return (out.detach(), dv, *grads)
     q, k = b200_pisa.qk_norm_rope(s["q"], s["k"], s["wq"], s["wk"], s["pos"], _axes(case), eps=EPS, **rotation)
     if case["pass"] == "forward":
         return q, k
-    if case["op"] == "layer":
-        out = b200_pisa.attention(q, k, s["v"], causal=case["causal"], key_lengths=s["lens"])
-        dv, *grads = torch.autograd.grad(out, [s[n] for n in ("v", "q", "k", "wq", "wk")], s["dout"])
-        return (out.detach(), dv, *grads)
     return (q.detach(), k.detach(),
             *torch.autograd.grad((q, k), [s[n] for n in ("q", "k", "wq", "wk")], (s["dq"], s["dk"])))
 

@@ -22,9 +22,14 @@
 // shared-memory bandwidth (about 3750 cycles a pair at 128 B a cycle, against
 // 7 * 512 for the products here).
 //
-// Warp roles (576 threads): warp 0 TMA producer and item scheduler, warp 1
-// MMA issuer and TMEM owner, warps 2..17 elementwise (warp % 4 is the TMEM
-// lane quadrant, and each group of four warps takes 32 columns of a tile).
+// The walked tiles are 128 rows for head dimensions above 64 and 64 rows up to
+// 64, where the elementwise work is what takes time: then two CTAs share an
+// SM (256 TMEM columns each), and one's exponentials run beside the other's
+// loads, stores and waits.
+//
+// Warp roles: warp 0 TMA producer and item scheduler, warp 1 MMA issuer and
+// TMEM owner, the other 16 (8) warps elementwise (warp % 4 is the TMEM lane
+// quadrant, and each group of four warps takes 32 columns of a tile).
 // Rings, barriers and tensor memory live across items: an item's first tiles
 // load and its first S and dP run while the one before stores its results.
 //
@@ -48,11 +53,8 @@ namespace {
 
 using namespace umma;
 
-constexpr int kTile = 128;
-constexpr int kElemWarps = 16;  // 4 TMEM lane quadrants x 4 column groups of 32
-constexpr int kThreads = 64 + 32 * kElemWarps;
+constexpr int kTile = 128;  // rows that an item owns
 constexpr uint32_t kHalfBytes = kTile * 128;  // 128 rows x 64 16-bit columns
-constexpr uint32_t kStatBytes = 2 * kTile * 4;
 // Rings of the walked tiles.  K (or Q) is read by the first and the last
 // product of its tile pair, so with two stages each pair waits for its load.
 constexpr int kStagesA = 3, kStagesB = 2;
@@ -60,16 +62,28 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kShiftP16 = 8;  // FP16 v: P is held times 2^8
 constexpr int kStatRows = 64;  // rows of a block of the statistics kernel
 
-// TMEM columns.
-//   dK/dV: S and dP take turns in kColX (each is free again as soon as the
-//     elementwise warps have loaded it), P, dS, dV, dK.
-//   dQ: S, dP, dQ, dS, and Q: as the A operand of S it costs no shared-memory
-//     reads there, whose 128 bytes a cycle A and B of a 128 x 128 product
-//     take all of (1.53 ms against 1.69 for all of dQ).  The same for V in the
-//     dK/dV items needs P and dS to share columns, and their products to wait
-//     for one another: 2.20 ms against 2.06.
-constexpr uint32_t kColX = 0, kColP = 128, kColDS = 192, kColDV = 256, kColDK = 384;
-constexpr uint32_t kColS = 0, kColDP = 128, kColDQ = 256, kColDSq = 384, kColQ = 448;
+// HALVES: 64-column halves of the head dimension that the products cover.
+template <int HALVES>
+struct Cfg {
+  static constexpr int kWalk = HALVES == 1 ? 64 : 128;  // rows of a walked tile
+  static constexpr int kGroups = kWalk / 32;            // column groups of 32
+  static constexpr int kElemWarps = 4 * kGroups;        // times the TMEM lane quadrants
+  static constexpr int kThreads = 64 + 32 * kElemWarps;
+  static constexpr int kCtas = HALVES == 1 ? 2 : 1;     // per SM
+  static constexpr uint32_t kStatBytes = 2 * kWalk * 4;
+  // TMEM columns.
+  //   dK/dV: S and dP take turns in kX (each is free again as soon as the
+  //     elementwise warps have loaded it), P, dS, dV, dK.
+  //   dQ: S, dP, dQ, dS, and Q: as the A operand of S it costs no
+  //     shared-memory reads there, whose 128 bytes a cycle A and B of a
+  //     128 x 128 product take all of (1.53 ms against 1.69 for all of dQ).
+  //     The same for V in the dK/dV items needs P and dS to share columns, and
+  //     their products to wait for one another: 2.20 ms against 2.06.
+  static constexpr uint32_t kX = 0, kP = kWalk, kDS = kP + kWalk / 2, kDV = 2 * kWalk, kDK = kDV + 64 * HALVES;
+  static constexpr uint32_t kS = 0, kDP = kWalk, kDQ = 2 * kWalk, kDSq = kDQ + 64 * HALVES, kQ = kDSq + kWalk / 2;
+  static constexpr uint32_t kTmem = kDK + 64 * HALVES;  // 512 or 256
+  static_assert(kQ + 32 * HALVES == kTmem, "both kinds of item fill the columns");
+};
 
 struct GradArgs {
   Rows dq, dk, dv;
@@ -81,7 +95,7 @@ struct GradArgs {
   const int32_t* key_lengths;
   int heads, kv_heads, group;
   int tq, tk, dim;
-  int q_tiles, k_tiles, v_blocks;
+  int q_tiles, k_tiles, q_walk, v_blocks;  // own tiles, walked query tiles
   int n_dkv, n_items;  // items of the dK/dV kind (they come first), and all
   int causal;
   float scale, scale_log2;
@@ -105,17 +119,19 @@ struct __align__(8) Misc {
 
 template <int HALVES>
 struct Smem {
-  static constexpr uint32_t tile = HALVES * kHalfBytes;
+  static constexpr uint32_t own_tile = HALVES * kHalfBytes, tile = HALVES * Cfg<HALVES>::kWalk * 128;
   static constexpr uint32_t own = 0;  // dK/dV: K and V; dQ: dO and Q
-  static constexpr uint32_t a = own + 2 * tile;
+  static constexpr uint32_t a = own + 2 * own_tile;
   static constexpr uint32_t b = a + kStagesA * tile;
   static constexpr uint32_t stat = b + kStagesB * tile;  // [2]
-  static constexpr uint32_t misc = stat + 2 * kStatBytes;
-  // one CTA per SM (each owns all 512 TMEM columns)
+  static constexpr uint32_t misc = stat + 2 * Cfg<HALVES>::kStatBytes;
+  // no more CTAs to an SM than its TMEM columns serve
   static constexpr uint32_t used = misc + sizeof(Misc);
-  static constexpr uint32_t total = used < 120 * 1024 ? 120 * 1024 : used;
+  static constexpr uint32_t least = (HALVES == 1 ? 80 : 120) * 1024;
+  static constexpr uint32_t total = used < least ? least : used;
 };
 static_assert(Smem<2>::total <= 232448, "shared memory budget");
+static_assert(2 * (Smem<1>::total + 1024) <= 233472, "two CTAs per SM");
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(
@@ -124,12 +140,19 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// 128 rows of one head as HALVES boxes of 64 columns.
+// A walked tile of one head: HALVES boxes of 64 columns.
 template <int HALVES>
 __device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uint64_t* bar, int row, int h, int b) {
 #pragma unroll
   for (int dh = 0; dh < HALVES; ++dh)
     tma_load_4d(static_cast<char*>(dst) + dh * kHalfBytes, map, bar, dh * 64, row, h, b);
+}
+// An own tile: 128 rows, by boxes of as many rows as a walked tile has.
+template <int HALVES>
+__device__ __forceinline__ void load_own(char* dst, const CUtensorMap* map, uint64_t* bar, int row, int h, int b) {
+  constexpr int kWalk = Cfg<HALVES>::kWalk;
+#pragma unroll
+  for (int r = 0; r < kTile; r += kWalk) load_tile<HALVES>(dst + r * 128, map, bar, row + r, h, b);
 }
 
 // Descriptors of a tile at shared-memory address `addr`, as rows of a product
@@ -140,10 +163,10 @@ __device__ __forceinline__ void load_tile(void* dst, const CUtensorMap* map, uin
 __device__ __forceinline__ uint64_t rows_desc(uint32_t addr) { return smem_desc_sw128(addr, 16, 1024); }
 __device__ __forceinline__ uint64_t cols_desc(uint32_t addr) { return smem_desc_sw128(addr, kHalfBytes, 1024); }
 
-// D[128 x 128] = A B^T over the head dimension, both tiles K-major in shared memory.
+// D[128 x walk] = A B^T over the head dimension, both tiles K-major in shared memory.
 template <bool BF16, int HALVES>
 __device__ __forceinline__ void product_rows(uint32_t d, uint64_t a_desc, uint64_t b_desc) {
-  constexpr uint32_t idesc = idesc_f16(128, 128, BF16, false, false);
+  constexpr uint32_t idesc = idesc_f16(128, Cfg<HALVES>::kWalk, BF16, false, false);
 #pragma unroll
   for (int kk = 0; kk < 4 * HALVES; ++kk) {
     const uint32_t off = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
@@ -154,19 +177,19 @@ __device__ __forceinline__ void product_rows(uint32_t d, uint64_t a_desc, uint64
 // The same with A (16-bit pairs: 32 * HALVES columns) in tensor memory at `a`.
 template <bool BF16, int HALVES>
 __device__ __forceinline__ void product_rows_ts(uint32_t d, uint32_t a, uint64_t b_desc) {
-  constexpr uint32_t idesc = idesc_f16(128, 128, BF16, false, false);
+  constexpr uint32_t idesc = idesc_f16(128, Cfg<HALVES>::kWalk, BF16, false, false);
 #pragma unroll
   for (int kk = 0; kk < 4 * HALVES; ++kk)
     mma_ts(d, a + kk * 8, b_desc + (((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4), idesc, kk > 0 ? 1u : 0u);
 }
 
-// D[128 x D] (+)= A B with A (128 x 128, 16-bit pairs: 64 columns) in tensor
-// memory at `a`, B's rows as contraction.
+// D[128 x D] (+)= A B with A (128 x walk, 16-bit pairs) in tensor memory at
+// `a`, B's rows as contraction.
 template <bool BF16, int HALVES>
 __device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint64_t b_desc, bool accumulate) {
   constexpr uint32_t idesc = idesc_f16(128, 64 * HALVES, BF16, false, true);
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk)
+  for (int kk = 0; kk < Cfg<HALVES>::kWalk / 16; ++kk)
     mma_ts(d, a + kk * 8, b_desc + kk * (2048 >> 4), idesc, kk > 0 ? 1u : accumulate ? 1u : 0u);
 }
 
@@ -217,7 +240,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
 // it: 128-byte rows, 16-byte chunks swizzled by the row) to tensor memory.
 template <int HALVES>
 __device__ __forceinline__ void row_to_tmem(uint32_t taddr, const char* tile, int row, int cg) {
-  if (cg >= 2 * HALVES) return;
   const char* src = tile + (cg >> 1) * kHalfBytes + row * 128;
   uint32_t w[16];
 #pragma unroll
@@ -340,7 +362,9 @@ struct Work {
   int first, per_head;  // dK/dV: the first query tile, and how many of each head
 };
 
+template <int HALVES>
 __device__ __forceinline__ Work decode(const GradArgs& a, int id) {
+  constexpr int kWalk = Cfg<HALVES>::kWalk;
   Work w;
   const int off = a.tk - a.tq;  // causal: query i sees keys up to i + off
   w.dkv = id < a.n_dkv;
@@ -351,8 +375,8 @@ __device__ __forceinline__ Work decode(const GradArgs& a, int id) {
     w.h = 0;
     w.hk = bhk - w.b * a.kv_heads;
     w.len = key_count(a, w.b);
-    w.first = a.causal ? max(0, w.r0 - off) / kTile : 0;
-    w.per_head = w.r0 < w.len ? a.q_tiles - w.first : 0;
+    w.first = a.causal ? max(0, w.r0 - off) / kWalk : 0;
+    w.per_head = w.r0 < w.len ? a.q_walk - w.first : 0;
     w.n = w.per_head * a.group;
   } else {
     id -= a.n_dkv;
@@ -364,7 +388,7 @@ __device__ __forceinline__ Work decode(const GradArgs& a, int id) {
     w.len = key_count(a, w.b);
     const int keys = a.causal ? min(w.len, min(w.r0 + kTile, a.tq) + off) : w.len;  // that any of the rows sees
     w.first = w.per_head = 0;
-    w.n = keys > 0 ? (keys + kTile - 1) / kTile : 0;
+    w.n = keys > 0 ? (keys + kWalk - 1) / kWalk : 0;
   }
   return w;
 }
@@ -390,6 +414,7 @@ template <int HALVES>
 __device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, const CUtensorMap* v_map,
                         const CUtensorMap* do_map, const GradArgs& a, char* smem, Misc& m) {
   using L = Smem<HALVES>;
+  constexpr int kWalk = Cfg<HALVES>::kWalk;
   volatile int* abort_flag = &m.abort_flag;
   Place<2> at, st;
   Place<kStagesA> pa;
@@ -403,20 +428,22 @@ __device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, cons
     mbar_arrive(&m.item_full[at.s]);
     at.next();
     if (id >= a.n_items) break;
-    const Work w = decode(a, id);
+    const Work w = decode<HALVES>(a, id);
     int g = 0, qt = w.first;  // dK/dV: head of the group and query tile
     for (int i = 0; ok && i < w.n; ++i) {
       const int h = w.hk * a.group + g;
-      const int row = (w.dkv ? qt : i) * kTile, head = w.dkv ? h : w.hk;
+      const int row = (w.dkv ? qt : i) * kWalk, head = w.dkv ? h : w.hk;
       if (!(ok = mbar_wait(&m.a_empty[pa.s], pa.ph ^ 1, abort_flag, a.status, 1))) break;
       mbar_expect_tx(&m.a_full[pa.s], L::tile);
       load_tile<HALVES>(smem + L::a + pa.s * L::tile, w.dkv ? q_map : k_map, &m.a_full[pa.s], row, head, w.b);
       pa.next(), ++na;
       if (w.dkv) {
         if (!(ok = mbar_wait(&m.stat_empty[st.s], st.ph ^ 1, abort_flag, a.status, 17))) break;
-        mbar_expect_tx(&m.stat_full[st.s], kStatBytes);
-        bulk_load(smem + L::stat + st.s * kStatBytes,
-                  a.stat + ((int64_t(w.b) * a.heads + h) * a.q_tiles + qt) * (2 * kTile), kStatBytes, &m.stat_full[st.s]);
+        mbar_expect_tx(&m.stat_full[st.s], Cfg<HALVES>::kStatBytes);
+        char* dst = smem + L::stat + st.s * Cfg<HALVES>::kStatBytes;
+        const float* src = a.stat + ((int64_t(w.b) * a.heads + h) * a.q_tiles + row / kTile) * (2 * kTile) + row % kTile;
+        bulk_load(dst, src, kWalk * 4, &m.stat_full[st.s]);
+        bulk_load(dst + kWalk * 4, src + kTile, kWalk * 4, &m.stat_full[st.s]);
         st.next(), ++ns;
       }
       if (!(ok = mbar_wait(&m.b_empty[pb.s], pb.ph ^ 1, abort_flag, a.status, 2))) break;
@@ -425,9 +452,9 @@ __device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, cons
       pb.next(), ++nb;
       if (i == 0) {  // the own tiles, once the item before has read its own
         if (!(ok = mbar_wait(&m.own_empty, (owns & 1) ^ 1, abort_flag, a.status, 22))) break;
-        mbar_expect_tx(&m.own_full, 2 * L::tile);
-        load_tile<HALVES>(smem + L::own, w.dkv ? k_map : do_map, &m.own_full, w.r0, w.dkv ? w.hk : w.h, w.b);
-        load_tile<HALVES>(smem + L::own + L::tile, w.dkv ? v_map : q_map, &m.own_full, w.r0, w.dkv ? w.hk : w.h, w.b);
+        mbar_expect_tx(&m.own_full, 2 * L::own_tile);
+        load_own<HALVES>(smem + L::own, w.dkv ? k_map : do_map, &m.own_full, w.r0, w.dkv ? w.hk : w.h, w.b);
+        load_own<HALVES>(smem + L::own + L::own_tile, w.dkv ? v_map : q_map, &m.own_full, w.r0, w.dkv ? w.hk : w.h, w.b);
         ++owns;
       }
       if (++qt == w.first + w.per_head) qt = w.first, ++g;
@@ -446,10 +473,11 @@ __device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, cons
 template <bool VBF16, bool QBF16, int HALVES>
 __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
   using L = Smem<HALVES>;
+  using C = Cfg<HALVES>;
   volatile int* abort_flag = &m.abort_flag;
   const uint32_t base = smem_u32(smem);
   constexpr uint32_t step = L::tile >> 4;  // stages are L::tile apart
-  const uint64_t own0 = rows_desc(base + L::own), own1 = rows_desc(base + L::own + L::tile);
+  const uint64_t own0 = rows_desc(base + L::own), own1 = rows_desc(base + L::own + L::own_tile);
   const uint64_t a_rows = rows_desc(base + L::a), a_cols = cols_desc(base + L::a);
   const uint64_t b_rows = rows_desc(base + L::b), b_cols = cols_desc(base + L::b);
   Place<2> at;
@@ -463,7 +491,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
     if (id < 0) break;
     mbar_arrive(&m.item_empty[at.s]);
     at.next();
-    const Work w = decode(a, id);
+    const Work w = decode<HALVES>(a, id);
     if (w.n == 0) continue;
     // the last item's products are complete: nothing is read any more from
     // the columns and tiles that this one fills
@@ -484,7 +512,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i < 0 || mbar_wait(&m.dp_read, ph, abort_flag, a.status, 8));
           if (!ok) break;
           tc_fence_after();
-          product_rows<QBF16, HALVES>(tmem + kColX, own0, a_rows + ta.s * step);
+          product_rows<QBF16, HALVES>(tmem + C::kX, own0, a_rows + ta.s * step);
           mma_commit(&m.s_full);
           ta.next();
         }
@@ -493,7 +521,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i > 0 || owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 25));
           if (!ok) break;
           tc_fence_after();
-          product_cols<VBF16, HALVES>(tmem + kColDV, tmem + kColP, b_cols + cb.s * step, i > 0);
+          product_cols<VBF16, HALVES>(tmem + C::kDV, tmem + C::kP, b_cols + cb.s * step, i > 0);
           mma_commit(&m.b_empty[cb.s]);
           cb.next();
         }
@@ -502,14 +530,14 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                mbar_wait(&m.s_read, next, abort_flag, a.status, 11);
           if (!ok) break;
           tc_fence_after();
-          product_rows<VBF16, HALVES>(tmem + kColX, own1, b_rows + tb.s * step);
+          product_rows<VBF16, HALVES>(tmem + C::kX, own1, b_rows + tb.s * step);
           mma_commit(&m.dp_full);
           tb.next();
         }
         if (i >= 0) {
           if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
           tc_fence_after();
-          product_cols<QBF16, HALVES>(tmem + kColDK, tmem + kColDS, a_cols + ca.s * step, i > 0);
+          product_cols<QBF16, HALVES>(tmem + C::kDK, tmem + C::kDS, a_cols + ca.s * step, i > 0);
           mma_commit(&m.dk_done);
           mma_commit(&m.a_empty[ca.s]);
           ca.next();
@@ -522,7 +550,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i < 0 || mbar_wait(&m.s_read, ph, abort_flag, a.status, 8));
           if (!ok) break;
           tc_fence_after();
-          product_rows_ts<QBF16, HALVES>(tmem + kColS, tmem + kColQ, a_rows + ta.s * step);
+          product_rows_ts<QBF16, HALVES>(tmem + C::kS, tmem + C::kQ, a_rows + ta.s * step);
           mma_commit(&m.s_full);
           ta.next();
         }
@@ -531,14 +559,14 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i > 0 || owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 25));
           if (!ok) break;
           tc_fence_after();
-          product_cols<QBF16, HALVES>(tmem + kColDQ, tmem + kColDSq, a_cols + ca.s * step, i > 0);
+          product_cols<QBF16, HALVES>(tmem + C::kDQ, tmem + C::kDSq, a_cols + ca.s * step, i > 0);
           mma_commit(&m.a_empty[ca.s]);
           ca.next();
         }
         if (more) {  // and dP(i) (ds_full says so)
           if (!(ok = mbar_wait(&m.b_full[tb.s], tb.ph, abort_flag, a.status, 10))) break;
           tc_fence_after();
-          product_rows<VBF16, HALVES>(tmem + kColDP, own0, b_rows + tb.s * step);
+          product_rows<VBF16, HALVES>(tmem + C::kDP, own0, b_rows + tb.s * step);
           mma_commit(&m.dp_full);
           mma_commit(&m.b_empty[tb.s]);
           tb.next(), cb.next();
@@ -566,6 +594,8 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
   using TS = typename std::conditional<QBF16, __nv_bfloat16, __half>::type;  // q, k, dS
   using TO = typename std::conditional<OUT32, float, TS>::type;              // dQ, dK
   using L = Smem<HALVES>;
+  using C = Cfg<HALVES>;
+  constexpr int kWalk = C::kWalk;
   constexpr int kShift = VBF16 ? 0 : kShiftP16;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -590,13 +620,13 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
     __syncwarp();
     if (lane == 0) mbar_arrive(&m.item_empty[at.s]);
     at.next();
-    w = decode(a, id);
+    w = decode<HALVES>(a, id);
     return true;
   };
   // Q of a dQ item (owns: the item's number among those with products)
   auto take_q = [&](int number) {
     if (!mbar_wait(&m.own_full, number & 1, abort_flag, a.status, 27)) return false;
-    row_to_tmem<HALVES>(tmem + lanes + kColQ, smem + L::own + L::tile, row, cg);
+    row_to_tmem<HALVES>(tmem + lanes + C::kQ, smem + L::own + L::own_tile, row, cg);
     tc_fence_before();
     __syncwarp();
     if (lane == 0) mbar_arrive(&m.own_tmem);
@@ -618,18 +648,18 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
     if constexpr (!QBF16) gain = ds_gain(a, w.b, w.hk, kShift, lane);
     const uint64_t gain2 = pack_f2(gain, gain);
     if (w.dkv) {
-      const uint32_t s_addr = tmem + lanes + kColX + cg * 32;
-      const uint32_t p_addr = tmem + lanes + kColP + cg * 16, ds_addr = tmem + lanes + kColDS + cg * 16;
-      int lim = own - off - w.first * kTile - cg * 32;  // causal: columns below it are queries before the key
+      const uint32_t s_addr = tmem + lanes + C::kX + cg * 32;
+      const uint32_t p_addr = tmem + lanes + C::kP + cg * 16, ds_addr = tmem + lanes + C::kDS + cg * 16;
+      int lim = own - off - w.first * kWalk - cg * 32;  // causal: columns below it are queries before the key
       int qt = 0;
       for (int i = 0; i < w.n; ++i) {
         const uint32_t ph = (it + i) & 1;
-        const float* stat = reinterpret_cast<const float*>(smem + L::stat + st.s * kStatBytes) + cg * 32;
+        const float* stat = reinterpret_cast<const float*>(smem + L::stat + st.s * C::kStatBytes) + cg * 32;
         uint32_t bad = 0u;
         if (a.causal) {
           bad = lim <= 0 ? 0u : lim >= 32 ? ~0u : (1u << lim) - 1u;
-          lim -= kTile;
-          if (++qt == w.per_head) lim += w.per_head * kTile, qt = 0;
+          lim -= kWalk;
+          if (++qt == w.per_head) lim += w.per_head * kWalk, qt = 0;
         }
         if (!(ok = mbar_wait(&m.stat_full[st.s], st.ph, abort_flag, a.status, 13))) break;
         if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
@@ -668,7 +698,7 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
         // dS = P (dP - delta)
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
-          const float4 nd = *reinterpret_cast<const float4*>(stat + kTile + c);
+          const float4 nd = *reinterpret_cast<const float4*>(stat + kWalk + c);
 #pragma unroll
           for (int e = c; e < c + 4; e += 2) {
             uint64_t pe = pack_f2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
@@ -694,9 +724,9 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
         st.next();
       }
     } else {
-      const uint32_t s_addr = tmem + lanes + kColS + cg * 32;
-      const uint32_t dp_addr = tmem + lanes + kColDP + cg * 32;
-      const uint32_t ds_addr = tmem + lanes + kColDSq + cg * 16;
+      const uint32_t s_addr = tmem + lanes + C::kS + cg * 32;
+      const uint32_t dp_addr = tmem + lanes + C::kDP + cg * 32;
+      const uint32_t ds_addr = tmem + lanes + C::kDSq + cg * 16;
       if (!q_ready) {
         // Q takes columns that a dK/dV item's results may still be read from
         ok = (owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 26)) && take_q(owns);
@@ -708,7 +738,7 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
       const int seen = a.causal ? min(w.len, own + off + 1) : w.len;  // keys this row sees
       for (int i = 0; i < w.n; ++i) {
         const uint32_t ph = (it + i) & 1;
-        const int lim = seen - i * kTile - cg * 32;  // columns from `lim` on are masked
+        const int lim = seen - i * kWalk - cg * 32;  // columns from `lim` on are masked
         const uint32_t bad = lim >= 32 ? 0u : lim <= 0 ? ~0u : ~0u << lim;
         if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
         tc_fence_after();
@@ -723,12 +753,12 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
           exp2_pair(fma_f2(pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1])), scale2, nl2), v[c], v[c + 1]);
         // a partly valid last key tile: rows past the keys may hold anything,
         // and dS's zeros times inf or NaN would reach dQ
-        const int k0 = i * kTile;
-        if (w.len < min(k0 + kTile, a.tk)) {
+        const int k0 = i * kWalk;
+        if (w.len < min(k0 + kWalk, a.tk)) {
           const int tid = threadIdx.x - 64;
-          const int from = w.len - k0, rows = min(kTile, a.tk - k0) - from;
+          const int from = w.len - k0, rows = min(kWalk, a.tk - k0) - from;
           char* tile = smem + L::a + ((it + i) % kStagesA) * L::tile;
-          for (int x = tid; x < rows * 8 * HALVES; x += 32 * kElemWarps) {
+          for (int x = tid; x < rows * 8 * HALVES; x += 32 * C::kElemWarps) {
             const int r = from + x / (8 * HALVES), ch = x % (8 * HALVES);
             *reinterpret_cast<uint4*>(tile + (ch >> 3) * kHalfBytes + r * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
           }
@@ -766,19 +796,19 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
     q_ready = have && !w.dkv && !next.dkv && next.n > 0;
     if (q_ready && !take_q(owns + 1)) break;
     const float p_mul = 1.f / static_cast<float>(1 << kShift);
-    if (w.dkv) {  // column groups 0 and 1 store the halves of dV, 2 and 3 those of dK
-      const int from = (cg & 1) * 32 * HALVES, to = from + 32 * HALVES;
-      if (cg >= 2) {
+    if (w.dkv) {  // the first half of the column groups stores dV, the second dK, 64 columns each
+      const int from = cg % (C::kGroups / 2) * 64, to = from + 64;
+      if (cg >= C::kGroups / 2) {
         const OutTile o{a.dk.row(static_cast<int>(bhk), w.r0), a.dk.st * int64_t(sizeof(TO)), a.tk - w.r0, a.dim};
-        store_rows<TO>(tmem + lanes + kColDK, o, row, lane, from, to, a.scale * p_mul / (gain * q_scale), own >= w.len);
+        store_rows<TO>(tmem + lanes + C::kDK, o, row, lane, from, to, a.scale * p_mul / (gain * q_scale), own >= w.len);
       } else {
         const OutTile o{a.dv.row(static_cast<int>(bhk), w.r0), a.dv.st * int64_t(sizeof(T)), a.tk - w.r0, a.dim};
-        store_rows<T>(tmem + lanes + kColDV, o, row, lane, from, to, p_mul, own >= w.len);
+        store_rows<T>(tmem + lanes + C::kDV, o, row, lane, from, to, p_mul, own >= w.len);
       }
-    } else if (cg < 2 * HALVES) {
+    } else {
       const OutTile o{a.dq.row(static_cast<int>(bh), w.r0), a.dq.st * int64_t(sizeof(TO)), a.tq - w.r0, a.dim};
       const bool none = (a.causal ? min(w.len, own + off + 1) : w.len) <= 0;
-      store_rows<TO>(tmem + lanes + kColDQ, o, row, lane, cg * 32, cg * 32 + 32, a.scale * p_mul / (gain * k_scale), none);
+      store_rows<TO>(tmem + lanes + C::kDQ, o, row, lane, cg * 32, cg * 32 + 32, a.scale * p_mul / (gain * k_scale), none);
     }
     tc_fence_before();
     __syncwarp();
@@ -790,11 +820,12 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
 }
 
 template <bool VBF16, bool QBF16, bool OUT32, int HALVES>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Cfg<HALVES>::kThreads, Cfg<HALVES>::kCtas)
 attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap do_map,
                  const __grid_constant__ GradArgs a) {
   extern __shared__ __align__(1024) char smem[];
+  constexpr int kElemWarps = Cfg<HALVES>::kElemWarps;
   Misc& m = *reinterpret_cast<Misc*>(smem + Smem<HALVES>::misc);
   const int warp = threadIdx.x >> 5;
   if (threadIdx.x == 0) {
@@ -834,7 +865,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     fence_proxy_async_smem();
   }
   grid_dep_wait();  // the statistics and the counter come from the kernel before
-  if (warp == 1) tmem_alloc<512>(&m.tmem);
+  if (warp == 1) tmem_alloc<Cfg<HALVES>::kTmem>(&m.tmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -850,7 +881,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc<512>(tmem);
+    tmem_dealloc<Cfg<HALVES>::kTmem>(tmem);
   }
 }
 
@@ -972,7 +1003,7 @@ struct Layout {
 Layout layout_of(int64_t bh, int64_t bhk, int64_t q_tiles, int64_t v_blocks) {
   Layout l;
   l.stat = 0;
-  l.do_norm = align256(size_t(bh) * q_tiles * kStatBytes);
+  l.do_norm = align256(size_t(bh) * q_tiles * 2 * kTile * 4);
   l.v_norm = l.do_norm + align256(size_t(bh) * q_tiles * 2 * 4);
   l.counter = l.v_norm + align256(size_t(bhk) * v_blocks * 4);
   l.total = l.counter + 256;
@@ -992,8 +1023,8 @@ cudaError_t launch_grad(const CUtensorMap* maps, const GradArgs& a, cudaStream_t
   const int smem = static_cast<int>(Smem<HALVES>::total);
   const cudaError_t err = ensure_smem(reinterpret_cast<const void*>(kernel), smem);
   if (err != cudaSuccess) return err;
-  const int sms = sm_count();
-  return launch_pdl(kernel, dim3(a.n_items < sms ? a.n_items : sms), dim3(kThreads), size_t(smem), st, maps[0], maps[1],
+  const int most = sm_count() * Cfg<HALVES>::kCtas;
+  return launch_pdl(kernel, dim3(a.n_items < most ? a.n_items : most), dim3(Cfg<HALVES>::kThreads), size_t(smem), st, maps[0], maps[1],
                     maps[2], maps[3], a);
 }
 
@@ -1017,7 +1048,7 @@ cudaError_t launch_attn_grad(const AttnGradCall& c, int* status, cudaStream_t st
   CUtensorMap maps[4];
   const b2_view* views[4] = {c.q, c.k, c.v, c.dout};
   for (int i = 0; i < 4; ++i)
-    if (!linear_rows_map(&maps[i], *views[i], kTile)) return cudaErrorInvalidValue;
+    if (!linear_rows_map(&maps[i], *views[i], q.head_dim <= 64 ? Cfg<1>::kWalk : Cfg<2>::kWalk)) return cudaErrorInvalidValue;
   const bool v_bf16 = c.v->dtype == B2_BF16, qk16 = c.qk_scale != nullptr;
   const int64_t bh = int64_t(q.batch) * q.heads, bhk = int64_t(q.batch) * k.heads;
   StatArgs s{};
@@ -1052,6 +1083,8 @@ cudaError_t launch_attn_grad(const AttnGradCall& c, int* status, cudaStream_t st
   a.heads = s.heads, a.kv_heads = s.kv_heads, a.group = q.heads / k.heads;
   a.tq = s.tq, a.tk = s.tk, a.dim = s.dim;
   a.q_tiles = s.q_tiles, a.v_blocks = s.v_blocks;
+  const int walk = q.head_dim <= 64 ? Cfg<1>::kWalk : Cfg<2>::kWalk;
+  a.q_walk = (q.tokens + walk - 1) / walk;
   a.k_tiles = (k.tokens + kTile - 1) / kTile;
   a.n_dkv = static_cast<int>(bhk * a.k_tiles);
   a.n_items = static_cast<int>(a.n_dkv + bh * a.q_tiles);

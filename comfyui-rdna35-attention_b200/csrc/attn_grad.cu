@@ -284,27 +284,6 @@ __device__ __forceinline__ float ds_gain(const GradArgs& a, int b, int hk, int s
   return ldexpf(1.f, min(max(e, -60), 60));
 }
 
-// 4 x 4 transpose of 16-byte chunks in every four lanes: chunk j of lane q
-// becomes chunk q of lane j.
-__device__ __forceinline__ void transpose_quads(uint32_t (&w)[16], int lane) {
-#pragma unroll
-  for (int bit = 1; bit <= 2; bit <<= 1) {
-    const bool upper = (lane & bit) != 0;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      if (c & bit) continue;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t& lo = w[4 * c + e];
-        uint32_t& hi = w[4 * (c + bit) + e];
-        const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? lo : hi, bit);
-        if (upper) lo = got;
-        else hi = got;
-      }
-    }
-  }
-}
-
 // Rows of a result tile in global memory.
 struct OutTile {
   char* base;  // row 0

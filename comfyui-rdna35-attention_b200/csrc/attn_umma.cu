@@ -750,7 +750,11 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     const float cw = tt * a.corr_scale;
     char* orow = store ? a.o.row(bh, tq_row) : nullptr;
     char* low_row = nullptr;
+    // the warp stores together (the rows of a general call are linear)
+    const bool whole = GEN != 0 && __all_sync(0xffffffffu, ok && !*abort_flag);
+    char* quad_row = nullptr;
     if constexpr (GEN != 0) {
+      if (half == 0 || has_b) quad_row = a.o.row(bh, tq_row - (lane & 3));
       if (store && a.o_low.base != nullptr && tk_ <= kLowKeys) low_row = a.o_low.row(bh, tq_row);
     }
     const uint32_t row_base = tmem + lane_base;
@@ -762,7 +766,36 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       if constexpr (NW == 2) tmem_ld32(row_base + 256 + c0, o1);
       if (a.has_corr) tmem_ld32(row_base + 128 + c0, cr);
       tmem_wait_ld();
-      if (store) {
+      if constexpr (GEN != 0) {
+        // Four lanes store 64 bytes of a row together: by its own lane alone,
+        // each row's 16 bytes touch a line of their own.
+        uint32_t w[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          const float f0 = lt == 0.f ? 0.f : __uint_as_float(o0[c]) * inv;  // no key seen: O may hold anything
+          const float f1 = lt == 0.f ? 0.f : __uint_as_float(o0[c + 1]) * inv;
+          w[c / 2] = Cvt<T>::pack2(f0, f1);
+          if (low_row != nullptr) {  // what the output's type cannot hold
+            float h0, h1;
+            Cvt<T>::unpack2(w[c / 2], h0, h1);
+            o0[c / 2] = Cvt<T>::pack2(f0 - h0, f1 - h1);
+          }
+        }
+        if (low_row != nullptr) {
+          uint4* dst = reinterpret_cast<uint4*>(low_row + c0 * 2);
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4)
+            if (c0 + 8 * q4 < a.o.dim)
+              dst[q4] = make_uint4(o0[4 * q4], o0[4 * q4 + 1], o0[4 * q4 + 2], o0[4 * q4 + 3]);
+        }
+        transpose_quads(w, lane);
+        const int q = lane & 3;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (whole && (half == 0 || has_b) && tq_row - q + j < a.tq && c0 + 8 * q < a.o.dim)
+            *reinterpret_cast<uint4*>(quad_row + j * a.o.st * 2 + (c0 + 8 * q) * 2) =
+                make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+      } else if (store) {
         uint32_t packed[16];
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
@@ -776,26 +809,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
             f0 = fmaf(__uint_as_float(cr[c]), cw, f0);
             f1 = fmaf(__uint_as_float(cr[c + 1]), cw, f1);
           }
-          if (GEN != 0 && lt == 0.f) f0 = f1 = 0.f;  // no key seen: O may hold anything
           packed[c / 2] = Cvt<T>::pack2(f0 * inv, f1 * inv);
-        }
-        if constexpr (GEN != 0) {
-          if (low_row != nullptr) {  // what the output's type cannot hold
-            uint32_t low[16];
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-              float h0, h1;
-              Cvt<T>::unpack2(packed[c / 2], h0, h1);
-              const float w0 = lt == 0.f ? 0.f : a0 * inv;
-              low[c / 2] = Cvt<T>::pack2(lt == 0.f ? 0.f : fmaf(__uint_as_float(o0[c]), w0, -h0),
-                                         lt == 0.f ? 0.f : fmaf(__uint_as_float(o0[c + 1]), w0, -h1));
-            }
-            uint4* dst = reinterpret_cast<uint4*>(low_row + c0 * 2);
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4)
-              if (c0 + 8 * q4 < a.o.dim)
-                dst[q4] = make_uint4(low[4 * q4], low[4 * q4 + 1], low[4 * q4 + 2], low[4 * q4 + 3]);
-          }
         }
         uint4* dst = reinterpret_cast<uint4*>(orow + c0 * 2);
         if (a.o.dim == 128) {

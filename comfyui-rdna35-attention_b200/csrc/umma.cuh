@@ -248,6 +248,27 @@ __device__ __forceinline__ void named_barrier_sync(int id, int count) {
   asm volatile("bar.sync %0, %1;\n" ::"r"(id), "r"(count) : "memory");
 }
 
+// 4 x 4 transpose of 16-byte chunks in every four lanes: chunk j of lane q
+// becomes chunk q of lane j.
+__device__ __forceinline__ void transpose_quads(uint32_t (&w)[16], int lane) {
+#pragma unroll
+  for (int bit = 1; bit <= 2; bit <<= 1) {
+    const bool upper = (lane & bit) != 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (c & bit) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t& lo = w[4 * c + e];
+        uint32_t& hi = w[4 * (c + bit) + e];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? lo : hi, bit);
+        if (upper) lo = got;
+        else hi = got;
+      }
+    }
+  }
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));

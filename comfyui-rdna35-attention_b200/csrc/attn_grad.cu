@@ -102,7 +102,23 @@ struct GradArgs {
   int* status;
 };
 
-struct __align__(8) Misc {
+// ------------------------------------------------------------ items
+// Decoded by the producer and read by the others from shared memory: their
+// code between two items runs once an item, instruction fetches and all, and
+// took half of an item of four tile pairs.
+struct __align__(16) Work {
+  int n;         // tile pairs; -1: no item is left
+  int dkv;
+  int b, h, hk;  // batch, query head (dQ), key/value head
+  int r0;        // the first of its own 128 rows
+  int len;       // keys of the batch
+  int first, per_head;  // dK/dV: the first query tile, and how many of each head
+  int rows;             // own rows that exist
+  char *out0, *out1;    // row r0 of dQ, or of dV and dK
+  const float* stat;    // dQ: statistics of row r0
+};
+
+struct __align__(16) Misc {
   uint64_t item_full[2], item_empty[2];
   uint64_t own_full, own_empty;  // the item's own two tiles in shared memory
   uint64_t own_tmem;             // dQ: Q in tensor memory
@@ -112,7 +128,7 @@ struct __align__(8) Misc {
   uint64_t s_full, s_read, p_full, dp_full, dp_read, ds_full, dk_done;
   uint64_t acc_full, acc_free;  // the item's results are complete; are stored
   uint64_t exit_done;
-  int item[2];
+  Work item[2];
   uint32_t tmem;
   int abort_flag;
 };
@@ -331,16 +347,6 @@ __device__ __forceinline__ void store_zero_row(char* row, int dim) {
   for (int c = 0; c < dim * int(sizeof(TO)); c += 16) *reinterpret_cast<uint4*>(row + c) = make_uint4(0u, 0u, 0u, 0u);
 }
 
-// ------------------------------------------------------------ items
-struct Work {
-  bool dkv;
-  int b, h, hk;  // batch, query head (dQ), key/value head
-  int r0;        // the first of its own 128 rows
-  int len;       // keys of the batch
-  int n;         // tile pairs
-  int first, per_head;  // dK/dV: the first query tile, and how many of each head
-};
-
 template <int HALVES>
 __device__ __forceinline__ Work decode(const GradArgs& a, int id) {
   constexpr int kWalk = Cfg<HALVES>::kWalk;
@@ -357,10 +363,15 @@ __device__ __forceinline__ Work decode(const GradArgs& a, int id) {
     w.first = a.causal ? max(0, w.r0 - off) / kWalk : 0;
     w.per_head = w.r0 < w.len ? a.q_walk - w.first : 0;
     w.n = w.per_head * a.group;
+    w.rows = a.tk - w.r0;
+    w.out0 = a.dv.row(bhk, w.r0);
+    w.out1 = a.dk.row(bhk, w.r0);
+    w.stat = nullptr;
   } else {
     id -= a.n_dkv;
     const int bh = id / a.q_tiles;
-    w.r0 = (a.q_tiles - 1 - (id - bh * a.q_tiles)) * kTile;  // causal: the longest first
+    const int qt = a.q_tiles - 1 - (id - bh * a.q_tiles);  // causal: the longest first
+    w.r0 = qt * kTile;
     w.b = bh / a.heads;
     w.h = bh - w.b * a.heads;
     w.hk = w.h / a.group;
@@ -368,6 +379,10 @@ __device__ __forceinline__ Work decode(const GradArgs& a, int id) {
     const int keys = a.causal ? min(w.len, min(w.r0 + kTile, a.tq) + off) : w.len;  // that any of the rows sees
     w.first = w.per_head = 0;
     w.n = keys > 0 ? (keys + kWalk - 1) / kWalk : 0;
+    w.rows = a.tq - w.r0;
+    w.out0 = a.dq.row(bh, w.r0);
+    w.out1 = nullptr;
+    w.stat = a.stat + (int64_t(bh) * a.q_tiles + qt) * (2 * kTile);
   }
   return w;
 }
@@ -382,10 +397,12 @@ struct Place {
   }
 };
 
-// The next item, published by the producer (-1: none left, or aborted).
-__device__ __forceinline__ int next_item(Misc& m, Place<2>& at, volatile int* abort_flag, int* status) {
-  if (!mbar_wait(&m.item_full[at.s], at.ph, abort_flag, status, 20)) return -1;
-  return *const_cast<volatile int*>(&m.item[at.s]);
+// The next item, once the producer has published it; false if none is left
+// (or on abort).
+__device__ __forceinline__ bool next_item(Misc& m, const Place<2>& at, volatile int* abort_flag, int* status, Work& w) {
+  if (!mbar_wait(&m.item_full[at.s], at.ph, abort_flag, status, 20)) return false;
+  w = m.item[at.s];
+  return w.n >= 0;
 }
 
 // ------------------------------------------------------------ TMA producer
@@ -403,11 +420,13 @@ __device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, cons
   while (ok) {
     const int id = atomicAdd(a.counter, 1);
     if (!(ok = mbar_wait(&m.item_empty[at.s], at.ph ^ 1, abort_flag, a.status, 21))) break;
-    *const_cast<volatile int*>(&m.item[at.s]) = id < a.n_items ? id : -1;
+    Work w;
+    if (id < a.n_items) w = decode<HALVES>(a, id);
+    else w.n = -1;
+    m.item[at.s] = w;
     mbar_arrive(&m.item_full[at.s]);
     at.next();
-    if (id >= a.n_items) break;
-    const Work w = decode<HALVES>(a, id);
+    if (w.n < 0) break;
     int g = 0, qt = w.first;  // dK/dV: head of the group and query tile
     for (int i = 0; ok && i < w.n; ++i) {
       const int h = w.hk * a.group + g;
@@ -466,11 +485,10 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
   int owns = 0, dqs = 0;
   bool ok = true;
   while (ok) {
-    const int id = next_item(m, at, abort_flag, a.status);
-    if (id < 0) break;
+    Work w;
+    if (!next_item(m, at, abort_flag, a.status, w)) break;
     mbar_arrive(&m.item_empty[at.s]);
     at.next();
-    const Work w = decode<HALVES>(a, id);
     if (w.n == 0) continue;
     // the last item's products are complete: nothing is read any more from
     // the columns and tiles that this one fills
@@ -588,19 +606,19 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
   if (a.qk_scale != nullptr) q_scale = a.qk_scale[0], k_scale = a.qk_scale[1];
   const float mul_s = a.scale_log2 / (q_scale * k_scale);
   const uint64_t scale2 = pack_f2(mul_s, mul_s);
+  constexpr float p_mul = 1.f / static_cast<float>(1 << kShift);
+  const float mul_dk = a.scale * p_mul / q_scale, mul_dq = a.scale * p_mul / k_scale;
+  const int64_t step_dv = a.dv.st * int64_t(sizeof(T)), step_dk = a.dk.st * int64_t(sizeof(TO)),
+                step_dq = a.dq.st * int64_t(sizeof(TO));
   Place<2> at, st;
   uint32_t it = 0;
   int owns = 0;
   bool ok = true;
   bool q_ready = false;  // dQ: the item's Q is in tensor memory already
-  auto fetch = [&](Work& w) {
-    const int id = next_item(m, at, abort_flag, a.status);
-    if (id < 0) return false;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&m.item_empty[at.s]);
-    at.next();
-    w = decode<HALVES>(a, id);
-    return true;
+  // Items stay in shared memory while they are worked on (copies of their
+  // fields would not fit the registers beside two tiles' columns).
+  auto have = [&](const Place<2>& p) {
+    return mbar_wait(&m.item_full[p.s], p.ph, abort_flag, a.status, 20) && m.item[p.s].n >= 0;
   };
   // Q of a dQ item (owns: the item's number among those with products)
   auto take_q = [&](int number) {
@@ -611,18 +629,23 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
     if (lane == 0) mbar_arrive(&m.own_tmem);
     return true;
   };
-  Work w;
-  bool have = fetch(w);
-  while (have) {
+  bool any = have(at);
+  while (any) {
+    const Work& w = m.item[at.s];
     const int own = w.r0 + row;  // key or query
-    const int64_t bhk = int64_t(w.b) * a.kv_heads + w.hk, bh = int64_t(w.b) * a.heads + w.h;
     if (w.n == 0) {  // column groups 0 and 1: zeros for dV and dK, or dQ
-      if (w.dkv && own < a.tk && cg == 0) store_zero_row<T>(a.dv.row(static_cast<int>(bhk), own), a.dim);
-      if (w.dkv && own < a.tk && cg == 1) store_zero_row<TO>(a.dk.row(static_cast<int>(bhk), own), a.dim);
-      if (!w.dkv && own < a.tq && cg == 0) store_zero_row<TO>(a.dq.row(static_cast<int>(bh), own), a.dim);
-      have = fetch(w);
+      if (row < w.rows && cg == 0) {
+        if (w.dkv) store_zero_row<T>(w.out0 + row * step_dv, a.dim);
+        else store_zero_row<TO>(w.out0 + row * step_dq, a.dim);
+      }
+      if (row < w.rows && cg == 1 && w.dkv) store_zero_row<TO>(w.out1 + row * step_dk, a.dim);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.item_empty[at.s]);
+      at.next();
+      any = have(at);
       continue;
     }
+    const int n = w.n, len = w.len;
     float gain = 1.f;
     if constexpr (!QBF16) gain = ds_gain(a, w.b, w.hk, kShift, lane);
     const uint64_t gain2 = pack_f2(gain, gain);
@@ -631,7 +654,7 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
       const uint32_t p_addr = tmem + lanes + C::kP + cg * 16, ds_addr = tmem + lanes + C::kDS + cg * 16;
       int lim = own - off - w.first * kWalk - cg * 32;  // causal: columns below it are queries before the key
       int qt = 0;
-      for (int i = 0; i < w.n; ++i) {
+      for (int i = 0; i < n; ++i) {
         const uint32_t ph = (it + i) & 1;
         const float* stat = reinterpret_cast<const float*>(smem + L::stat + st.s * C::kStatBytes) + cg * 32;
         uint32_t bad = 0u;
@@ -711,11 +734,10 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
         ok = (owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 26)) && take_q(owns);
         if (!ok) break;
       }
-      const float* stat = a.stat + (bh * a.q_tiles + w.r0 / kTile) * (2 * kTile) + row;
-      const float nl = stat[0], nd = stat[kTile];
+      const float nl = w.stat[row], nd = w.stat[kTile + row];
       const uint64_t nl2 = pack_f2(nl, nl), nd2 = pack_f2(nd, nd);
-      const int seen = a.causal ? min(w.len, own + off + 1) : w.len;  // keys this row sees
-      for (int i = 0; i < w.n; ++i) {
+      const int seen = a.causal ? min(len, own + off + 1) : len;  // keys this row sees
+      for (int i = 0; i < n; ++i) {
         const uint32_t ph = (it + i) & 1;
         const int lim = seen - i * kWalk - cg * 32;  // columns from `lim` on are masked
         const uint32_t bad = lim >= 32 ? 0u : lim <= 0 ? ~0u : ~0u << lim;
@@ -733,9 +755,9 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
         // a partly valid last key tile: rows past the keys may hold anything,
         // and dS's zeros times inf or NaN would reach dQ
         const int k0 = i * kWalk;
-        if (w.len < min(k0 + kWalk, a.tk)) {
+        if (len < min(k0 + kWalk, a.tk)) {
           const int tid = threadIdx.x - 64;
-          const int from = w.len - k0, rows = min(kWalk, a.tk - k0) - from;
+          const int from = len - k0, rows = min(kWalk, a.tk - k0) - from;
           char* tile = smem + L::a + ((it + i) % kStagesA) * L::tile;
           for (int x = tid; x < rows * 8 * HALVES; x += 32 * C::kElemWarps) {
             const int r = from + x / (8 * HALVES), ch = x % (8 * HALVES);
@@ -770,31 +792,35 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
     tc_fence_after();
     // between dQ items the next Q goes in first, so that the next S and dP run
     // while this item's results are stored
-    Work next;
-    have = fetch(next);
-    q_ready = have && !w.dkv && !next.dkv && next.n > 0;
+    Place<2> then = at;
+    then.next();
+    any = have(then);
+    q_ready = any && !w.dkv && !m.item[then.s].dkv && m.item[then.s].n > 0;
     if (q_ready && !take_q(owns + 1)) break;
-    const float p_mul = 1.f / static_cast<float>(1 << kShift);
+    float inv_gain = 1.f;
+    if constexpr (!QBF16) inv_gain = 1.f / gain;
     if (w.dkv) {  // the first half of the column groups stores dV, the second dK, 64 columns each
       const int from = cg % (C::kGroups / 2) * 64, to = from + 64;
-      if (cg >= C::kGroups / 2) {
-        const OutTile o{a.dk.row(static_cast<int>(bhk), w.r0), a.dk.st * int64_t(sizeof(TO)), a.tk - w.r0, a.dim};
-        store_rows<TO>(tmem + lanes + C::kDK, o, row, lane, from, to, a.scale * p_mul / (gain * q_scale), own >= w.len);
-      } else {
-        const OutTile o{a.dv.row(static_cast<int>(bhk), w.r0), a.dv.st * int64_t(sizeof(T)), a.tk - w.r0, a.dim};
-        store_rows<T>(tmem + lanes + C::kDV, o, row, lane, from, to, p_mul, own >= w.len);
-      }
+      if (cg >= C::kGroups / 2)
+        store_rows<TO>(tmem + lanes + C::kDK, OutTile{w.out1, step_dk, w.rows, a.dim}, row, lane, from, to,
+                       mul_dk * inv_gain, own >= len);
+      else
+        store_rows<T>(tmem + lanes + C::kDV, OutTile{w.out0, step_dv, w.rows, a.dim}, row, lane, from, to, p_mul,
+                      own >= len);
     } else {
-      const OutTile o{a.dq.row(static_cast<int>(bh), w.r0), a.dq.st * int64_t(sizeof(TO)), a.tq - w.r0, a.dim};
-      const bool none = (a.causal ? min(w.len, own + off + 1) : w.len) <= 0;
-      store_rows<TO>(tmem + lanes + C::kDQ, o, row, lane, cg * 32, cg * 32 + 32, a.scale * p_mul / (gain * k_scale), none);
+      const bool none = (a.causal ? min(len, own + off + 1) : len) <= 0;
+      store_rows<TO>(tmem + lanes + C::kDQ, OutTile{w.out0, step_dq, w.rows, a.dim}, row, lane, cg * 32, cg * 32 + 32,
+                     mul_dq * inv_gain, none);
     }
     tc_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&m.acc_free);
-    it += w.n;
+    if (lane == 0) {
+      mbar_arrive(&m.acc_free);
+      mbar_arrive(&m.item_empty[at.s]);
+    }
+    it += n;
     ++owns;
-    w = next;
+    at = then;
   }
 }
 
@@ -897,15 +923,15 @@ __global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_consta
   const int r0 = (id - head * per_head) * kStatRows;
   float most = 0.f;
   if (queries) {
-    bool use_low = a.out_low.base != nullptr;
-    if (use_low && a.key_lengths != nullptr) use_low = min(max(a.key_lengths[head / a.heads], 0), a.tk) <= kLowKeys;
-    else if (use_low) use_low = a.tk <= kLowKeys;
+    const int len = a.key_lengths != nullptr ? min(max(a.key_lengths[head / a.heads], 0), a.tk) : a.tk;
+    const bool use_low = a.out_low.base != nullptr && len <= kLowKeys;
+    const bool needed = active && len > 0;  // rows without a key have no gradient
     uint4 o[4], d[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int r = r0 + u * 16 + g;
       o[u] = d[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (active && r < a.tq) {
+      if (needed && r < a.tq) {
         o[u] = reinterpret_cast<const uint4*>(a.out.row(head, r))[l];
         d[u] = reinterpret_cast<const uint4*>(a.dout.row(head, r))[l];
       }
@@ -915,7 +941,7 @@ __global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_consta
       const int r = r0 + u * 16 + g;
       const uint32_t ow[4] = {o[u].x, o[u].y, o[u].z, o[u].w}, dw[4] = {d[u].x, d[u].y, d[u].z, d[u].w};
       uint4 low = make_uint4(0u, 0u, 0u, 0u);
-      if (use_low && active && r < a.tq) low = reinterpret_cast<const uint4*>(a.out_low.row(head, r))[l];
+      if (use_low && needed && r < a.tq) low = reinterpret_cast<const uint4*>(a.out_low.row(head, r))[l];
       const uint32_t lw[4] = {low.x, low.y, low.z, low.w};
       float sum = 0.f, norm = 0.f;
 #pragma unroll

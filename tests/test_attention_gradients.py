@@ -256,3 +256,204 @@ def test_forward_and_backward_match_fp64(case):
 def test_peaked_rows(dtype):
     """Logits spread by 3 * 3: most of a row's weight on few keys."""
     run_case(1, 2, 2, 300, 500, 128, dtype, False, None, "bthd", seed=10, spread=3.0 ** 0.5)
+
+
+# ---------------------------------------------------------------- calls no plain case makes (GPU)
+def plain_grads(q, k, v, dout, scale, causal=False):
+    res, allow = reference(q, k, v, dout, scale, causal, None)
+    return res, allow
+
+
+def check_all(got, res, allow, dtype, names=("out", "dq", "dk", "dv")):
+    u = torch.finfo(dtype).eps / 2
+    for name, x in zip(names, got):
+        close(name, x, res[name], allow[name](u))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_autograd_broadcast_inputs_and_gradients(dtype):
+    """Expanded keys and values (one head for all), and the gradient of sum(),
+    which is one broadcast value."""
+    import b200_pisa
+
+    q = make(2, 4, 70, 64, dtype, "bthd", 1).requires_grad_()
+    k1, v1 = (make(2, 1, 90, 64, dtype, "bhtd", i).requires_grad_() for i in (2, 3))
+    out = b200_pisa.attention(q, k1.expand(2, 4, 90, 64), v1.expand(2, 4, 90, 64))
+    grads = torch.autograd.grad(out.sum(), (q, k1, v1))
+    res, allow = plain_grads(q.detach(), k1.detach(), v1.detach(), torch.ones_like(q), 64 ** -0.5)
+    u = torch.finfo(dtype).eps / 2
+    close("out", out.detach(), res["out"], allow["out"](u))
+    close("dq", grads[0], res["dq"], allow["dq"](u))
+    # four heads' gradients rounded to the type one by one, then summed by autograd in it
+    full, fallow = plain_grads(q.detach(), k1.detach().expand(2, 4, 90, 64), v1.detach().expand(2, 4, 90, 64),
+                               torch.ones_like(q), 64 ** -0.5)
+    for i, name in ((1, "dk"), (2, "dv")):
+        total = full[name].sum(1, keepdim=True)
+        allowed = fallow[name](u).sum(1, keepdim=True) + 4 * u * full[name].abs().sum(1, keepdim=True)
+        close(name, grads[i], total, allowed)
+
+
+@gpu
+def test_three_dimensional_calls_and_unaligned_gradients():
+    import b200_pisa
+
+    q, k, v = (make(1, 6, t, 40, torch.bfloat16, "bhtd", i)[0] for i, t in ((1, 33), (2, 65), (3, 65)))
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    out = b200_pisa.attention(*leaves, scale=0.3)
+    assert out.shape == q.shape
+    wide = torch.randn(6, 33, 43, device=DEV).to(torch.bfloat16)
+    dout = wide[..., 1:41]  # rows off the 16-byte boundaries
+    grads = torch.autograd.grad(out, leaves, dout)
+    four = [x[None] for x in (q, k, v)]
+    res, allow = plain_grads(*four, dout[None], 0.3)
+    check_all([x[None] for x in (out.detach(), *grads)], res, allow, torch.bfloat16)
+
+
+@gpu
+def test_gradients_match_differences():
+    """Against central differences of the FP64 formula along a few directions."""
+    import b200_pisa
+
+    q, k, v = (make(1, 2, t, 64, torch.float16, "bthd", i) for i, t in ((1, 17), (2, 23), (3, 23)))
+    dout = make(1, 2, 17, 64, torch.float16, "bthd", 4)
+    out, lse = b200_pisa.attention_forward(q, k, v, causal=True)
+    grads = b200_pisa.attention_backward(dout, q, k, v, out, lse, causal=True)
+
+    def loss(*x):
+        res, _ = reference(*x, None, 64 ** -0.5, True, None)
+        return (res["out"] * dout.double()).sum().item()
+
+    base = [x.double() for x in (q, k, v)]
+    for i, g in enumerate(grads):
+        way = torch.randn_like(base[i], dtype=torch.float64)
+        step = 1e-5
+        moved = [[x + s * step * way if j == i else x for j, x in enumerate(base)] for s in (1, -1)]
+        slope = (loss(*moved[0]) - loss(*moved[1])) / (2 * step)
+        # the gradient's FP16 terms add up to half a unit of FP16 of their sum at worst, a few times over
+        assert abs((g.double() * way).sum().item() - slope) <= 4 * 2.0 ** -11 * (g.double() * way).abs().sum().item() + 1e-6
+
+
+@gpu
+@pytest.mark.parametrize("scale_dout,scale_v", [(1e-6, 1.0), (1e-7, 1e3), (3e2, 30.0)])
+def test_fp16_gradients_of_any_size(scale_dout, scale_v):
+    """dS neither underflows nor overflows FP16: what is lost is the last
+    rounding (step 2^-24) of results that are themselves FP16."""
+    import b200_pisa
+
+    q, k = (make(1, 2, t, 128, torch.float16, "bthd", i) for i, t in ((1, 300), (2, 500)))
+    v = make(1, 2, 500, 128, torch.float16, "bthd", 3, scale_v)
+    dout = make(1, 2, 300, 128, torch.float16, "bthd", 4, scale_dout)
+    out, lse = b200_pisa.attention_forward(q, k, v)
+    grads = b200_pisa.attention_backward(dout, q, k, v, out, lse)
+    res, allow = reference(q, k, v, dout, 128 ** -0.5, False, None)
+    check_all((out, *grads), res, allow, torch.float16)
+
+
+@gpu
+def test_few_keys_keep_their_accuracy_through_autograd():
+    """With two keys delta cancels against two dP terms: the rounding of out
+    (2^-9) would be several times the error of everything else."""
+    import b200_pisa
+
+    for tk, lens in ((2, None), (300, (2, 300))):
+        q = make(2, 4, 128, 64, torch.bfloat16, "bthd", 1).requires_grad_()
+        k, v = (make(2, 4, tk, 64, torch.bfloat16, "bthd", i).requires_grad_() for i in (2, 3))
+        lens_t = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=DEV)
+        dout = make(2, 4, 128, 64, torch.bfloat16, "bthd", 4)
+        out = b200_pisa.attention(q, k, v, key_lengths=lens_t)
+        dq, dk, _ = torch.autograd.grad(out, (q, k, v), dout)
+        res, _ = reference(q.detach(), k.detach(), v.detach(), dout, 64 ** -0.5, False, lens_t)
+        for got, want in ((dq[0], res["dq"][0]), (dk[0], res["dk"][0])):  # the batch of two keys
+            # roundings of P's and dS's 2^-9 and the result's, uniform and independent: their
+            # root mean square is 2^-9 / sqrt(3) each, 2^-9 in all; delta's would add more than that again
+            assert ((got.double() - want).norm() / want.norm()).item() < 2.0 ** -8.25
+
+
+@gpu
+def test_streams_two_calls_at_once_and_graph_replays():
+    import b200_pisa
+    from b200_pisa import _lib
+
+    q, k, v = (make(1, h, t, 128, torch.bfloat16, "bthd", i) for i, h, t in ((1, 8, 700), (2, 4, 900), (3, 4, 900)))
+    dout = make(1, 8, 700, 128, torch.bfloat16, "bthd", 4)
+
+    def call():
+        out, lse = b200_pisa.attention_forward(q, k, v, causal=True)
+        return (out, lse, *b200_pisa.attention_backward(dout, q, k, v, out, lse, causal=True))
+
+    eager = call()
+    streams = [torch.cuda.Stream(DEV) for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream(DEV))
+    at_once = []
+    for _ in range(3):
+        for s in streams:
+            with torch.cuda.stream(s):
+                at_once.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for got in at_once for x, y in zip(eager, got))
+    graphs, captured = [], []
+    for s in streams:  # two graphs with workspaces of their own, replayed at once
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            captured.append(call())
+        graphs.append(g)
+    q.mul_(0.5)
+    fresh = call()
+    torch.cuda.synchronize()
+    for _ in range(2):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for got in captured for x, y in zip(fresh, got))
+    _lib.check_status()
+
+
+@gpu
+def test_long_sequences_and_many_heads():
+    import b200_pisa
+    from b200_pisa import _lib
+
+    # 33000 keys: the whole gradient of one head against FP64
+    q, k, v, dout = (make(1, 1, t, 64, torch.bfloat16, "bthd", i) for i, t in ((1, 200), (2, 33000), (3, 33000), (4, 200)))
+    out, lse = b200_pisa.attention_forward(q, k, v)
+    res, allow = reference(q, k, v, dout, 0.125, False, None)
+    check_all((out, *b200_pisa.attention_backward(dout, q, k, v, out, lse)), res, allow, torch.bfloat16)
+    # 6000 heads of 5 tokens
+    q, k, v, dout = (make(2, 3000, 5, 16, torch.float16, "bhtd", i) for i in range(4))
+    out, lse = b200_pisa.attention_forward(q, k, v)
+    res, allow = reference(q, k, v, dout, 0.25, False, None)
+    check_all((out, *b200_pisa.attention_backward(dout, q, k, v, out, lse)), res, allow, torch.float16)
+    _lib.check_status()
+
+
+@gpu
+def test_rows_past_32_bit_offsets():
+    import b200_pisa
+
+    storage = torch.empty(2 ** 31 + 2 ** 22, device=DEV, dtype=torch.bfloat16)
+    far = lambda t: storage.as_strided((1, 2, t, 64), (0, 2 ** 31, 64, 1))  # noqa: E731
+    near = [make(1, 2, t, 64, torch.bfloat16, "bthd", i) for i, t in ((1, 100), (2, 200), (3, 200), (4, 100))]
+    want_out, want_lse = b200_pisa.attention_forward(*near[:3])
+    want = b200_pisa.attention_backward(near[3], *near[:3], want_out, want_lse)
+    for i, x in enumerate(near):
+        y = far(x.shape[2])
+        y.copy_(x)
+        args = [*near[:i], y, *near[i + 1:]]
+        out, lse = b200_pisa.attention_forward(*args[:3])
+        got = b200_pisa.attention_backward(args[3], *args[:3], out, lse)
+        assert torch.equal(out, want_out) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+def test_equal_to_full_attention_and_to_the_node_default():
+    """The forward-only entry point and this one agree within the rounding of
+    their results (their products and order of sums are the same)."""
+    import b200_pisa
+
+    q, k, v = (make(1, 4, t, 128, torch.bfloat16, "bthd", i) for i, t in ((1, 130), (2, 260), (3, 260)))
+    a = b200_pisa.full_attention(q, k, v, 128 ** -0.5)
+    b = b200_pisa.attention(q, k, v)
+    assert ((a.float() - b.float()).abs() <= 2.0 ** -8 * a.float().abs() + 1e-6).all()

@@ -382,3 +382,36 @@ def test_long_rows_pass_32_bit_offsets():
     x.copy_(torch.randn(1, 2, 4, 64, device=DEV))
     pos = grid_positions(4, (64,), "int")
     close(b200_pisa.axial_rope(x, pos, (64,)), rotate_ref(x.double(), pos, (64,), 1e4, True), pair_scale(x.double(), (64,), True))
+
+
+@gpu
+def test_eps_zero_with_lanes_and_groups_left_over():
+    """Heads that do not fill the groups of a block, and no eps to keep the
+    empty lanes' reciprocal root finite."""
+    import b200_pisa
+
+    q, k = make(1, 3, 7, 40, torch.float32, "bthd", 1), make(1, 5, 7, 40, torch.float32, "bthd", 2)
+    w = torch.ones(40, device=DEV).requires_grad_()
+    lq = q.clone().requires_grad_()
+    pos = grid_positions(7, (40,), "int")
+    yq, yk = b200_pisa.qk_norm_rope(lq, k, w, w, pos, (40,), eps=0.0)
+    dq, dw = torch.autograd.grad((yq, yk), (lq, w), (torch.ones_like(yq), torch.ones_like(yk)))
+    assert all(torch.isfinite(x).all() for x in (yq, yk, dq, dw))
+    z = norm_ref(q.double(), None, 0.0)
+    close(yq.detach(), rotate_ref(z, pos, (40,), 1e4, True), pair_scale(z, (40,), True))
+
+
+@gpu
+def test_one_tensor_as_queries_and_keys():
+    import b200_pisa
+
+    x = make(1, 4, 33, 64, torch.bfloat16, "bthd", 1).requires_grad_()
+    w = torch.ones(64, device=DEV, dtype=torch.bfloat16)
+    pos = grid_positions(33, (64,), "int")
+    yq, yk = b200_pisa.qk_norm_rope(x, x, w, w, pos, (64,))
+    assert torch.equal(yq, yk)
+    (dx,) = torch.autograd.grad((yq, yk), x, (torch.ones_like(yq), torch.ones_like(yk)))
+    lone = x.detach().clone().requires_grad_()
+    zq, _ = b200_pisa.qk_norm_rope(lone, lone.detach(), w, w, pos, (64,))
+    (half,) = torch.autograd.grad(zq, lone, torch.ones_like(zq))
+    assert torch.equal(dx, half * 2)

@@ -905,9 +905,46 @@ struct StatArgs {
   int q_blocks;  // blocks of the query part; the rest walks V (NORMS)
 };
 
+// A group of 16 lanes sums x[u] for each u: lane l returns that of u = l >> 2
+// (the exchanges halve the values still held: 5 shuffles for the 4 sums).
+__device__ __forceinline__ float sum_rows(const float (&x)[4], int l) {
+  const bool h8 = l & 8, h4 = l & 4;
+  const float y0 = (h8 ? x[2] : x[0]) + __shfl_xor_sync(0xffffffffu, h8 ? x[0] : x[2], 8);
+  const float y1 = (h8 ? x[3] : x[1]) + __shfl_xor_sync(0xffffffffu, h8 ? x[1] : x[3], 8);
+  float z = (h4 ? y1 : y0) + __shfl_xor_sync(0xffffffffu, h4 ? y0 : y1, 4);
+  z += __shfl_xor_sync(0xffffffffu, z, 2);
+  return z + __shfl_xor_sync(0xffffffffu, z, 1);
+}
+
+// (a + low) . b of eight elements; LOW: whether there is a low part.
+template <typename T, bool LOW>
+__device__ __forceinline__ float dot8(const uint4& a, const uint4& low, const uint4& b) {
+  const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, lw[4] = {low.x, low.y, low.z, low.w}, bw[4] = {b.x, b.y, b.z, b.w};
+  uint64_t sum = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a0, a1, b0, b1;
+    Cvt<T>::unpack2(aw[i], a0, a1);
+    Cvt<T>::unpack2(bw[i], b0, b1);
+    uint64_t a2 = pack_f2(a0, a1);
+    if constexpr (LOW) {
+      Cvt<T>::unpack2(lw[i], a0, a1);
+      a2 = add_f2(a2, pack_f2(a0, a1));
+    }
+    sum = fma_f2(a2, pack_f2(b0, b1), sum);
+  }
+  float s0, s1;
+  unpack_f2(sum, s0, s1);
+  return s0 + s1;
+}
+
 // -lse*log2e and -delta of every query row, padded to whole tiles with rows
 // that give P = 0.  NORMS: also the largest squared norms of 64 dO rows and of
 // 64 valid V rows.  Block 0 resets the item counter of the kernel after.
+// A block takes 64 rows of one head, 16 lanes a row and four rows of each
+// lane at a time.  What counts is instructions: with a row address and
+// separate shuffles for each row it took 80 us for 64 heads of 9216 x 128 (16
+// of them without keys, so not read), and takes 56.
 template <typename T, bool NORMS>
 __global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_constant__ StatArgs a) {
   constexpr int kShift = std::is_same<T, __half>::value ? kShiftP16 : 0;
@@ -921,75 +958,64 @@ __global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_consta
   const int per_head = queries ? a.q_tiles * (kTile / kStatRows) : a.v_blocks;
   const int head = id / per_head;
   const int r0 = (id - head * per_head) * kStatRows;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
   float most = 0.f;
   if (queries) {
     const int len = a.key_lengths != nullptr ? min(max(a.key_lengths[head / a.heads], 0), a.tk) : a.tk;
-    const bool use_low = a.out_low.base != nullptr && len <= kLowKeys;
-    const bool needed = active && len > 0;  // rows without a key have no gradient
+    const int mine = r0 + (l >> 2) * 16 + g;  // the row this lane writes
+    const float lse = (l & 3) == 0 && mine < a.tq ? a.lse[int64_t(head) * a.tq + mine] : -INFINITY;
+    const int rows = active && len > 0 ? a.tq - r0 - g : 0;  // rows without a key have no gradient
+    float sum[4] = {}, norm[4] = {};
+    const int64_t o_step = a.out.st * int64_t(16 * sizeof(T)), d_step = a.dout.st * int64_t(16 * sizeof(T));
+    const char* op = a.out.row(head, r0 + g) + l * 16;
+    const char* dp = a.dout.row(head, r0 + g) + l * 16;
     uint4 o[4], d[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int r = r0 + u * 16 + g;
-      o[u] = d[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (needed && r < a.tq) {
-        o[u] = reinterpret_cast<const uint4*>(a.out.row(head, r))[l];
-        d[u] = reinterpret_cast<const uint4*>(a.dout.row(head, r))[l];
-      }
+      const bool in = u * 16 < rows;
+      o[u] = in ? *reinterpret_cast<const uint4*>(op + u * o_step) : zero;
+      d[u] = in ? *reinterpret_cast<const uint4*>(dp + u * d_step) : zero;
     }
+    if (a.out_low.base != nullptr && len <= kLowKeys) {
+      const char* lp = a.out_low.row(head, r0 + g) + l * 16;
+      const int64_t l_step = a.out_low.st * int64_t(16 * sizeof(T));
+      uint4 low[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int r = r0 + u * 16 + g;
-      const uint32_t ow[4] = {o[u].x, o[u].y, o[u].z, o[u].w}, dw[4] = {d[u].x, d[u].y, d[u].z, d[u].w};
-      uint4 low = make_uint4(0u, 0u, 0u, 0u);
-      if (use_low && needed && r < a.tq) low = reinterpret_cast<const uint4*>(a.out_low.row(head, r))[l];
-      const uint32_t lw[4] = {low.x, low.y, low.z, low.w};
-      float sum = 0.f, norm = 0.f;
+      for (int u = 0; u < 4; ++u) low[u] = u * 16 < rows ? *reinterpret_cast<const uint4*>(lp + u * l_step) : zero;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float o0, o1, l0, l1, d0, d1;
-        Cvt<T>::unpack2(ow[i], o0, o1);
-        Cvt<T>::unpack2(lw[i], l0, l1);
-        Cvt<T>::unpack2(dw[i], d0, d1);
-        sum = fmaf(o0 + l0, d0, sum);
-        sum = fmaf(o1 + l1, d1, sum);
-        if constexpr (NORMS) norm = fmaf(d0, d0, fmaf(d1, d1, norm));
-      }
+      for (int u = 0; u < 4; ++u) sum[u] = dot8<T, true>(o[u], low[u], d[u]);
+    } else {
 #pragma unroll
-      for (int w = 8; w > 0; w >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffu, sum, w);
-        if constexpr (NORMS) norm += __shfl_xor_sync(0xffffffffu, norm, w);
-      }
-      most = fmaxf(most, norm);
-      if (l == 0) {
-        const float lse = r < a.tq ? a.lse[int64_t(head) * a.tq + r] : -INFINITY;
-        float* dst = a.stat + (int64_t(head) * a.q_tiles + r / kTile) * (2 * kTile) + r % kTile;
-        dst[0] = lse == -INFINITY ? -INFINITY : -lse * kLog2e + static_cast<float>(kShift);
-        dst[kTile] = -sum;
-      }
+      for (int u = 0; u < 4; ++u) sum[u] = dot8<T, false>(o[u], zero, d[u]);
+    }
+    const float delta = sum_rows(sum, l);
+    if constexpr (NORMS) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) norm[u] = dot8<T, false>(d[u], zero, d[u]);
+      most = sum_rows(norm, l);
+    }
+    if ((l & 3) == 0) {
+      float* dst = a.stat + (int64_t(head) * a.q_tiles + mine / kTile) * (2 * kTile) + mine % kTile;
+      dst[0] = lse == -INFINITY ? -INFINITY : -lse * kLog2e + static_cast<float>(kShift);
+      dst[kTile] = -delta;
     }
   } else if constexpr (NORMS) {
     const int b = head / a.kv_heads;
     const int len = a.key_lengths != nullptr ? min(a.key_lengths[b], a.tk) : a.tk;
+    const int rows = active ? len - r0 - g : 0;
+    const char* vp = a.v.row(head, r0 + g) + l * 16;
+    const int64_t v_step = a.v.st * int64_t(16 * sizeof(T));
+    uint4 x[4];
+    float norm[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int r = r0 + u * 16 + g;
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (active && r < len) x = reinterpret_cast<const uint4*>(a.v.row(head, r))[l];
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-      float norm = 0.f;
+    for (int u = 0; u < 4; ++u) x[u] = u * 16 < rows ? *reinterpret_cast<const uint4*>(vp + u * v_step) : zero;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float v0, v1;
-        Cvt<T>::unpack2(w[i], v0, v1);
-        norm = fmaf(v0, v0, fmaf(v1, v1, norm));
-      }
-#pragma unroll
-      for (int s = 8; s > 0; s >>= 1) norm += __shfl_xor_sync(0xffffffffu, norm, s);
-      most = fmaxf(most, norm);
-    }
+    for (int u = 0; u < 4; ++u) norm[u] = dot8<T, false>(x[u], zero, x[u]);
+    most = sum_rows(norm, l);
   }
   if constexpr (NORMS) {
-    most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 16));
+#pragma unroll
+    for (int w = 16; w >= 4; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
     __syncthreads();
     if (threadIdx.x == 0) {

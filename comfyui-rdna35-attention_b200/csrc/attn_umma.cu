@@ -182,7 +182,7 @@ __device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
 // The buffer last held P(j-4): the caller issues S(j) only once that P.V has
 // completed (it reads P from these TMEM columns).
 template <bool BF16, int NW, int HALVES>
-__device__ __forceinline__ bool issue_s(Misc& m, char* k_s, uint32_t q_addr, uint32_t tmem, const UmmaArgs& a,
+__device__ __forceinline__ bool issue_s(Misc& m, uint64_t k_desc, uint64_t q_desc, uint32_t tmem, const UmmaArgs& a,
                                         volatile int* abort_flag, int j, long long* trace) {
   constexpr int kStages = Cfg<NW>::kStagesK;
   const int s = j % kStages;
@@ -193,11 +193,11 @@ __device__ __forceinline__ bool issue_s(Misc& m, char* k_s, uint32_t q_addr, uin
   tc_fence_after();
   if (trace && j < 256) trace[6 * j + 1] = clock64();
   const uint32_t idesc_s = idesc_f16(128, 64, BF16, false, false);
-  const uint32_t k_addr = smem_u32(k_s + s * kSlotBytes);
+  k_desc += s * (kSlotBytes >> 4);
 #pragma unroll
   for (int kk = 0; kk < 4 * HALVES; ++kk) {
-    const uint64_t da = smem_desc_sw128(q_addr + (kk >> 2) * 16384 + (kk & 3) * 32, 16, 1024);
-    const uint64_t db = smem_desc_sw128(k_addr + (kk >> 2) * 8192 + (kk & 3) * 32, 16, 1024);
+    const uint64_t da = q_desc + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
+    const uint64_t db = k_desc + (((kk >> 2) * 8192 + (kk & 3) * 32) >> 4);
     mma_ss(tmem + w * 256 + 128 + 64 * sb, da, db, idesc_s, kk > 0 ? 1u : 0u);
   }
   mma_commit(&m.s_full[w][sb]);
@@ -209,7 +209,7 @@ __device__ __forceinline__ bool issue_s(Misc& m, char* k_s, uint32_t q_addr, uin
 // O(w) += P(jj) V(jj) for key tile jj (warpgroup w = jj % 2); P is read from
 // TMEM, where the softmax wrote it over the tile's S columns.
 template <bool BF16, int NW, int HALVES>
-__device__ __forceinline__ bool issue_pv(Misc& m, char* smem, uint32_t tmem, const UmmaArgs& a,
+__device__ __forceinline__ bool issue_pv(Misc& m, uint64_t v_desc, uint32_t tmem, const UmmaArgs& a,
                                          volatile int* abort_flag, int jj, long long* trace) {
   constexpr int kStages = Cfg<NW>::kStagesV;
   const int w = jj % NW;
@@ -219,12 +219,10 @@ __device__ __forceinline__ bool issue_pv(Misc& m, char* smem, uint32_t tmem, con
   if (!mbar_wait(&m.v_full[jj % kStages], (jj / kStages) & 1, abort_flag, a.status, 12)) return false;
   tc_fence_after();
   const uint32_t idesc_o = idesc_f16(128, 64 * HALVES, BF16, false, true);
-  const uint32_t v_addr = smem_u32(smem + SmemLayout<NW>::v + (jj % kStages) * kSlotBytes);
+  v_desc += (jj % kStages) * (kSlotBytes >> 4);
 #pragma unroll
-  for (int kk = 0; kk < 4; ++kk) {
-    const uint64_t db = smem_desc_sw128(v_addr + kk * 2048, 8192, 1024);
-    mma_ts(tmem + w * 256, p_tmem + kk * 8, db, idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
-  }
+  for (int kk = 0; kk < 4; ++kk)
+    mma_ts(tmem + w * 256, p_tmem + kk * 8, v_desc + kk * (2048 >> 4), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
   mma_commit(&m.pv_done[w][i & 1]);
   mma_commit(&m.v_empty[jj % kStages]);
   if (trace && jj < 256) trace[6 * 256 + 1 + jj] = clock64();
@@ -465,6 +463,9 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     if (elect_one()) {
       const int w = warp == 1 ? 0 : 1;
       const uint32_t q_addr = smem_u32(q_s);
+      // one add per MMA steps a descriptor (its address field is the low bits)
+      const uint64_t q_desc = smem_desc_sw128(q_addr, 16, 1024), k_desc = smem_desc_sw128(smem_u32(k_s), 16, 1024),
+                     v_desc = smem_desc_sw128(smem_u32(v_s), 8192, 1024);
       const int cnt = (n - w + NW - 1) / NW;
       // S(i) may go out once P.V(i-2) (same S buffer) has completed and its K
       // tile is in; P.V(i) once P(i) and V(i) are.  S is preferred.
@@ -477,7 +478,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           const int j = NW * ns + w;
           const bool buf_free = ns < 2 || (ns - 2 < npv && mbar_test_wait(&m.pv_done[w][ns & 1], ((ns - 2) >> 1) & 1));
           if (buf_free && mbar_test_wait(&m.k_full[j % kStagesK], (j / kStagesK) & 1)) {
-            ok = issue_s<BF16 && !QK16, NW, kHalves>(m, k_s, q_addr, tmem, a, abort_flag, j, trace);
+            ok = issue_s<BF16 && !QK16, NW, kHalves>(m, k_desc, q_desc, tmem, a, abort_flag, j, trace);
             ++ns;
             did = true;
           }
@@ -486,7 +487,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           const int j = NW * npv + w;
           if (mbar_test_wait(&m.p_full[w][npv & 1], (npv >> 1) & 1) &&
               mbar_test_wait(&m.v_full[j % kStagesV], (j / kStagesV) & 1)) {
-            ok = issue_pv<BF16, NW, kHalves>(m, smem, tmem, a, abort_flag, j, trace);
+            ok = issue_pv<BF16, NW, kHalves>(m, v_desc, tmem, a, abort_flag, j, trace);
             ++npv;
             did = true;
           }

@@ -71,6 +71,7 @@ struct Cfg {
   static constexpr int kThreads = 64 + 32 * kElemWarps;
   static constexpr int kCtas = HALVES == 1 ? 2 : 1;     // per SM
   static constexpr uint32_t kStatBytes = 2 * kWalk * 4;
+  static constexpr bool kDpEarly = HALVES == 2;         // dQ: dP(i+1) is issued before dQ(i)
   // TMEM columns.
   //   dK/dV: S and dP take turns in kX (each is free again as soon as the
   //     elementwise warps have loaded it), P, dS, dV, dK.
@@ -276,6 +277,9 @@ __device__ __forceinline__ void clear_pairs(uint32_t (&w)[16], uint32_t bad) {
   }
 }
 
+// The first n of 32 columns.
+__device__ __forceinline__ uint32_t bad_below(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
 __device__ __forceinline__ int key_count(const GradArgs& a, int b) {
   return a.key_lengths != nullptr ? min(max(a.key_lengths[b], 0), a.tk) : a.tk;
 }
@@ -474,6 +478,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
   using C = Cfg<HALVES>;
   volatile int* abort_flag = &m.abort_flag;
   const uint32_t base = smem_u32(smem);
+  constexpr bool kDpEarly = C::kDpEarly;
   constexpr uint32_t step = L::tile >> 4;  // stages are L::tile apart
   const uint64_t own0 = rows_desc(base + L::own), own1 = rows_desc(base + L::own + L::own_tile);
   const uint64_t a_rows = rows_desc(base + L::a), a_cols = cols_desc(base + L::a);
@@ -540,8 +545,22 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
           ca.next();
         }
       } else {
-        // Order S(i+1), dQ(i), dP(i+1): S runs ahead of the exponentials of
-        // the tile before, dP under those of its own.
+        // Order S(i+1), dP(i+1), dQ(i): each goes out as soon as the
+        // elementwise warps have read the one before, and runs under their
+        // arithmetic of tile i.  With two CTAs per SM the other's products
+        // do that, and the wait it saves counts: dP(i+1) last (288 us
+        // against 300 for 16 x 4096 x 64).
+        auto dp = [&] {
+          if (!(ok = mbar_wait(&m.b_full[tb.s], tb.ph, abort_flag, a.status, 10))) return;
+          if constexpr (kDpEarly) {
+            if (i >= 0 && !(ok = mbar_wait(&m.dp_read, ph, abort_flag, a.status, 11))) return;
+          }
+          tc_fence_after();
+          product_rows<VBF16, HALVES>(tmem + C::kDP, own0, b_rows + tb.s * step);
+          mma_commit(&m.dp_full);
+          mma_commit(&m.b_empty[tb.s]);
+          tb.next(), cb.next();
+        };
         if (more) {  // the elementwise warps hold S(i)
           ok = mbar_wait(&m.a_full[ta.s], ta.ph, abort_flag, a.status, 7) &&
                (i < 0 || mbar_wait(&m.s_read, ph, abort_flag, a.status, 8));
@@ -551,22 +570,23 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
           mma_commit(&m.s_full);
           ta.next();
         }
+        if (kDpEarly && more) {
+          dp();
+          if (!ok) break;
+        }
         if (i >= 0) {
           ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9) &&
                (i > 0 || owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 25));
           if (!ok) break;
           tc_fence_after();
           product_cols<QBF16, HALVES>(tmem + C::kDQ, tmem + C::kDSq, a_cols + ca.s * step, i > 0);
+          if constexpr (kDpEarly) mma_commit(&m.dk_done);
           mma_commit(&m.a_empty[ca.s]);
           ca.next();
         }
-        if (more) {  // and dP(i) (ds_full says so)
-          if (!(ok = mbar_wait(&m.b_full[tb.s], tb.ph, abort_flag, a.status, 10))) break;
-          tc_fence_after();
-          product_rows<VBF16, HALVES>(tmem + C::kDP, own0, b_rows + tb.s * step);
-          mma_commit(&m.dp_full);
-          mma_commit(&m.b_empty[tb.s]);
-          tb.next(), cb.next();
+        if (!kDpEarly && more) {
+          dp();
+          if (!ok) break;
         }
       }
     }
@@ -657,12 +677,12 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
       for (int i = 0; i < n; ++i) {
         const uint32_t ph = (it + i) & 1;
         const float* stat = reinterpret_cast<const float*>(smem + L::stat + st.s * C::kStatBytes) + cg * 32;
-        uint32_t bad = 0u;
+        const int before = lim;
         if (a.causal) {
-          bad = lim <= 0 ? 0u : lim >= 32 ? ~0u : (1u << lim) - 1u;
           lim -= kWalk;
           if (++qt == w.per_head) lim += w.per_head * kWalk, qt = 0;
         }
+        const bool masked = a.causal && before > 0;
         if (!(ok = mbar_wait(&m.stat_full[st.s], st.ph, abort_flag, a.status, 13))) break;
         if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
         tc_fence_after();
@@ -682,7 +702,7 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
           p[c / 2] = Cvt<T>::pack2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
           p[c / 2 + 1] = Cvt<T>::pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
         }
-        if (bad != 0u) clear_pairs(p, bad);
+        if (masked) clear_pairs(p, bad_below(before));
         // dP(i) was issued after dV(i-1), so with it done P's columns are free
         if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
         tc_fence_after();
@@ -712,7 +732,7 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
             p[e / 2] = Cvt<TS>::pack2(x0, x1);
           }
         }
-        if (bad != 0u) clear_pairs(p, bad);  // 0 * inf
+        if (masked) clear_pairs(p, bad_below(before));  // 0 * inf
         if (i > 0 && !(ok = mbar_wait(&m.dk_done, ph ^ 1, abort_flag, a.status, 19))) break;  // the last dS is read
         tc_fence_after();
         tmem_st16(ds_addr, p);
@@ -740,7 +760,6 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
       for (int i = 0; i < n; ++i) {
         const uint32_t ph = (it + i) & 1;
         const int lim = seen - i * kWalk - cg * 32;  // columns from `lim` on are masked
-        const uint32_t bad = lim >= 32 ? 0u : lim <= 0 ? ~0u : ~0u << lim;
         if (!(ok = mbar_wait(&m.s_full, ph, abort_flag, a.status, 14))) break;
         tc_fence_after();
         uint32_t v[32];
@@ -770,6 +789,11 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
         uint32_t d[32], ds[16];
         tmem_ld32(dp_addr, d);
         tmem_wait_ld();
+        if constexpr (C::kDpEarly) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m.dp_read);
+        }
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
           uint64_t p = pack_f2(__uint_as_float(v[c]), __uint_as_float(v[c + 1]));
@@ -778,8 +802,11 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
           unpack_f2(mul_f2(p, add_f2(pack_f2(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), nd2)), x0, x1);
           ds[c / 2] = Cvt<TS>::pack2(x0, x1);
         }
-        if (bad != 0u) clear_pairs(ds, bad);
-        // dP(i) was issued after dQ(i-1), so dS's columns are free
+        if (lim < 32) clear_pairs(ds, ~bad_below(lim));
+        if constexpr (C::kDpEarly) {
+          if (i > 0 && !(ok = mbar_wait(&m.dk_done, ph ^ 1, abort_flag, a.status, 19))) break;  // the last dS is read
+          tc_fence_after();
+        }  // otherwise dP(i) was issued after dQ(i-1)
         tmem_st16(ds_addr, ds);
         tmem_wait_st();
         tc_fence_before();

@@ -71,6 +71,12 @@ struct Cfg {
   static constexpr int kThreads = 64 + 32 * kElemWarps;
   static constexpr int kCtas = HALVES == 1 ? 2 : 1;     // per SM
   static constexpr uint32_t kStatBytes = 2 * kWalk * 4;
+  // dK/dV: P and dS take the columns of S and dP that they come from.  With
+  // one CTA per SM the waits of the issuing thread that this needs are not
+  // hidden (3.56 against 3.48 ms for 32 heads of 9216^2 x 128); with two they
+  // are, and it saves the other warps two waits a tile (274 against 292 us
+  // for 16 of 4096^2 x 64).
+  static constexpr bool kInPlace = HALVES == 1;
   static constexpr bool kDpEarly = HALVES == 2;         // dQ: dP(i+1) is issued before dQ(i)
   // TMEM columns.
   //   dK/dV: S and dP take turns in kX (each is free again as soon as the
@@ -126,7 +132,7 @@ struct __align__(16) Misc {
   uint64_t a_full[kStagesA], a_empty[kStagesA];  // walked tiles: Q or K
   uint64_t b_full[kStagesB], b_empty[kStagesB];  // dO or V
   uint64_t stat_full[2], stat_empty[2];          // -lse and -delta of a query tile
-  uint64_t s_full, s_read, p_full, dp_full, dp_read, ds_full, dk_done;
+  uint64_t s_full, s_read, p_full, dp_full, dp_read, ds_full, dv_done, dk_done;
   uint64_t acc_full, acc_free;  // the item's results are complete; are stored
   uint64_t exit_done;
   Work item[2];
@@ -202,12 +208,12 @@ __device__ __forceinline__ void product_rows_ts(uint32_t d, uint32_t a, uint64_t
 
 // D[128 x D] (+)= A B with A (128 x walk, 16-bit pairs) in tensor memory at
 // `a`, B's rows as contraction.
-template <bool BF16, int HALVES>
+template <bool BF16, int HALVES, bool IN_PLACE = false>
 __device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint64_t b_desc, bool accumulate) {
   constexpr uint32_t idesc = idesc_f16(128, 64 * HALVES, BF16, false, true);
 #pragma unroll
   for (int kk = 0; kk < Cfg<HALVES>::kWalk / 16; ++kk)
-    mma_ts(d, a + kk * 8, b_desc + kk * (2048 >> 4), idesc, kk > 0 ? 1u : accumulate ? 1u : 0u);
+    mma_ts(d, a + (IN_PLACE ? (kk >> 1) * 32 + (kk & 1) * 8 : kk * 8), b_desc + kk * (2048 >> 4), idesc, kk > 0 ? 1u : accumulate ? 1u : 0u);
 }
 
 __device__ __forceinline__ uint64_t pack_f2(float a, float b) {
@@ -505,7 +511,47 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
     for (int i = -1; i < w.n; ++i) {
       const uint32_t ph = (it + i) & 1, next = ph ^ 1;
       const bool more = i + 1 < w.n;
-      if (w.dkv) {
+      if (C::kInPlace && w.dkv) {
+        // Order dV(i), S(i+1), dK(i), dP(i+1): P and dS are written over the
+        // columns of the S and dP they come from, and S(i+1) and dP(i+1) wait
+        // for the product that reads them.
+        if (i >= 0) {
+          ok = mbar_wait(&m.p_full, ph, abort_flag, a.status, 6) &&
+               (i > 0 || owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 25));
+          if (!ok) break;
+          tc_fence_after();
+          product_cols<VBF16, HALVES, true>(tmem + C::kDV, tmem + C::kS, b_cols + cb.s * step, i > 0);
+          mma_commit(&m.b_empty[cb.s]);
+          mma_commit(&m.dv_done);
+          cb.next();
+        }
+        if (more) {
+          ok = mbar_wait(&m.a_full[ta.s], ta.ph, abort_flag, a.status, 7) &&
+               (i < 0 || mbar_wait(&m.dv_done, ph, abort_flag, a.status, 8));
+          if (!ok) break;
+          tc_fence_after();
+          product_rows<QBF16, HALVES>(tmem + C::kS, own0, a_rows + ta.s * step);
+          mma_commit(&m.s_full);
+          ta.next();
+        }
+        if (i >= 0) {
+          if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
+          tc_fence_after();
+          product_cols<QBF16, HALVES, true>(tmem + C::kDK, tmem + C::kDP, a_cols + ca.s * step, i > 0);
+          mma_commit(&m.dk_done);
+          mma_commit(&m.a_empty[ca.s]);
+          ca.next();
+        }
+        if (more) {
+          ok = mbar_wait(&m.b_full[tb.s], tb.ph, abort_flag, a.status, 10) &&
+               (i < 0 || mbar_wait(&m.dk_done, ph, abort_flag, a.status, 11));
+          if (!ok) break;
+          tc_fence_after();
+          product_rows<VBF16, HALVES>(tmem + C::kDP, own1, b_rows + tb.s * step);
+          mma_commit(&m.dp_full);
+          tb.next();
+        }
+      } else if (w.dkv) {
         // Order S(i+1), dV(i), dP(i+1), dK(i): S and dP wait for the
         // elementwise warps to have loaded the other out of their common
         // columns, and dV or dK runs while they do.
@@ -670,8 +716,10 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
     if constexpr (!QBF16) gain = ds_gain(a, w.b, w.hk, kShift, lane);
     const uint64_t gain2 = pack_f2(gain, gain);
     if (w.dkv) {
-      const uint32_t s_addr = tmem + lanes + C::kX + cg * 32;
-      const uint32_t p_addr = tmem + lanes + C::kP + cg * 16, ds_addr = tmem + lanes + C::kDS + cg * 16;
+      const uint32_t s_addr = tmem + lanes + C::kX + cg * 32;  // kX is kS
+      const uint32_t dp_addr = C::kInPlace ? tmem + lanes + C::kDP + cg * 32 : s_addr;
+      const uint32_t p_addr = C::kInPlace ? s_addr : tmem + lanes + C::kP + cg * 16;
+      const uint32_t ds_addr = C::kInPlace ? dp_addr : tmem + lanes + C::kDS + cg * 16;
       int lim = own - off - w.first * kWalk - cg * 32;  // causal: columns below it are queries before the key
       int qt = 0;
       for (int i = 0; i < n; ++i) {
@@ -689,9 +737,11 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
         uint32_t v[32], p[16];
         tmem_ld32(s_addr, v);
         tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&m.s_read);
+        if constexpr (!C::kInPlace) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m.s_read);
+        }
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
           const float4 nl = *reinterpret_cast<const float4*>(stat + c);
@@ -703,19 +753,31 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
           p[c / 2 + 1] = Cvt<T>::pack2(__uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
         }
         if (masked) clear_pairs(p, bad_below(before));
+        if constexpr (C::kInPlace) {
+          tmem_st16(p_addr, p);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&m.p_full);
+            mbar_arrive(&m.s_read);  // for the parity of dQ items' waits
+          }
+        }
         // dP(i) was issued after dV(i-1), so with it done P's columns are free
         if (!(ok = mbar_wait(&m.dp_full, ph, abort_flag, a.status, 15))) break;
         tc_fence_after();
         uint32_t d[32];
-        tmem_st16(p_addr, p);
-        tmem_ld32(s_addr, d);
-        tmem_wait_st();
+        if constexpr (!C::kInPlace) tmem_st16(p_addr, p);
+        tmem_ld32(dp_addr, d);
+        if constexpr (!C::kInPlace) tmem_wait_st();
         tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&m.dp_read);
-          mbar_arrive(&m.p_full);
+        if constexpr (!C::kInPlace) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&m.dp_read);
+            mbar_arrive(&m.p_full);
+          }
         }
         // dS = P (dP - delta)
 #pragma unroll
@@ -733,8 +795,10 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
           }
         }
         if (masked) clear_pairs(p, bad_below(before));  // 0 * inf
-        if (i > 0 && !(ok = mbar_wait(&m.dk_done, ph ^ 1, abort_flag, a.status, 19))) break;  // the last dS is read
-        tc_fence_after();
+        if constexpr (!C::kInPlace) {
+          if (i > 0 && !(ok = mbar_wait(&m.dk_done, ph ^ 1, abort_flag, a.status, 19))) break;  // the last dS is read
+          tc_fence_after();
+        }
         tmem_st16(ds_addr, p);
         tmem_wait_st();
         tc_fence_before();
@@ -889,6 +953,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     mbar_init(&m.dp_full, 1);
     mbar_init(&m.dp_read, kElemWarps);
     mbar_init(&m.ds_full, kElemWarps);
+    mbar_init(&m.dv_done, 1);
     mbar_init(&m.dk_done, 1);
     mbar_init(&m.acc_full, 1);
     mbar_init(&m.acc_free, kElemWarps);

@@ -1133,13 +1133,6 @@ Layout layout_of(int64_t bh, int64_t bhk, int64_t q_tiles, int64_t v_blocks) {
   return l;
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 1;
-  return n;
-}
-
 template <bool VBF16, bool QBF16, bool OUT32, int HALVES>
 cudaError_t launch_grad(const CUtensorMap* maps, const GradArgs& a, cudaStream_t st) {
   const auto kernel = attn_grad_kernel<VBF16, QBF16, OUT32, HALVES>;

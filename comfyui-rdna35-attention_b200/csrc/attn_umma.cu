@@ -136,12 +136,11 @@ __device__ __forceinline__ Tile tile_at(const UmmaArgs& a, const Misc& m, int j,
   return t;
 }
 
-// TMA load of 64 rows (one key/query block) x 64 columns (half of D=128) of
-// (batch, head) bh of `heads` heads.
+// TMA load of 64 rows (one key/query block) x 64 columns (half of D=128).
 __device__ __forceinline__ void load_block(const CUtensorMap* map, const UmmaArgs& a, void* dst, uint64_t* bar,
-                                           int kind, int heads, int bh, int blk, int dh) {
-  const int b = bh / heads;
-  const int h = bh - b * heads;
+                                           int kind, int bh, int blk, int dh) {
+  const int b = bh / a.heads;
+  const int h = bh - b * a.heads;
   if (kind == 0) {
     tma_load_4d(dst, map, bar, dh * 64, blk * 64, h, b);
   } else {
@@ -181,7 +180,7 @@ __device__ __forceinline__ void add2(float& a0, float& a1, float b0, float b1) {
 // S(j) = Q K(j)^T into the S buffer of warpgroup j%2; frees K slot on completion.
 // The buffer last held P(j-4): the caller issues S(j) only once that P.V has
 // completed (it reads P from these TMEM columns).
-template <bool BF16, int NW, int HALVES>
+template <bool BF16, int NW>
 __device__ __forceinline__ bool issue_s(Misc& m, uint64_t k_desc, uint64_t q_desc, uint32_t tmem, const UmmaArgs& a,
                                         volatile int* abort_flag, int j, long long* trace) {
   constexpr int kStages = Cfg<NW>::kStagesK;
@@ -195,7 +194,7 @@ __device__ __forceinline__ bool issue_s(Misc& m, uint64_t k_desc, uint64_t q_des
   const uint32_t idesc_s = idesc_f16(128, 64, BF16, false, false);
   k_desc += s * (kSlotBytes >> 4);
 #pragma unroll
-  for (int kk = 0; kk < 4 * HALVES; ++kk) {
+  for (int kk = 0; kk < 8; ++kk) {
     const uint64_t da = q_desc + (((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
     const uint64_t db = k_desc + (((kk >> 2) * 8192 + (kk & 3) * 32) >> 4);
     mma_ss(tmem + w * 256 + 128 + 64 * sb, da, db, idesc_s, kk > 0 ? 1u : 0u);
@@ -208,7 +207,7 @@ __device__ __forceinline__ bool issue_s(Misc& m, uint64_t k_desc, uint64_t q_des
 
 // O(w) += P(jj) V(jj) for key tile jj (warpgroup w = jj % 2); P is read from
 // TMEM, where the softmax wrote it over the tile's S columns.
-template <bool BF16, int NW, int HALVES>
+template <bool BF16, int NW>
 __device__ __forceinline__ bool issue_pv(Misc& m, uint64_t v_desc, uint32_t tmem, const UmmaArgs& a,
                                          volatile int* abort_flag, int jj, long long* trace) {
   constexpr int kStages = Cfg<NW>::kStagesV;
@@ -218,7 +217,7 @@ __device__ __forceinline__ bool issue_pv(Misc& m, uint64_t v_desc, uint32_t tmem
   if (!mbar_wait(&m.p_full[w][i & 1], (i >> 1) & 1, abort_flag, a.status, 2)) return false;
   if (!mbar_wait(&m.v_full[jj % kStages], (jj / kStages) & 1, abort_flag, a.status, 12)) return false;
   tc_fence_after();
-  const uint32_t idesc_o = idesc_f16(128, 64 * HALVES, BF16, false, true);
+  const uint32_t idesc_o = idesc_f16(128, 128, BF16, false, true);
   v_desc += (jj % kStages) * (kSlotBytes >> 4);
 #pragma unroll
   for (int kk = 0; kk < 4; ++kk)
@@ -234,13 +233,8 @@ __device__ __forceinline__ bool issue_pv(Misc& m, uint64_t v_desc, uint32_t tmem
 // DIAG with a mask): every row adds its FP32 mask terms a.bias to the scaled
 // scores, and a row whose keys are all masked stores NaN.  MIRROR (head-
 // sharded calls): every output row is also stored into a.n_mirror peer
-// copies of the output buffer.  GEN (general exact attention, mode ALL): keys
-// limited per batch (a.key_lengths) and causally (query i sees keys up to
-// i + a.causal_off), key/value heads shared by groups of query heads, rows
-// that see no key written as 0 with lse -inf; its value is the number of
-// 64-column halves of the head dimension the products cover.  QK16: q and k
-// are FP16 copies held times a.qk_scale, whatever the type of v.
-template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR, int GEN, bool QK16>
+// copies of the output buffer.
+template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR>
 __global__ void __launch_bounds__(Cfg<NW>::kThreads, Cfg<NW>::kCtasPerSm)
 attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                  const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap kc_map,
@@ -251,17 +245,14 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   constexpr int kThreads = Cfg<NW>::kThreads;
   constexpr int kStagesK = Cfg<NW>::kStagesK;
   constexpr int kStagesV = Cfg<NW>::kStagesV;
-  constexpr int kHalves = GEN == 1 ? 1 : 2;
   Misc& m = *reinterpret_cast<Misc*>(smem + SmemLayout<NW>::misc);
   char* q_s = smem + SmemLayout<NW>::q;
   char* k_s = smem + SmemLayout<NW>::k;
   char* v_s = smem + SmemLayout<NW>::v;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  // causal: the CTAs with the most keys first
-  const int pair = GEN && a.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const int pair = blockIdx.x;
   const int bh = blockIdx.y;
-  int kv_heads = a.heads, kv_bh = bh, tk_ = a.tk;
   int qa = 2 * pair;
   int qb = 2 * pair + 1;
   bool has_b = qb < a.nqb;  // the pairing kernel's output is read after grid_dep_wait
@@ -314,16 +305,6 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   // launched with programmatic stream serialization: everything below reads
   // the routing results (or the inputs) and writes the output
   grid_dep_wait();
-  if constexpr (GEN != 0) {
-    const int b = bh / a.heads;
-    kv_heads = a.kv_heads;
-    kv_bh = b * kv_heads + (bh - b * a.heads) / (a.heads / kv_heads);
-    if (a.key_lengths != nullptr) tk_ = min(max(a.key_lengths[b], 0), a.tk);
-    if (threadIdx.x == 0) {
-      const int keys = a.causal ? min(tk_, min(pair * 128 + 128, a.tq) + a.causal_off) : tk_;
-      m.nlist = m.ntiles = keys > 0 ? (keys + 63) / 64 : 0;
-    }
-  }
   if (a.pairs != nullptr) {
     qa = a.pairs[(int64_t(bh) * gridDim.x + pair) * 2];
     qb = a.pairs[(int64_t(bh) * gridDim.x + pair) * 2 + 1];
@@ -408,10 +389,10 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       tma_prefetch_desc(&q_map);
       tma_prefetch_desc(&k_map);
       if constexpr (!WITHHOLD) {
-        mbar_expect_tx(&m.q_full, kQBytes / 2 * kHalves);
+        mbar_expect_tx(&m.q_full, kQBytes);
         for (int half = 0; half < 2; ++half)
-          for (int dh = 0; dh < kHalves; ++dh)
-            load_block(&q_map, a, q_s + dh * 16384 + half * 8192, &m.q_full, a.q_kind, a.heads, bh, half ? qb : qa, dh);
+          for (int dh = 0; dh < 2; ++dh)
+            load_block(&q_map, a, q_s + dh * 16384 + half * 8192, &m.q_full, a.q_kind, bh, half ? qb : qa, dh);
       }
       // key tiles 0..n-1, then the two 64-column halves of H as "tiles" n, n+1
       const int total = n + (a.has_corr ? 2 : 0);
@@ -422,11 +403,11 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         char* slot = k_s + s * kSlotBytes;
         if (trace && j < 256) trace[6 * j] = clock64();
         if (j < n) {
-          mbar_expect_tx(&m.k_full[s], kSlotBytes / 2 * kHalves);
+          mbar_expect_tx(&m.k_full[s], kSlotBytes);
           const Tile t = tile_at(a, m, j, ntail);
-          for (int dh = 0; dh < kHalves; ++dh) {
+          for (int dh = 0; dh < 2; ++dh) {
             if (t.tail) tma_load_3d(slot + dh * 8192, &kc_map, &m.k_full[s], dh * 64, t.blk * 64, bh);
-            else load_block(&k_map, a, slot + dh * 8192, &m.k_full[s], a.kv_kind, kv_heads, kv_bh, t.blk, dh);
+            else load_block(&k_map, a, slot + dh * 8192, &m.k_full[s], a.kv_kind, bh, t.blk, dh);
           }
         } else {
           // H[:, 64*(j-n) : 64*(j-n)+64]: 128 rows x 128 B
@@ -445,11 +426,11 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         const int s = j % kStagesV;
         if (!mbar_wait(&m.v_empty[s], ((j / kStagesV) & 1) ^ 1, abort_flag, a.status, 13)) break;
         char* slot = v_s + s * kSlotBytes;
-        mbar_expect_tx(&m.v_full[s], kSlotBytes / 2 * kHalves);
+        mbar_expect_tx(&m.v_full[s], kSlotBytes);
         const Tile t = tile_at(a, m, j, ntail);
-        for (int dh = 0; dh < kHalves; ++dh) {
+        for (int dh = 0; dh < 2; ++dh) {
           if (t.tail) tma_load_3d(slot + dh * 8192, &vc_map, &m.v_full[s], dh * 64, t.blk * 64, bh);
-          else load_block(&v_map, a, slot + dh * 8192, &m.v_full[s], a.kv_kind, kv_heads, kv_bh, t.blk, dh);
+          else load_block(&v_map, a, slot + dh * 8192, &m.v_full[s], a.kv_kind, bh, t.blk, dh);
         }
       }
       if (*abort_flag) drain_loads(m.v_full, kStagesV, issued, nullptr, a.status);
@@ -478,7 +459,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           const int j = NW * ns + w;
           const bool buf_free = ns < 2 || (ns - 2 < npv && mbar_test_wait(&m.pv_done[w][ns & 1], ((ns - 2) >> 1) & 1));
           if (buf_free && mbar_test_wait(&m.k_full[j % kStagesK], (j / kStagesK) & 1)) {
-            ok = issue_s<BF16 && !QK16, NW, kHalves>(m, k_desc, q_desc, tmem, a, abort_flag, j, trace);
+            ok = issue_s<BF16, NW>(m, k_desc, q_desc, tmem, a, abort_flag, j, trace);
             ++ns;
             did = true;
           }
@@ -487,7 +468,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
           const int j = NW * npv + w;
           if (mbar_test_wait(&m.p_full[w][npv & 1], (npv >> 1) & 1) &&
               mbar_test_wait(&m.v_full[j % kStagesV], (j / kStagesV) & 1)) {
-            ok = issue_pv<BF16, NW, kHalves>(m, v_desc, tmem, a, abort_flag, j, trace);
+            ok = issue_pv<BF16, NW>(m, v_desc, tmem, a, abort_flag, j, trace);
             ++npv;
             did = true;
           }
@@ -544,11 +525,8 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     const uint32_t o_base = tmem + lane_base + wg * 256;
     const int tq_row = qblk * 64 + (row & 63);
     float mrun = -INFINITY, lrun = 0.f, tmass = 0.f;
-    const int nb_ = a.nb, causal_ = a.causal;
-    const int causal_row = tq_row + (GEN ? a.causal_off : 0);  // the last key the row sees
-    const float log2_last_ = a.log2_last;
-    float scale_log2_ = a.scale_log2;
-    if constexpr (QK16) scale_log2_ /= a.qk_scale[0] * a.qk_scale[1];
+    const int nb_ = a.nb, causal_ = a.causal, tk_ = a.tk;
+    const float log2_last_ = a.log2_last, scale_log2_ = a.scale_log2;
     int i = 0;
     bool ok = true;
     for (int j = wg; j < n; j += NW, ++i) {
@@ -563,8 +541,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       tc_fence_after();
       const uint32_t s_addr = o_base + 128 + 64 * sb;
       const int klen = t.tail ? 64 : min(64, tk_ - t.blk * 64);
-      const bool plain =
-          !MASKED && !t.tail && klen == 64 && (!causal_ || (GEN != 0 && causal_row - t.blk * 64 >= 63));
+      const bool plain = !MASKED && !t.tail && klen == 64 && !causal_;
       // masked columns of this tile as two 32-bit words (bit c = column c),
       // and the column that carries the last (ragged) block's log2 length
       uint32_t bad0 = 0u, bad1 = 0u;
@@ -584,7 +561,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         } else {
           bad = klen < 64 ? (~0ull << klen) : 0ull;
           if (causal_) {
-            const int lim = causal_row - t.blk * 64;  // columns > lim are masked
+            const int lim = tq_row - t.blk * 64;  // columns > lim are masked
             if (lim < 63) bad |= lim < 0 ? ~0ull : (~0ull << (lim + 1));
           }
         }
@@ -667,7 +644,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
         }
         tc_fence_after();
 #pragma unroll 1
-        for (int c0 = 0; c0 < 64 * kHalves; c0 += 32) {
+        for (int c0 = 0; c0 < 128; c0 += 32) {
           uint32_t o[32];
           tmem_ld32(o_base + c0, o);
           tmem_wait_ld();
@@ -700,23 +677,6 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       }
       tmem_st32(s_addr, v);
       tmem_wait_st();
-      if constexpr (GEN != 0) {
-        // V rows past the batch's keys may hold anything: P is 0 there, but
-        // 0 * inf is not, so they are cleared in the tile first
-        if (klen < min(64, a.tk - t.blk * 64)) {
-          if (!mbar_wait(&m.v_full[j % kStagesV], (j / kStagesV) & 1, abort_flag, a.status, 25)) {
-            ok = false;
-            break;
-          }
-          char* tile = v_s + (j % kStagesV) * kSlotBytes;
-          const int rows = min(64, a.tk - t.blk * 64) - klen;
-          for (int x = threadIdx.x - 64; x < rows * 8 * kHalves; x += 128) {
-            const int r = klen + x / (8 * kHalves), ch = x % (8 * kHalves);
-            *reinterpret_cast<uint4*>(tile + (ch >> 3) * 8192 + r * 128 + (ch & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-        }
-      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&m.p_full[wg][sb]);
@@ -750,53 +710,16 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
     const float inv = lt > 0.f ? 1.f / lt : (MASKED ? __int_as_float(0x7fc00000) : 0.f);
     const float cw = tt * a.corr_scale;
     char* orow = store ? a.o.row(bh, tq_row) : nullptr;
-    char* low_row = nullptr;
-    // the warp stores together (the rows of a general call are linear)
-    const bool whole = GEN != 0 && __all_sync(0xffffffffu, ok && !*abort_flag);
-    char* quad_row = nullptr;
-    if constexpr (GEN != 0) {
-      if (half == 0 || has_b) quad_row = a.o.row(bh, tq_row - (lane & 3));
-      if (store && a.o_low.base != nullptr && tk_ <= kLowKeys) low_row = a.o_low.row(bh, tq_row);
-    }
     const uint32_t row_base = tmem + lane_base;
 #pragma unroll 1
-    for (int c0 = wg * (128 / NW); c0 < (GEN == 1 ? 64 : (wg + 1) * (128 / NW)); c0 += 32) {
+    for (int c0 = wg * (128 / NW); c0 < (wg + 1) * (128 / NW); c0 += 32) {
       // each warpgroup stores 128 / NW of the output columns
       uint32_t o0[32], o1[32], cr[32];
       tmem_ld32(row_base + c0, o0);
       if constexpr (NW == 2) tmem_ld32(row_base + 256 + c0, o1);
       if (a.has_corr) tmem_ld32(row_base + 128 + c0, cr);
       tmem_wait_ld();
-      if constexpr (GEN != 0) {
-        // Four lanes store 64 bytes of a row together: by its own lane alone,
-        // each row's 16 bytes touch a line of their own.
-        uint32_t w[16];
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          const float f0 = lt == 0.f ? 0.f : __uint_as_float(o0[c]) * inv;  // no key seen: O may hold anything
-          const float f1 = lt == 0.f ? 0.f : __uint_as_float(o0[c + 1]) * inv;
-          w[c / 2] = Cvt<T>::pack2(f0, f1);
-          if (low_row != nullptr) {  // what the output's type cannot hold
-            float h0, h1;
-            Cvt<T>::unpack2(w[c / 2], h0, h1);
-            o0[c / 2] = Cvt<T>::pack2(f0 - h0, f1 - h1);
-          }
-        }
-        if (low_row != nullptr) {
-          uint4* dst = reinterpret_cast<uint4*>(low_row + c0 * 2);
-#pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4)
-            if (c0 + 8 * q4 < a.o.dim)
-              dst[q4] = make_uint4(o0[4 * q4], o0[4 * q4 + 1], o0[4 * q4 + 2], o0[4 * q4 + 3]);
-        }
-        transpose_quads(w, lane);
-        const int q = lane & 3;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (whole && (half == 0 || has_b) && tq_row - q + j < a.tq && c0 + 8 * q < a.o.dim)
-            *reinterpret_cast<uint4*>(quad_row + j * a.o.st * 2 + (c0 + 8 * q) * 2) =
-                make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-      } else if (store) {
+      if (store) {
         uint32_t packed[16];
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
@@ -869,8 +792,7 @@ attn_umma_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       }
     }
     if (store && wg == 0 && a.lse != nullptr) {
-      const float none = GEN != 0 && lt != 0.f ? lt : -INFINITY;  // NaN rows stay NaN
-      a.lse[int64_t(bh) * a.tq + tq_row] = lt > 0.f ? (mm + __log2f(lt)) * 0.6931471805599453f : none;
+      a.lse[int64_t(bh) * a.tq + tq_row] = lt > 0.f ? (mm + __log2f(lt)) * 0.6931471805599453f : -INFINITY;
     }
   }
   tc_fence_before();
@@ -966,6 +888,13 @@ int* device_status_ptr() {
   return static_cast<int*>(ptr);
 }
 
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 1;
+  return n;
+}
+
 bool umma_supported(const b2_view& q, const b2_view& k, const b2_view& v, const b2_view& o) {
   // D < 128 (multiples of 8): the TMA boxes stay 64 columns wide and read
   // the columns past D as zeros, which changes no dot product
@@ -990,15 +919,15 @@ int attn_warpgroups() {
   return nw;
 }
 
-template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR, int GEN = 0, bool QK16 = false>
+template <bool BF16, int NW, bool WITHHOLD, bool MASKED, bool MIRROR>
 cudaError_t launch_variant(dim3 grid, cudaStream_t stream, const CUtensorMap& q_map, const CUtensorMap& k_map,
                            const CUtensorMap& v_map, const CUtensorMap& kc_map, const CUtensorMap& vc_map,
                            const CUtensorMap& h_map, const UmmaArgs& a) {
   const int smem = static_cast<int>(SmemLayout<NW>::total);
   const cudaError_t err =
-      ensure_smem(reinterpret_cast<const void*>(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR, GEN, QK16>), smem);
+      ensure_smem(reinterpret_cast<const void*>(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR>), smem);
   if (err != cudaSuccess) return err;
-  return launch_pdl(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR, GEN, QK16>, grid, dim3(Cfg<NW>::kThreads), size_t(smem), stream,
+  return launch_pdl(attn_umma_kernel<BF16, NW, WITHHOLD, MASKED, MIRROR>, grid, dim3(Cfg<NW>::kThreads), size_t(smem), stream,
                     q_map, k_map, v_map, kc_map, vc_map, h_map, a);
 }
 
@@ -1091,41 +1020,6 @@ cudaError_t launch_attn_umma(const b2_view& qv, const b2_view& kv, const b2_view
   if (err != cudaSuccess) return err;
   *launched = true;
   return cudaGetLastError();
-}
-
-cudaError_t launch_attn_general(const AttnGeneralCall& c, int* status, cudaStream_t stream) {
-  const b2_view &q = *c.q, &k = *c.k;
-  CUtensorMap q_map, k_map, v_map;
-  if (!linear_rows_map(&q_map, q, 64) || !linear_rows_map(&k_map, k, 64) || !linear_rows_map(&v_map, *c.v, 64))
-    return cudaErrorInvalidValue;
-  UmmaArgs a{};
-  a.heads = q.heads;
-  a.kv_heads = k.heads;
-  a.tq = q.tokens;
-  a.tk = k.tokens;
-  a.nqb = (q.tokens + 63) / 64;
-  a.frames = a.tiles_per_row = a.tiles_per_frame = 1;
-  a.scale_log2 = c.scale * 1.4426950408889634f;
-  a.causal = c.causal;
-  a.causal_off = k.tokens - q.tokens;
-  a.key_lengths = c.key_lengths;
-  a.o = make_rows(*c.out);
-  a.lse = c.lse;
-  a.status = status;
-  if (c.out_low != nullptr) a.o_low = make_rows(*c.out_low);
-  a.qk_scale = c.qk_scale;
-  const dim3 grid((a.nqb + 1) / 2, q.batch * q.heads);
-  auto launch = [&](auto bf16, auto halves) {
-    constexpr bool kBf16 = decltype(bf16)::value;
-    constexpr int kGen = decltype(halves)::value;
-    if (c.qk_scale != nullptr)
-      return launch_variant<kBf16, 1, false, false, false, kGen, true>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a);
-    return launch_variant<kBf16, 1, false, false, false, kGen>(grid, stream, q_map, k_map, v_map, k_map, v_map, k_map, a);
-  };
-  using One = std::integral_constant<int, 1>;
-  using Two = std::integral_constant<int, 2>;
-  if (c.v->dtype == B2_BF16) return q.head_dim <= 64 ? launch(std::true_type{}, One{}) : launch(std::true_type{}, Two{});
-  return q.head_dim <= 64 ? launch(std::false_type{}, One{}) : launch(std::false_type{}, Two{});
 }
 
 }  // namespace b2

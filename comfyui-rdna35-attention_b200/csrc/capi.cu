@@ -775,8 +775,8 @@ int b2_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, c
   if (rc || (out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q)))) return rc;
   int* status = device_status_ptr();
   if (status == nullptr) return fail(B2_ERR_CUDA, "device status word unavailable");
-  const AttnGeneralCall c{q, k, v, out, key_lengths, scale, causal ? 1 : 0, lse, out_low, nullptr};
-  const cudaError_t err = launch_attn_general(c, status, static_cast<cudaStream_t>(stream));
+  const AttnForwardCall c{q, k, v, out, key_lengths, scale, causal ? 1 : 0, lse, out_low, nullptr};
+  const cudaError_t err = launch_attn_forward(c, status, static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) return cuda_fail(err, "attention launch");
   g_last_kernel = "tcgen05";
   return ok();
@@ -1013,8 +1013,8 @@ int b2_norm_rope_attention_forward(const b2_view* q, const b2_view* k, const b2_
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t err = launch_rotary(r, st);
   if (err != cudaSuccess) return cuda_fail(err, "norm and rotary launch");
-  const AttnGeneralCall c{&q16, &k16, v, out, key_lengths, scale, causal ? 1 : 0, lse, out_low, qk_scale};
-  err = launch_attn_general(c, status, st);
+  const AttnForwardCall c{&q16, &k16, v, out, key_lengths, scale, causal ? 1 : 0, lse, out_low, qk_scale};
+  err = launch_attn_forward(c, status, st);
   if (err != cudaSuccess) return cuda_fail(err, "attention launch");
   g_last_kernel = "tcgen05";
   return ok();

@@ -8,6 +8,7 @@ namespace b2 {
 // 4D TMA map (D,T,H,B) of a linear view: boxes of 64 columns x box_rows rows,
 // zeros past D and T.  False for views TMA cannot address.
 bool linear_rows_map(CUtensorMap* map, const b2_view& v, int box_rows);
+int sm_count();  // of the current device
 // Where a batch has at most this many keys, the forward pass also writes what
 // the output's type cannot hold: delta = rowsum(dout * out) then cancels
 // against few dP terms, and BF16's rounding of out would be the largest error
@@ -64,12 +65,6 @@ struct UmmaArgs {
   int n_mirror;  // peer output copies, see AttnParams
   char* mirror[kMaxMirrors];
   int mirror_multicast;
-  // general exact attention: shared key/value heads, key limits
-  int kv_heads;
-  const int32_t* key_lengths;  // [B] or NULL
-  int causal_off;              // causal: query i sees keys up to i + causal_off
-  Rows o_low;                  // what o's type cannot hold of the output (rows of few keys), or no base
-  const float* qk_scale;       // the powers of two FP16 q and k are held times
 };
 bool umma_supported(const b2_view& q, const b2_view& k, const b2_view& v, const b2_view& o);
 cudaError_t launch_attn_umma(const b2_view& qv, const b2_view& kv, const b2_view& vv, const b2_view& ov,
@@ -105,8 +100,8 @@ cudaError_t launch_fixed_f32(const Rows& q, const Rows& k, const Rows& v, const 
 cudaError_t launch_block_bias(const void* mask, int mask_dtype, int64_t s_bh, int64_t s_row, int64_t s_col,
                               int mask_rows_bh, int tokens, float* bias, cudaStream_t stream);
 // Exact attention with shared key/value heads, per-batch key counts and a
-// causal mask aligned to the last key (attn_umma.cu).
-struct AttnGeneralCall {
+// causal mask aligned to the last key (attn_forward.cu).
+struct AttnForwardCall {
   const b2_view *q, *k, *v, *out;
   const int32_t* key_lengths;
   float scale;
@@ -115,7 +110,7 @@ struct AttnGeneralCall {
   const b2_view* out_low;   // or NULL
   const float* qk_scale;    // FP16 q, k held times these (whatever v's type), or NULL
 };
-cudaError_t launch_attn_general(const AttnGeneralCall& call, int* status, cudaStream_t stream);
+cudaError_t launch_attn_forward(const AttnForwardCall& call, int* status, cudaStream_t stream);
 struct AttnGradCall {
   const b2_view *q, *k, *v, *out, *dout, *dq, *dk, *dv;
   const b2_view* out_low;  // what out's type could not hold of the output, or NULL

@@ -568,21 +568,22 @@ rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
         for (int i = 0; i < 8; ++i) x[i] = g[i] = 0.f;
       }
       turn<LAYOUT>(k, g, t, a.rot_pairs);  // dz
-      float sum = 0.f, dot = 0.f;
+      float sum = 0.f, dot = 0.f, gw[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         sum = fmaf(x[i], x[i], sum);
-        dot = fmaf(g[i] * w[i], x[i], dot);
+        gw[i] = g[i] * w[i];
+        dot = fmaf(gw[i], x[i], dot);
       }
       float sums[2] = {sum, dot};
       group_sums<2>(sums, a.group_log2);
       const float r = counts ? rsqrtf(sums[0] * inv_dim + a.eps) : 0.f;  // eps may be 0
-      const float back = -sums[1] * inv_dim * r * r * r;  // xh mean(g w xh) r = -back x
+      const float back = -sums[1] * inv_dim * r;  // -mean(g w xh)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        g[i] *= r;
+        x[i] *= r;  // xh
         dw[i] = fmaf(g[i], x[i], dw[i]);
-        g[i] = fmaf(g[i], w[i], back * x[i]);
+        g[i] = fmaf(back, x[i], gw[i]) * r;
       }
       if (j < rows) {
         rx.narrow(g);

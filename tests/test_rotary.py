@@ -415,3 +415,27 @@ def test_one_tensor_as_queries_and_keys():
     zq, _ = b200_pisa.qk_norm_rope(lone, lone.detach(), w, w, pos, (64,))
     (half,) = torch.autograd.grad(zq, lone, torch.ones_like(zq))
     assert torch.equal(dx, half * 2)
+
+
+@gpu
+@pytest.mark.parametrize("size", [1e-17, 1e15])
+def test_tiny_and_huge_rows_without_eps(size):
+    """r^3 of such rows is out of FP32's range, their gradient is not; the
+    sums of squares (1e-34, 1e30) still are in it."""
+    import b200_pisa
+
+    x = (make(1, 4, 9, 64, torch.float32, "bthd", 1) * size).requires_grad_()
+    dy = make(1, 4, 9, 64, torch.float32, "bthd", 2)
+    w = torch.ones(64, device=DEV)
+    pos = grid_positions(9, (64,), "int")
+    y, _ = b200_pisa.qk_norm_rope(x, x.detach(), w, w, pos, (64,), eps=0.0)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    leaf = x.detach().double().requires_grad_()
+    ref = rotate_ref(norm_ref(leaf, None, 0.0), pos, (64,), 1e4, True)
+    (want,) = torch.autograd.grad(ref, leaf, dy.double())
+    close(y.detach(), ref.detach(), pair_scale(ref.detach(), (64,), True))
+    # dx = r (g - xh mean(g xh)): a hundred roundings of terms as large as r |g|, r |xh| sum|g xh| / 64
+    r = leaf.detach().square().mean(-1, keepdim=True).rsqrt()
+    g = dy.double().abs().amax(-1, keepdim=True) * 2 ** 0.5
+    xh = (leaf.detach() * r).abs()
+    assert ((dx.double() - want).abs() <= 128 * 2.0 ** -24 * r * g * (1 + xh * xh.mean(-1, keepdim=True))).all()

@@ -48,7 +48,11 @@ def raw_stream(x: torch.Tensor) -> int:
 
 def require_one_device(name: str, *tensors: torch.Tensor | None) -> None:
     first = tensors[0].device
-    if first.type != "cuda" or any(t is not None and t.device != first for t in tensors):
+    one = first.type == "cuda"
+    for t in tensors:
+        if t is not None and t.device != first:
+            one = False
+    if not one:
         raise ValueError(f"{name} requires its tensors on one CUDA device.")
 
 
@@ -100,10 +104,19 @@ def signature(x: torch.Tensor):
     return x.shape, x.stride(), x.dtype
 
 
-def as_rows(x: torch.Tensor, broadcast: bool = True) -> torch.Tensor:
-    """x where the kernels can read it in place, else a contiguous copy.
-    broadcast: whether stride 0 can be read in place (TMA cannot)."""
-    shape, strides, dtype = signature(x)
-    if x.data_ptr() % 16 == 0 and addressable(shape, strides, dtype) and (broadcast or not repeats(shape, strides)):
-        return x
-    return x.contiguous()
+@functools.lru_cache(maxsize=PLANS)
+def _tail_in_place(shape, strides, dtype: torch.dtype, broadcast: bool) -> bytes | None:
+    if addressable(shape, strides, dtype) and (broadcast or not repeats(shape, strides)):
+        return view_tail(shape, strides, dtype)
+    return None
+
+
+def as_rows(x: torch.Tensor, broadcast: bool = True) -> tuple[torch.Tensor, bytes]:
+    """x where the kernels can read it in place, else a contiguous copy, and
+    its packed view.  broadcast: whether stride 0 can be read in place (TMA
+    cannot)."""
+    tail = _tail_in_place(*signature(x), broadcast)
+    if tail is None or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format) if x.data_ptr() % 16 else x.contiguous()
+        tail = view_tail(*signature(x))
+    return x, with_base(x, tail)

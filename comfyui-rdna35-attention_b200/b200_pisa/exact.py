@@ -84,7 +84,7 @@ def _planned(q, k, v, scale, key_lengths):
         if x.data_ptr() % 16:
             raise ValueError(f"{name} needs a contiguous head dimension and rows that start on 16-byte boundaries.")
     if plan[1]:
-        q, k, v = (as_rows(x, broadcast=False) for x in (q, k, v))
+        q, k, v = (as_rows(x, broadcast=False)[0] for x in (q, k, v))
         plan = _plan(signature(q), signature(k), signature(v), lens_sig, scale)
     return q, k, v, plan
 
@@ -127,6 +127,11 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
     return (out, lse, low) if with_low else (out, lse)
 
 
+@functools.lru_cache(maxsize=PLANS)
+def _workspace_bytes(*sizes: int) -> int:
+    return LIB.b2_attention_backward_workspace_bytes(*sizes)
+
+
 def check_saved(q: torch.Tensor, flat: bool, lse, **rows) -> list:
     """Checked four-dimensional ``rows`` (like q) a backward pass is given."""
     got = []
@@ -156,17 +161,15 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     require_one_device("attention_backward", q, k, v, key_lengths, out, dout, lse, out_low)
     batch, heads, tokens, _ = q.shape
     with on_device(q):
-        out, dout, lse = as_rows(out, broadcast=False), as_rows(dout, broadcast=False), lse.contiguous()
-        low = None if out_low is None else as_rows(out_low, broadcast=False)
+        (out, out_view), (dout, dout_view) = as_rows(out, broadcast=False), as_rows(dout, broadcast=False)
+        low, low_view = (None, None) if out_low is None else as_rows(out_low, broadcast=False)
+        lse = lse.contiguous()
         dq, dk, dv = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1]), new_rows(k, k.shape, strides[1])
-        ws = torch.empty(LIB.b2_attention_backward_workspace_bytes(batch, heads, k.shape[1], tokens, k.shape[2]),
-                         device=q.device, dtype=torch.uint8)
+        ws = torch.empty(_workspace_bytes(batch, heads, k.shape[1], tokens, k.shape[2]), device=q.device, dtype=torch.uint8)
         check(LIB.b2_attention_backward(
             with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]),
-            with_base(out, view_tail(*signature(out))), None if low is None else with_base(low, view_tail(*signature(low))),
-            with_base(dout, view_tail(*signature(dout))), ptr(lse), with_base(dq, grad_tails[0]),
-            with_base(dk, grad_tails[1]), with_base(dv, grad_tails[1]), scale, 1 if causal else 0, ptr(key_lengths),
-            ptr(ws), raw_stream(q)))
+            out_view, low_view, dout_view, ptr(lse), with_base(dq, grad_tails[0]), with_base(dk, grad_tails[1]),
+            with_base(dv, grad_tails[1]), scale, 1 if causal else 0, ptr(key_lengths), ptr(ws), raw_stream(q)))
     return (dq.squeeze(1), dk.squeeze(1), dv.squeeze(1)) if flat else (dq, dk, dv)
 
 

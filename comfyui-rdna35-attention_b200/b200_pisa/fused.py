@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import exact, rotary
-from ._args import (as_rows, new_rows, on_device, raw_stream, require_one_device, signature, view_tail, with_base)
+from ._args import as_rows, new_rows, on_device, raw_stream, require_one_device, with_base
 from ._lib import LIB, check, ptr
 
 
@@ -60,13 +60,13 @@ def _backward(dout, q, k, v, q_weight, k_weight, positions, out, lse, low, saved
                                                                                         positions, call)
     batch, heads, tokens, dim = q.shape
     with on_device(q):
-        dout = as_rows(dout, broadcast=False)
+        dout, dout_view = as_rows(dout, broadcast=False)
         dq, dk, dv = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1]), new_rows(k, k.shape, strides[1])
         dwq, dwk = (torch.empty_like(w) if w is not None and weight_grads else None for w in (q_weight, k_weight))
         ws = torch.empty(_saved_bytes(batch, heads, k.shape[1], tokens, dim)[1], device=q.device, dtype=torch.uint8)
         check(LIB.b2_norm_rope_attention_backward(
             with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]), with_base(out, grad_tails[0]),
-            exact.with_optional(low, grad_tails[0]), with_base(dout, view_tail(*signature(dout))), ptr(lse),
+            exact.with_optional(low, grad_tails[0]), dout_view, ptr(lse),
             ptr(q_weight), ptr(k_weight), w_code, eps, with_base(positions, rot), scale, 1 if causal else 0,
             ptr(key_lengths), ptr(saved), with_base(dq, grad_tails[0]), with_base(dk, grad_tails[1]),
             with_base(dv, grad_tails[1]), ptr(dwq), ptr(dwk), ptr(ws), raw_stream(q)))

@@ -111,7 +111,7 @@ class _AxialRope(torch.autograd.Function):
     def backward(ctx, dy):
         axes_dims, theta, interleaved, inverse = ctx.rotation
         (positions,) = ctx.saved_tensors
-        return _rope_call(as_rows(dy), positions, axes_dims, theta, interleaved, not inverse), None, None, None, None, None
+        return _rope_call(as_rows(dy)[0], positions, axes_dims, theta, interleaved, not inverse), None, None, None, None, None
 
 
 def axial_rope(x: torch.Tensor, positions: torch.Tensor, axes_dims: Sequence[int], *, theta=10000.0,
@@ -202,17 +202,16 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
             raise ValueError(f"{name} must be a tensor of its output's shape and dtype.")
     require_one_device("qk_norm_rope_backward", q, k, q_weight, k_weight, positions, dq_out, dk_out)
     with on_device(q):
-        dq_out, dk_out = as_rows(dq_out), as_rows(dk_out)
+        (dq_out, dq_view), (dk_out, dk_view) = as_rows(dq_out), as_rows(dk_out)
         dq, dk = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1])
         dwq, dwk = (torch.empty_like(w) if w is not None and weight_grads else None for w in (q_weight, k_weight))
         ws = None
         if dwq is not None or dwk is not None:
             ws = torch.empty(LIB.b2_qk_norm_rope_workspace_bytes(q.shape[-1]), device=q.device, dtype=torch.uint8)
         check(LIB.b2_qk_norm_rope_backward(
-            with_base(q, tails[0]), with_base(k, tails[1]), with_base(dq_out, view_tail(*signature(dq_out))),
-            with_base(dk_out, view_tail(*signature(dk_out))), with_base(dq, out_tails[0]), with_base(dk, out_tails[1]),
-            ptr(q_weight), ptr(k_weight), w_code, float(eps), with_base(positions, rot), ptr(dwq), ptr(dwk), ptr(ws),
-            raw_stream(q)))
+            with_base(q, tails[0]), with_base(k, tails[1]), dq_view, dk_view, with_base(dq, out_tails[0]),
+            with_base(dk, out_tails[1]), ptr(q_weight), ptr(k_weight), w_code, float(eps), with_base(positions, rot),
+            ptr(dwq), ptr(dwk), ptr(ws), raw_stream(q)))
     return dq, dk, dwq, dwk
 
 

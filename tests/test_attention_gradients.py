@@ -457,3 +457,56 @@ def test_equal_to_full_attention_and_to_the_node_default():
     a = b200_pisa.full_attention(q, k, v, 128 ** -0.5)
     b = b200_pisa.attention(q, k, v)
     assert ((a.float() - b.float()).abs() <= 2.0 ** -8 * a.float().abs() + 1e-6).all()
+
+
+@gpu
+def test_contiguous_gradients_off_the_16_byte_boundaries():
+    """contiguous() leaves such a tensor where it is."""
+    import b200_pisa
+
+    q, k, v, dout = (make(1, 2, 40, 64, torch.bfloat16, "bhtd", i) for i in range(4))
+    out, lse = b200_pisa.attention_forward(q, k, v)
+    want = b200_pisa.attention_backward(dout, q, k, v, out, lse)
+    off = torch.empty(dout.numel() + 1, device=DEV, dtype=torch.bfloat16)[1:].view_as(dout)
+    off.copy_(dout)
+    assert off.is_contiguous() and off.data_ptr() % 16
+    got = b200_pisa.attention_backward(off, q, k, v, out, lse)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    pos = torch.arange(40, device=DEV)[:, None]
+    x = q.clone().requires_grad_()
+    y = b200_pisa.axial_rope(x, pos, (64,))
+    assert torch.equal(torch.autograd.grad(y, x, off, retain_graph=True)[0], torch.autograd.grad(y, x, dout)[0])
+
+
+@gpu
+def test_training_step_captured_whole():
+    """Forward and backward through autograd in one graph, as a captured
+    training step has them (no eager graph of the leaves is alive)."""
+    import b200_pisa
+
+    q, k, v = (make(1, 4, 200, 64, torch.bfloat16, "bthd", i).requires_grad_() for i in (1, 2, 3))
+    w = torch.ones(64, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    pos = torch.arange(200, device=DEV)[:, None]
+    dout = make(1, 4, 200, 64, torch.bfloat16, "bthd", 4)
+
+    def step():
+        a = b200_pisa.norm_rope_attention(q, k, v, w, w, pos, (64,), causal=True)
+        b = b200_pisa.attention(q, k, v)
+        return torch.autograd.grad((a, b), (q, k, v, w), (dout, dout))
+
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream(DEV).wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    with torch.no_grad():
+        q.mul_(0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [x.clone() for x in captured]
+    assert all(torch.equal(a, b) for a, b in zip(got, step()))

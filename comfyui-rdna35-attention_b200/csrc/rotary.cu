@@ -562,12 +562,12 @@ rotary_grad_kernel(const __grid_constant__ RotaryArgs a) {
       rx.widen(x);
       rdy.widen(g);
       fetch(j + kAheadGrad);
+      turn<LAYOUT>(k, g, t, a.rot_pairs);  // dz
       const bool counts = j < rows && !dead;
-      if (!counts) {  // what a slot held before may be NaN
+      if (!counts) {  // what a slot held before may be NaN, and so may the angles of a token past the last
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = g[i] = 0.f;
       }
-      turn<LAYOUT>(k, g, t, a.rot_pairs);  // dz
       float sum = 0.f, dot = 0.f, gw[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {

@@ -439,3 +439,23 @@ def test_tiny_and_huge_rows_without_eps(size):
     g = dy.double().abs().amax(-1, keepdim=True) * 2 ** 0.5
     xh = (leaf.detach() * r).abs()
     assert ((dx.double() - want).abs() <= 128 * 2.0 ** -24 * r * g * (1 + xh * xh.mean(-1, keepdim=True))).all()
+
+
+@gpu
+@pytest.mark.parametrize("h,t,d,axis", [(2, 887, 64, 64), (1, 17, 128, 128), (3, 5, 40, 40), (2, 33, 24, 12)])
+def test_weight_gradients_of_ragged_token_tiles(h, t, d, axis):
+    """Tokens past the last of a block's tile have no angles: what an earlier
+    call left in their place (here NaN, from NaN positions) does not reach the
+    sums."""
+    import b200_pisa
+
+    x = make(1, h, 20000, d, torch.float32, "bthd", 1)  # the same tiles, on every SM
+    w = torch.ones(d, device=DEV)
+    dirty = torch.full((20000, 1), math.nan, device=DEV)
+    q, k, dq, dk = (make(1, n, t, d, torch.float32, "bthd", i) for i, n in ((1, h), (2, 1), (3, h), (4, 1)))
+    pos = grid_positions(t, (axis,), "int")
+    for _ in range(3):
+        b200_pisa.qk_norm_rope_backward(x, x, x, x, w, w, dirty, (axis,))
+        b200_pisa.qk_norm_rope(x, x, w, w, dirty, (axis,))
+        got = b200_pisa.qk_norm_rope_backward(dq, dk, q, k, w, w, pos, (axis,))
+        assert all(torch.isfinite(g).all() for g in got)

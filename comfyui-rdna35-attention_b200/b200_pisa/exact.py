@@ -22,7 +22,7 @@ from ._args import (PLANS, addressable, as_rows, new_rows, on_device, raw_stream
 from ._lib import LIB, check, ptr
 
 MAX_HEAD_DIM = 128
-#: keys of a batch up to which out's rounding error is kept for the backward pass (kLowKeys of the library)
+#: keys that a row sees up to which out's rounding error is kept for the backward pass (kLowKeys of the library)
 LOW_KEYS = 64
 _DTYPES = (torch.bfloat16, torch.float16)
 
@@ -89,10 +89,10 @@ def _planned(q, k, v, scale, key_lengths):
     return q, k, v, plan
 
 
-def new_low(q: torch.Tensor, strides, key_tokens: int, key_lengths) -> torch.Tensor | None:
+def new_low(q: torch.Tensor, strides, key_tokens: int, key_lengths, causal: bool) -> torch.Tensor | None:
     """Room for what BF16 cannot hold of the output, where the backward pass
-    may need it: batches of at most LOW_KEYS keys."""
-    if q.dtype != torch.bfloat16 or (key_lengths is None and key_tokens > LOW_KEYS):
+    may need it: rows that see at most LOW_KEYS keys."""
+    if q.dtype != torch.bfloat16 or (key_lengths is None and not causal and key_tokens > LOW_KEYS):
         return None
     return new_rows(q, q.shape, strides)
 
@@ -110,14 +110,15 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
     up to i + Tk - Tq.  A query that sees no key gives out 0 and lse -inf.
 
     with_low: (out, lse, out_low), for attention_backward: out's rounding
-    error (like out, BF16) in batches of at most 64 keys, whose gradients it
-    is the largest error of; None where no batch can have so few."""
+    error (like out, BF16) in rows that see at most 64 keys, whose gradients
+    it is the largest error of (its other rows are not written); None where no
+    row can see so few."""
     flat = isinstance(q, torch.Tensor) and q.ndim == 3
     q, k, v, (scale, _, tails, strides, out_tails) = _planned(q, k, v, scale, key_lengths)
     require_one_device("attention", q, k, v, key_lengths)
     with on_device(q):
         out = new_rows(q, q.shape, strides[0])
-        low = new_low(q, strides[0], k.shape[2], key_lengths) if with_low else None
+        low = new_low(q, strides[0], k.shape[2], key_lengths, causal) if with_low else None
         lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32)
         check(LIB.b2_attention_forward(with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]),
                                        with_base(out, out_tails[0]), scale, 1 if causal else 0, ptr(key_lengths), ptr(lse),

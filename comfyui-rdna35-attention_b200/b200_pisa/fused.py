@@ -44,7 +44,7 @@ def _forward(q, k, v, q_weight, k_weight, positions, call, with_low: bool):
     batch, heads, tokens, dim = q.shape
     with on_device(q):
         out = new_rows(q, q.shape, strides[0])
-        low = exact.new_low(q, strides[0], tokens, key_lengths) if with_low else None
+        low = exact.new_low(q, strides[0], tokens, key_lengths, causal) if with_low else None
         lse = torch.empty((batch, heads, tokens), device=q.device, dtype=torch.float32)
         saved = torch.empty(_saved_bytes(batch, heads, k.shape[1], tokens, dim)[0], device=q.device, dtype=torch.uint8)
         check(LIB.b2_norm_rope_attention_forward(

@@ -278,10 +278,10 @@ __device__ void softmax(const ForwardArgs& a, char* smem, Misc& m, uint32_t tmem
   for (int id = blockIdx.x; id < a.n_items; id += gridDim.x) {
     const Item w = decode(a, id);
     const int r = w.r0 + row;
-    const bool low = a.o_low.base != nullptr && w.len <= kLowKeys;
-    if (w.n == 0) {
+    const bool low = a.o_low.base != nullptr && r < low_rows(w.len, a.tq, a.causal, a.off);
+    if (w.n == 0) {  // no row sees a key, so all of them have a low part
       store_zeros(a.o, w.bh, w.r0 + sub * 32, a.tq, lane);
-      if (low) store_zeros(a.o_low, w.bh, w.r0 + sub * 32, a.tq, lane);
+      if (a.o_low.base != nullptr) store_zeros(a.o_low, w.bh, w.r0 + sub * 32, a.tq, lane);
       if (r < a.tq && a.lse != nullptr) a.lse[int64_t(w.bh) * a.tq + r] = -INFINITY;
       continue;
     }

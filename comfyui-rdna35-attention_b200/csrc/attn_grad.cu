@@ -993,6 +993,7 @@ struct StatArgs {
   const int32_t* key_lengths;
   int heads, kv_heads;
   int tq, tk, dim;
+  int causal;
   int q_tiles, v_blocks;
   int q_blocks;  // blocks of the query part; the rest walks V (NORMS)
 };
@@ -1068,12 +1069,13 @@ __global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_consta
       o[u] = in ? *reinterpret_cast<const uint4*>(op + u * o_step) : zero;
       d[u] = in ? *reinterpret_cast<const uint4*>(dp + u * d_step) : zero;
     }
-    if (a.out_low.base != nullptr && len <= kLowKeys) {
+    const int low_end = a.out_low.base != nullptr ? low_rows(len, a.tq, a.causal, a.tk - a.tq) : 0;
+    if (r0 < low_end) {
       const char* lp = a.out_low.row(head, r0 + g) + l * 16;
       const int64_t l_step = a.out_low.st * int64_t(16 * sizeof(T));
       uint4 low[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) low[u] = u * 16 < rows ? *reinterpret_cast<const uint4*>(lp + u * l_step) : zero;
+      for (int u = 0; u < 4; ++u) low[u] = u * 16 < min(rows, low_end - r0 - g) ? *reinterpret_cast<const uint4*>(lp + u * l_step) : zero;
 #pragma unroll
       for (int u = 0; u < 4; ++u) sum[u] = dot8<T, true>(o[u], low[u], d[u]);
     } else {
@@ -1174,6 +1176,7 @@ cudaError_t launch_attn_grad(const AttnGradCall& c, int* status, cudaStream_t st
   s.key_lengths = c.key_lengths;
   s.heads = q.heads, s.kv_heads = k.heads;
   s.tq = q.tokens, s.tk = k.tokens, s.dim = q.head_dim;
+  s.causal = c.causal;
   s.q_tiles = (q.tokens + kTile - 1) / kTile;
   s.v_blocks = (k.tokens + kStatRows - 1) / kStatRows;
   const Layout l = layout_of(bh, bhk, s.q_tiles, s.v_blocks);

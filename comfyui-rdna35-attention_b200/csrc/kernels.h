@@ -9,11 +9,18 @@ namespace b2 {
 // zeros past D and T.  False for views TMA cannot address.
 bool linear_rows_map(CUtensorMap* map, const b2_view& v, int box_rows);
 int sm_count();  // of the current device
-// Where a batch has at most this many keys, the forward pass also writes what
+// For rows that see at most this many keys, the forward pass also writes what
 // the output's type cannot hold: delta = rowsum(dout * out) then cancels
 // against few dP terms, and BF16's rounding of out would be the largest error
 // of dQ and dK (5e-3 of dQ for 2 keys, 1e-3 from 64 on).
 constexpr int kLowKeys = 64;
+// Those rows of a batch of len keys: all below the one returned (causal: row r
+// sees r + off + 1 keys).
+__host__ __device__ inline int low_rows(int len, int tq, int causal, int off) {
+  if (len <= kLowKeys) return tq;
+  const int64_t rows = causal ? int64_t(kLowKeys) - off : 0;
+  return rows < 0 ? 0 : rows < tq ? static_cast<int>(rows) : tq;
+}
 constexpr int kMaxMirrors = 7;  // peer copies of an output (head-sharded calls over up to 8 GPUs)
 // Parameters of the fused attention kernel (see attn_mma.cu).
 struct AttnParams {

@@ -315,7 +315,7 @@ int b2_fixed_block_attention_masked(const b2_view* q, const b2_view* k,
  * that sees no key gives out = 0, lse = -inf and gradient 0.
  * lse: [B,H,Tq] FP32, the natural log of the sum of exp(scale * scores); NULL
  * if not wanted.  out_low (NULL if not wanted): like out, receives out's
- * rounding error in batches of at most 64 keys, where the backward pass needs
+ * rounding error in rows that see at most 64 keys, where the backward pass needs
  * it; elsewhere it is neither written nor read. */
 int b2_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out, float scale,
                          int32_t causal, const int32_t* key_lengths, float* lse, const b2_view* out_low, void* stream);

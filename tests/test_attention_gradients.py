@@ -510,3 +510,32 @@ def test_training_step_captured_whole():
     torch.cuda.synchronize()
     got = [x.clone() for x in captured]
     assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+@gpu
+@pytest.mark.parametrize("tq,tk,lens", [(113, 113, None), (300, 300, None), (70, 200, None), (200, 70, (70, 9)), (129, 400, (400, 60))])
+def test_causal_rows_of_few_keys_keep_their_accuracy(tq, tk, lens):
+    """The first rows of a causal call see few keys, and with_low's rounding
+    error of out takes part in their gradients."""
+    import b200_pisa
+
+    q, k, v, dout = (make(2, 2, t, 64, torch.bfloat16, "bthd", i) for i, t in ((1, tq), (2, tk), (3, tk), (4, tq)))
+    lens_t = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=DEV)
+    torch.cuda.empty_cache()
+    out, lse, low = b200_pisa.attention_forward(q, k, v, causal=True, key_lengths=lens_t, with_low=True)
+    dq, dk, dv = b200_pisa.attention_backward(dout, q, k, v, out, lse, causal=True, key_lengths=lens_t, out_low=low)
+    res, allow = reference(q, k, v, dout, 0.125, True, lens_t)
+    check_all((out, dq, dk, dv), res, allow, torch.bfloat16)
+    seen = torch.arange(tq, device=DEV)[None] + 1 + tk - tq
+    limit = torch.full((2, 1), tk, device=DEV) if lens is None else lens_t[:, None]
+    few = (torch.minimum(seen.expand(2, tq), limit.long()) <= 64)[:, None, :, None].expand_as(out)
+    whole = out.double() + torch.where(few, low, torch.zeros_like(low)).double()
+    p = res["out"]
+    # P's rounding only: the row's output is exact but for 2^-9 of its P V terms
+    err = ((whole - p) * few).norm() / (p * few).norm().clamp_min(1e-30)
+    plain = ((out.double() - p) * few).norm() / (p * few).norm().clamp_min(1e-30)
+    assert not few.any() or err < 0.85 * plain
+    rows = few[..., 0]
+    if rows.any():  # as for few keys without a mask: two roundings and P's in delta
+        e = (dq.double() - res["dq"])[rows].norm() / res["dq"][rows].norm().clamp_min(1e-30)
+        assert e < 2.0 ** -8.25

@@ -29,6 +29,7 @@ from ._lib import LIB, check, ptr, stream_of, view
 from .exact import attention, attention_backward, attention_forward
 from .fused import norm_rope_attention
 from .rotary import axial_rope, qk_norm_rope, qk_norm_rope_backward
+from . import compiled as _compiled  # noqa: F401  (registers their custom ops)
 
 __version__ = "0.1.0"
 

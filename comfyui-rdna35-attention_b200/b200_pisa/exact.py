@@ -89,12 +89,14 @@ def _planned(q, k, v, scale, key_lengths):
     return q, k, v, plan
 
 
+def wants_low(dtype: torch.dtype, key_tokens: int, key_lengths, causal: bool) -> bool:
+    """Whether the backward pass may need what the type cannot hold of the
+    output: BF16, and rows that see at most LOW_KEYS keys."""
+    return dtype == torch.bfloat16 and (key_lengths is not None or causal or key_tokens <= LOW_KEYS)
+
+
 def new_low(q: torch.Tensor, strides, key_tokens: int, key_lengths, causal: bool) -> torch.Tensor | None:
-    """Room for what BF16 cannot hold of the output, where the backward pass
-    may need it: rows that see at most LOW_KEYS keys."""
-    if q.dtype != torch.bfloat16 or (key_lengths is None and not causal and key_tokens > LOW_KEYS):
-        return None
-    return new_rows(q, q.shape, strides)
+    return new_rows(q, q.shape, strides) if wants_low(q.dtype, key_tokens, key_lengths, causal) else None
 
 
 def with_optional(x: torch.Tensor | None, tail: bytes) -> bytes | None:
@@ -195,6 +197,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | 
               key_lengths: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(scale q k^T) v, differentiable in q, k and v (see
     attention_forward for the masks and layouts; scale defaults to D^-0.5)."""
+    if torch.compiler.is_compiling():
+        scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+        return torch.ops.b200_pisa.attention(q, k, v, scale, bool(causal), key_lengths)[0]
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
         return _Attention.apply(q, k, v, scale, causal, key_lengths)
     return attention_forward(q, k, v, scale, causal=causal, key_lengths=key_lengths)[0]

@@ -20,7 +20,7 @@ from ._lib import LIB, check, ptr
 
 
 @functools.lru_cache(maxsize=256)
-def _saved_bytes(batch: int, heads: int, kv_heads: int, tokens: int, dim: int) -> tuple[int, int]:
+def saved_bytes(batch: int, heads: int, kv_heads: int, tokens: int, dim: int) -> tuple[int, int]:
     sizes = (batch, heads, kv_heads, tokens, dim)
     return LIB.b2_norm_rope_attention_saved_bytes(*sizes), LIB.b2_norm_rope_attention_workspace_bytes(*sizes)
 
@@ -46,7 +46,7 @@ def _forward(q, k, v, q_weight, k_weight, positions, call, with_low: bool):
         out = new_rows(q, q.shape, strides[0])
         low = exact.new_low(q, strides[0], tokens, key_lengths, causal) if with_low else None
         lse = torch.empty((batch, heads, tokens), device=q.device, dtype=torch.float32)
-        saved = torch.empty(_saved_bytes(batch, heads, k.shape[1], tokens, dim)[0], device=q.device, dtype=torch.uint8)
+        saved = torch.empty(saved_bytes(batch, heads, k.shape[1], tokens, dim)[0], device=q.device, dtype=torch.uint8)
         check(LIB.b2_norm_rope_attention_forward(
             with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]), with_base(out, out_tails[0]),
             ptr(q_weight), ptr(k_weight), w_code, eps, with_base(positions, rot), scale, 1 if causal else 0,
@@ -63,7 +63,7 @@ def _backward(dout, q, k, v, q_weight, k_weight, positions, out, lse, low, saved
         dout, dout_view = as_rows(dout, broadcast=False)
         dq, dk, dv = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1]), new_rows(k, k.shape, strides[1])
         dwq, dwk = (torch.empty_like(w) if w is not None and weight_grads else None for w in (q_weight, k_weight))
-        ws = torch.empty(_saved_bytes(batch, heads, k.shape[1], tokens, dim)[1], device=q.device, dtype=torch.uint8)
+        ws = torch.empty(saved_bytes(batch, heads, k.shape[1], tokens, dim)[1], device=q.device, dtype=torch.uint8)
         check(LIB.b2_norm_rope_attention_backward(
             with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]), with_base(out, grad_tails[0]),
             exact.with_optional(low, grad_tails[0]), dout_view, ptr(lse),
@@ -99,6 +99,11 @@ def norm_rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     key_lengths of the attention (K rows past a batch's keys are not used,
     whatever they hold).  Differentiable in q, k, v and the weights."""
     axes_dims, theta = rotary._hashable(axes_dims, theta)
+    if torch.compiler.is_compiling():
+        scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+        return torch.ops.b200_pisa.norm_rope_attention(q, k, v, q_weight, k_weight, positions, axes_dims, scale, float(eps),
+                                                       rotary.rates(axes_dims, theta), bool(interleaved), bool(causal),
+                                                       key_lengths)[0]
     call = (axes_dims, None if scale is None else float(scale), float(eps), theta, bool(interleaved), bool(causal),
             key_lengths)
     leaves = (q, k, v, q_weight, k_weight)

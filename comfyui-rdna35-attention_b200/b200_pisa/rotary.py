@@ -54,7 +54,7 @@ def _rotary_tail(shape, pos_sig, axes_dims, theta, interleaved: bool, inverse: b
     dims = list(axes_dims)
     if not 1 <= len(dims) <= _lib.MAX_AXES or any(d <= 0 or d % 2 for d in dims) or sum(dims) > shape[-1]:
         raise ValueError(f"axes_dims must be 1..{_lib.MAX_AXES} positive even sizes that sum to at most D={shape[-1]}.")
-    thetas = list(theta) if isinstance(theta, tuple) else [theta] * len(dims)
+    thetas = rates(dims, theta)
     if len(thetas) != len(dims) or not all(0.0 < t < math.inf for t in thetas):
         raise ValueError("theta must be one positive number, or one for each axis.")
     batch, _, tokens, _ = shape
@@ -72,6 +72,11 @@ def _hashable(axes_dims, theta):
     """The rotation's sizes and rates as plain numbers, for the plan's key."""
     theta = tuple(float(t) for t in theta) if isinstance(theta, Sequence) else float(theta)
     return tuple(operator.index(d) for d in axes_dims), theta
+
+
+def rates(axes_dims, theta) -> list[float]:
+    """theta of each axis, as the custom ops take it."""
+    return list(theta) if isinstance(theta, tuple) else [theta] * len(axes_dims)
 
 
 @functools.lru_cache(maxsize=PLANS)
@@ -127,6 +132,8 @@ def axial_rope(x: torch.Tensor, positions: torch.Tensor, axes_dims: Sequence[int
     positions keep their accuracy; the result is rounded once to x's type.
     Differentiable in x."""
     rotation = (*_hashable(axes_dims, theta), bool(interleaved), bool(inverse))
+    if torch.compiler.is_compiling():
+        return torch.ops.b200_pisa.axial_rope(x, positions, rotation[0], rates(*rotation[:2]), *rotation[2:])
     if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
         return _AxialRope.apply(x, positions, *rotation)
     return _rope_call(x, positions, *rotation)
@@ -238,6 +245,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     (``axial_rope``), in one launch with one rounding at the end.
     Differentiable in q, k and the weights."""
     axes_dims, theta = _hashable(axes_dims, theta)
+    if torch.compiler.is_compiling():
+        return torch.ops.b200_pisa.qk_norm_rope(q, k, q_weight, k_weight, positions, axes_dims, float(eps),
+                                                rates(axes_dims, theta), bool(interleaved))
     args = (q, k, q_weight, k_weight, positions, axes_dims, float(eps), theta, bool(interleaved))
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in args[:4]):
         return _QkNormRope.apply(*args)

@@ -758,10 +758,10 @@ int check_attention(const b2_view* q, const b2_view* k, const b2_view* v, const 
     return fail(B2_ERR_INVALID, "scale must be representable as a positive finite float32 value.");
   if (reinterpret_cast<uintptr_t>(key_lengths) % 4) return fail(B2_ERR_INVALID, "key_lengths must be 4-byte aligned");
   const int64_t bh = int64_t(q->batch) * q->heads;
-  if (bh > 65535) return fail(B2_ERR_UNSUPPORTED, "attention supports at most 65535 (batch, head) pairs");
   if (q->tokens > (1 << 24) || k->tokens > (1 << 24))
     return fail(B2_ERR_UNSUPPORTED, "attention supports at most 2^24 tokens");
-  if (bh * (int64_t(q->tokens) + k->tokens + 256) / 64 > 0x7fffffff)
+  // 64-row tiles of queries and keys, padded to 128
+  if (bh * ((int64_t(q->tokens) + 127) / 128 + (int64_t(k->tokens) + 127) / 128) > 0x7fffffff / 2)
     return fail(B2_ERR_UNSUPPORTED, "too many tiles for one launch");
   return B2_OK;
 }
@@ -790,12 +790,12 @@ int64_t b2_attention_backward_workspace_bytes(int32_t batch, int32_t heads, int3
 
 int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
                           const b2_view* out_low, const b2_view* dout, const float* lse, const b2_view* dq,
-                          const b2_view* dk, const b2_view* dv, float scale, int32_t causal, const int32_t* key_lengths, void* workspace,
-                          void* stream) {
+                          const b2_view* dk, const b2_view* dv, float scale, int32_t causal, const int32_t* key_lengths,
+                          void* workspace, void* stream) {
   int rc = check_attention(q, k, v, out, scale, key_lengths);
   if (rc) return rc;
-  if ((out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q))) || (rc = check_grad_view(dout, "dout", q)) || (rc = check_grad_view(dq, "dq", q)) ||
-      (rc = check_grad_view(dk, "dk", k)) || (rc = check_grad_view(dv, "dv", v)))
+  if ((out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q))) || (rc = check_grad_view(dout, "dout", q)) ||
+      (rc = check_grad_view(dq, "dq", q)) || (rc = check_grad_view(dk, "dk", k)) || (rc = check_grad_view(dv, "dv", v)))
     return rc;
   if (lse == nullptr || reinterpret_cast<uintptr_t>(lse) % 4) return fail(B2_ERR_INVALID, "lse must be non-NULL");
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16)

@@ -61,7 +61,7 @@ __device__ __forceinline__ void mma16816<__half>(float* c, const uint32_t* a, ui
 template <typename T>
 __device__ __forceinline__ void issue_block_load(StatsSmem<T>& s, int stage, const Rows& q, const Rows& k,
                                                  const Rows& v, int bh, int start, int len) {
-  // 3 tensors x 64 rows x 16 vectors of 16 bytes = 3072 copies / 256 threads
+  // 3 tensors x 64 rows x 16 vectors of 16 bytes / 256 threads
   for (int idx = threadIdx.x; idx < 3 * kBlock * 16; idx += kStatsThreads) {
     const int tensor = idx / (kBlock * 16);
     const int rem = idx - tensor * kBlock * 16;

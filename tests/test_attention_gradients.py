@@ -180,7 +180,7 @@ def test_c_entries_check_their_arguments():
     assert forward(*(changed(a, dtype=_lib.B2_F32) for a in (q, k, k, q))) == unsupported
     wide = dict(head_dim=136, stride_t=136)
     assert forward(*(changed(a, **wide) for a in (q, k, k, q))) == unsupported
-    many = dict(batch=65536 // 2, stride_b=64)
+    many = dict(batch=1 << 10, heads=1 << 10, tokens=1 << 20, stride_b=64)  # more tiles than a launch has blocks
     assert forward(*(changed(a, **many) for a in (q, k, k, q))) == unsupported
     assert backward(lse=None) == invalid and backward(ws=None) == invalid and backward(ws=ctypes.c_void_p(8)) == invalid
     assert backward(dk=q) == invalid and backward(dq=changed(q, stride_t=0)) == invalid
@@ -539,3 +539,19 @@ def test_causal_rows_of_few_keys_keep_their_accuracy(tq, tk, lens):
     if rows.any():  # as for few keys without a mask: two roundings and P's in delta
         e = (dq.double() - res["dq"])[rows].norm() / res["dq"][rows].norm().clamp_min(1e-30)
         assert e < 2.0 ** -8.25
+
+
+@gpu
+def test_more_heads_than_a_grid_dimension_holds():
+    import b200_pisa
+    from b200_pisa import _lib
+
+    q, k, v, dout = (make(2, 35000, 3, 8, torch.float16, "bhtd", i) for i in range(4))
+    out, lse = b200_pisa.attention_forward(q, k, v, causal=True)
+    res, allow = reference(q, k, v, dout, 8 ** -0.5, True, None)
+    check_all((out, *b200_pisa.attention_backward(dout, q, k, v, out, lse, causal=True)), res, allow, torch.float16)
+    pos = torch.arange(3, device=DEV)[:, None]
+    fused = b200_pisa.norm_rope_attention(q, k, v, None, None, pos, (8,), causal=True)
+    some = b200_pisa.norm_rope_attention(q[1:, 34000:], k[1:, 34000:], v[1:, 34000:], None, None, pos, (8,), causal=True)
+    assert torch.equal(fused[1:, 34000:], some)
+    _lib.check_status()

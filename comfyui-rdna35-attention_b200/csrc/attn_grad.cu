@@ -44,8 +44,8 @@
 
 #include <type_traits>
 
-#include "kernels.h"
-#include "umma.cuh"
+#include "/root/repo/comfyui-rdna35-attention_b200/csrc/kernels.h"
+#include "/root/repo/comfyui-rdna35-attention_b200/csrc/umma.cuh"
 
 namespace b2 {
 
@@ -127,7 +127,7 @@ struct __align__(16) Work {
 
 struct __align__(16) Misc {
   uint64_t item_full[2], item_empty[2];
-  uint64_t own_full, own_empty;  // the item's own two tiles in shared memory
+  uint64_t own_full[2], own_empty[2];  // the item's own two tiles in shared memory
   uint64_t own_tmem;             // dQ: Q in tensor memory
   uint64_t a_full[kStagesA], a_empty[kStagesA];  // walked tiles: Q or K
   uint64_t b_full[kStagesB], b_empty[kStagesB];  // dO or V
@@ -425,8 +425,15 @@ __device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, cons
   Place<2> at, st;
   Place<kStagesA> pa;
   Place<kStagesB> pb;
-  int na = 0, nb = 0, ns = 0, owns = 0;
+  int na = 0, nb = 0, ns = 0, owns = 0, own_loads[2] = {};
   bool ok = !*abort_flag;
+  auto own_tile = [&](int which, const CUtensorMap* map, const Work& w) {
+    if (!mbar_wait(&m.own_empty[which], (owns & 1) ^ 1, abort_flag, a.status, 22)) return false;
+    mbar_expect_tx(&m.own_full[which], L::own_tile);
+    load_own<HALVES>(smem + L::own + which * L::own_tile, map, &m.own_full[which], w.r0, w.dkv ? w.hk : w.h, w.b);
+    ++own_loads[which];
+    return true;
+  };
   while (ok) {
     const int id = atomicAdd(a.counter, 1);
     if (!(ok = mbar_wait(&m.item_empty[at.s], at.ph ^ 1, abort_flag, a.status, 21))) break;
@@ -437,6 +444,8 @@ __device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, cons
     mbar_arrive(&m.item_full[at.s]);
     at.next();
     if (w.n < 0) break;
+    // Q of a dQ item first: its tile is free once the item before has Q in tensor memory
+    if (!w.dkv && w.n > 0 && !(ok = own_tile(1, q_map, w))) break;
     int g = 0, qt = w.first;  // dK/dV: head of the group and query tile
     for (int i = 0; ok && i < w.n; ++i) {
       const int h = w.hk * a.group + g;
@@ -458,11 +467,9 @@ __device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, cons
       mbar_expect_tx(&m.b_full[pb.s], L::tile);
       load_tile<HALVES>(smem + L::b + pb.s * L::tile, w.dkv ? do_map : v_map, &m.b_full[pb.s], row, head, w.b);
       pb.next(), ++nb;
-      if (i == 0) {  // the own tiles, once the item before has read its own
-        if (!(ok = mbar_wait(&m.own_empty, (owns & 1) ^ 1, abort_flag, a.status, 22))) break;
-        mbar_expect_tx(&m.own_full, 2 * L::own_tile);
-        load_own<HALVES>(smem + L::own, w.dkv ? k_map : do_map, &m.own_full, w.r0, w.dkv ? w.hk : w.h, w.b);
-        load_own<HALVES>(smem + L::own + L::own_tile, w.dkv ? v_map : q_map, &m.own_full, w.r0, w.dkv ? w.hk : w.h, w.b);
+      if (i == 0) {  // the other own tiles, once the item before has read its own
+        if (!(ok = own_tile(0, w.dkv ? k_map : do_map, w))) break;
+        if (w.dkv && !(ok = own_tile(1, v_map, w))) break;
         ++owns;
       }
       if (++qt == w.first + w.per_head) qt = w.first, ++g;
@@ -473,7 +480,8 @@ __device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, cons
     drain_loads(m.a_full, kStagesA, na, nullptr, a.status);
     drain_loads(m.b_full, kStagesB, nb, nullptr, a.status);
     drain_loads(m.stat_full, 2, ns, nullptr, a.status);
-    if (owns > 0) mbar_wait(&m.own_full, (owns - 1) & 1, &no_abort, a.status, 31);
+    for (int t = 0; t < 2; ++t)
+      if (own_loads[t] > 0) mbar_wait(&m.own_full[t], (own_loads[t] - 1) & 1, &no_abort, a.status, 31);
   }
 }
 
@@ -504,10 +512,17 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
     // the last item's products are complete: nothing is read any more from
     // the columns and tiles that this one fills
     ok = (owns == 0 || mbar_wait(&m.acc_full, (owns - 1) & 1, abort_flag, a.status, 24)) &&
-         mbar_wait(&m.own_full, owns & 1, abort_flag, a.status, 3) &&
-         (w.dkv || mbar_wait(&m.own_tmem, dqs & 1, abort_flag, a.status, 4));
+         (w.dkv ? mbar_wait(&m.own_full[0], owns & 1, abort_flag, a.status, 3) &&
+                      mbar_wait(&m.own_full[1], owns & 1, abort_flag, a.status, 3)
+                : mbar_wait(&m.own_tmem, dqs & 1, abort_flag, a.status, 4));
     if (!ok) break;
+    if (!w.dkv) mbar_arrive(&m.own_empty[1]);
     tc_fence_after();
+    auto own_read = [&](int i) {  // after dP(i): the last reads of the own tiles have been issued
+      if (i + 1 < w.n) return;
+      mma_commit(&m.own_empty[0]);
+      if (w.dkv) mma_commit(&m.own_empty[1]);
+    };
     for (int i = -1; i < w.n; ++i) {
       const uint32_t ph = (it + i) & 1, next = ph ^ 1;
       const bool more = i + 1 < w.n;
@@ -549,6 +564,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
           tc_fence_after();
           product_rows<VBF16, HALVES>(tmem + C::kDP, own1, b_rows + tb.s * step);
           mma_commit(&m.dp_full);
+          own_read(i + 1);
           tb.next();
         }
       } else if (w.dkv) {
@@ -580,6 +596,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
           tc_fence_after();
           product_rows<VBF16, HALVES>(tmem + C::kX, own1, b_rows + tb.s * step);
           mma_commit(&m.dp_full);
+          own_read(i + 1);
           tb.next();
         }
         if (i >= 0) {
@@ -597,7 +614,9 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
         // do that, and the wait it saves counts: dP(i+1) last (288 us
         // against 300 for 16 x 4096 x 64).
         auto dp = [&] {
-          if (!(ok = mbar_wait(&m.b_full[tb.s], tb.ph, abort_flag, a.status, 10))) return;
+          ok = mbar_wait(&m.b_full[tb.s], tb.ph, abort_flag, a.status, 10) &&
+               (i >= 0 || mbar_wait(&m.own_full[0], owns & 1, abort_flag, a.status, 3));
+          if (!ok) return;
           if constexpr (kDpEarly) {
             if (i >= 0 && !(ok = mbar_wait(&m.dp_read, ph, abort_flag, a.status, 11))) return;
           }
@@ -605,6 +624,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
           product_rows<VBF16, HALVES>(tmem + C::kDP, own0, b_rows + tb.s * step);
           mma_commit(&m.dp_full);
           mma_commit(&m.b_empty[tb.s]);
+          own_read(i + 1);
           tb.next(), cb.next();
         };
         if (more) {  // the elementwise warps hold S(i)
@@ -638,7 +658,6 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
     }
     if (!ok) break;
     mma_commit(&m.acc_full);
-    mma_commit(&m.own_empty);
     it += w.n;
     ++owns;
     dqs += w.dkv ? 0 : 1;
@@ -688,7 +707,7 @@ __device__ void elementwise(const GradArgs& a, char* smem, Misc& m, uint32_t tme
   };
   // Q of a dQ item (owns: the item's number among those with products)
   auto take_q = [&](int number) {
-    if (!mbar_wait(&m.own_full, number & 1, abort_flag, a.status, 27)) return false;
+    if (!mbar_wait(&m.own_full[1], number & 1, abort_flag, a.status, 27)) return false;
     row_to_tmem<HALVES>(tmem + lanes + C::kQ, smem + L::own + L::own_tile, row, cg);
     tc_fence_before();
     __syncwarp();
@@ -944,8 +963,10 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
       mbar_init(&m.b_full[s], 1);
       mbar_init(&m.b_empty[s], 1);
     }
-    mbar_init(&m.own_full, 1);
-    mbar_init(&m.own_empty, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&m.own_full[t], 1);
+      mbar_init(&m.own_empty[t], 1);
+    }
     mbar_init(&m.own_tmem, kElemWarps);
     mbar_init(&m.s_full, 1);
     mbar_init(&m.s_read, kElemWarps);

@@ -22,6 +22,13 @@
 // shared-memory bandwidth (about 3750 cycles a pair at 128 B a cycle, against
 // 7 * 512 for the products here).
 //
+// What bounds it: the products, for D > 64 and long walks (70 % of the cycles,
+// at the power limit in a run of calls: 2 x 16 x 9216^2 x 128 takes 3.48 ms in a
+// burst, 1399 TFLOP/s of the seven, 4.0 sustained); for D <= 64 the chain of a
+// tile (product, exponentials, product, dS; 16 x 4096^2 x 64: 271 us); for few
+// keys what an item costs beside its tiles, about 5000 cycles of first loads,
+// results and cold code (64 heads of 9216 queries and 512 keys: 550 us).
+//
 // The walked tiles are 128 rows for head dimensions above 64 and 64 rows up to
 // 64, where the elementwise work is what takes time: then two CTAs share an
 // SM (256 TMEM columns each), and one's exponentials run beside the other's
@@ -80,7 +87,8 @@ struct Cfg {
   static constexpr bool kDpEarly = HALVES == 2;         // dQ: dP(i+1) is issued before dQ(i)
   // TMEM columns.
   //   dK/dV: S and dP take turns in kX (each is free again as soon as the
-  //     elementwise warps have loaded it), P, dS, dV, dK.
+  //     elementwise warps have loaded it), P, dS, dV, dK; in place (below):
+  //     S, dP, dV, dK.
   //   dQ: S, dP, dQ, dS, and Q: as the A operand of S it costs no
   //     shared-memory reads there, whose 128 bytes a cycle A and B of a
   //     128 x 128 product take all of (1.53 ms against 1.69 for all of dQ).

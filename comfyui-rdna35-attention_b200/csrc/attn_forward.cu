@@ -199,12 +199,13 @@ struct Cursor {
 };
 
 // S runs up to two tiles, and into the next item, ahead of P V; whichever can
-// go out does, S first.
-template <bool BF16, bool QBF16, int HALVES>
+// go out does, S first.  STEPS: the 16-column steps of the head dimension that
+// products cover, all that it has (what pads it is zeros).
+template <bool BF16, bool QBF16, int HALVES, int STEPS>
 __device__ void issue(const ForwardArgs& a, char* smem, Misc& m, uint32_t tmem) {
   using L = Smem<HALVES>;
   constexpr uint32_t idesc_s = idesc_f16(128, kKeys, QBF16, false, false);
-  constexpr uint32_t idesc_o = idesc_f16(128, 64 * HALVES, BF16, false, true);
+  constexpr uint32_t idesc_o = idesc_f16(128, 16 * STEPS, BF16, false, true);
   volatile int* abort_flag = &m.abort_flag;
   const uint64_t q_desc = smem_desc_sw128(smem_u32(smem + L::q), 16, 1024);
   const uint64_t k_desc = smem_desc_sw128(smem_u32(smem + L::k), 16, 1024);
@@ -221,7 +222,7 @@ __device__ void issue(const ForwardArgs& a, char* smem, Misc& m, uint32_t tmem) 
         (s.j > 0 || mbar_test_wait(&m.q_full, s.own & 1)) && mbar_test_wait(&m.k_full[sk], (s.g / kStagesK) & 1)) {
       tc_fence_after();
 #pragma unroll
-      for (int kk = 0; kk < 4 * HALVES; ++kk)
+      for (int kk = 0; kk < STEPS; ++kk)
         mma_ss(tmem + kS + kKeys * (s.g & 1), q_desc + (((kk >> 2) * kRows * 128 + (kk & 3) * 32) >> 4),
                k_desc + ((sk * L::tile + (kk >> 2) * kKeys * 128 + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
       mma_commit(&m.s_full[s.g & 1]);
@@ -477,7 +478,8 @@ attn_forward_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_cons
   if (warp == 0) {
     if ((threadIdx.x & 31) == 0) produce_qk<HALVES>(&q_map, &k_map, a, smem, m);
   } else if (warp == 1) {
-    if (elect_one()) issue<BF16, BF16 && !QK16, HALVES>(a, smem, m, tmem);
+    if (elect_one())
+      with_steps<HALVES>(a.o.dim, [&](auto steps) { issue<BF16, BF16 && !QK16, HALVES, decltype(steps)::value>(a, smem, m, tmem); });
   } else if (warp == kVWarp) {
     if ((threadIdx.x & 31) == 0) produce_v<HALVES>(&v_map, a, smem, m);
   } else {

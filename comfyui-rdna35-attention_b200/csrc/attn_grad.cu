@@ -194,31 +194,33 @@ __device__ __forceinline__ void load_own(char* dst, const CUtensorMap* map, uint
 __device__ __forceinline__ uint64_t rows_desc(uint32_t addr) { return smem_desc_sw128(addr, 16, 1024); }
 __device__ __forceinline__ uint64_t cols_desc(uint32_t addr) { return smem_desc_sw128(addr, kHalfBytes, 1024); }
 
+// Products cover STEPS 16-column steps of the head dimension: all that it has
+// (what pads it to 64 or 128 columns is zeros).
 // D[128 x walk] = A B^T over the head dimension, both tiles K-major in shared memory.
-template <bool BF16, int HALVES>
+template <bool BF16, int HALVES, int STEPS>
 __device__ __forceinline__ void product_rows(uint32_t d, uint64_t a_desc, uint64_t b_desc) {
   constexpr uint32_t idesc = idesc_f16(128, Cfg<HALVES>::kWalk, BF16, false, false);
 #pragma unroll
-  for (int kk = 0; kk < 4 * HALVES; ++kk) {
+  for (int kk = 0; kk < STEPS; ++kk) {
     const uint32_t off = ((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4;
     mma_ss(d, a_desc + off, b_desc + off, idesc, kk > 0 ? 1u : 0u);
   }
 }
 
 // The same with A (16-bit pairs: 32 * HALVES columns) in tensor memory at `a`.
-template <bool BF16, int HALVES>
+template <bool BF16, int HALVES, int STEPS>
 __device__ __forceinline__ void product_rows_ts(uint32_t d, uint32_t a, uint64_t b_desc) {
   constexpr uint32_t idesc = idesc_f16(128, Cfg<HALVES>::kWalk, BF16, false, false);
 #pragma unroll
-  for (int kk = 0; kk < 4 * HALVES; ++kk)
+  for (int kk = 0; kk < STEPS; ++kk)
     mma_ts(d, a + kk * 8, b_desc + (((kk >> 2) * kHalfBytes + (kk & 3) * 32) >> 4), idesc, kk > 0 ? 1u : 0u);
 }
 
 // D[128 x D] (+)= A B with A (128 x walk, 16-bit pairs) in tensor memory at
 // `a`, B's rows as contraction.
-template <bool BF16, int HALVES, bool IN_PLACE = false>
+template <bool BF16, int HALVES, int STEPS, bool IN_PLACE = false>
 __device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint64_t b_desc, bool accumulate) {
-  constexpr uint32_t idesc = idesc_f16(128, 64 * HALVES, BF16, false, true);
+  constexpr uint32_t idesc = idesc_f16(128, 16 * STEPS, BF16, false, true);
 #pragma unroll
   for (int kk = 0; kk < Cfg<HALVES>::kWalk / 16; ++kk)
     mma_ts(d, a + (IN_PLACE ? (kk >> 1) * 32 + (kk & 1) * 8 : kk * 8), b_desc + kk * (2048 >> 4), idesc, kk > 0 ? 1u : accumulate ? 1u : 0u);
@@ -494,7 +496,7 @@ __device__ void produce(const CUtensorMap* q_map, const CUtensorMap* k_map, cons
 }
 
 // ------------------------------------------------------------ MMA issuer
-template <bool VBF16, bool QBF16, int HALVES>
+template <bool VBF16, bool QBF16, int HALVES, int STEPS>
 __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
   using L = Smem<HALVES>;
   using C = Cfg<HALVES>;
@@ -543,7 +545,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i > 0 || owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 25));
           if (!ok) break;
           tc_fence_after();
-          product_cols<VBF16, HALVES, true>(tmem + C::kDV, tmem + C::kS, b_cols + cb.s * step, i > 0);
+          product_cols<VBF16, HALVES, STEPS, true>(tmem + C::kDV, tmem + C::kS, b_cols + cb.s * step, i > 0);
           mma_commit(&m.b_empty[cb.s]);
           mma_commit(&m.dv_done);
           cb.next();
@@ -553,14 +555,14 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i < 0 || mbar_wait(&m.dv_done, ph, abort_flag, a.status, 8));
           if (!ok) break;
           tc_fence_after();
-          product_rows<QBF16, HALVES>(tmem + C::kS, own0, a_rows + ta.s * step);
+          product_rows<QBF16, HALVES, STEPS>(tmem + C::kS, own0, a_rows + ta.s * step);
           mma_commit(&m.s_full);
           ta.next();
         }
         if (i >= 0) {
           if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
           tc_fence_after();
-          product_cols<QBF16, HALVES, true>(tmem + C::kDK, tmem + C::kDP, a_cols + ca.s * step, i > 0);
+          product_cols<QBF16, HALVES, STEPS, true>(tmem + C::kDK, tmem + C::kDP, a_cols + ca.s * step, i > 0);
           mma_commit(&m.dk_done);
           mma_commit(&m.a_empty[ca.s]);
           ca.next();
@@ -570,7 +572,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i < 0 || mbar_wait(&m.dk_done, ph, abort_flag, a.status, 11));
           if (!ok) break;
           tc_fence_after();
-          product_rows<VBF16, HALVES>(tmem + C::kDP, own1, b_rows + tb.s * step);
+          product_rows<VBF16, HALVES, STEPS>(tmem + C::kDP, own1, b_rows + tb.s * step);
           mma_commit(&m.dp_full);
           own_read(i + 1);
           tb.next();
@@ -584,7 +586,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i < 0 || mbar_wait(&m.dp_read, ph, abort_flag, a.status, 8));
           if (!ok) break;
           tc_fence_after();
-          product_rows<QBF16, HALVES>(tmem + C::kX, own0, a_rows + ta.s * step);
+          product_rows<QBF16, HALVES, STEPS>(tmem + C::kX, own0, a_rows + ta.s * step);
           mma_commit(&m.s_full);
           ta.next();
         }
@@ -593,7 +595,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i > 0 || owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 25));
           if (!ok) break;
           tc_fence_after();
-          product_cols<VBF16, HALVES>(tmem + C::kDV, tmem + C::kP, b_cols + cb.s * step, i > 0);
+          product_cols<VBF16, HALVES, STEPS>(tmem + C::kDV, tmem + C::kP, b_cols + cb.s * step, i > 0);
           mma_commit(&m.b_empty[cb.s]);
           cb.next();
         }
@@ -602,7 +604,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                mbar_wait(&m.s_read, next, abort_flag, a.status, 11);
           if (!ok) break;
           tc_fence_after();
-          product_rows<VBF16, HALVES>(tmem + C::kX, own1, b_rows + tb.s * step);
+          product_rows<VBF16, HALVES, STEPS>(tmem + C::kX, own1, b_rows + tb.s * step);
           mma_commit(&m.dp_full);
           own_read(i + 1);
           tb.next();
@@ -610,7 +612,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
         if (i >= 0) {
           if (!(ok = mbar_wait(&m.ds_full, ph, abort_flag, a.status, 9))) break;
           tc_fence_after();
-          product_cols<QBF16, HALVES>(tmem + C::kDK, tmem + C::kDS, a_cols + ca.s * step, i > 0);
+          product_cols<QBF16, HALVES, STEPS>(tmem + C::kDK, tmem + C::kDS, a_cols + ca.s * step, i > 0);
           mma_commit(&m.dk_done);
           mma_commit(&m.a_empty[ca.s]);
           ca.next();
@@ -629,7 +631,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
             if (i >= 0 && !(ok = mbar_wait(&m.dp_read, ph, abort_flag, a.status, 11))) return;
           }
           tc_fence_after();
-          product_rows<VBF16, HALVES>(tmem + C::kDP, own0, b_rows + tb.s * step);
+          product_rows<VBF16, HALVES, STEPS>(tmem + C::kDP, own0, b_rows + tb.s * step);
           mma_commit(&m.dp_full);
           mma_commit(&m.b_empty[tb.s]);
           own_read(i + 1);
@@ -640,7 +642,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i < 0 || mbar_wait(&m.s_read, ph, abort_flag, a.status, 8));
           if (!ok) break;
           tc_fence_after();
-          product_rows_ts<QBF16, HALVES>(tmem + C::kS, tmem + C::kQ, a_rows + ta.s * step);
+          product_rows_ts<QBF16, HALVES, STEPS>(tmem + C::kS, tmem + C::kQ, a_rows + ta.s * step);
           mma_commit(&m.s_full);
           ta.next();
         }
@@ -653,7 +655,7 @@ __device__ void issue(const GradArgs& a, char* smem, Misc& m, uint32_t tmem) {
                (i > 0 || owns == 0 || mbar_wait(&m.acc_free, (owns - 1) & 1, abort_flag, a.status, 25));
           if (!ok) break;
           tc_fence_after();
-          product_cols<QBF16, HALVES>(tmem + C::kDQ, tmem + C::kDSq, a_cols + ca.s * step, i > 0);
+          product_cols<QBF16, HALVES, STEPS>(tmem + C::kDQ, tmem + C::kDSq, a_cols + ca.s * step, i > 0);
           if constexpr (kDpEarly) mma_commit(&m.dk_done);
           mma_commit(&m.a_empty[ca.s]);
           ca.next();
@@ -999,7 +1001,8 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constan
   if (warp == 0) {
     if ((threadIdx.x & 31) == 0) produce<HALVES>(&q_map, &k_map, &v_map, &do_map, a, smem, m);
   } else if (warp == 1) {
-    if (elect_one()) issue<VBF16, QBF16, HALVES>(a, smem, m, tmem);
+    if (elect_one())
+      with_steps<HALVES>(a.dim, [&](auto steps) { issue<VBF16, QBF16, HALVES, decltype(steps)::value>(a, smem, m, tmem); });
   } else {
     elementwise<VBF16, QBF16, OUT32, HALVES>(a, smem, m, tmem);
   }

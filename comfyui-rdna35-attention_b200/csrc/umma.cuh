@@ -17,6 +17,8 @@
 #include <cuda.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace b2 {
@@ -267,6 +269,21 @@ __device__ __forceinline__ void transpose_quads(uint32_t (&w)[16], int lane) {
       }
     }
   }
+}
+
+// f with the 16-column steps that a head dimension of `dim` needs, as a constant:
+// the last four of 4 * HALVES.  Products of these alone instead of 64 * HALVES
+// columns: backward of 16 x 4096^2, D = 40: 265 us against 279, 80: 320 against
+// 358, 96: 337 against 369.  (A branch at each MMA instead of four copies of the
+// issuing code cost 11 % of the forward pass at D = 128.)
+template <int HALVES, typename F>
+__device__ __forceinline__ void with_steps(int dim, F&& f) {
+  constexpr int kMost = 4 * HALVES;
+  const int steps = (dim + 15) >> 4;
+  if (steps >= kMost) f(std::integral_constant<int, kMost>{});
+  else if (steps == kMost - 1) f(std::integral_constant<int, kMost - 1>{});
+  else if (steps == kMost - 2) f(std::integral_constant<int, kMost - 2>{});
+  else f(std::integral_constant<int, kMost - 3>{});
 }
 
 __device__ __forceinline__ float ex2(float x) {

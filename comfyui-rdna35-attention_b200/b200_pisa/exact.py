@@ -103,6 +103,19 @@ def with_optional(x: torch.Tensor | None, tail: bytes) -> bytes | None:
     return None if x is None else with_base(x, tail)
 
 
+def _run_forward(q, k, v, plan, causal: bool, key_lengths, with_low: bool):
+    """The pass on checked four-dimensional tensors."""
+    scale, _, tails, strides, out_tails = plan
+    with on_device(q):
+        out = new_rows(q, q.shape, strides[0])
+        low = new_low(q, strides[0], k.shape[2], key_lengths, causal) if with_low else None
+        lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32)
+        check(LIB.b2_attention_forward(with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]),
+                                       with_base(out, out_tails[0]), scale, 1 if causal else 0, ptr(key_lengths),
+                                       ptr(lse), with_optional(low, out_tails[0]), raw_stream(q)))
+    return out, lse, low
+
+
 def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None, *,
                       causal: bool = False, key_lengths: torch.Tensor | None = None, with_low: bool = False):
     """(out, lse) of softmax(scale q k^T) v: out like q, lse FP32 [B,H,Tq]
@@ -116,15 +129,9 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
     it is the largest error of (its other rows are not written); None where no
     row can see so few."""
     flat = isinstance(q, torch.Tensor) and q.ndim == 3
-    q, k, v, (scale, _, tails, strides, out_tails) = _planned(q, k, v, scale, key_lengths)
+    q, k, v, plan = _planned(q, k, v, scale, key_lengths)
     require_one_device("attention", q, k, v, key_lengths)
-    with on_device(q):
-        out = new_rows(q, q.shape, strides[0])
-        low = new_low(q, strides[0], k.shape[2], key_lengths, causal) if with_low else None
-        lse = torch.empty(q.shape[:3], device=q.device, dtype=torch.float32)
-        check(LIB.b2_attention_forward(with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]),
-                                       with_base(out, out_tails[0]), scale, 1 if causal else 0, ptr(key_lengths), ptr(lse),
-                                       with_optional(low, out_tails[0]), raw_stream(q)))
+    out, lse, low = _run_forward(q, k, v, plan, causal, key_lengths, with_low)
     if flat:
         out, lse, low = out.squeeze(1), lse.squeeze(1), None if low is None else low.squeeze(1)
     return (out, lse, low) if with_low else (out, lse)
@@ -151,6 +158,22 @@ def check_saved(q: torch.Tensor, flat: bool, lse, **rows) -> list:
     return got
 
 
+def _run_backward(dout, q, k, v, out, lse, low, plan, causal: bool, key_lengths):
+    scale, _, tails, strides, grad_tails = plan
+    batch, heads, tokens, _ = q.shape
+    with on_device(q):
+        (out, out_view), (dout, dout_view) = as_rows(out, broadcast=False), as_rows(dout, broadcast=False)
+        low, low_view = (None, None) if low is None else as_rows(low, broadcast=False)
+        dq, dk, dv = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1]), new_rows(k, k.shape, strides[1])
+        ws = torch.empty(_workspace_bytes(batch, heads, k.shape[1], tokens, k.shape[2]), device=q.device,
+                         dtype=torch.uint8)
+        check(LIB.b2_attention_backward(
+            with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]), out_view, low_view, dout_view,
+            ptr(lse), with_base(dq, grad_tails[0]), with_base(dk, grad_tails[1]), with_base(dv, grad_tails[1]), scale,
+            1 if causal else 0, ptr(key_lengths), ptr(ws), raw_stream(q)))
+    return dq, dk, dv
+
+
 def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
                        lse: torch.Tensor, scale: float | None = None, *, causal: bool = False,
                        key_lengths: torch.Tensor | None = None, out_low: torch.Tensor | None = None):
@@ -159,38 +182,33 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     from lse; dk and dv of a shared head are summed over its group in FP32;
     rows of dk and dv past a batch's keys are 0.  Bit-reproducible."""
     flat = isinstance(q, torch.Tensor) and q.ndim == 3
-    q, k, v, (scale, _, tails, strides, grad_tails) = _planned(q, k, v, scale, key_lengths)
+    q, k, v, plan = _planned(q, k, v, scale, key_lengths)
     out, dout, out_low = check_saved(q, flat, lse, out=out, dout=dout, out_low=out_low)
     require_one_device("attention_backward", q, k, v, key_lengths, out, dout, lse, out_low)
-    batch, heads, tokens, _ = q.shape
     with on_device(q):
-        (out, out_view), (dout, dout_view) = as_rows(out, broadcast=False), as_rows(dout, broadcast=False)
-        low, low_view = (None, None) if out_low is None else as_rows(out_low, broadcast=False)
         lse = lse.contiguous()
-        dq, dk, dv = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1]), new_rows(k, k.shape, strides[1])
-        ws = torch.empty(_workspace_bytes(batch, heads, k.shape[1], tokens, k.shape[2]), device=q.device, dtype=torch.uint8)
-        check(LIB.b2_attention_backward(
-            with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]),
-            out_view, low_view, dout_view, ptr(lse), with_base(dq, grad_tails[0]), with_base(dk, grad_tails[1]),
-            with_base(dv, grad_tails[1]), scale, 1 if causal else 0, ptr(key_lengths), ptr(ws), raw_stream(q)))
-    return (dq.squeeze(1), dk.squeeze(1), dv.squeeze(1)) if flat else (dq, dk, dv)
+    grads = _run_backward(dout, q, k, v, out, lse, out_low, plan, causal, key_lengths)
+    return tuple(g.squeeze(1) for g in grads) if flat else grads
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, causal, key_lengths):
-        out, lse, low = attention_forward(q, k, v, scale, causal=causal, key_lengths=key_lengths, with_low=True)
+        flat = q.ndim == 3
+        q, k, v, plan = _planned(q, k, v, scale, key_lengths)
+        require_one_device("attention", q, k, v, key_lengths)
+        out, lse, low = _run_forward(q, k, v, plan, causal, key_lengths, True)
         ctx.save_for_backward(q, k, v, out, lse, low, key_lengths)
-        ctx.call = (scale, causal)
-        return out
+        ctx.call = (plan, causal, flat)
+        return out.squeeze(1) if flat else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, low, key_lengths = ctx.saved_tensors
-        scale, causal = ctx.call
-        grads = attention_backward(dout, q, k, v, out, lse, scale, causal=causal, key_lengths=key_lengths, out_low=low)
-        return (*grads, None, None, None)
+        plan, causal, flat = ctx.call
+        grads = _run_backward(dout.unsqueeze(1) if flat else dout, q, k, v, out, lse, low, plan, causal, key_lengths)
+        return (*(g.squeeze(1) if flat else g for g in grads), None, None, None)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None, *, causal: bool = False,

@@ -37,10 +37,15 @@ def _checked(q, k, v, q_weight, k_weight, positions, call):
 
 
 def _forward(q, k, v, q_weight, k_weight, positions, call, with_low: bool):
+    q, k, v, *plans = _checked(q, k, v, q_weight, k_weight, positions, call)
+    require_one_device("norm_rope_attention", q, k, v, q_weight, k_weight, positions, call[-1])
+    return _run_forward(q, k, v, q_weight, k_weight, positions, call, plans, with_low)
+
+
+def _run_forward(q, k, v, q_weight, k_weight, positions, call, plans, with_low: bool):
+    """The pass on checked tensors."""
     _, _, eps, _, _, causal, key_lengths = call
-    q, k, v, (rot, _, _, _, w_code), (scale, _, tails, strides, out_tails) = _checked(q, k, v, q_weight, k_weight,
-                                                                                       positions, call)
-    require_one_device("norm_rope_attention", q, k, v, q_weight, k_weight, positions, key_lengths)
+    (rot, _, _, _, w_code), (scale, _, tails, strides, out_tails) = plans
     batch, heads, tokens, dim = q.shape
     with on_device(q):
         out = new_rows(q, q.shape, strides[0])
@@ -55,9 +60,13 @@ def _forward(q, k, v, q_weight, k_weight, positions, call, with_low: bool):
 
 
 def _backward(dout, q, k, v, q_weight, k_weight, positions, out, lse, low, saved, call, weight_grads: bool):
+    q, k, v, *plans = _checked(q, k, v, q_weight, k_weight, positions, call)
+    return _run_backward(dout, q, k, v, q_weight, k_weight, positions, out, lse, low, saved, call, plans, weight_grads)
+
+
+def _run_backward(dout, q, k, v, q_weight, k_weight, positions, out, lse, low, saved, call, plans, weight_grads: bool):
     _, _, eps, _, _, causal, key_lengths = call
-    q, k, v, (rot, _, _, _, w_code), (scale, _, tails, strides, grad_tails) = _checked(q, k, v, q_weight, k_weight,
-                                                                                        positions, call)
+    (rot, _, _, _, w_code), (scale, _, tails, strides, grad_tails) = plans
     batch, heads, tokens, dim = q.shape
     with on_device(q):
         dout, dout_view = as_rows(dout, broadcast=False)
@@ -76,9 +85,11 @@ def _backward(dout, q, k, v, q_weight, k_weight, positions, out, lse, low, saved
 class _NormRopeAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_weight, k_weight, positions, call):
-        out, lse, low, saved = _forward(q, k, v, q_weight, k_weight, positions, call, True)
+        q, k, v, *plans = _checked(q, k, v, q_weight, k_weight, positions, call)
+        require_one_device("norm_rope_attention", q, k, v, q_weight, k_weight, positions, call[-1])
+        out, lse, low, saved = _run_forward(q, k, v, q_weight, k_weight, positions, call, plans, True)
         ctx.save_for_backward(q, k, v, q_weight, k_weight, positions, out, lse, low, saved, call[-1])
-        ctx.call = call[:-1]
+        ctx.call, ctx.plans = call[:-1], plans
         return out
 
     @staticmethod
@@ -86,7 +97,7 @@ class _NormRopeAttention(torch.autograd.Function):
     def backward(ctx, dout):
         *tensors, key_lengths = ctx.saved_tensors
         wanted = ctx.needs_input_grad[3] or ctx.needs_input_grad[4]
-        return (*_backward(dout, *tensors, (*ctx.call, key_lengths), wanted), None, None)
+        return (*_run_backward(dout, *tensors, (*ctx.call, key_lengths), ctx.plans, wanted), None, None)
 
 
 def norm_rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor | None,

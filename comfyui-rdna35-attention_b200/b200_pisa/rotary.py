@@ -182,8 +182,12 @@ def _plan_of(q, k, q_weight, k_weight, positions, axes_dims, eps, theta, interle
 
 
 def _norm_rope_call(q, k, q_weight, k_weight, positions, axes_dims, eps, theta, interleaved):
-    rot, tails, out_tails, strides, w_code = _plan_of(q, k, q_weight, k_weight, positions, axes_dims, eps, theta,
-                                                      interleaved)
+    plan = _plan_of(q, k, q_weight, k_weight, positions, axes_dims, eps, theta, interleaved)
+    return _run_norm_rope(q, k, q_weight, k_weight, positions, eps, plan)
+
+
+def _run_norm_rope(q, k, q_weight, k_weight, positions, eps, plan):
+    rot, tails, out_tails, strides, w_code = plan
     require_one_device("qk_norm_rope", q, k, q_weight, k_weight, positions)
     with on_device(q):
         q_out, k_out = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1])
@@ -191,6 +195,28 @@ def _norm_rope_call(q, k, q_weight, k_weight, positions, axes_dims, eps, theta, 
                                   with_base(k_out, out_tails[1]), ptr(q_weight), ptr(k_weight), w_code, eps,
                                   with_base(positions, rot), raw_stream(q)))
     return q_out, k_out
+
+
+def _run_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, eps, plan, weight_grads: bool):
+    """The pass on checked tensors."""
+    rot, tails, out_tails, strides, w_code = plan
+    with on_device(q):
+        (dq_out, dq_view), (dk_out, dk_view) = as_rows(dq_out), as_rows(dk_out)
+        dq, dk = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1])
+        dwq, dwk = (torch.empty_like(w) if w is not None and weight_grads else None for w in (q_weight, k_weight))
+        ws = None
+        if dwq is not None or dwk is not None:
+            ws = torch.empty(_workspace_bytes(q.shape[-1]), device=q.device, dtype=torch.uint8)
+        check(LIB.b2_qk_norm_rope_backward(
+            with_base(q, tails[0]), with_base(k, tails[1]), dq_view, dk_view, with_base(dq, out_tails[0]),
+            with_base(dk, out_tails[1]), ptr(q_weight), ptr(k_weight), w_code, eps, with_base(positions, rot), ptr(dwq),
+            ptr(dwk), ptr(ws), raw_stream(q)))
+    return dq, dk, dwq, dwk
+
+
+@functools.lru_cache(maxsize=PLANS)
+def _workspace_bytes(dim: int) -> int:
+    return LIB.b2_qk_norm_rope_workspace_bytes(dim)
 
 
 def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
@@ -202,38 +228,27 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     None without weights or with weight_grads=False.  The statistics are
     recomputed from q and k.  Bit-reproducible."""
     axes_dims, theta = _hashable(axes_dims, theta)
-    rot, tails, out_tails, strides, w_code = _plan_of(q, k, q_weight, k_weight, positions, axes_dims, float(eps), theta,
-                                                      bool(interleaved))
+    plan = _plan_of(q, k, q_weight, k_weight, positions, axes_dims, float(eps), theta, bool(interleaved))
     for name, dy, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
         if not isinstance(dy, torch.Tensor) or dy.shape != x.shape or dy.dtype != x.dtype:
             raise ValueError(f"{name} must be a tensor of its output's shape and dtype.")
     require_one_device("qk_norm_rope_backward", q, k, q_weight, k_weight, positions, dq_out, dk_out)
-    with on_device(q):
-        (dq_out, dq_view), (dk_out, dk_view) = as_rows(dq_out), as_rows(dk_out)
-        dq, dk = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1])
-        dwq, dwk = (torch.empty_like(w) if w is not None and weight_grads else None for w in (q_weight, k_weight))
-        ws = None
-        if dwq is not None or dwk is not None:
-            ws = torch.empty(LIB.b2_qk_norm_rope_workspace_bytes(q.shape[-1]), device=q.device, dtype=torch.uint8)
-        check(LIB.b2_qk_norm_rope_backward(
-            with_base(q, tails[0]), with_base(k, tails[1]), dq_view, dk_view, with_base(dq, out_tails[0]),
-            with_base(dk, out_tails[1]), ptr(q_weight), ptr(k_weight), w_code, float(eps), with_base(positions, rot),
-            ptr(dwq), ptr(dwk), ptr(ws), raw_stream(q)))
-    return dq, dk, dwq, dwk
+    return _run_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, positions, float(eps), plan, weight_grads)
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, axes_dims, eps, theta, interleaved):
         ctx.save_for_backward(q, k, q_weight, k_weight, positions)
-        ctx.rotation = dict(axes_dims=axes_dims, eps=eps, theta=theta, interleaved=interleaved)
-        return _norm_rope_call(q, k, q_weight, k_weight, positions, axes_dims, eps, theta, interleaved)
+        plan = _plan_of(q, k, q_weight, k_weight, positions, axes_dims, eps, theta, interleaved)
+        ctx.call = (eps, plan)
+        return _run_norm_rope(q, k, q_weight, k_weight, positions, eps, plan)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
         wanted = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
-        grads = qk_norm_rope_backward(dq_out, dk_out, *ctx.saved_tensors, weight_grads=wanted, **ctx.rotation)
+        grads = _run_norm_rope_backward(dq_out, dk_out, *ctx.saved_tensors, *ctx.call, wanted)
         return (*grads, None, None, None, None, None)
 
 

@@ -194,7 +194,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, causal, key_lengths):
-        flat = q.ndim == 3
+        flat = isinstance(q, torch.Tensor) and q.ndim == 3
         q, k, v, plan = _planned(q, k, v, scale, key_lengths)
         require_one_device("attention", q, k, v, key_lengths)
         out, lse, low = _run_forward(q, k, v, plan, causal, key_lengths, True)

@@ -328,7 +328,8 @@ int64_t b2_attention_backward_workspace_bytes(int32_t batch, int32_t heads, int3
                                               int32_t k_tokens);
 int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, const b2_view* out,
                           const b2_view* out_low, const b2_view* dout, const float* lse, const b2_view* dq,
-                          const b2_view* dk, const b2_view* dv, float scale, int32_t causal, const int32_t* key_lengths, void* workspace,
+                          const b2_view* dk, const b2_view* dv, float scale, int32_t causal,
+                          const int32_t* key_lengths, void* workspace,
                           void* stream);
 
 /* ---- Per-head RMS norm of queries and keys and rotary positions with several

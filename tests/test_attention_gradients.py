@@ -555,3 +555,12 @@ def test_more_heads_than_a_grid_dimension_holds():
     some = b200_pisa.norm_rope_attention(q[1:, 34000:], k[1:, 34000:], v[1:, 34000:], None, None, pos, (8,), causal=True)
     assert torch.equal(fused[1:, 34000:], some)
     _lib.check_status()
+
+
+def test_wrong_types_are_refused_with_gradients_wanted_too():
+    import b200_pisa
+
+    x = _x(1, 2, 4, 16).requires_grad_()
+    for args in ((None, x, x), (x, 3.0, x), (x, x, "v")):
+        with pytest.raises(TypeError):
+            b200_pisa.attention(*args)

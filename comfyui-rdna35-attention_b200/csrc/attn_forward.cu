@@ -18,8 +18,10 @@
 //
 // What bounds it: the softmax chain of a tile (load S, maximum, exponentials,
 // store P), which two CTAs overlap; tensor and exponential pipes are each half
-// used.  2 x 16 x 9216^2 x 128: 1.265 ms, 1100 TFLOP/s (a CTA an item: 1.455);
-// 64 heads of 9216 queries and 512 keys: 204 us (249).
+// used.  2 x 16 x 9216^2 x 128: 1.22 ms, 1141 TFLOP/s (a CTA an item: 1.455);
+// 64 heads of 9216 queries and 512 keys: 197 us (249).  Three CTAs per SM with
+// one S buffer and half a row's logits in registers, for D <= 64: 211 us
+// against 133 (16 x 4096^2 x 64).
 #include <cudaTypedefs.h>
 
 #include <type_traits>
@@ -305,30 +307,26 @@ __device__ void softmax(const ForwardArgs& a, char* smem, Misc& m, uint32_t tmem
       // logits in the log2 domain, masked ones -inf; unmasked tiles keep raw S
       // and fold the scale into the argument of the exponential
       const int k0 = j * kKeys, klen = min(kKeys, w.len - k0);
-      float mul = scale_log2, mx;
-      if (klen == kKeys && (!a.causal || last - k0 >= kKeys - 1)) {
-        float m0 = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
-        float m1 = fmaxf(__uint_as_float(v[2]), __uint_as_float(v[3]));
-#pragma unroll
-        for (int c = 4; c < kKeys; c += 4) {
-          m0 = max3(m0, __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
-          m1 = max3(m1, __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
-        }
-        mx = fmaxf(m0, m1) * scale_log2;
-      } else {
+      const bool plain = klen == kKeys && (!a.causal || last - k0 >= kKeys - 1);
+      if (!plain) {
         uint64_t bad = klen < kKeys ? ~0ull << klen : 0ull;
         if (a.causal && last - k0 < kKeys - 1) bad |= last < k0 ? ~0ull : ~0ull << (last - k0 + 1);
-        const uint32_t bad0 = static_cast<uint32_t>(bad), bad1 = static_cast<uint32_t>(bad >> 32);
-        mx = -INFINITY;
 #pragma unroll
         for (int c = 0; c < kKeys; ++c) {
+          const uint32_t word = static_cast<uint32_t>(c < 32 ? bad : bad >> 32);
           const float x = __uint_as_float(v[c]) * scale_log2;
-          const float xm = (((c < 32 ? bad0 : bad1) >> (c & 31)) & 1u) ? -INFINITY : x;
-          v[c] = __float_as_uint(xm);
-          mx = fmaxf(mx, xm);
+          v[c] = (word >> (c & 31)) & 1u ? __float_as_uint(-INFINITY) : __float_as_uint(x);
         }
-        mul = 1.f;
       }
+      const float mul = plain ? scale_log2 : 1.f;
+      float m0 = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
+      float m1 = fmaxf(__uint_as_float(v[2]), __uint_as_float(v[3]));
+#pragma unroll
+      for (int c = 4; c < kKeys; c += 4) {
+        m0 = max3(m0, __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
+        m1 = max3(m1, __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
+      }
+      const float mx = fmaxf(m0, m1) * mul;
       float alpha = 1.f;
       bool rescale = false;
       const float mnew = fmaxf(mrun, mx);

@@ -51,8 +51,8 @@
 
 #include <type_traits>
 
-#include "/root/repo/comfyui-rdna35-attention_b200/csrc/kernels.h"
-#include "/root/repo/comfyui-rdna35-attention_b200/csrc/umma.cuh"
+#include "kernels.h"
+#include "umma.cuh"
 
 namespace b2 {
 

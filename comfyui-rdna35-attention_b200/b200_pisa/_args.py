@@ -120,3 +120,35 @@ def as_rows(x: torch.Tensor, broadcast: bool = True) -> tuple[torch.Tensor, byte
         x = x.clone(memory_format=torch.contiguous_format) if x.data_ptr() % 16 else x.contiguous()
         tail = view_tail(*signature(x))
     return x, with_base(x, tail)
+
+
+def layouts(*tensors: torch.Tensor | None):
+    """What came_back() compares."""
+    return tuple(None if x is None else signature(x) for x in tensors)
+
+
+def came_back(name: str, tensors, were) -> bool:
+    """Whether the tensors that a forward pass saved came back to its backward
+    pass laid out as they ``were``, so that the forward pass's plan holds for
+    them.  Saved-tensor hooks (offloading, compression) may return copies with
+    other strides or off the 16-byte boundaries; copies of another shape or
+    type are refused."""
+    same = True
+    for x, was in zip(tensors, were):
+        if was is None:
+            continue
+        now = signature(x)
+        if now != was:
+            if now[0] != was[0] or now[2] != was[2]:
+                raise ValueError(f"{name}: a saved tensor came back with another shape or dtype.")
+            same = False
+        elif x.data_ptr() % 16:
+            same = False
+    return same
+
+
+def dense(x: torch.Tensor | None, alignment: int = 1) -> torch.Tensor | None:
+    """x itself if contiguous from a multiple of ``alignment``, else a copy that is."""
+    if x is None or (x.is_contiguous() and x.data_ptr() % alignment == 0):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)

@@ -17,8 +17,8 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._args import (PLANS, addressable, as_rows, new_rows, on_device, raw_stream, repeats, require_one_device, signature,
-                    token_major_strides, view_tail, with_base)
+from ._args import (PLANS, addressable, as_rows, came_back, dense, layouts, new_rows, on_device, raw_stream, repeats,
+                    require_one_device, signature, token_major_strides, view_tail, with_base)
 from ._lib import LIB, check, ptr
 
 MAX_HEAD_DIM = 128
@@ -164,6 +164,7 @@ def _run_backward(dout, q, k, v, out, lse, low, plan, causal: bool, key_lengths)
     with on_device(q):
         (out, out_view), (dout, dout_view) = as_rows(out, broadcast=False), as_rows(dout, broadcast=False)
         low, low_view = (None, None) if low is None else as_rows(low, broadcast=False)
+        lse = dense(lse)
         dq, dk, dv = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1]), new_rows(k, k.shape, strides[1])
         ws = torch.empty(_workspace_bytes(batch, heads, k.shape[1], tokens, k.shape[2]), device=q.device,
                          dtype=torch.uint8)
@@ -185,8 +186,6 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     q, k, v, plan = _planned(q, k, v, scale, key_lengths)
     out, dout, out_low = check_saved(q, flat, lse, out=out, dout=dout, out_low=out_low)
     require_one_device("attention_backward", q, k, v, key_lengths, out, dout, lse, out_low)
-    with on_device(q):
-        lse = lse.contiguous()
     grads = _run_backward(dout, q, k, v, out, lse, out_low, plan, causal, key_lengths)
     return tuple(g.squeeze(1) for g in grads) if flat else grads
 
@@ -198,16 +197,24 @@ class _Attention(torch.autograd.Function):
         q, k, v, plan = _planned(q, k, v, scale, key_lengths)
         require_one_device("attention", q, k, v, key_lengths)
         out, lse, low = _run_forward(q, k, v, plan, causal, key_lengths, True)
-        ctx.save_for_backward(q, k, v, out, lse, low, key_lengths)
-        ctx.call = (plan, causal, flat)
+        saved = (q, k, v, out, lse, low, key_lengths)
+        ctx.save_for_backward(*saved)
+        ctx.call = (plan, causal, flat, layouts(*saved))
         return out.squeeze(1) if flat else out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse, low, key_lengths = ctx.saved_tensors
-        plan, causal, flat = ctx.call
-        grads = _run_backward(dout.unsqueeze(1) if flat else dout, q, k, v, out, lse, low, plan, causal, key_lengths)
+        saved = ctx.saved_tensors  # each access unpacks them anew
+        q, k, v, out, lse, low, key_lengths = saved
+        plan, causal, flat, were = ctx.call
+        dout = dout.unsqueeze(1) if flat else dout
+        require_one_device("attention", *saved, dout)
+        if not came_back("attention", saved, were):
+            q, k, v = (as_rows(x, broadcast=False)[0] for x in (q, k, v))
+            key_lengths = dense(key_lengths)
+            q, k, v, plan = _planned(q, k, v, plan[0], key_lengths)
+        grads = _run_backward(dout, q, k, v, out, lse, low, plan, causal, key_lengths)
         return (*(g.squeeze(1) if flat else g for g in grads), None, None, None)
 
 

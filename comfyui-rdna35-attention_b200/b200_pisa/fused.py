@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import exact, rotary
-from ._args import as_rows, new_rows, on_device, raw_stream, require_one_device, with_base
+from ._args import as_rows, came_back, dense, layouts, new_rows, on_device, raw_stream, require_one_device, with_base
 from ._lib import LIB, check, ptr
 
 
@@ -69,13 +69,14 @@ def _run_backward(dout, q, k, v, q_weight, k_weight, positions, out, lse, low, s
     (rot, _, _, _, w_code), (scale, _, tails, strides, grad_tails) = plans
     batch, heads, tokens, dim = q.shape
     with on_device(q):
-        dout, dout_view = as_rows(dout, broadcast=False)
+        (out, out_view), (dout, dout_view) = as_rows(out, broadcast=False), as_rows(dout, broadcast=False)
+        low, low_view = (None, None) if low is None else as_rows(low, broadcast=False)
+        lse, saved = dense(lse), dense(saved, 256)
         dq, dk, dv = new_rows(q, q.shape, strides[0]), new_rows(k, k.shape, strides[1]), new_rows(k, k.shape, strides[1])
         dwq, dwk = (torch.empty_like(w) if w is not None and weight_grads else None for w in (q_weight, k_weight))
         ws = torch.empty(saved_bytes(batch, heads, k.shape[1], tokens, dim)[1], device=q.device, dtype=torch.uint8)
         check(LIB.b2_norm_rope_attention_backward(
-            with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]), with_base(out, grad_tails[0]),
-            exact.with_optional(low, grad_tails[0]), dout_view, ptr(lse),
+            with_base(q, tails[0]), with_base(k, tails[1]), with_base(v, tails[2]), out_view, low_view, dout_view, ptr(lse),
             ptr(q_weight), ptr(k_weight), w_code, eps, with_base(positions, rot), scale, 1 if causal else 0,
             ptr(key_lengths), ptr(saved), with_base(dq, grad_tails[0]), with_base(dk, grad_tails[1]),
             with_base(dv, grad_tails[1]), ptr(dwq), ptr(dwk), ptr(ws), raw_stream(q)))
@@ -88,16 +89,24 @@ class _NormRopeAttention(torch.autograd.Function):
         q, k, v, *plans = _checked(q, k, v, q_weight, k_weight, positions, call)
         require_one_device("norm_rope_attention", q, k, v, q_weight, k_weight, positions, call[-1])
         out, lse, low, saved = _run_forward(q, k, v, q_weight, k_weight, positions, call, plans, True)
-        ctx.save_for_backward(q, k, v, q_weight, k_weight, positions, out, lse, low, saved, call[-1])
-        ctx.call, ctx.plans = call[:-1], plans
+        kept = (q, k, v, q_weight, k_weight, positions, out, lse, low, saved, call[-1])
+        ctx.save_for_backward(*kept)
+        ctx.call, ctx.plans, ctx.layouts = call[:-1], plans, layouts(*kept)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        *tensors, key_lengths = ctx.saved_tensors
+        kept = ctx.saved_tensors  # each access unpacks them anew
+        q, k, v, q_weight, k_weight, positions, *results, key_lengths = kept
         wanted = ctx.needs_input_grad[3] or ctx.needs_input_grad[4]
-        return (*_run_backward(dout, *tensors, (*ctx.call, key_lengths), ctx.plans, wanted), None, None)
+        call, plans = (*ctx.call, key_lengths), ctx.plans
+        require_one_device("norm_rope_attention", *kept, dout)
+        if not came_back("norm_rope_attention", kept, ctx.layouts):
+            q, k, v = (as_rows(x, broadcast=False)[0] for x in (q, k, v))
+            q_weight, k_weight, call = dense(q_weight), dense(k_weight), (*ctx.call, dense(key_lengths))
+            q, k, v, *plans = _checked(q, k, v, q_weight, k_weight, positions, call)
+        return (*_run_backward(dout, q, k, v, q_weight, k_weight, positions, *results, call, plans, wanted), None, None)
 
 
 def norm_rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor | None,

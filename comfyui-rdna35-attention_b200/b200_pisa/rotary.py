@@ -17,8 +17,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._args import (PLANS, addressable, as_rows, new_rows, on_device, raw_stream, require_one_device, signature,
-                    token_major_strides, view_tail, with_base)
+from ._args import (PLANS, addressable, as_rows, came_back, dense, layouts, new_rows, on_device, raw_stream,
+                    require_one_device, signature, token_major_strides, view_tail, with_base)
 from ._lib import LIB, check, ptr
 
 MAX_ROTARY_DIM = 256
@@ -239,16 +239,24 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, positions, axes_dims, eps, theta, interleaved):
-        ctx.save_for_backward(q, k, q_weight, k_weight, positions)
-        plan = _plan_of(q, k, q_weight, k_weight, positions, axes_dims, eps, theta, interleaved)
-        ctx.call = (eps, plan)
+        saved = (q, k, q_weight, k_weight, positions)
+        ctx.save_for_backward(*saved)
+        plan = _plan_of(*saved, axes_dims, eps, theta, interleaved)
+        ctx.call = (axes_dims, eps, theta, interleaved)
+        ctx.plan, ctx.layouts = plan, layouts(*saved)
         return _run_norm_rope(q, k, q_weight, k_weight, positions, eps, plan)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
         wanted = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
-        grads = _run_norm_rope_backward(dq_out, dk_out, *ctx.saved_tensors, *ctx.call, wanted)
+        saved, plan = ctx.saved_tensors, ctx.plan
+        require_one_device("qk_norm_rope", *saved, dq_out, dk_out)
+        if not came_back("qk_norm_rope", saved, ctx.layouts):
+            q, k, q_weight, k_weight, positions = saved
+            saved = (as_rows(q)[0], as_rows(k)[0], dense(q_weight), dense(k_weight), positions)
+            plan = _plan_of(*saved, *ctx.call)
+        grads = _run_norm_rope_backward(dq_out, dk_out, *saved, ctx.call[1], plan, wanted)
         return (*grads, None, None, None, None, None)
 
 

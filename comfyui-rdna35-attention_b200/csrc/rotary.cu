@@ -198,8 +198,8 @@ struct Raw {
     } else if constexpr (LAYOUT == kInterleaved) {
       cp_async16(to, row + c0 * 2, 16);
     } else {
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to), "l"(row + c0 * 2));
-      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to + 8), "l"(row + c1 * 2));
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to), "l"(row + c0 * 2) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;\n" ::"r"(to + 8), "l"(row + c1 * 2) : "memory");
     }
   }
   __device__ __forceinline__ void take(const char* slot) {

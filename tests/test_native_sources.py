@@ -38,3 +38,15 @@ def test_a_copy_elsewhere_reads_its_own_headers(tmp_path):
         deps = [pathlib.Path(d).resolve() for d in out.replace("\\\n", " ").split(":", 1)[1].split()]
         foreign = [str(d) for d in deps if ROOT in d.parents]
         assert not foreign, f"{name} of the copy reads {foreign}"
+
+
+# Instructions that copy to or wait for memory which ordinary loads and stores read and write: without the clobber the
+# compiler may move those across them.
+MEMORY = re.compile(r"\b(cp\.async|mbarrier\.|fence\.|bar\.sync|griddepcontrol\.)")
+
+
+@pytest.mark.parametrize("path", FILES, ids=lambda p: p.name)
+def test_copies_and_waits_clobber_memory(path):
+    for match in re.finditer(r"\basm\s+volatile\s*\((.*?)\)\s*;", path.read_text(), re.S):
+        if MEMORY.search(match[1]):
+            assert '"memory"' in match[1], f"{path.name}: {match[0]}"

@@ -13,6 +13,7 @@ import functools
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import LIB, check
@@ -54,6 +55,16 @@ def require_one_device(name: str, *tensors: torch.Tensor | None) -> None:
             one = False
     if not one:
         raise ValueError(f"{name} requires its tensors on one CUDA device.")
+
+
+def refuse_tangents(name: str, *tensors: torch.Tensor | None) -> None:
+    """Forward-mode derivatives do not exist here; results without them would pass for constants."""
+    if forward_ad._current_level < 0:  # no dual level is open, so no tensor has a tangent
+        return
+    tracing = torch.compiler.is_compiling()  # a traced tensor does not show its tangent
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and (tracing or forward_ad.unpack_dual(t).tangent is not None):
+            raise ValueError(f"{name} has no forward-mode derivatives; its tensors must not carry tangents.")
 
 
 def row_strides(shape, strides) -> tuple[int, ...]:

@@ -17,8 +17,8 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
-from ._args import (PLANS, addressable, as_rows, came_back, dense, layouts, new_rows, on_device, raw_stream, repeats,
-                    require_one_device, signature, token_major_strides, view_tail, with_base)
+from ._args import (PLANS, addressable, as_rows, came_back, dense, layouts, new_rows, on_device, raw_stream, refuse_tangents,
+                    repeats, require_one_device, signature, token_major_strides, view_tail, with_base)
 from ._lib import LIB, check, ptr
 
 MAX_HEAD_DIM = 128
@@ -128,6 +128,7 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: 
     error (like out, BF16) in rows that see at most 64 keys, whose gradients
     it is the largest error of (its other rows are not written); None where no
     row can see so few."""
+    refuse_tangents("attention_forward", q, k, v)
     flat = isinstance(q, torch.Tensor) and q.ndim == 3
     q, k, v, plan = _planned(q, k, v, scale, key_lengths)
     require_one_device("attention", q, k, v, key_lengths)
@@ -182,6 +183,7 @@ def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: 
     and what it returned (out_low is optional).  Probabilities are recomputed
     from lse; dk and dv of a shared head are summed over its group in FP32;
     rows of dk and dv past a batch's keys are 0.  Bit-reproducible."""
+    refuse_tangents("attention_backward", dout, q, k, v, out, lse, out_low)
     flat = isinstance(q, torch.Tensor) and q.ndim == 3
     q, k, v, plan = _planned(q, k, v, scale, key_lengths)
     out, dout, out_low = check_saved(q, flat, lse, out=out, dout=dout, out_low=out_low)
@@ -205,6 +207,7 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        refuse_tangents("attention", dout)
         saved = ctx.saved_tensors  # each access unpacks them anew
         q, k, v, out, lse, low, key_lengths = saved
         plan, causal, flat, were = ctx.call
@@ -221,7 +224,9 @@ class _Attention(torch.autograd.Function):
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float | None = None, *, causal: bool = False,
               key_lengths: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(scale q k^T) v, differentiable in q, k and v (see
-    attention_forward for the masks and layouts; scale defaults to D^-0.5)."""
+    attention_forward for the masks and layouts; scale defaults to D^-0.5).
+    Tensors that carry forward-mode tangents are refused."""
+    refuse_tangents("attention", q, k, v)
     if torch.compiler.is_compiling():
         scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
         return torch.ops.b200_pisa.attention(q, k, v, scale, bool(causal), key_lengths)[0]

@@ -15,7 +15,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import exact, rotary
-from ._args import as_rows, came_back, dense, layouts, new_rows, on_device, raw_stream, require_one_device, with_base
+from ._args import (as_rows, came_back, dense, layouts, new_rows, on_device, raw_stream, refuse_tangents, require_one_device,
+                    with_base)
 from ._lib import LIB, check, ptr
 
 
@@ -97,6 +98,7 @@ class _NormRopeAttention(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
+        refuse_tangents("norm_rope_attention", dout)
         kept = ctx.saved_tensors  # each access unpacks them anew
         q, k, v, q_weight, k_weight, positions, *results, key_lengths = kept
         wanted = ctx.needs_input_grad[3] or ctx.needs_input_grad[4]
@@ -117,7 +119,9 @@ def norm_rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     q [B,H,T,D], k and v [B,Hk,T,D] (BF16 or FP16, D <= 128), weights [D] or
     None, positions and axes_dims of the rotation, scale, causal and
     key_lengths of the attention (K rows past a batch's keys are not used,
-    whatever they hold).  Differentiable in q, k, v and the weights."""
+    whatever they hold).  Differentiable in q, k, v and the weights (reverse
+    mode; tangents are refused)."""
+    refuse_tangents("norm_rope_attention", q, k, v, q_weight, k_weight, positions)
     axes_dims, theta = rotary._hashable(axes_dims, theta)
     if torch.compiler.is_compiling():
         scale = float(q.shape[-1] ** -0.5 if scale is None else scale)

@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._args import (PLANS, addressable, as_rows, came_back, dense, layouts, new_rows, on_device, raw_stream,
+from ._args import (PLANS, addressable, as_rows, came_back, dense, layouts, new_rows, on_device, raw_stream, refuse_tangents,
                     require_one_device, signature, token_major_strides, view_tail, with_base)
 from ._lib import LIB, check, ptr
 
@@ -114,6 +114,7 @@ class _AxialRope(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        refuse_tangents("axial_rope", dy)
         axes_dims, theta, interleaved, inverse = ctx.rotation
         (positions,) = ctx.saved_tensors
         return _rope_call(as_rows(dy)[0], positions, axes_dims, theta, interleaved, not inverse), None, None, None, None, None
@@ -130,7 +131,8 @@ def axial_rope(x: torch.Tensor, positions: torch.Tensor, axes_dims: Sequence[int
     be one number per axis).  interleaved: pair p is columns (2p, 2p+1), else
     (p, p + R/2).  inverse rotates back.  Angles are reduced in FP64, so far
     positions keep their accuracy; the result is rounded once to x's type.
-    Differentiable in x."""
+    Differentiable in x (reverse mode; tangents are refused)."""
+    refuse_tangents("axial_rope", x, positions)
     rotation = (*_hashable(axes_dims, theta), bool(interleaved), bool(inverse))
     if torch.compiler.is_compiling():
         return torch.ops.b200_pisa.axial_rope(x, positions, rotation[0], rates(*rotation[:2]), *rotation[2:])
@@ -227,6 +229,7 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     k_weight_grad) from the gradients of its two outputs; the weights' are
     None without weights or with weight_grads=False.  The statistics are
     recomputed from q and k.  Bit-reproducible."""
+    refuse_tangents("qk_norm_rope_backward", dq_out, dk_out, q, k, q_weight, k_weight, positions)
     axes_dims, theta = _hashable(axes_dims, theta)
     plan = _plan_of(q, k, q_weight, k_weight, positions, axes_dims, float(eps), theta, bool(interleaved))
     for name, dy, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
@@ -249,6 +252,7 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
+        refuse_tangents("qk_norm_rope", dq_out, dk_out)
         wanted = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
         saved, plan = ctx.saved_tensors, ctx.plan
         require_one_device("qk_norm_rope", *saved, dq_out, dk_out)
@@ -266,7 +270,9 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     """RMS-norm every row of q [B,Hq,T,D] and k [B,Hk,T,D] over D, scale it by
     its weight [D] (None for none) and rotate it by the tokens' positions
     (``axial_rope``), in one launch with one rounding at the end.
-    Differentiable in q, k and the weights."""
+    Differentiable in q, k and the weights (reverse mode; tangents are
+    refused)."""
+    refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, positions)
     axes_dims, theta = _hashable(axes_dims, theta)
     if torch.compiler.is_compiling():
         return torch.ops.b200_pisa.qk_norm_rope(q, k, q_weight, k_weight, positions, axes_dims, float(eps),

@@ -153,7 +153,7 @@ def norm_rope_attention_op(q: Tensor, k: Tensor, v: Tensor, q_weight: Optional[T
 def _(q, k, v, q_weight, k_weight, positions, axes_dims, scale, eps, theta, interleaved, causal, key_lengths):
     batch, heads, tokens, dim = q.shape
     low = _like(q) if exact.wants_low(q.dtype, tokens, key_lengths, causal) else q.new_empty(0)
-    saved = fused.saved_bytes(batch, heads, k.shape[1], tokens, dim)[0]
+    saved = fused.saved_size(batch, heads, k.shape[1], tokens, dim)
     return _like(q), q.new_empty(q.shape[:3], dtype=torch.float32), low, q.new_empty(saved, dtype=torch.uint8)
 
 

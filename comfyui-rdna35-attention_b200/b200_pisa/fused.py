@@ -26,6 +26,14 @@ def saved_bytes(batch: int, heads: int, kv_heads: int, tokens: int, dim: int) ->
     return LIB.b2_norm_rope_attention_saved_bytes(*sizes), LIB.b2_norm_rope_attention_workspace_bytes(*sizes)
 
 
+def saved_size(batch, heads, kv_heads, tokens, dim):
+    """saved_bytes()[0] of sizes that need not be numbers: a traced call's are
+    symbols, which neither a cache nor the library takes.  FP16 queries and keys
+    and two FP32 scales, each from a multiple of 256 bytes."""
+    queries, keys = (2 * batch * h * tokens * dim for h in (heads, kv_heads))
+    return (queries + 255) // 256 * 256 + (keys + 255) // 256 * 256 + 256
+
+
 def _checked(q, k, v, q_weight, k_weight, positions, call):
     """Both operators' checks; (q, k, v, rotation plan, attention plan)."""
     axes_dims, scale, eps, theta, interleaved, causal, key_lengths = call

@@ -6,7 +6,10 @@
 //   S = Q K^T in tensor memory (two buffers), P = exp(scale S - max) rounded to
 //   the type of v and written back over S, O += P V, O /= sum at the end.
 // O is rescaled only when a row's maximum has grown by 2^8 (P stays below
-// that, and the sum is of the same P).
+// that).  The sum is of P before its rounding.  FP16 P is held times 2^8, as in
+// the backward pass: without, keys below 2^-25 of the largest would leave P V
+// and stay in the sum (65535 at 2^-25.5: 1.4e-3 of the row, all of it lost).  O
+// is then rescaled from 2^7 on, and P stays below 2^15.
 //
 // Persistent CTAs, two per SM (112 KB of shared memory, 256 TMEM columns
 // each), step through the items by the grid's size: barriers, rings and tensor
@@ -42,6 +45,7 @@ constexpr int kVWarp = 6;   // warp 0: Q and K, warp 1: MMA and TMEM, warps 2-5:
 constexpr int kThreads = 32 * (kVWarp + 1);
 constexpr uint32_t kTmem = 256, kO = 0, kS = 128;  // columns: O, and S by kKeys
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kShiftP16 = 8.f;  // FP16 v: P is held times 2^8
 
 struct ForwardArgs {
   Rows o, o_low;  // o_low: what o's type cannot hold, or no base
@@ -275,6 +279,7 @@ template <bool BF16, bool QK16, int HALVES>
 __device__ void softmax(const ForwardArgs& a, char* smem, Misc& m, uint32_t tmem) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   using L = Smem<HALVES>;
+  constexpr float kGrowth = BF16 ? 8.f : 7.f;
   volatile int* abort_flag = &m.abort_flag;
   const int lane = threadIdx.x & 31;
   const int sub = (threadIdx.x >> 5) & 3;  // TMEM sub-partition of this warp
@@ -294,7 +299,7 @@ __device__ void softmax(const ForwardArgs& a, char* smem, Misc& m, uint32_t tmem
       continue;
     }
     const int last = r + a.off;  // causal: the last key the row sees
-    float mrun = -INFINITY, lrun = 0.f;
+    float mrun = -INFINITY, lrun = 0.f;  // mrun: the maximum less P's shift
     for (int j = 0; j < w.n; ++j, ++g) {
       const uint32_t sb = g & 1;
       if (!mbar_wait(&m.s_full[sb], (g >> 1) & 1, abort_flag, a.status, 8)) return;
@@ -326,13 +331,13 @@ __device__ void softmax(const ForwardArgs& a, char* smem, Misc& m, uint32_t tmem
         m0 = max3(m0, __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
         m1 = max3(m1, __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
       }
-      const float mx = fmaxf(m0, m1) * mul;
+      const float mx = BF16 ? fmaxf(m0, m1) * mul : fmaf(fmaxf(m0, m1), mul, -kShiftP16);
       float alpha = 1.f;
       bool rescale = false;
       const float mnew = fmaxf(mrun, mx);
       if (mrun == -INFINITY) {
         mrun = mnew;
-      } else if (mnew > mrun + 8.0f) {
+      } else if (mnew > mrun + kGrowth) {
         alpha = ex2(mrun - mnew);
         mrun = mnew;
         rescale = true;

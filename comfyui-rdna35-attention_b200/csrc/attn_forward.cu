@@ -357,23 +357,19 @@ __device__ void softmax(const ForwardArgs& a, char* smem, Misc& m, uint32_t tmem
         }
         tmem_wait_st();
       }
-      if (mrun != -INFINITY) {
-        const float neg = -mrun;
-        float s0 = 0.f, s1 = 0.f;
+      // no maximum yet: masked keys (-inf) give 0, and NaN, which no maximum shows, stays
+      const float neg = mrun == -INFINITY ? 0.f : -mrun;
+      float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-        for (int c = 0; c < kKeys; c += 2) {
-          float x0, x1;
-          fma2(x0, x1, __uint_as_float(v[c]), __uint_as_float(v[c + 1]), mul, neg);
-          const float p0 = ex2(x0);
-          const float p1 = ex2(x1);
-          add2(s0, s1, p0, p1);
-          v[c / 2] = Cvt<T>::pack2(p0, p1);
-        }
-        lrun = lrun * alpha + (s0 + s1);
-      } else {
-#pragma unroll
-        for (int c = 0; c < kKeys / 2; ++c) v[c] = 0u;
+      for (int c = 0; c < kKeys; c += 2) {
+        float x0, x1;
+        fma2(x0, x1, __uint_as_float(v[c]), __uint_as_float(v[c + 1]), mul, neg);
+        const float p0 = ex2(x0);
+        const float p1 = ex2(x1);
+        add2(s0, s1, p0, p1);
+        v[c / 2] = Cvt<T>::pack2(p0, p1);
       }
+      lrun = lrun * alpha + (s0 + s1);
       tmem_st32(s_addr, v);
       tmem_wait_st();
       // V rows past the batch's keys may hold anything: P is 0 there, but
@@ -395,6 +391,7 @@ __device__ void softmax(const ForwardArgs& a, char* smem, Misc& m, uint32_t tmem
     if (!mbar_wait(&m.pv_done[(g - 1) & 1], ((g - 1) >> 1) & 1, abort_flag, a.status, 10)) return;
     tc_fence_after();
     const float inv = lrun > 0.f ? 1.f / lrun : 0.f;
+    const float empty = a.causal && last < 0 ? 0.f : NAN;  // without a sum: no key seen, or -inf from all (0 / 0)
     const int q = lane & 3;
     char* quad_row = a.o.row(w.bh, r - q);
     char* low_row = low ? a.o_low.row(w.bh, r) : nullptr;
@@ -407,8 +404,8 @@ __device__ void softmax(const ForwardArgs& a, char* smem, Misc& m, uint32_t tmem
       // each row's 16 bytes touch a line of their own.
 #pragma unroll
       for (int c = 0; c < 32; c += 2) {
-        const float f0 = lrun == 0.f ? 0.f : __uint_as_float(o[c]) * inv;  // no key seen: O may hold anything
-        const float f1 = lrun == 0.f ? 0.f : __uint_as_float(o[c + 1]) * inv;
+        const float f0 = lrun == 0.f ? empty : __uint_as_float(o[c]) * inv;
+        const float f1 = lrun == 0.f ? empty : __uint_as_float(o[c + 1]) * inv;
         x[c / 2] = Cvt<T>::pack2(f0, f1);
         if (low) {  // what the output's type cannot hold
           float h0, h1;

@@ -132,6 +132,7 @@ def norm_rope_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
     refuse_tangents("norm_rope_attention", q, k, v, q_weight, k_weight, positions)
     axes_dims, theta = rotary._hashable(axes_dims, theta)
     if torch.compiler.is_compiling():
+        rotary._no_position_gradient(positions)
         scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
         return torch.ops.b200_pisa.norm_rope_attention(q, k, v, q_weight, k_weight, positions, axes_dims, scale, float(eps),
                                                        rotary.rates(axes_dims, theta), bool(interleaved), bool(causal),

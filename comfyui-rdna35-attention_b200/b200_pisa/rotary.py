@@ -89,7 +89,7 @@ def _rope_plan(sig, pos_sig, axes_dims, theta, interleaved, inverse):
 
 
 def _no_position_gradient(positions) -> None:
-    if positions.requires_grad:
+    if isinstance(positions, torch.Tensor) and positions.requires_grad:
         raise ValueError("positions have no gradient here; detach them.")
 
 
@@ -135,6 +135,7 @@ def axial_rope(x: torch.Tensor, positions: torch.Tensor, axes_dims: Sequence[int
     refuse_tangents("axial_rope", x, positions)
     rotation = (*_hashable(axes_dims, theta), bool(interleaved), bool(inverse))
     if torch.compiler.is_compiling():
+        _no_position_gradient(positions)  # the op would not see it
         return torch.ops.b200_pisa.axial_rope(x, positions, rotation[0], rates(*rotation[:2]), *rotation[2:])
     if torch.is_grad_enabled() and isinstance(x, torch.Tensor) and x.requires_grad:
         return _AxialRope.apply(x, positions, *rotation)
@@ -275,6 +276,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor | None
     refuse_tangents("qk_norm_rope", q, k, q_weight, k_weight, positions)
     axes_dims, theta = _hashable(axes_dims, theta)
     if torch.compiler.is_compiling():
+        _no_position_gradient(positions)
         return torch.ops.b200_pisa.qk_norm_rope(q, k, q_weight, k_weight, positions, axes_dims, float(eps),
                                                 rates(axes_dims, theta), bool(interleaved))
     args = (q, k, q_weight, k_weight, positions, axes_dims, float(eps), theta, bool(interleaved))

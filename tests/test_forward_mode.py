@@ -1,7 +1,7 @@
-"""Forward-mode derivatives do not exist for the rotary and the differentiable
-attention entry points: a tensor that carries a tangent is refused, in eager
-calls, under torch.compile and in a backward pass (CPU; the refusal comes
-before anything that needs a GPU)."""
+"""Derivatives that are refused (CPU; before anything that needs a GPU).
+Forward-mode ones do not exist for the rotary and the differentiable attention
+entry points: a tensor that carries a tangent is refused, in eager calls, under
+torch.compile and in a backward pass.  Positions have no gradient."""
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -111,3 +111,16 @@ def test_a_gradient_with_a_tangent_is_refused(monkeypatch, name):
     out = out[0] if isinstance(out, tuple) else out
     with forward_ad.dual_level(), pytest.raises(ValueError, match="forward-mode"):
         out.backward(forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+@pytest.mark.parametrize("name", ["axial_rope", "qk_norm_rope", "norm_rope_attention"])
+@pytest.mark.parametrize("fullgraph", [False, True])
+def test_derivatives_of_positions_are_refused_under_compile(name, fullgraph):
+    torch._dynamo.reset()
+    names, call = calls()[name]
+    args = tensors()
+    args["pos"].requires_grad_()
+    compiled = torch.compile(call, backend="eager", fullgraph=fullgraph)
+    with pytest.raises(torch._dynamo.exc.Unsupported if fullgraph else ValueError, match="no gradient"):
+        compiled(*(args[n] for n in names))
+    torch._dynamo.reset()

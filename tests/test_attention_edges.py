@@ -110,3 +110,19 @@ def test_a_layer_query_that_is_not_a_number_stays_one():
     assert got[0, 1, 33].isnan().all()
     clean[0, 1, 33] = got[0, 1, 33] = 0.0
     assert torch.equal(clean, got)
+
+
+@gpu
+def test_the_benchmark_node_s_default_sizes_equal_full_attention():
+    """1 x 4 heads, 128 tokens x 64, FP16: two kernels that round P and their result once each, at worst apart by
+    both roundings of both, u (P |V|) + u |out| each, and the FP32 part 2^-18 P |V|."""
+    import b200_pisa
+
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    q, k, v = (torch.randn(1, 4, 128, 64, generator=gen, device=DEV).to(torch.float16) for _ in range(3))
+    a = b200_pisa.full_attention(q, k, v, 64 ** -0.5).double()
+    b = b200_pisa.attention(q, k, v).double()
+    p = (q.double() @ k.double().transpose(-1, -2) * 64 ** -0.5).softmax(-1)
+    u = 2.0 ** -11
+    allowed = 2 * (((u + 2.0 ** -18) * p) @ v.double().abs() + u * (p @ v.double()).abs()) * (1 + 2 ** -8) + 128 * 2.0 ** -25 * v.abs().max()
+    assert ((a - b).abs() <= allowed).all()

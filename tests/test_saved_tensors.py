@@ -210,3 +210,36 @@ def test_gradients_under_hooks(op, hook):
     got = torch.autograd.grad(outs, leaves, douts)
     assert all(torch.equal(a, b) and a.stride() == b.stride() for a, b in zip(got, want))
     _lib.check_status()
+
+
+@gpu
+@pytest.mark.parametrize("op", ["axial_rope", "qk_norm_rope", "attention", "flat attention", "norm_rope_attention"])
+def test_gradients_under_checkpointing(op):
+    """The forward pass runs again and hands over its own saved tensors."""
+    from torch.utils.checkpoint import checkpoint
+
+    *leaves, pos, lens = inputs(DEV)
+    outs, used = run(op, *leaves, pos, lens)
+    douts = [torch.randn_like(x) for x in outs]
+    want = torch.autograd.grad(outs, used, douts)
+    outs = checkpoint(lambda *x: run(op, *x, pos, lens)[0], *leaves, use_reentrant=False)
+    got = torch.autograd.grad(outs, used, douts)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@gpu
+@pytest.mark.parametrize("how", ["no leaf wants one", "no_grad"])
+@pytest.mark.parametrize("op", ["axial_rope", "qk_norm_rope", "attention", "flat attention", "norm_rope_attention"])
+def test_calls_without_gradients_keep_their_results_alone(op, how):
+    tensors = inputs(DEV, tokens=700)
+    if how != "no_grad":
+        tensors = [x.detach() for x in tensors]
+    with torch.no_grad() if how == "no_grad" else contextlib.nullcontext():
+        run(op, *tensors)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated(DEV)
+        outs, _ = run(op, *tensors)
+        torch.cuda.synchronize()
+    kept = torch.cuda.memory_allocated(DEV) - before
+    rounded = sum(-(-x.numel() * x.element_size() // 512) * 512 for x in outs)
+    assert kept == rounded and not any(x.requires_grad for x in outs)

@@ -773,6 +773,7 @@ int b2_attention_forward(const b2_view* q, const b2_view* k, const b2_view* v, c
                          int32_t causal, const int32_t* key_lengths, float* lse, const b2_view* out_low, void* stream) {
   int rc = check_attention(q, k, v, out, scale, key_lengths);
   if (rc || (out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q)))) return rc;
+  if (reinterpret_cast<uintptr_t>(lse) % 4) return fail(B2_ERR_INVALID, "lse must be 4-byte aligned");
   int* status = device_status_ptr();
   if (status == nullptr) return fail(B2_ERR_CUDA, "device status word unavailable");
   const AttnForwardCall c{q, k, v, out, key_lengths, scale, causal ? 1 : 0, lse, out_low, nullptr};
@@ -797,7 +798,7 @@ int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, 
   if ((out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q))) || (rc = check_grad_view(dout, "dout", q)) ||
       (rc = check_grad_view(dq, "dq", q)) || (rc = check_grad_view(dk, "dk", k)) || (rc = check_grad_view(dv, "dv", v)))
     return rc;
-  if (lse == nullptr || reinterpret_cast<uintptr_t>(lse) % 4) return fail(B2_ERR_INVALID, "lse must be non-NULL");
+  if (lse == nullptr || reinterpret_cast<uintptr_t>(lse) % 4) return fail(B2_ERR_INVALID, "lse must be non-NULL and 4-byte aligned");
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16)
     return fail(B2_ERR_INVALID, "workspace must be non-NULL and 16-byte aligned");
   int* status = device_status_ptr();
@@ -814,6 +815,8 @@ namespace {
 int check_rotary(const b2_rotary* r, const b2_view* v) {
   if (r == nullptr || r->positions == nullptr) return fail(B2_ERR_INVALID, "positions must be non-NULL");
   if (r->pos_dtype < B2_POS_I32 || r->pos_dtype > B2_POS_F64) return fail(B2_ERR_INVALID, "unknown position dtype");
+  const uintptr_t size = r->pos_dtype == B2_POS_I64 || r->pos_dtype == B2_POS_F64 ? 8 : 4;
+  if (reinterpret_cast<uintptr_t>(r->positions) % size) return fail(B2_ERR_INVALID, "positions must be aligned to their type");
   if (r->n_axes < 1 || r->n_axes > B2_MAX_AXES) return fail(B2_ERR_INVALID, "rotary axes must be 1..%d", B2_MAX_AXES);
   int64_t sum = 0;
   for (int i = 0; i < r->n_axes; ++i) {
@@ -834,6 +837,15 @@ int check_rotary_view(const b2_view* v, const char* name, const b2_view* like) {
   if (int64_t(v->batch) * v->tokens > (1 << 30)) return fail(B2_ERR_UNSUPPORTED, "%s has more than 2^30 tokens", name);
   if (like != nullptr && (!same_bht(v, like) || v->dtype != like->dtype))
     return fail(B2_ERR_INVALID, "%s must have its input's [B,H,T,D] and dtype", name);
+  return B2_OK;
+}
+
+// Rows that a call writes: not twice.
+int check_rotary_out(const b2_view* v, const char* name, const b2_view* like) {
+  const int rc = check_rotary_view(v, name, like);
+  if (rc) return rc;
+  if ((v->batch > 1 && v->stride_b <= 0) || (v->heads > 1 && v->stride_h <= 0) || (v->tokens > 1 && v->stride_t <= 0))
+    return fail(B2_ERR_INVALID, "%s strides must be positive", name);
   return B2_OK;
 }
 
@@ -858,7 +870,7 @@ extern "C" {
 
 int b2_axial_rope(const b2_view* x, const b2_view* out, const b2_rotary* rot, void* stream) {
   int rc;
-  if ((rc = check_rotary_view(x, "x", nullptr)) || (rc = check_rotary_view(out, "out", x)) || (rc = check_rotary(rot, x)))
+  if ((rc = check_rotary_view(x, "x", nullptr)) || (rc = check_rotary_out(out, "out", x)) || (rc = check_rotary(rot, x)))
     return rc;
   RotaryCall c{};
   c.x[0] = x;
@@ -874,7 +886,7 @@ int b2_qk_norm_rope(const b2_view* q, const b2_view* k, const b2_view* q_out, co
                     const b2_rotary* rot, void* stream) {
   int rc = check_qk(q, k, q_weight, k_weight, weight_dtype, eps, rot);
   if (rc) return rc;
-  if ((rc = check_rotary_view(q_out, "q_out", q)) || (rc = check_rotary_view(k_out, "k_out", k))) return rc;
+  if ((rc = check_rotary_out(q_out, "q_out", q)) || (rc = check_rotary_out(k_out, "k_out", k))) return rc;
   RotaryCall c{};
   c.x[0] = q, c.x[1] = k;
   c.y[0] = q_out, c.y[1] = k_out;
@@ -900,7 +912,7 @@ int b2_qk_norm_rope_backward(const b2_view* q, const b2_view* k, const b2_view* 
   int rc = check_qk(q, k, q_weight, k_weight, weight_dtype, eps, rot);
   if (rc) return rc;
   if ((rc = check_rotary_view(dq_out, "dq_out", q)) || (rc = check_rotary_view(dk_out, "dk_out", k)) ||
-      (rc = check_rotary_view(q_grad, "q_grad", q)) || (rc = check_rotary_view(k_grad, "k_grad", k)))
+      (rc = check_rotary_out(q_grad, "q_grad", q)) || (rc = check_rotary_out(k_grad, "k_grad", k)))
     return rc;
   const uintptr_t mask = weight_dtype == B2_F32 ? 3 : 1;
   if ((reinterpret_cast<uintptr_t>(q_weight_grad) | reinterpret_cast<uintptr_t>(k_weight_grad)) & mask)
@@ -995,6 +1007,7 @@ int b2_norm_rope_attention_forward(const b2_view* q, const b2_view* k, const b2_
                                    void* saved, float* lse, const b2_view* out_low, void* stream) {
   int rc = check_fused(q, k, v, out, q_weight, k_weight, weight_dtype, eps, rot, scale, key_lengths, saved);
   if (rc || (out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q)))) return rc;
+  if (reinterpret_cast<uintptr_t>(lse) % 4) return fail(B2_ERR_INVALID, "lse must be 4-byte aligned");
   int* status = device_status_ptr();
   if (status == nullptr) return fail(B2_ERR_CUDA, "device status word unavailable");
   const FusedSaved f = fused_saved(q->batch, q->heads, k->heads, q->tokens, q->head_dim);
@@ -1031,7 +1044,7 @@ int b2_norm_rope_attention_backward(const b2_view* q, const b2_view* k, const b2
   if ((out_low != nullptr && (rc = check_grad_view(out_low, "out_low", q))) || (rc = check_grad_view(dout, "dout", q)) ||
       (rc = check_grad_view(dq, "dq", q)) || (rc = check_grad_view(dk, "dk", k)) || (rc = check_grad_view(dv, "dv", v)))
     return rc;
-  if (lse == nullptr || reinterpret_cast<uintptr_t>(lse) % 4) return fail(B2_ERR_INVALID, "lse must be non-NULL");
+  if (lse == nullptr || reinterpret_cast<uintptr_t>(lse) % 4) return fail(B2_ERR_INVALID, "lse must be non-NULL and 4-byte aligned");
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(B2_ERR_INVALID, "workspace must be non-NULL and 256-byte aligned");
   const uintptr_t mask = weight_dtype == B2_F32 ? 3 : 1;

@@ -342,7 +342,8 @@ int b2_attention_backward(const b2_view* q, const b2_view* k, const b2_view* v, 
  * and cover the first R = sum(axes_dims) columns, the others pass through.
  * interleaved: pair p is columns (2p, 2p+1), else (p, p + R/2).  inverse:
  * rotate by the negative angle (the rotation's gradient).  Angles are reduced
- * in FP64. */
+ * in FP64.  positions lies on a boundary of its type; strides of outputs are
+ * positive (inputs may repeat rows). */
 enum b2_pos_dtype { B2_POS_I32 = 0, B2_POS_I64 = 1, B2_POS_F32 = 2, B2_POS_F64 = 3 };
 #define B2_MAX_AXES 4
 typedef struct b2_rotary {

@@ -175,3 +175,37 @@ def test_sharded_and_mask_entry_points_check_arguments_without_a_gpu():
     assert values == sorted(values) and values[0] == 0 and values[-1] < total
     assert all(o % 256 == 0 for o in values)
     assert lib.b2_pisa_workspace_layout(32, 9216, 64, 23, offs, _lib.WS_FIELDS) == _lib.B2_ERR_INVALID
+
+
+def test_rotary_and_attention_entries_refuse_addresses_the_kernels_cannot_use():
+    """Positions and lse off their type's boundaries, and outputs whose rows repeat."""
+    import torch
+    from b200_pisa import _lib
+
+    lib = _lib.LIB
+    x = torch.zeros((1, 2, 4, 64), dtype=torch.bfloat16)
+    view, buffer, at = _lib.view(x), torch.zeros(8192), ctypes.byref
+    good = at(view)
+    ws = -(-buffer.data_ptr() // 256) * 256
+
+    def refused(rc, what):
+        assert rc == _lib.B2_ERR_INVALID and what in lib.b2_last_error(), (rc, lib.b2_last_error())
+
+    for code, size in ((_lib.POS_I32, 4), (_lib.POS_I64, 8), (_lib.POS_F32, 4), (_lib.POS_F64, 8)):
+        rot = _lib.Rotary(ws + size // 2, 0, 1, 1, code, 1)
+        rot.axes_dims[0], rot.theta[0] = 64, 1e4
+        refused(lib.b2_axial_rope(good, good, at(rot), None), b"positions must be aligned")
+        refused(lib.b2_qk_norm_rope(good, good, good, good, None, None, _lib.B2_F32, 1e-6, at(rot), None), b"positions must be aligned")
+        refused(lib.b2_norm_rope_attention_forward(good, good, good, good, None, None, _lib.B2_F32, 1e-6, at(rot), 0.1, 0, None,
+                                                   ws, ws, None, None), b"positions must be aligned")
+    rot.positions = ws
+    refused(lib.b2_attention_forward(good, good, good, good, 0.1, 0, None, ws + 2, None, None), b"lse must be")
+    refused(lib.b2_norm_rope_attention_forward(good, good, good, good, None, None, _lib.B2_F32, 1e-6, at(rot), 0.1, 0, None,
+                                               ws, ws + 2, None, None), b"lse must be")
+    for field in ("stride_h", "stride_t"):
+        bad = _lib.view(x)
+        setattr(bad, field, 0)
+        refused(lib.b2_axial_rope(good, at(bad), at(rot), None), b"out strides must be positive")
+        refused(lib.b2_qk_norm_rope(good, good, good, at(bad), None, None, _lib.B2_F32, 1e-6, at(rot), None), b"k_out strides")
+        refused(lib.b2_qk_norm_rope_backward(good, good, good, good, at(bad), good, None, None, _lib.B2_F32, 1e-6, at(rot), None,
+                                             None, None, None), b"q_grad strides")

@@ -309,15 +309,20 @@ __device__ __forceinline__ float warp_most(const float* x, int64_t n, int lane) 
   return most;
 }
 
+// The least n with x < 2^n for a square x; of one that is 0 in FP32, of its least value.
+__device__ __forceinline__ int square_log2(float x) { return x > 0.f ? ilogbf(x) + 1 : -148; }
+
 // FP16 dS: the power of two it is held times (the shift of P aside), so that
 // 2^shift * 2 max|dO| max|V| times it stays below 2^15.
 __device__ __forceinline__ float ds_gain(const GradArgs& a, int b, int hk, int shift, int lane) {
   const int64_t bh = int64_t(b) * a.heads + int64_t(hk) * a.group, bhk = int64_t(b) * a.kv_heads + hk;
-  const float bound2 = warp_most(a.do_norm + bh * 2 * a.q_tiles, int64_t(a.group) * 2 * a.q_tiles, lane) *
-                       warp_most(a.v_norm + bhk * a.v_blocks, a.v_blocks, lane);
-  if (!(bound2 > 0.f) || !(bound2 < 3e38f)) return 1.f;
-  const int e = 15 - shift - 1 - 1 - (ilogbf(bound2) >> 1);  // bound < 2^(ilogb(bound2)/2 + 1)
-  return ldexpf(1.f, min(max(e, -60), 60));
+  const float do2 = warp_most(a.do_norm + bh * 2 * a.q_tiles, int64_t(a.group) * 2 * a.q_tiles, lane);
+  const float v2 = warp_most(a.v_norm + bhk * a.v_blocks, a.v_blocks, lane);
+  const float bound2 = do2 * v2;
+  // the product where FP32 holds it: its exponent may be one less than the factors' together
+  const int twice = bound2 > 1e-36f && bound2 < 3e38f ? square_log2(bound2) : square_log2(do2) + square_log2(v2);
+  const int e = 15 - shift - 1 - ((twice + 1) >> 1);  // bound < 2^ceil(twice / 2)
+  return ldexpf(1.f, min(max(e, -100), 100));
 }
 
 // Rows of a result tile in global memory.
@@ -1064,8 +1069,8 @@ __device__ __forceinline__ float dot8(const uint4& a, const uint4& low, const ui
 }
 
 // -lse*log2e and -delta of every query row, padded to whole tiles with rows
-// that give P = 0.  NORMS: also the largest squared norms of 64 dO rows and of
-// 64 valid V rows.  Block 0 resets the item counter of the kernel after.
+// that give P = 0.  NORMS: also the largest finite squared norms of 64 dO rows
+// and of 64 valid V rows (rows that are not finite say nothing of the others).  Block 0 resets the item counter of the kernel after.
 // A block takes 64 rows of one head, 16 lanes a row and four rows of each
 // lane at a time.  What counts is instructions: with a row address and
 // separate shuffles for each row it took 80 us for 64 heads of 9216 x 128 (16
@@ -1140,6 +1145,7 @@ __global__ void __launch_bounds__(256) attn_grad_stat_kernel(const __grid_consta
     most = sum_rows(norm, l);
   }
   if constexpr (NORMS) {
+    if (!(most < INFINITY)) most = 0.f;
 #pragma unroll
     for (int w = 16; w >= 4; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;

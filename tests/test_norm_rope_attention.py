@@ -214,3 +214,53 @@ def test_c_sizes():
     assert lib.b2_norm_rope_attention_saved_bytes(1, 4, 2, 100, 136) == -1
     assert lib.b2_norm_rope_attention_workspace_bytes(1, 4, 2, 100, 64) >= 4 * 100 * 64 * (4 + 2)
     assert lib.b2_norm_rope_attention_workspace_bytes(0, 4, 2, 100, 64) == -1
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("power", [60, 57, 30, -50, -75, -85])
+def test_gradients_scale_with_dout(d, power):
+    """Gradients of dout * 2^n are those of dout times 2^n, whatever power of two FP16 holds dS times in between: exactly
+    where it can follow dout's rows.  Below, their squares leave FP32 and dS is held up to 2^10 lower than it could be,
+    its small entries as subnormals: results may round to the next BF16 value, 2^-7 of theirs."""
+    import b200_pisa
+
+    t, axes = 200, (d,)
+    q, k, v = (make(1, h, t, d, torch.bfloat16, "bthd", i) for i, h in ((1, 4), (2, 2), (3, 2)))
+    dout = make(1, 4, t, d, torch.bfloat16, "bthd", 4)
+    pos = torch.arange(t, device=DEV)[:, None]
+    w = torch.ones(d, device=DEV)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v, w, w)]
+    out = b200_pisa.norm_rope_attention(*leaves, pos, axes)
+    want = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+    got = torch.autograd.grad(out, leaves, dout * 2.0 ** power)
+    for name, a, b in zip(("dq", "dk", "dv", "dwq", "dwk"), want, got):
+        a, b = a.double(), b.double() * 2.0 ** -power
+        if power > -70:
+            assert torch.equal(a, b), name
+        else:
+            assert ((a - b).norm() <= 2.0 ** -7 * a.norm()).item(), name
+
+
+
+@gpu
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("d,dtype,layer", [(64, torch.float16, False), (128, torch.float16, False), (128, torch.bfloat16, True)])
+def test_a_dout_row_that_is_not_finite_leaves_the_others(d, dtype, layer, value):
+    """Their dq is that beside a row of zeros, bit for bit."""
+    import b200_pisa
+
+    q, k, v, dout = (make(1, 3, 150, d, dtype, "bthd", i) for i in range(4))
+    dout *= 2.0 ** -12
+    pos = torch.arange(150, device=DEV)[:, None]
+    grads = []
+    for x in (0.0, value):
+        dout[0, 1, 77] = 0.0
+        dout[0, 1, 77, 5] = x
+        leaf = q.clone().requires_grad_()
+        out = b200_pisa.norm_rope_attention(leaf, k, v, None, None, pos, (d,)) if layer else b200_pisa.attention(leaf, k, v)
+        grads.append(torch.autograd.grad(out, leaf, dout)[0])
+    assert not grads[1][0, 1, 77].isfinite().any()
+    for g in grads:
+        g[0, 1, 77] = 0.0
+    assert torch.equal(*grads)

@@ -21,8 +21,8 @@
 //
 // What bounds it: the softmax chain of a tile (load S, maximum, exponentials,
 // store P), which two CTAs overlap; tensor and exponential pipes are each half
-// used.  2 x 16 x 9216^2 x 128: 1.22 ms, 1141 TFLOP/s (a CTA an item: 1.455);
-// 64 heads of 9216 queries and 512 keys: 197 us (249).  Three CTAs per SM with
+// used.  2 x 16 x 9216^2 x 128: 1.18 ms, 1177 TFLOP/s (a CTA an item: 1.455;
+// FP16 1.22); 64 heads of 9216 queries and 512 keys: 192 us (249).  Three CTAs per SM with
 // one S buffer and half a row's logits in registers, for D <= 64: 211 us
 // against 133 (16 x 4096^2 x 64).
 #include <cudaTypedefs.h>

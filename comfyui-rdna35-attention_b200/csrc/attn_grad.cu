@@ -39,14 +39,18 @@
 // quadrant, and each group of four warps takes 32 columns of a tile).
 // Rings, barriers and tensor memory live across items: an item's first tiles
 // load and its first S and dP run while the one before stores its results.
+// 18 warps put five on one scheduler, which caps registers at 96: for D > 64
+// the elementwise warps spill 116 to 140 bytes (8 to 24 up to 64).
 //
 // Precision: products of 16-bit operands accumulated in FP32; P and dS are
 // rounded once, as operands: P to the type of v, dS to that of q and k.  FP16
 // has too small a range for them.  With FP16 v, P is held times 2^8; FP16 dS
 // is held times a power of two chosen from the largest norms of dO and V rows
 // (|dP - delta| <= 2 |dO||V|), which cannot overflow; both are taken out again
-// in FP32 at the end.  QK16: q and k are FP16 copies (times a power of two
-// each) of what v's BF16 could hold less exactly, and dQ, dK leave in FP32.
+// in FP32 at the end.  So held, a dS below 2^-29 of that bound (rows of dO far
+// smaller than the head's largest) loses bits to FP16's subnormals, and one
+// below 2^-40 is 0.  QK16: q and k are FP16 copies (times a power of two each)
+// of what v's BF16 could hold less exactly, and dQ, dK leave in FP32.
 #include <cudaTypedefs.h>
 
 #include <type_traits>

@@ -28,8 +28,8 @@
 // writes, fetches them by asynchronous copies into slots that only their own
 // thread reads: 142 us against 204 (9170 tokens of 56 + 56 heads x 128) for
 // loads into registers.
-// 9216 x (16 + 16) x 128, norm and rotation forward: 32 us (HBM alone: 23);
-// 32760 x 40 x 128, rotation: 111 us (102.6).
+// 9216 x (16 + 16) x 128, norm and rotation forward: 34 us (HBM alone: 23);
+// 32760 x 40 x 128, rotation: 114 us (102.6).
 #include <math.h>
 #include <string.h>
 
